@@ -41,7 +41,7 @@
 extern "C" {
 #endif
 
-#define SMX_VERSION 14
+#define SMX_VERSION 15
 
 /* Status codes. */
 #define SMX_OK 0
@@ -382,6 +382,131 @@ int smx_scale_rows(int64_t m, int64_t n, const void* x, int64_t ldx, const float
 int smx_qk_norm_rope(int64_t m, int64_t n, const float* x, int64_t ldx, const void* rope_cos, const void* rope_sin,
                      const void* rope_scale, int32_t dtypes, int32_t bn, int32_t head_dim, float eps, void* out,
                      int64_t ldo, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Serving: a paged key/value cache, attention over it, 4-bit weights. These
+ * have no counterpart in the reference, whose decoder keeps no cache.
+ * ------------------------------------------------------------------------ */
+
+#define SMX_PAGED_MAX_REQUESTS 8192
+#define SMX_PAGED_MAX_TOKENS (1 << 20)
+
+/* What became of a request in a plan (smx_paged_plan's status). */
+#define SMX_PAGED_OK 0
+#define SMX_PAGED_BAD_LENGTH 1   /* a negative length, over max_new new tokens or past max_context */
+#define SMX_PAGED_OUT_OF_ROWS 2  /* its rows end behind the step's last */
+#define SMX_PAGED_OUT_OF_PAGES 3 /* the free list does not hold the pages it needs */
+#define SMX_PAGED_BAD_PAGE 4     /* the page its context ends in is not one of the cache */
+
+/* dtype bits of smx_paged_write: float32 scales and RoPE tables (else bf16). */
+#define SMX_PAGED_Q_SCALE_F32 1
+#define SMX_PAGED_K_SCALE_F32 2
+#define SMX_PAGED_ROPE_F32 4
+
+/* bf16 keys and values of one layer: [num_pages, page_size, kv_heads, head_dim], any strides
+ * (in elements) whose head rows are 16-byte aligned runs, the same for both. Powers of two
+ * from 8 to 4096 as page_size, head_dim 64 or 128. */
+typedef struct smx_paged_cache {
+  void *k, *v;
+  int64_t page_stride, slot_stride, head_stride;
+  int32_t num_pages, page_size, kv_heads, head_dim;
+} smx_paged_cache;
+
+/* bf16 head rows [tokens, heads, head_dim], strides in elements, rows 16-byte aligned. */
+typedef struct smx_heads {
+  void* data;
+  int64_t token_stride, head_stride;
+  int32_t heads;
+} smx_heads;
+
+/* What smx_paged_attention reads of a plan (device pointers). */
+typedef struct smx_paged_step {
+  int32_t requests, tokens, max_new;
+  const int32_t* block_tables;
+  int64_t table_stride;
+  const int32_t *starts, *rows, *context, *positions;
+} smx_paged_step;
+
+/*
+ * Plan of one serving step, built on the device from the requests' lengths (all
+ * pointers are device pointers, int32 but for slots). Request b holds
+ * context_lens[b] tokens in the cache and appends new_lens[b]; the new tokens of all
+ * requests are consecutive rows 0 .. tokens - 1 of the step, padding rows behind
+ * them. With a free list, request b takes ceil((c + n) / page_size) - ceil(c / page_size)
+ * pages from free_pages in request order, and its entries in
+ * block_tables [requests, width] are filled in; without one (NULL) the tables must
+ * hold every page already. Out:
+ *   starts [requests + 1]: first row of each request;
+ *   rows, context, status [requests]: new and context tokens of the requests that are
+ *     admitted (0 for others), and SMX_PAGED_* for each;
+ *   positions [tokens]: position in its request, -1 for rows of no admitted request;
+ *   slots [tokens]: page * page_size + offset, -1 where there is no such page;
+ *   pages [2]: how many of free_pages were taken, from its front; and how many the
+ *     requests up to the last admitted one need together, admitted or not (more than are free
+ *     once they ran out).
+ * A request that is not admitted changes neither table nor cache; one that needs no new page
+ * is admitted though others before it ran out of pages. Asynchronous on stream.
+ */
+int smx_paged_plan(int32_t requests, int32_t width, int32_t page_size, int32_t num_pages, int32_t tokens,
+                   int32_t max_new, int32_t max_context, const int32_t* context_lens, const int32_t* new_lens,
+                   int32_t* block_tables, int64_t table_stride, const int32_t* free_pages, int32_t free_count,
+                   int32_t* starts, int32_t* rows, int32_t* context, int32_t* positions, int64_t* slots,
+                   int32_t* status, int32_t* pages, void* stream);
+
+/*
+ * Stores a step's key and value heads in the cache, at the plan's slots (rows of
+ * slot -1 are left out). Optionally the keys, and the query heads q -> q_out
+ * (dense [tokens, heads, head_dim], rows of position -1 zero), are RMS-normalised over
+ * head_dim (q_scale, k_scale [head_dim]) and rotated by their positions (rope_cos,
+ * rope_sin: row `position`, head_dim / 2 values), in FP32 with one rounding.
+ * q and q_out, scales and tables may be NULL. Asynchronous on stream.
+ */
+int smx_paged_write(const smx_paged_cache* cache, int32_t tokens, const int32_t* positions, const int64_t* slots,
+                    const smx_heads* q, const smx_heads* k, const smx_heads* v, const void* rope_cos,
+                    const void* rope_sin, int32_t rope_rows, int64_t rope_stride, const void* q_scale,
+                    const void* k_scale, int32_t dtypes, float eps, void* q_out, void* stream);
+
+/*
+ * Attention of a step's query heads over the cache, which holds the step's own keys and
+ * values already: the row at position p of its request sees that request's keys j <= p, and with
+ * window > 0 only those with j > p - window. Query head h reads key/value head
+ * h / (heads / kv_heads). softmax(scale q k) in FP32, its weights rounded to bf16 for the
+ * product with the values, one bf16 rounding of the result. Keys of pages that are
+ * not in the cache (0 .. num_pages - 1) are not seen, and a row that sees none is zero. Rows of no
+ * request stay as they are, or become zero with zero_rows. The workspace
+ * (smx_paged_attention_workspace_bytes, for the current device) is overwritten.
+ * Asynchronous on stream.
+ */
+int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step, const smx_heads* q,
+                        const smx_heads* out, float scale, int32_t window, int32_t zero_rows, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+int smx_paged_attention_workspace_bytes(int32_t head_dim, int64_t* bytes);
+
+/*
+ * A [k, n] weight of 4-bit codes with a scale and a zero point per group of k and column:
+ * W = (code - zero) scale. Laid out once: columns in tiles of 16 (for swiglu the
+ * tiles of the gate half and of the up half in turn; an even number of tiles, padded
+ * with scale 0), k in tiles of 128 (padded likewise).
+ *   codes: per column tile and k tile 64 lanes of four words; word s of lane l holds
+ *     column l % 16, k = 32 s + 8 (l / 16) + j, j = 0 .. 7, at bit 16 (j % 2) + 4 (j / 2);
+ *   scales: per column tile, group (of 32, 64 or 128) and column one word: the bf16
+ *     scale in the upper half, bf16(-(16 + zero)) in the lower.
+ */
+typedef struct smx_int4_weight {
+  const void *codes, *scales;
+  int64_t k, n;
+  int32_t group, swiglu;
+} smx_int4_weight;
+
+/*
+ * out [m, n] = epilogue(x [m, k] W), bf16 in and out, FP32 sums, one rounding. Epilogues:
+ * SMX_EPI_NONE; SMX_EPI_SWIGLU (out [m, n / 2] = silu(gate) up, a weight laid out for
+ * it); SMX_EPI_RESIDUAL_ADD and SMX_EPI_BIAS_ADD (extra [m, n] or [n], bf16, or float32 with
+ * extra_f32). k % 32 == 0. Meant for few rows: every 64 rows read the weight again.
+ * An infinity in x makes its row NaN. Asynchronous on stream.
+ */
+int smx_int4_matmul(const smx_int4_weight* w, int64_t m, const void* x, int64_t ldx, int32_t epilogue,
+                    const void* extra, int64_t lde, int32_t extra_f32, void* out, int64_t ldo, void* stream);
 
 /* Message of the last failing call on this thread ("" if none). */
 const char* smx_last_error(void);

@@ -22,5 +22,10 @@ from .packing import (  # noqa: F401
 )
 from .strassen import PlainWeightPackWarning  # noqa: F401
 from .tuning import tuned_matmul  # noqa: F401
+from .paged import (  # noqa: F401
+    PAGED_BAD_LENGTH, PAGED_BAD_PAGE, PAGED_OK, PAGED_OUT_OF_PAGES, PAGED_OUT_OF_ROWS, PagedPlan, paged_attention,
+    paged_plan, paged_write,
+)
+from .int4 import Int4Operand, int4_matmul, int4_quantize, int4_weight_layout  # noqa: F401
 
 __version__ = "0.5.0"

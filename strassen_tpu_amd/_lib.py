@@ -59,9 +59,16 @@ SMX_NRA_OUT_F32 = 4
 SMX_QK_SCALE_F32 = 1
 SMX_QK_OUT_F32 = 4
 
+SMX_PAGED_MAX_REQUESTS = 8192
+SMX_PAGED_MAX_TOKENS = 1 << 20
+SMX_PAGED_Q_SCALE_F32 = 1
+SMX_PAGED_K_SCALE_F32 = 2
+SMX_PAGED_ROPE_F32 = 4
+
 EXPORTS = ("smx_gemm", "smx_gemm_noalloc", "smx_gemm_workspace_bytes", "smx_matmul", "smx_matmul_workspace_bytes", "smx_matmul_plan",
            "smx_tile_requirements", "smx_packed_bytes", "smx_pack_operand", "smx_pack_rhs_transposed", "smx_norm_residual_add", "smx_rms_norm",
-           "smx_row_squares", "smx_scale_rows", "smx_qk_norm_rope", "smx_last_error", "smx_version")
+           "smx_row_squares", "smx_scale_rows", "smx_qk_norm_rope", "smx_paged_plan", "smx_paged_write",
+           "smx_paged_attention", "smx_paged_attention_workspace_bytes", "smx_int4_matmul", "smx_last_error", "smx_version")
 
 
 class SmxGemmDesc(ctypes.Structure):
@@ -86,6 +93,28 @@ class SmxMatmulLaunch(ctypes.Structure):
 
     _fields_ = [(name, ctypes.c_int32) for name in ("streaming", "tile_rows", "tile_cols", "head_columns",
                                                     "whole_tiles", "split_tiles", "shares", "readers")]
+
+
+class SmxPagedCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("slot_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("num_pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class SmxHeads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("heads", ctypes.c_int32)]
+
+
+class SmxPagedStep(ctypes.Structure):
+    _fields_ = [("requests", ctypes.c_int32), ("tokens", ctypes.c_int32), ("max_new", ctypes.c_int32),
+                ("block_tables", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("starts", ctypes.c_void_p),
+                ("rows", ctypes.c_void_p), ("context", ctypes.c_void_p), ("positions", ctypes.c_void_p)]
+
+
+class SmxInt4Weight(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("k", ctypes.c_int64), ("n", ctypes.c_int64),
+                ("group", ctypes.c_int32), ("swiglu", ctypes.c_int32)]
 
 
 _lib = None
@@ -137,6 +166,17 @@ def load():
     lib.smx_scale_rows.restype = ctypes.c_int
     lib.smx_qk_norm_rope.argtypes = [i64, i64, vp, i64, vp, vp, vp, i32, i32, i32, f32, vp, i64, vp]
     lib.smx_qk_norm_rope.restype = ctypes.c_int
+    lib.smx_paged_plan.argtypes = [i32] * 7 + [vp, vp, vp, i64, vp, i32] + [vp] * 8
+    lib.smx_paged_plan.restype = ctypes.c_int
+    cache, heads, step = (ctypes.POINTER(t) for t in (SmxPagedCache, SmxHeads, SmxPagedStep))
+    lib.smx_paged_write.argtypes = [cache, i32, vp, vp, heads, heads, heads, vp, vp, i32, i64, vp, vp, i32, f32, vp, vp]
+    lib.smx_paged_write.restype = ctypes.c_int
+    lib.smx_paged_attention.argtypes = [cache, step, heads, heads, f32, i32, i32, vp, i64, vp]
+    lib.smx_paged_attention.restype = ctypes.c_int
+    lib.smx_paged_attention_workspace_bytes.argtypes = [i32, ctypes.POINTER(i64)]
+    lib.smx_paged_attention_workspace_bytes.restype = ctypes.c_int
+    lib.smx_int4_matmul.argtypes = [ctypes.POINTER(SmxInt4Weight), i64, vp, i64, i32, vp, i64, i32, vp, i64, vp]
+    lib.smx_int4_matmul.restype = ctypes.c_int
     lib.smx_last_error.argtypes = []
     lib.smx_last_error.restype = ctypes.c_char_p
     lib.smx_version.argtypes = []

@@ -1,8 +1,9 @@
 """Build the gfx950 C-ABI library in-tree.
 
 ``python -m strassen_tpu_amd.build`` (or ``build()``) compiles the C ABI's
-translation unit (``csrc/strassen_gemm.hip``) and the six units that
-instantiate the GEMM kernels (``csrc/gemm_*.hip``) with hipcc, in parallel,
+translation unit (``csrc/strassen_gemm.hip``), the six units that
+instantiate the GEMM kernels (``csrc/gemm_*.hip``) and the three of the serving
+operators (``csrc/paged_*.hip``, ``csrc/int4_matmul.hip``) with hipcc, in parallel,
 checks each unit's device assembly, and links ``libstrassen_mi355x.so`` next
 to this file. hipcc cross-compiles for gfx950 without a GPU.
 """
@@ -21,7 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
 SOURCES = tuple(os.path.join(HERE, "csrc", name) for name in (
     "strassen_gemm.hip", "gemm_strassen.hip", "gemm_strassen_thin.hip", "gemm_strassen_pm.hip", "gemm_cubic.hip",
-    "gemm_cubic_thin.hip", "gemm_stream.hip"))
+    "gemm_cubic_thin.hip", "gemm_stream.hip", "paged_cache.hip", "paged_attention.hip", "int4_matmul.hip"))
 LIBRARY = os.path.join(HERE, "libstrassen_mi355x.so")
 INCLUDE = os.path.join(REPO, "include")
 
@@ -126,13 +127,14 @@ _SPLIT = re.compile(r"gemm_splitILi(\d+)ELi(\d+)ELb(\d)E")
 _PM = re.compile(r"gemm_pmILi(\d+)ELi(\d+)EE")
 _STREAM = re.compile(r"gemm_streamILi(\d+)E")
 _PACKED = re.compile(r"gemm_packedILi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)ELb(\d)E")
+_SERVING = re.compile(r"(paged_attend|paged_join|int4_matmul)")
 _QUAD_CUBIC_PARTIAL = 1
 PARTIAL_SCRATCH_CAP = 1024
 
 
 def scratch_limit(name):
     """Allowed scratch bytes per lane of a kernel (None: not a GEMM kernel)."""
-    if _SPLIT.search(name) or _PM.search(name) or _STREAM.search(name):
+    if _SPLIT.search(name) or _PM.search(name) or _STREAM.search(name) or _SERVING.search(name):
         return 0
     m = _PACKED.search(name)
     if m:
@@ -192,10 +194,11 @@ def build(verbose=False, jobs=None):
             # The C ABI's unit holds the compact kernels and the packers; the
             # GEMM scratch limits live in the kernel units, each of which must
             # hold some, and inline-asm MFMAs in all of those but the streaming
-            # kernels', whose MFMAs are the compiler's builtins.
+            # kernels', whose MFMAs are the compiler's builtins (as are the serving
+            # operators', whose registers are held to the same limit).
             unit = os.path.basename(source)
-            kernel_unit = unit != "strassen_gemm.hip"
-            if kernel_unit and unit != "gemm_stream.hip":
+            kernel_unit = unit not in ("strassen_gemm.hip", "paged_cache.hip")
+            if kernel_unit and unit not in ("gemm_stream.hip", "paged_attention.hip", "int4_matmul.hip"):
                 checked += verify_inline_asm_kernels(text)
             gemms += verify_kernel_scratch(text, require=kernel_unit)
         cmd = link_command([obj for obj, _, _ in units], tmp)

@@ -12,6 +12,12 @@ namespace smx {
 // Records the message of a failing call (smx_last_error) and returns code.
 int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 
+// Compute units of the current device.
+int device_cus(int* cus);
+
+// Checks the description of a paged cache (paged_cache.hip).
+int paged_layout(const smx_paged_cache* c);
+
 inline int check_launch() {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(SMX_ERR_LAUNCH, "kernel launch: %s", hipGetErrorString(e));

@@ -1,0 +1,626 @@
+// Attention of new tokens over a paged key/value cache (smx_paged_attention):
+// requests of ragged lengths, grouped query heads, causal, optionally within a
+// sliding window.
+//
+// Mathematics. For a request with c tokens before the step and n new ones, new
+// token i stands at position p = c + i and sees the keys j with p - window < j <= p.
+// out_i = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m), s_j = scale q_i . k_j,
+// m = max_j s_j, in one pass over the keys with a running maximum and sum (FP32). The
+// exponentials are powers of two (scale carries log2 e) and are rounded to bf16 for the
+// product with the values; their sum is taken before that rounding.
+//
+// Rows. The g query heads of a key/value head share its keys: a tile holds
+// whole tokens, row r of it being token r / g, head r % g.
+//
+// Matrix products (v_mfma_f32_32x32x16_bf16, both transposed): S^T = K Q^T gives
+// lane l the scores of row l % 32, so that maxima and sums need one exchange
+// between lanes l and l ^ 32; O^T = V^T P^T takes P^T as the scores' own registers:
+// the sum over keys may run in any order, and the order in which the lanes hold the
+// scores (register i of half h: key 8 (i / 4) + 4 h + i % 4) is the one in which the
+// transposing LDS reads hand out V^T.
+//
+// Work. The key tiles of all (key/value head, request, row tile) items, one behind
+// the other, are cut into equal spans, one per workgroup: decode steps and long
+// prompts, alone or mixed, fill the chip alike. An item cut by a span's end leaves
+// partial sums in the workspace that paged_join adds up. Counts of tiles have closed
+// forms, so every workgroup finds its span by itself, from the lengths on the device.
+#include "kernel_packed.hpp"
+#include "launch.hpp"
+
+namespace smx {
+
+namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+struct AttentionArgs {
+  const uint16_t* q;
+  uint16_t* out;
+  int64_t q_token, q_head, out_token, out_head;
+  const uint16_t *k, *v;
+  int64_t page_stride, slot_stride, head_stride;
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t *starts, *rows, *context, *positions;
+  int32_t requests, tokens, group, kv_heads, page_shift, num_pages, window, tile_tokens, zero_rows, min_span;
+  float scale;  // times log2 e
+  float* partial;
+  int32_t* records;
+};
+
+// What paged_join needs to know of an item that workgroup w begins and others
+// finish: its place and the number of those others (0: no such item).
+struct Record {
+  int32_t others, worker, head, request, tile, unused[3];
+};
+
+// sum_{i < n} floor((a i + b) / m), for 0 <= a, b and n a + b < 2^32 once a, b < m.
+__device__ int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+  int64_t sum = 0;
+  while (n) {
+    if (a >= m) sum += (int64_t)n * (n - 1) / 2 * (a / m), a %= m;
+    if (b >= m) sum += (int64_t)n * (b / m), b %= m;
+    const uint32_t top = a * n + b;
+    if (top < m) break;
+    n = top / m, b = top % m;
+    const uint32_t old = m;
+    m = a, a = old;
+  }
+  return sum;
+}
+
+// The row tiles of one request and the key tiles (of kKeys keys) that each sees.
+template <int kKeys>
+struct Request {
+  int32_t context, fresh, per_tile, window, tiles;
+
+  __device__ Request(const AttentionArgs& p, int b)
+      : context(p.context[b]), fresh(p.rows[b]), per_tile(p.tile_tokens), window(p.window) {
+    tiles = (fresh + per_tile - 1) / per_tile;
+  }
+  __device__ int first(int t) const {
+    return window ? max(0, context + t * per_tile - window + 1) / kKeys : 0;
+  }
+  __device__ int last(int t) const { return (context + min(fresh, (t + 1) * per_tile) + kKeys - 1) / kKeys; }
+  __device__ int count(int t) const { return last(t) - first(t); }
+  // Key tiles of the row tiles before t < tiles.
+  __device__ int64_t before(int t) const {
+    if (!t) return 0;
+    int64_t sum = floor_sum(t, kKeys, per_tile, context + per_tile + kKeys - 1);
+    if (window) {
+      const int x = context - window + 1;  // first(s) = max(0, x + s per_tile) / kKeys
+      const int skip = x >= 0 ? 0 : (-x + per_tile - 1) / per_tile;
+      if (skip < t) sum -= floor_sum(t - skip, kKeys, per_tile, x + skip * per_tile);
+    }
+    return sum;
+  }
+  __device__ int64_t all() const { return fresh > 0 ? before(tiles - 1) + count(tiles - 1) : 0; }
+};
+
+// A workgroup's span of the key tiles, and the item in which it begins.
+struct Span {
+  int64_t left;         // key tiles to do
+  int64_t each;         // key tiles of a span
+  int64_t begin;        // of this one, over all key/value heads
+  int32_t worker;       // which span this is
+  int32_t head, request, tile, skip;  // skip: key tiles of that item done by others
+};
+
+__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+  return x;
+}
+
+// Finds the workgroup's span (256 threads, uniform result). Consecutive spans lie
+// on one XCD, whose L2 then serves one key/value head's pages at a time.
+template <int kKeys>
+__device__ bool find_span(const AttentionArgs& p, Span* s) {
+  __shared__ int64_t waves[4], found_rest;
+  __shared__ int32_t found;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t total = 0;
+  for (int b = threadIdx.x; b < p.requests; b += 256) total += Request<kKeys>(p, b).all();
+  total = wave_sum(total);
+  if (lane == 0) waves[wave] = total;
+  __syncthreads();
+  total = waves[0] + waves[1] + waves[2] + waves[3];
+  const int64_t everything = total * p.kv_heads;
+  s->each = max((int64_t)p.min_span, (everything + gridDim.x - 1) / gridDim.x);
+  const int64_t spans = (everything + s->each - 1) / s->each, per_xcd = (spans + 7) / 8;
+  s->worker = (int)((blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3));
+  if ((blockIdx.x >> 3) >= per_xcd || s->worker >= spans) return false;
+  s->begin = (int64_t)s->worker * s->each;
+  s->left = min(s->each, everything - s->begin);
+  s->head = (int)(s->begin / total);
+  const int64_t at = s->begin - (int64_t)s->head * total;
+
+  int64_t base = 0;
+  for (int first = 0; first < p.requests; first += 256) {
+    const int b = first + (int)threadIdx.x;
+    const int64_t mine = b < p.requests ? Request<kKeys>(p, b).all() : 0;
+    int64_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t y = __shfl_up(upto, d);
+      if (lane >= d) upto += y;
+    }
+    __syncthreads();
+    if (lane == 63) waves[wave] = upto;
+    __syncthreads();
+    int64_t all = 0;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) upto += waves[w];
+      all += waves[w];
+    }
+    upto += base;
+    if (at >= upto - mine && at < upto) found = b, found_rest = at - (upto - mine);
+    base += all;
+    if (at < base) break;  // uniform
+  }
+  __syncthreads();
+  s->request = __builtin_amdgcn_readfirstlane(found);
+  int64_t rest = found_rest;
+  const Request<kKeys> r(p, s->request);
+  int low = 0, high = r.tiles;  // the last tile with before(tile) <= rest
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (r.before(mid) <= rest) low = mid; else high = mid;
+  }
+  s->tile = __builtin_amdgcn_readfirstlane(low);
+  s->skip = __builtin_amdgcn_readfirstlane((int)(rest - r.before(low)));
+  return true;
+}
+
+// One page's rows as a buffer for the DMA into LDS: a page that is not in the
+// cache, and rows behind `rows`, read as zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const uint16_t* base, const AttentionArgs& p, int page,
+                                                            int slot, int head, int rows) {
+  const bool held = (uint32_t)page < (uint32_t)p.num_pages;
+  const int64_t at = (held ? (int64_t)page * p.page_stride : 0) + (int64_t)slot * p.slot_stride + head * p.head_stride;
+  return packed::panel_rsrc(reinterpret_cast<const uint8_t*>(base + at),
+                            held && rows > 0 ? (uint32_t)rows * (uint32_t)p.slot_stride * 2 : 0);
+}
+
+// LDS tiles of keys and values: rows of D bf16. Keys are stored with their 16-byte
+// chunks, values with their 32-byte pairs of chunks, XORed with bits of the row, so
+// that neither reads (a wave's 32 rows of one chunk; the transposing reads' 4 rows of one pair)
+// fall on the same banks. The DMA stores lane l's 16 bytes at 16 l, so the
+// lane fetches the chunk that belongs there.
+template <int D>
+struct Tile {
+  static constexpr int kRow = 2 * D, kChunks = D / 8, kDmaRows = 64 / kChunks;  // rows per DMA
+  __device__ static int key_chunk(int chunk, int row) { return chunk ^ (row & (kChunks - 1)); }
+  __device__ static int value_chunk(int chunk, int row) {
+    return chunk ^ (2 * ((D == 128 ? row : row >> 1) & (kChunks / 2 - 1)));
+  }
+};
+
+// V^T fragments of 16 keys: for each block of 32 columns, lane l's 8 values of column
+// l % 32 by two transposing LDS reads (4 keys each; lane group l / 16 reads 4
+// rows of 16 columns). `at`: LDS address of the block's first read. Written as one asm
+// block with its wait: before the builtin of this read the compiler waits for every
+// DMA in flight, the next step's too.
+template <int D, int kOffset>
+__device__ __forceinline__ void read_values(bf16x8 (&v)[D / 32], const uint32_t (&at)[D / 32]) {
+  u32x2 a[D / 32], b[D / 32];
+  if constexpr (D == 128) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]), "=&v"(b[2]), "=&v"(a[3]), "=&v"(b[3])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(kOffset), "n"(kOffset + 8 * 2 * D));
+  } else {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1])
+        : "v"(at[0]), "v"(at[1]), "n"(kOffset), "n"(kOffset + 8 * 2 * D));
+  }
+#pragma unroll
+  for (int x = 0; x < D / 32; ++x) v[x] = __builtin_bit_cast(bf16x8, u32x4{a[x][0], a[x][1], b[x][0], b[x][1]});
+}
+
+__device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
+}
+
+// Running softmax and output of a wave's 32 rows: lane l holds row l % 32; register e
+// of block x is column 32 x + 8 (e / 4) + 4 (l / 32) + e % 4 of the output.
+template <int D>
+struct Rows {
+  f32x16 o[D / 32];
+  float top, sum;  // the reference maximum (scores times scale); this lane's share of the sum
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[x][e] = 0.f;
+    top = -INFINITY, sum = 0.f;
+  }
+};
+
+__device__ __forceinline__ float other_half(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return (threadIdx.x & 32) ? __uint_as_float(r[0]) : __uint_as_float(r[1]);
+}
+
+// One step: the wave's 32 rows against 32 kBlocks keys in LDS. `seen` is called for
+// score registers only if kMask. The maximum that the exponentials are taken against
+// moves only once it is exceeded by 2^8, so that most steps rescale nothing; sums
+// stay below 2^8 times their number of keys.
+template <int D, int kBlocks>
+__device__ __forceinline__ void attend(Rows<D>& r, const bf16x8 (&q)[D / 16], const uint8_t* keys, const uint8_t* values,
+                                       float scale, bool masked, int rel, int window, uint64_t held) {
+  using T = Tile<D>;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  f32x16 s[kBlocks];
+#pragma unroll
+  for (int x = 0; x < kBlocks; ++x)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[x][e] = 0.f;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+    for (int x = 0; x < kBlocks; ++x) {
+      const bf16x8 k = packed::ld_frag(keys + (32 * x + (lane & 31)) * T::kRow + 16 * T::key_chunk(2 * t + half, lane & 31));
+      s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[t], s[x], 0, 0, 0);
+    }
+  if (masked) {
+    // key - first key of the step = 32 x + 8 (e / 4) + 4 half + e % 4; `rel` is the
+    // row's position less the step's first key
+    const int mine = rel - 4 * half;
+    const uint64_t bits = held >> (4 * half);
+#pragma unroll
+    for (int x = 0; x < kBlocks; ++x)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int key = 32 * x + 8 * (e >> 2) + (e & 3);
+        const bool ok = key <= mine && (!window || key > mine - window) && ((bits >> key) & 1);
+        s[x][e] = ok ? s[x][e] : -INFINITY;
+      }
+  }
+  float top = s[0][0];
+#pragma unroll
+  for (int x = 0; x < kBlocks; ++x)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, s[x][e]);
+  top = fmaxf(top, other_half(top)) * scale;
+  if (__any(top > r.top + 8.f)) {
+    const float next = fmaxf(r.top, top);
+    const float factor = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(r.top - next);
+    r.top = next;
+    r.sum *= factor;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) r.o[x][e] *= factor;
+  }
+  const float base = r.top == -INFINITY ? 0.f : r.top;
+  bf16x8 w[2 * kBlocks];
+#pragma unroll
+  for (int x = 0; x < kBlocks; ++x) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      s[x][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], scale, -base));
+      r.sum += s[x][e];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x4 b;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = pack_bf16(s[x][8 * h + 2 * i], s[x][8 * h + 2 * i + 1]);
+      w[2 * x + h] = __builtin_bit_cast(bf16x8, b);
+    }
+  }
+  // Lane group lane / 16 reads rows 4 half .. + 3 of 16 columns: lane's row and piece there.
+  const int row = 4 * half + ((lane & 15) >> 2), piece = lane & 3, side = (lane >> 4) & 1;
+  uint32_t at[D / 32];
+#pragma unroll
+  for (int x = 0; x < D / 32; ++x)
+    at[x] = lds_address(values) + row * T::kRow + 16 * T::value_chunk(2 * (2 * x + side), row) + 8 * piece;
+  auto product = [&](auto step) __attribute__((always_inline)) {
+    constexpr int t = decltype(step)::value;
+    bf16x8 v[D / 32];
+    read_values<D, 16 * t * T::kRow>(v, at);
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) r.o[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[x], w[t], r.o[x], 0, 0, 0);
+  };
+  product(std::integral_constant<int, 0>{});
+  product(std::integral_constant<int, 1>{});
+  if constexpr (kBlocks == 2) {
+    product(std::integral_constant<int, 2>{});
+    product(std::integral_constant<int, 3>{});
+  }
+}
+
+// A tile's output or partial sums. kWaves row groups of 32 in a tile. Partial layout per
+// worker and slot: D / 8 chunks of [256] float4, then [256] tops and [256] sums.
+template <int D>
+constexpr int kPartialFloats = 256 * (D / 2 + 2);
+
+// Rows of 32 D-wide outputs to memory: lane l of half h holds columns 8 (e / 4) + 4 h ..
+// of block x; two lanes exchange halves so that each stores 16 bytes.
+template <int D>
+__device__ __forceinline__ void store_rows(const AttentionArgs& p, const f32x16 (&o)[D / 32], float inverse, bool valid,
+                                           int64_t token, int head) {
+  const int half = (threadIdx.x & 63) >> 5;
+  uint16_t* const to = p.out + token * p.out_token + head * p.out_head;
+#pragma unroll
+  for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+    for (int e = 0; e < 16; e += 8) {
+      // columns 4 h .. of groups e / 4 (mine if half 0) and e / 4 + 1 (mine if half 1)
+      const uint32_t a0 = pack_bf16(o[x][e] * inverse, o[x][e + 1] * inverse);
+      const uint32_t a1 = pack_bf16(o[x][e + 2] * inverse, o[x][e + 3] * inverse);
+      const uint32_t b0 = pack_bf16(o[x][e + 4] * inverse, o[x][e + 5] * inverse);
+      const uint32_t b1 = pack_bf16(o[x][e + 6] * inverse, o[x][e + 7] * inverse);
+      // swap: a's upper half with b's lower half
+      const auto r0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+      const auto r1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+      const u32x4 v = {r0[0], r1[0], r0[1], r1[1]};
+      if (valid) *reinterpret_cast<u32x4*>(to + 32 * x + 8 * ((e >> 2) + half)) = v;
+    }
+}
+
+__device__ __forceinline__ float inverse_of(float sum) { return sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum; }
+
+// 128 rows a tile (four waves of 32), 64 keys a step, keys and values double buffered.
+template <int D>
+__global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
+  using T = Tile<D>;
+  constexpr int kKeys = 64, kDmas = 16 / T::kDmaRows;  // DMAs of a wave's 16 keys
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  constexpr int kTileBytes = kKeys * T::kRow;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+
+  // Rows that belong to no request are zeroed on the way.
+  if (p.zero_rows) {
+    const int chunks = p.group * p.kv_heads * (D / 8);
+    for (int64_t row = blockIdx.x; row < p.tokens; row += gridDim.x)
+      if (p.positions[row] < 0)
+        for (int c = threadIdx.x; c < chunks; c += 256)
+          *reinterpret_cast<u32x4*>(p.out + row * p.out_token + c / (D / 8) * p.out_head + c % (D / 8) * 8) = u32x4{0, 0, 0, 0};
+  }
+  Record* const record = reinterpret_cast<Record*>(p.records) + blockIdx.x;
+  if (threadIdx.x == 0) record->others = 0;
+  Span s;
+  if (!find_span<kKeys>(p, &s)) return;
+
+  // the DMA's lane offsets within a page: row and chunk
+  uint32_t key_at[kDmas], value_at[kDmas];
+#pragma unroll
+  for (int i = 0; i < kDmas; ++i) {
+    const int in = lane / T::kChunks, row = i * T::kDmaRows + in, chunk = lane % T::kChunks;
+    key_at[i] = (uint32_t)in * (uint32_t)p.slot_stride * 2 + 16 * T::key_chunk(chunk, row);
+    value_at[i] = (uint32_t)in * (uint32_t)p.slot_stride * 2 + 16 * T::value_chunk(chunk, row);
+  }
+
+  while (s.left > 0) {
+    const Request<kKeys> r(p, s.request);
+    const int tile_first = r.first(s.tile), tile_count = r.count(s.tile);
+    const int count = (int)min((int64_t)(tile_count - s.skip), s.left);
+    const int from = tile_first + s.skip;
+    const int tile_tokens = min(r.per_tile, r.fresh - s.tile * r.per_tile), tile_rows = tile_tokens * p.group;
+    const int row = min(32 * wave + (lane & 31), tile_rows - 1);
+    const int local = s.tile * r.per_tile + row / p.group, head = s.head * p.group + row % p.group;
+    const int64_t token = p.starts[s.request] + local;
+    const int position = r.context + local;
+    const int length = r.context + r.fresh;
+    // positions of the wave's first and last row
+    const int low = __builtin_amdgcn_readfirstlane(position);
+    const int high = __builtin_amdgcn_readlane(position, 31);
+    const bool active = 32 * wave < tile_rows;  // rows of its own
+    const int32_t* const table = p.tables + s.request * p.table_stride;
+
+    bf16x8 q[D / 16];
+    const uint16_t* const q_row = p.q + token * p.q_token + head * p.q_head + 8 * half;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) q[t] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q_row + 16 * t));
+
+    Rows<D> o;
+    o.clear();
+    // lane l's page of a step: that of its key 64 step + l
+    auto pages_of = [&](int step) __attribute__((always_inline)) {
+      return table[min(step * kKeys + lane, length - 1) >> p.page_shift];
+    };
+    auto fetch = [&](int step, int pages, int buffer) __attribute__((always_inline)) {
+      const int key0 = step * kKeys + 16 * wave;
+      uint8_t* const to = lds + buffer * 2 * kTileBytes + 16 * wave * T::kRow;
+#pragma unroll
+      for (int i = 0; i < kDmas; ++i) {
+        const int key = key0 + i * T::kDmaRows;
+        const int page = __builtin_amdgcn_readlane(pages, 16 * wave + i * T::kDmaRows);
+        const int slot = key & ((1 << p.page_shift) - 1), rows = min(length - key, T::kDmaRows);
+        packed::dma_frag(page_rsrc(p.k, p, page, slot, s.head, rows), key_at[i], 0, to + i * T::kDmaRows * T::kRow);
+        packed::dma_frag(page_rsrc(p.v, p, page, slot, s.head, rows), value_at[i], 0,
+                         to + kTileBytes + i * T::kDmaRows * T::kRow);
+      }
+    };
+    int pages = pages_of(from);
+    uint64_t held = __ballot((uint32_t)pages < (uint32_t)p.num_pages);
+    packed::stage_barrier<0>();  // the item before is done with the buffers
+    fetch(from, pages, 0);
+    int next_pages = pages_of(from + 1);
+    for (int i = 0; i < count; ++i) {
+      const int step = from + i;
+      packed::stage_barrier<0>();
+      const uint64_t now = held;
+      if (i + 1 < count) {
+        held = __ballot((uint32_t)next_pages < (uint32_t)p.num_pages);
+        fetch(step + 1, next_pages, (i + 1) & 1);
+        next_pages = pages_of(step + 2);
+      }
+      const int key0 = step * kKeys;
+      if (active && key0 <= high && (!p.window || key0 + kKeys - 1 > low - p.window)) {
+        const bool masked = key0 + kKeys - 1 > low || (p.window && key0 <= high - p.window) || now != ~0ull;
+        const uint8_t* const at = lds + (i & 1) * 2 * kTileBytes;
+        attend<D, 2>(o, q, at, at + kTileBytes, p.scale, masked, position - key0, p.window, now);
+      }
+    }
+
+    const bool whole = count == tile_count;
+    const float sum = o.sum + other_half(o.sum);
+    if (whole) {
+      store_rows<D>(p, o.o, inverse_of(sum), 32 * wave + (lane & 31) < tile_rows, token, head);
+    } else {
+      float* const to = p.partial + (2 * (int64_t)s.worker + (s.skip == 0)) * kPartialFloats<D>;
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          reinterpret_cast<f32x4*>(to)[(4 * x + e) * 256 + threadIdx.x] =
+              f32x4{o.o[x][4 * e], o.o[x][4 * e + 1], o.o[x][4 * e + 2], o.o[x][4 * e + 3]};
+      to[256 * (D / 2) + threadIdx.x] = o.top;
+      to[256 * (D / 2 + 1) + threadIdx.x] = sum;
+      if (s.skip == 0 && threadIdx.x == 0) {
+        record->worker = s.worker, record->head = s.head, record->request = s.request, record->tile = s.tile;
+        // the item goes on for tile_count - count key tiles in the spans behind this one
+        record->others = (int)((tile_count - count + s.each - 1) / s.each);
+      }
+    }
+    s.left -= count;
+    if (s.left <= 0) break;
+    s.skip = 0;
+    if (++s.tile < r.tiles) continue;
+    s.tile = 0;
+    do {
+      if (++s.request == p.requests) s.request = 0, ++s.head;
+    } while (p.rows[s.request] <= 0);
+  }
+}
+
+// Adds up the partial sums of the items that spans cut: one workgroup per
+// record, its threads in the layout that paged_attend wrote them in.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join(AttentionArgs p) {
+  const Record record = reinterpret_cast<const Record*>(p.records)[blockIdx.x];
+  if (record.others <= 0) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto slot = [&](int i) { return p.partial + (2 * (int64_t)(record.worker + i) + (i == 0)) * kPartialFloats<D>; };
+  float top = -INFINITY;
+  for (int i = 0; i <= record.others; ++i) top = fmaxf(top, slot(i)[256 * (D / 2) + threadIdx.x]);
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[x][e] = 0.f;
+  float sum = 0.f;
+  for (int i = 0; i <= record.others; ++i) {
+    const float* const from = slot(i);
+    const float mine = from[256 * (D / 2) + threadIdx.x];
+    const float factor = mine == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - top);
+    sum += from[256 * (D / 2 + 1) + threadIdx.x] * factor;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 v = reinterpret_cast<const f32x4*>(from)[(4 * x + e) * 256 + threadIdx.x];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[x][4 * e + j] += v[j] * factor;
+      }
+  }
+  const int fresh = p.rows[record.request];
+  const int tile_rows = min(p.tile_tokens, fresh - record.tile * p.tile_tokens) * p.group;
+  const int at = 32 * wave + (lane & 31), row = min(at, tile_rows - 1);
+  const int64_t token = p.starts[record.request] + record.tile * p.tile_tokens + row / p.group;
+  store_rows<D>(p, o, inverse_of(sum), at < tile_rows, token, record.head * p.group + row % p.group);
+}
+
+// Workgroups of a launch: two per CU (LDS holds two), a multiple of the 8 XCDs.
+int workgroups(int cus) { return (2 * cus + 7) / 8 * 8; }
+
+constexpr int64_t kRecordBytes = sizeof(Record);
+
+int64_t workspace_of(int cus, int head_dim) {
+  const int64_t floats = 256 * (head_dim / 2 + 2);
+  return workgroups(cus) * (kRecordBytes + 2 * floats * 4);
+}
+
+template <int D>
+int launch_attention(AttentionArgs& p, int cus, hipStream_t stream) {
+  const int lds = 4 * 64 * 2 * D;
+  hipError_t e = hipFuncSetAttribute((const void*)paged_attend<D>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (e != hipSuccess) return fail(SMX_ERR_LAUNCH, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+  const unsigned blocks = (unsigned)workgroups(cus);
+  p.tile_tokens = 128 / p.group;
+  hipLaunchKernelGGL(paged_attend<D>, dim3(blocks), dim3(256), lds, stream, p);
+  if (int rc = check_launch()) return rc;
+  hipLaunchKernelGGL(paged_join<D>, dim3(blocks), dim3(256), 0, stream, p);
+  return check_launch();
+}
+
+}  // namespace
+}  // namespace smx
+
+using namespace smx;
+
+extern "C" {
+
+int smx_paged_attention_workspace_bytes(int32_t head_dim, int64_t* bytes) {
+  smx::fail(SMX_OK, "%s", "");
+  if (!bytes) return fail(SMX_ERR_INVALID, "null pointer");
+  if (head_dim != 64 && head_dim != 128) return fail(SMX_ERR_UNSUPPORTED, "head_dim must be 64 or 128, got %d", head_dim);
+  int cus = 0;
+  if (int rc = device_cus(&cus)) return rc;
+  *bytes = workspace_of(cus, head_dim);
+  return SMX_OK;
+}
+
+int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step, const smx_heads* q,
+                        const smx_heads* out, float scale, int32_t window, int32_t zero_rows, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  smx::fail(SMX_OK, "%s", "");
+  if (int rc = paged_layout(cache)) return rc;
+  if (!step || !step->block_tables || !step->starts || !step->rows || !step->context || !step->positions || !q ||
+      !q->data || !out || !out->data)
+    return fail(SMX_ERR_INVALID, "null pointer");
+  if (step->requests <= 0 || step->requests > SMX_PAGED_MAX_REQUESTS || step->tokens <= 0 ||
+      step->tokens > SMX_PAGED_MAX_TOKENS || step->max_new < 0 || step->table_stride <= 0)
+    return fail(SMX_ERR_INVALID, "a step has 1 to %d requests and 1 to %d tokens (requests=%d, tokens=%d)",
+                SMX_PAGED_MAX_REQUESTS, SMX_PAGED_MAX_TOKENS, step->requests, step->tokens);
+  if (q->heads <= 0 || q->heads % cache->kv_heads || q->heads / cache->kv_heads > 128)
+    return fail(SMX_ERR_INVALID, "%d query heads are not 1 to 128 for each of %d key/value heads", q->heads,
+                cache->kv_heads);
+  if (out->heads != q->heads) return fail(SMX_ERR_INVALID, "out must have the %d query heads", q->heads);
+  for (const smx_heads* x : {q, out})
+    if ((uintptr_t)x->data % 16 || x->token_stride % 8 || x->head_stride % 8 || x->token_stride < 0 ||
+        x->head_stride < 0)
+      return fail(SMX_ERR_INVALID, "head rows must be 16-byte aligned");
+  if (!(scale > 0.f) || !(scale < INFINITY)) return fail(SMX_ERR_INVALID, "scale must be positive and finite");
+  if (window < 0) return fail(SMX_ERR_INVALID, "window must not be negative (0: none)");
+  int cus = 0;
+  if (int rc = device_cus(&cus)) return rc;
+  const int64_t need = workspace_of(cus, cache->head_dim);
+  if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)
+    return fail(SMX_ERR_INVALID, "the call needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+  AttentionArgs p{};
+  p.q = (const uint16_t*)q->data, p.q_token = q->token_stride, p.q_head = q->head_stride;
+  p.out = (uint16_t*)out->data, p.out_token = out->token_stride, p.out_head = out->head_stride;
+  p.k = (const uint16_t*)cache->k, p.v = (const uint16_t*)cache->v;
+  p.page_stride = cache->page_stride, p.slot_stride = cache->slot_stride, p.head_stride = cache->head_stride;
+  p.tables = step->block_tables, p.table_stride = step->table_stride;
+  p.starts = step->starts, p.rows = step->rows, p.context = step->context, p.positions = step->positions;
+  p.requests = step->requests, p.tokens = step->tokens;
+  p.kv_heads = cache->kv_heads, p.group = q->heads / cache->kv_heads;
+  p.page_shift = __builtin_ctz(cache->page_size), p.num_pages = cache->num_pages;
+  p.window = window, p.zero_rows = zero_rows, p.min_span = 2;
+  p.scale = scale * 1.44269504088896341f;
+  p.records = (int32_t*)workspace;
+  p.partial = (float*)((char*)workspace + workgroups(cus) * kRecordBytes);
+  return cache->head_dim == 128 ? launch_attention<128>(p, cus, (hipStream_t)stream)
+                                : launch_attention<64>(p, cus, (hipStream_t)stream);
+}
+
+}  // extern "C"

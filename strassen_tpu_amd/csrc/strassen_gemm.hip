@@ -459,6 +459,8 @@ int gemm_params(const smx_gemm_desc* d, const void* a, const void* b, void* c, c
 
 constexpr int kMaxDevices = 64;
 
+}  // namespace
+
 // Compute units of the current device, looked up once per device.
 int device_cus(int* cus) {
   static std::atomic<int> known[kMaxDevices] = {};
@@ -475,6 +477,8 @@ int device_cus(int* cus) {
   *cus = v;
   return SMX_OK;
 }
+
+namespace {
 
 // The CUs a launch is planned for: those given, or the current device's.
 int planned_cus(int* cus) { return *cus > 0 ? SMX_OK : device_cus(cus); }
