@@ -211,7 +211,7 @@ def _own_pass(s):
     case, kind = s["case"], s["case"]["kind"]
     if kind == "plan":
         plan = _plan(s)
-        return [plan.starts, plan.positions, plan.slots, plan.status, plan.pages_used, s["tables"]]
+        return [plan.starts, plan.positions, plan.slots, plan.status, plan.pages_needed, s["tables"]]
     if kind == "write":
         q = smx.paged_write(s["k"], s["v"], s["k_cache"], s["v_cache"], s["plan"], q=s["q"], rope_cos=s["cos"],
                             rope_sin=s["sin"], q_scale=s["q_scale"], k_scale=s["k_scale"], eps=EPS)
