@@ -112,19 +112,38 @@ __device__ __forceinline__ int64_t wave_sum(int64_t x) {
   return x;
 }
 
-// Finds the workgroup's span (256 threads, uniform result). Consecutive spans lie
+// Inclusive sum of x over a wave's lanes.
+__device__ __forceinline__ int64_t wave_scan(int64_t x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up(x, d);
+    if ((int)(threadIdx.x & 63) >= d) x += y;
+  }
+  return x;
+}
+
+__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, lane) |
+         (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
+}
+
+// Finds the workgroup's span (kWaves waves, uniform result). Consecutive spans lie
 // on one XCD, whose L2 then serves one key/value head's pages at a time.
-template <int kKeys>
+template <int kKeys, int kWaves>
 __device__ bool find_span(const AttentionArgs& p, Span* s) {
-  __shared__ int64_t waves[4], found_rest;
+  constexpr int kThreads = 64 * kWaves;
+  __shared__ int64_t waves[kWaves], found_rest;
   __shared__ int32_t found;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int64_t total = 0;
-  for (int b = threadIdx.x; b < p.requests; b += 256) total += Request<kKeys>(p, b).all();
-  total = wave_sum(total);
-  if (lane == 0) waves[wave] = total;
-  __syncthreads();
-  total = waves[0] + waves[1] + waves[2] + waves[3];
+  for (int b = threadIdx.x; b < p.requests; b += kThreads) total += Request<kKeys>(p, b).all();
+  total = lane_value(wave_scan(total), 63);
+  if constexpr (kWaves > 1) {
+    if (lane == 0) waves[wave] = total;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < kWaves; ++w) total += waves[w];
+  }
   const int64_t everything = total * p.kv_heads;
   s->each = max((int64_t)p.min_span, (everything + gridDim.x - 1) / gridDim.x);
   const int64_t spans = (everything + s->each - 1) / s->each, per_xcd = (spans + 7) / 8;
@@ -135,32 +154,40 @@ __device__ bool find_span(const AttentionArgs& p, Span* s) {
   s->head = (int)(s->begin / total);
   const int64_t at = s->begin - (int64_t)s->head * total;
 
-  int64_t base = 0;
-  for (int first = 0; first < p.requests; first += 256) {
+  int64_t base = 0, rest = 0;
+  for (int first = 0; first < p.requests; first += kThreads) {
     const int b = first + (int)threadIdx.x;
     const int64_t mine = b < p.requests ? Request<kKeys>(p, b).all() : 0;
-    int64_t upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t y = __shfl_up(upto, d);
-      if (lane >= d) upto += y;
-    }
-    __syncthreads();
-    if (lane == 63) waves[wave] = upto;
-    __syncthreads();
-    int64_t all = 0;
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) upto += waves[w];
-      all += waves[w];
+    int64_t upto = wave_scan(mine), all;
+    if constexpr (kWaves > 1) {
+      __syncthreads();
+      if (lane == 63) waves[wave] = upto;
+      __syncthreads();
+      all = 0;
+      for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) upto += waves[w];
+        all += waves[w];
+      }
+    } else {
+      all = lane_value(upto, 63);
     }
     upto += base;
-    if (at >= upto - mine && at < upto) found = b, found_rest = at - (upto - mine);
+    const bool here = at >= upto - mine && at < upto;
+    if constexpr (kWaves > 1) {
+      if (here) found = b, found_rest = at - (upto - mine);
+    } else if (const uint64_t who = __ballot(here)) {
+      const int l = __builtin_ctzll(who);
+      s->request = first + l;
+      rest = at - lane_value(upto - mine, l);
+    }
     base += all;
     if (at < base) break;  // uniform
   }
-  __syncthreads();
-  s->request = __builtin_amdgcn_readfirstlane(found);
-  int64_t rest = found_rest;
+  if constexpr (kWaves > 1) {
+    __syncthreads();
+    s->request = __builtin_amdgcn_readfirstlane(found);
+    rest = found_rest;
+  }
   const Request<kKeys> r(p, s->request);
   int low = 0, high = r.tiles;  // the last tile with before(tile) <= rest
   while (high - low > 1) {
@@ -172,14 +199,26 @@ __device__ bool find_span(const AttentionArgs& p, Span* s) {
   return true;
 }
 
-// One page's rows as a buffer for the DMA into LDS: a page that is not in the
-// cache, and rows behind `rows`, read as zeros.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rsrc(const uint16_t* base, const AttentionArgs& p, int page,
-                                                            int slot, int head, int rows) {
-  const bool held = (uint32_t)page < (uint32_t)p.num_pages;
-  const int64_t at = (held ? (int64_t)page * p.page_stride : 0) + (int64_t)slot * p.slot_stride + head * p.head_stride;
-  return packed::panel_rsrc(reinterpret_cast<const uint8_t*>(base + at),
-                            held && rows > 0 ? (uint32_t)rows * (uint32_t)p.slot_stride * 2 : 0);
+// On to the next item with rows.
+__device__ __forceinline__ void next_item(const AttentionArgs& p, Span* s, int tiles) {
+  s->skip = 0;
+  if (++s->tile < tiles) return;
+  s->tile = 0;
+  do {
+    if (++s->request == p.requests) s->request = 0, ++s->head;
+  } while (p.rows[s->request] <= 0);
+}
+
+// Rows that belong to no request are zeroed on the way.
+template <int D, int kThreads>
+__device__ __forceinline__ void clear_rows(const AttentionArgs& p) {
+  if (!p.zero_rows) return;
+  const int chunks = p.group * p.kv_heads * (D / 8);
+  for (int64_t row = blockIdx.x; row < p.tokens; row += gridDim.x)
+    if (p.positions[row] < 0)
+      for (int c = threadIdx.x; c < chunks; c += kThreads)
+        *reinterpret_cast<u32x4*>(p.out + row * p.out_token + c / (D / 8) * p.out_head + c % (D / 8) * 8) =
+            u32x4{0, 0, 0, 0};
 }
 
 // LDS tiles of keys and values: rows of D bf16. Keys are stored with their 16-byte
@@ -193,6 +232,51 @@ struct Tile {
   __device__ static int key_chunk(int chunk, int row) { return chunk ^ (row & (kChunks - 1)); }
   __device__ static int value_chunk(int chunk, int row) {
     return chunk ^ (2 * ((D == 128 ? row : row >> 1) & (kChunks / 2 - 1)));
+  }
+};
+
+// Lane offsets, within eight rows of a page, of the DMAs that bring kRows rows of keys
+// and of values into LDS: row and chunk.
+template <int D, int kRows>
+struct Lanes {
+  using T = Tile<D>;
+  static constexpr int kDmas = kRows / T::kDmaRows, kPer8 = 8 / T::kDmaRows;
+  uint32_t key[kDmas], value[kDmas];
+
+  __device__ explicit Lanes(int64_t slot_stride) {
+    const int in = (threadIdx.x & 63) / T::kChunks, chunk = (threadIdx.x & 63) % T::kChunks;
+#pragma unroll
+    for (int i = 0; i < kDmas; ++i) {
+      const int row = i * T::kDmaRows + in;  // the wave's first row is a multiple of 16
+      const uint32_t at = (uint32_t)(i % kPer8 * T::kDmaRows + in) * (uint32_t)slot_stride * 2;
+      key[i] = at + 16 * T::key_chunk(chunk, row);
+      value[i] = at + 16 * T::value_chunk(chunk, row);
+    }
+  }
+
+  // Starts the DMAs of rows key0 .. key0 + kRows - 1 of a head to LDS. A page holds whole
+  // groups of eight rows: each group is one buffer, whose rows behind `length`, and
+  // all of whose rows if its page is not in the cache, read as zeros. Lane
+  // lane0 + r of `pages` holds row r's page.
+  __device__ __forceinline__ void fetch(const AttentionArgs& p, int head, int key0, int length, int pages, int lane0,
+                                        uint8_t* keys, uint8_t* values) const {
+    const uint8_t* const k = reinterpret_cast<const uint8_t*>(p.k + head * p.head_stride);
+    const uint8_t* const v = reinterpret_cast<const uint8_t*>(p.v + head * p.head_stride);
+#pragma unroll
+    for (int g = 0; g < kRows / 8; ++g) {
+      const int first = key0 + 8 * g, page = __builtin_amdgcn_readlane(pages, lane0 + 8 * g);
+      const bool held = (uint32_t)page < (uint32_t)p.num_pages;
+      const int64_t at =
+          ((int64_t)(held ? page : 0) * p.page_stride + (int64_t)(first & ((1 << p.page_shift) - 1)) * p.slot_stride) * 2;
+      const int rows = held ? max(0, min(8, length - first)) : 0;
+      const uint32_t bytes = (uint32_t)rows * (uint32_t)p.slot_stride * 2;
+      const auto from_k = packed::panel_rsrc(k + at, bytes), from_v = packed::panel_rsrc(v + at, bytes);
+#pragma unroll
+      for (int i = g * kPer8; i < (g + 1) * kPer8; ++i) {
+        packed::dma_frag(from_k, key[i], 0, keys + i * T::kDmaRows * T::kRow);
+        packed::dma_frag(from_v, value[i], 0, values + i * T::kDmaRows * T::kRow);
+      }
+    }
   }
 };
 
@@ -216,7 +300,8 @@ __device__ __forceinline__ void read_values(bf16x8 (&v)[D / 32], const uint32_t 
         "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]), "=&v"(b[2]), "=&v"(a[3]), "=&v"(b[3])
-        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(kOffset), "n"(kOffset + 8 * 2 * D));
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(kOffset), "n"(kOffset + 8 * 2 * D)
+        : "memory");
   } else {
     asm volatile(
         "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
@@ -225,7 +310,8 @@ __device__ __forceinline__ void read_values(bf16x8 (&v)[D / 32], const uint32_t 
         "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1])
-        : "v"(at[0]), "v"(at[1]), "n"(kOffset), "n"(kOffset + 8 * 2 * D));
+        : "v"(at[0]), "v"(at[1]), "n"(kOffset), "n"(kOffset + 8 * 2 * D)
+        : "memory");
   }
 #pragma unroll
   for (int x = 0; x < D / 32; ++x) v[x] = __builtin_bit_cast(bf16x8, u32x4{a[x][0], a[x][1], b[x][0], b[x][1]});
@@ -349,6 +435,9 @@ __device__ __forceinline__ void attend(Rows<D>& r, const bf16x8 (&q)[D / 16], co
 // worker and slot: D / 8 chunks of [256] float4, then [256] tops and [256] sums.
 template <int D>
 constexpr int kPartialFloats = 256 * (D / 2 + 2);
+// The same of paged_attend_few: [32][D] values, [32] tops, [32] sums.
+template <int D>
+constexpr int kFewPartialFloats = 32 * (D + 2);
 
 // Rows of 32 D-wide outputs to memory: lane l of half h holds columns 8 (e / 4) + 4 h ..
 // of block x; two lanes exchange halves so that each stores 16 bytes.
@@ -380,32 +469,18 @@ __device__ __forceinline__ float inverse_of(float sum) { return sum > 0.f ? 1.f 
 template <int D>
 __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
   using T = Tile<D>;
-  constexpr int kKeys = 64, kDmas = 16 / T::kDmaRows;  // DMAs of a wave's 16 keys
+  constexpr int kKeys = 64;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   constexpr int kTileBytes = kKeys * T::kRow;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
 
-  // Rows that belong to no request are zeroed on the way.
-  if (p.zero_rows) {
-    const int chunks = p.group * p.kv_heads * (D / 8);
-    for (int64_t row = blockIdx.x; row < p.tokens; row += gridDim.x)
-      if (p.positions[row] < 0)
-        for (int c = threadIdx.x; c < chunks; c += 256)
-          *reinterpret_cast<u32x4*>(p.out + row * p.out_token + c / (D / 8) * p.out_head + c % (D / 8) * 8) = u32x4{0, 0, 0, 0};
-  }
+  clear_rows<D, 256>(p);
   Record* const record = reinterpret_cast<Record*>(p.records) + blockIdx.x;
   if (threadIdx.x == 0) record->others = 0;
   Span s;
-  if (!find_span<kKeys>(p, &s)) return;
+  if (!find_span<kKeys, 4>(p, &s)) return;
 
-  // the DMA's lane offsets within a page: row and chunk
-  uint32_t key_at[kDmas], value_at[kDmas];
-#pragma unroll
-  for (int i = 0; i < kDmas; ++i) {
-    const int in = lane / T::kChunks, row = i * T::kDmaRows + in, chunk = lane % T::kChunks;
-    key_at[i] = (uint32_t)in * (uint32_t)p.slot_stride * 2 + 16 * T::key_chunk(chunk, row);
-    value_at[i] = (uint32_t)in * (uint32_t)p.slot_stride * 2 + 16 * T::value_chunk(chunk, row);
-  }
+  const Lanes<D, 16> lanes(p.slot_stride);
 
   while (s.left > 0) {
     const Request<kKeys> r(p, s.request);
@@ -436,17 +511,8 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
       return table[min(step * kKeys + lane, length - 1) >> p.page_shift];
     };
     auto fetch = [&](int step, int pages, int buffer) __attribute__((always_inline)) {
-      const int key0 = step * kKeys + 16 * wave;
       uint8_t* const to = lds + buffer * 2 * kTileBytes + 16 * wave * T::kRow;
-#pragma unroll
-      for (int i = 0; i < kDmas; ++i) {
-        const int key = key0 + i * T::kDmaRows;
-        const int page = __builtin_amdgcn_readlane(pages, 16 * wave + i * T::kDmaRows);
-        const int slot = key & ((1 << p.page_shift) - 1), rows = min(length - key, T::kDmaRows);
-        packed::dma_frag(page_rsrc(p.k, p, page, slot, s.head, rows), key_at[i], 0, to + i * T::kDmaRows * T::kRow);
-        packed::dma_frag(page_rsrc(p.v, p, page, slot, s.head, rows), value_at[i], 0,
-                         to + kTileBytes + i * T::kDmaRows * T::kRow);
-      }
+      lanes.fetch(p, s.head, step * kKeys + 16 * wave, length, pages, 16 * wave, to, to + kTileBytes);
     };
     int pages = pages_of(from);
     uint64_t held = __ballot((uint32_t)pages < (uint32_t)p.num_pages);
@@ -492,13 +558,158 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
     }
     s.left -= count;
     if (s.left <= 0) break;
-    s.skip = 0;
-    if (++s.tile < r.tiles) continue;
-    s.tile = 0;
-    do {
-      if (++s.request == p.requests) s.request = 0, ++s.head;
-    } while (p.rows[s.request] <= 0);
+    next_item(p, &s, r.tiles);
   }
+}
+
+// Steps of few rows (decoding): a workgroup is one wave with 32 rows a tile, which streams 32
+// keys a step through its own two buffers, so that no barrier joins it to others and
+// five of them (LDS: 32 KB each at head_dim 128) keep up to 160 KB of a CU's reads in
+// flight. Rows are few: what bounds it is the cache's bytes.
+template <int D>
+__global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
+  using T = Tile<D>;
+  constexpr int kKeys = 32, kDmas = kKeys / T::kDmaRows, kTileBytes = kKeys * T::kRow;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int lane = threadIdx.x, half = lane >> 5;
+
+  clear_rows<D, 64>(p);
+  Record* const record = reinterpret_cast<Record*>(p.records) + blockIdx.x;
+  if (lane == 0) record->others = 0;
+  Span s;
+  if (!find_span<kKeys, 1>(p, &s)) return;
+
+  const Lanes<D, kKeys> lanes(p.slot_stride);
+
+  while (s.left > 0) {
+    const Request<kKeys> r(p, s.request);
+    const int tile_first = r.first(s.tile), tile_count = r.count(s.tile);
+    const int count = (int)min((int64_t)(tile_count - s.skip), s.left);
+    const int from = tile_first + s.skip;
+    const int tile_rows = min(r.per_tile, r.fresh - s.tile * r.per_tile) * p.group;
+    const int row = min(lane & 31, tile_rows - 1);
+    const int local = s.tile * r.per_tile + row / p.group, head = s.head * p.group + row % p.group;
+    const int64_t token = p.starts[s.request] + local;
+    const int position = r.context + local, length = r.context + r.fresh;
+    const int low = __builtin_amdgcn_readfirstlane(position), high = __builtin_amdgcn_readlane(position, 31);
+    const bool valid = (lane & 31) < tile_rows;
+    const int32_t* const table = p.tables + s.request * p.table_stride;
+
+    // lane l's page of a step: that of its key l % 32 of the step
+    auto pages_of = [&](int step) __attribute__((always_inline)) {
+      return table[min(step * kKeys + (lane & 31), length - 1) >> p.page_shift];
+    };
+    // Steps past the item's last are fetched as no rows (zeros, no reads), so that the
+    // number of operations in flight stays the same.
+    auto fetch = [&](int i, int pages) __attribute__((always_inline)) {
+      uint8_t* const to = lds + (i & 1) * 2 * kTileBytes;
+      lanes.fetch(p, s.head, (from + i) * kKeys, i < count ? length : 0, pages, 0, to, to + kTileBytes);
+    };
+    int pages = pages_of(from), next = pages_of(from + 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the item before: its last fetches and stores
+    bf16x8 q[D / 16];
+    const uint16_t* const q_row = p.q + token * p.q_token + head * p.q_head + 8 * half;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) q[t] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q_row + 16 * t));
+    uint32_t held = (uint32_t)__ballot((uint32_t)pages < (uint32_t)p.num_pages);
+    fetch(0, pages);
+    int after = pages_of(from + 2);
+    uint32_t next_held = (uint32_t)__ballot((uint32_t)next < (uint32_t)p.num_pages);
+    fetch(1, next);
+
+    Rows<D> o;
+    o.clear();
+    for (int i = 0; i < count; ++i) {
+      // all but the page list and the DMAs of the step behind this one
+      asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * kDmas + 1) : "memory");
+      const int key0 = (from + i) * kKeys;
+      const bool masked = key0 + kKeys - 1 > low || (p.window && key0 <= high - p.window) || held != ~0u;
+      const uint8_t* const at = lds + (i & 1) * 2 * kTileBytes;
+      attend<D, 1>(o, q, at, at + kTileBytes, p.scale, masked, position - key0, p.window, held);
+      held = next_held;
+      next_held = (uint32_t)__ballot((uint32_t)after < (uint32_t)p.num_pages);
+      const int now = after;
+      after = pages_of(from + i + 3);
+      fetch(i + 2, now);
+    }
+
+    const float sum = o.sum + other_half(o.sum);
+    if (count == tile_count) {
+      store_rows<D>(p, o.o, inverse_of(sum), valid, token, head);
+    } else {
+      float* const to = p.partial + (2 * (int64_t)s.worker + (s.skip == 0)) * kFewPartialFloats<D>;
+      if (valid) {
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<f32x4*>(to + row * D + 32 * x + 8 * e + 4 * half) =
+                f32x4{o.o[x][4 * e], o.o[x][4 * e + 1], o.o[x][4 * e + 2], o.o[x][4 * e + 3]};
+        if (!half) {
+          to[32 * D + row] = o.top;
+          to[32 * D + 32 + row] = sum;
+        }
+      }
+      if (s.skip == 0 && lane == 0) {
+        record->worker = s.worker, record->head = s.head, record->request = s.request, record->tile = s.tile;
+        record->others = (int)((tile_count - count + s.each - 1) / s.each);
+      }
+    }
+    s.left -= count;
+    if (s.left <= 0) break;
+    next_item(p, &s, r.tiles);
+  }
+  // no DMA outlives the wave
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// Adds up the partial sums of paged_attend_few: a workgroup per record, a thread per
+// row and four columns; threads that are left divide the partial sums among them. Each
+// keeps a running maximum, and the parts meet in LDS.
+template <int D>
+__global__ __launch_bounds__(1024) void paged_join_few(AttentionArgs p) {
+  const Record record = reinterpret_cast<const Record*>(p.records)[blockIdx.x];
+  if (record.others <= 0) return;
+  __shared__ f32x4 values[1024];
+  __shared__ float tops[1024], totals[1024];
+  const int fresh = p.rows[record.request];
+  const int rows = min(p.tile_tokens, fresh - record.tile * p.tile_tokens) * p.group;
+  const int items = rows * (D / 4), parts = 1024 / items;  // rows <= 32: at least one part
+  const int part = (int)threadIdx.x / items, item = (int)threadIdx.x - part * items;
+  const int row = item / (D / 4), column = item % (D / 4) * 4;
+  const float* const base = p.partial + 2 * (int64_t)record.worker * kFewPartialFloats<D>;
+  constexpr int64_t kWorker = 2 * (int64_t)kFewPartialFloats<D>;
+  float top = -INFINITY, total = 0.f;
+  f32x4 value = {0.f, 0.f, 0.f, 0.f};
+  if (part < parts)
+#pragma unroll 4
+    for (int i = part; i <= record.others; i += parts) {
+      const float* const from = base + i * kWorker + (i == 0 ? kFewPartialFloats<D> : 0);
+      const float mine = from[32 * D + row], sum = from[32 * D + 32 + row];
+      const f32x4 v = *reinterpret_cast<const f32x4*>(from + row * D + column);
+      const float next = fmaxf(top, mine), ref = next == -INFINITY ? 0.f : next;
+      const float keep = __builtin_amdgcn_exp2f(top - ref), add = __builtin_amdgcn_exp2f(mine - ref);
+      top = next;
+      total = total * keep + sum * add;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) value[j] = value[j] * keep + v[j] * add;
+    }
+  values[threadIdx.x] = value, tops[threadIdx.x] = top, totals[threadIdx.x] = total;
+  __syncthreads();
+  if (part) return;
+  for (int i = 1; i < parts; ++i) {
+    const int at = i * items + item;
+    const float next = fmaxf(top, tops[at]), ref = next == -INFINITY ? 0.f : next;
+    const float keep = __builtin_amdgcn_exp2f(top - ref), add = __builtin_amdgcn_exp2f(tops[at] - ref);
+    top = next;
+    total = total * keep + totals[at] * add;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) value[j] = value[j] * keep + values[at][j] * add;
+  }
+  const float inverse = inverse_of(total);
+  const int64_t token = p.starts[record.request] + record.tile * p.tile_tokens + row / p.group;
+  *reinterpret_cast<uint2*>(p.out + token * p.out_token + (record.head * p.group + row % p.group) * p.out_head + column) =
+      make_uint2(pack_bf16(value[0] * inverse, value[1] * inverse), pack_bf16(value[2] * inverse, value[3] * inverse));
 }
 
 // Adds up the partial sums of the items that spans cut: one workgroup per
@@ -538,26 +749,31 @@ __global__ __launch_bounds__(256) void paged_join(AttentionArgs p) {
   store_rows<D>(p, o, inverse_of(sum), at < tile_rows, token, record.head * p.group + row % p.group);
 }
 
-// Workgroups of a launch: two per CU (LDS holds two), a multiple of the 8 XCDs.
-int workgroups(int cus) { return (2 * cus + 7) / 8 * 8; }
+// Workgroups of a launch, a multiple of the 8 XCDs: as many as a CU's LDS holds (two of paged_attend;
+// five of paged_attend_few, its registers would allow eight).
+int workgroups(int cus, bool few) { return ((few ? 4 : 2) * cus + 7) / 8 * 8; }
 
 constexpr int64_t kRecordBytes = sizeof(Record);
 
 int64_t workspace_of(int cus, int head_dim) {
-  const int64_t floats = 256 * (head_dim / 2 + 2);
-  return workgroups(cus) * (kRecordBytes + 2 * floats * 4);
+  const int64_t many = kRecordBytes + 2 * 4 * 256 * (int64_t)(head_dim / 2 + 2);
+  const int64_t few = kRecordBytes + 2 * 4 * 32 * (int64_t)(head_dim + 2);
+  return max(workgroups(cus, false) * many, workgroups(cus, true) * few);
 }
 
+// Requests whose new rows fill one tile of 32 at most take the kernel for few rows: its waves
+// share no work, so a tile of four times the rows reads the cache four times less.
+bool few_rows(int64_t max_new, int group) { return max_new * group <= 32; }
+
 template <int D>
-int launch_attention(AttentionArgs& p, int cus, hipStream_t stream) {
-  const int lds = 4 * 64 * 2 * D;
-  hipError_t e = hipFuncSetAttribute((const void*)paged_attend<D>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+int launch_attention(AttentionArgs& p, bool few, unsigned blocks, hipStream_t stream) {
+  auto kern = few ? paged_attend_few<D> : paged_attend<D>;
+  const int lds = (few ? 4 * 32 : 4 * 64) * 2 * D;
+  hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return fail(SMX_ERR_LAUNCH, "hipFuncSetAttribute: %s", hipGetErrorString(e));
-  const unsigned blocks = (unsigned)workgroups(cus);
-  p.tile_tokens = 128 / p.group;
-  hipLaunchKernelGGL(paged_attend<D>, dim3(blocks), dim3(256), lds, stream, p);
+  hipLaunchKernelGGL(kern, dim3(blocks), dim3(few ? 64 : 256), lds, stream, p);
   if (int rc = check_launch()) return rc;
-  hipLaunchKernelGGL(paged_join<D>, dim3(blocks), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL(few ? paged_join_few<D> : paged_join<D>, dim3(blocks), dim3(few ? 1024 : 256), 0, stream, p);
   return check_launch();
 }
 
@@ -615,12 +831,16 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
   p.requests = step->requests, p.tokens = step->tokens;
   p.kv_heads = cache->kv_heads, p.group = q->heads / cache->kv_heads;
   p.page_shift = __builtin_ctz(cache->page_size), p.num_pages = cache->num_pages;
-  p.window = window, p.zero_rows = zero_rows, p.min_span = 2;
+  p.window = window, p.zero_rows = zero_rows;
+  const bool few = few_rows(step->max_new, p.group);
+  const int blocks = workgroups(cus, few);
+  p.tile_tokens = (few ? 32 : 128) / p.group;
+  p.min_span = few ? 4 : 2;
   p.scale = scale * 1.44269504088896341f;
   p.records = (int32_t*)workspace;
-  p.partial = (float*)((char*)workspace + workgroups(cus) * kRecordBytes);
-  return cache->head_dim == 128 ? launch_attention<128>(p, cus, (hipStream_t)stream)
-                                : launch_attention<64>(p, cus, (hipStream_t)stream);
+  p.partial = (float*)((char*)workspace + blocks * kRecordBytes);
+  return cache->head_dim == 128 ? launch_attention<128>(p, few, blocks, (hipStream_t)stream)
+                                : launch_attention<64>(p, few, blocks, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -23,7 +23,6 @@ tables and the heads changed in place.
 from __future__ import annotations
 
 import ctypes
-import dataclasses
 import functools
 import math
 
@@ -38,7 +37,6 @@ __all__ = ["PagedPlan", "paged_plan", "paged_write", "paged_attention", "PAGED_O
 PAGED_OK, PAGED_BAD_LENGTH, PAGED_OUT_OF_ROWS, PAGED_OUT_OF_PAGES, PAGED_BAD_PAGE = range(5)
 
 
-@dataclasses.dataclass(frozen=True)
 class PagedPlan:
     """Rows, positions and slots of one step (``paged_plan``); tensors on the device.
 
@@ -52,50 +50,41 @@ class PagedPlan:
     * ``pages_used`` int32 [1]: how many free pages were taken, from the list's front.
     * ``pages_needed`` int32 [1]: how many the requests up to the last admitted one need together,
       admitted or not; more than the list holds once it ran out.
-    """
 
-    starts: torch.Tensor
-    rows: torch.Tensor
-    context: torch.Tensor
-    status: torch.Tensor
-    positions: torch.Tensor
-    slots: torch.Tensor
-    pages_used: torch.Tensor
-    pages_needed: torch.Tensor
-    block_tables: torch.Tensor
-    page_size: int
-    num_pages: int
-    max_new: int
-    max_context: int
+    It also holds the step's ``block_tables`` and sizes. One plan serves all layers of its step."""
 
-    @property
-    def tokens(self):
-        return self.positions.shape[0]
+    __slots__ = ("starts", "rows", "context", "status", "positions", "slots", "pages_used", "pages_needed",
+                 "block_tables", "page_size", "num_pages", "max_new", "max_context", "requests", "tokens", "device",
+                 "_positions", "_slots", "_step")
 
-    @property
-    def requests(self):
-        return self.rows.shape[0]
-
-    @property
-    def device(self):
-        return self.positions.device
+    def __repr__(self):
+        return (f"PagedPlan(requests={self.requests}, tokens={self.tokens}, page_size={self.page_size}, "
+                f"num_pages={self.num_pages}, max_new={self.max_new}, max_context={self.max_context})")
 
 
 def _check_device(name, x, device=None):
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(x).__name__}")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError(f"the gfx950 kernel needs tensors on the HIP device (got {name} on {x.device})")
     if device is not None and x.device != device:
         raise ValueError(f"{name} is on {x.device}, the call on {device}")
 
 
+# The stream's handle itself: torch.cuda.current_stream makes an object of it first, which takes as long as
+# the launch of a decode step's kernel.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _call(device, function, *args):
     """One library call on the device's current stream."""
     if torch.cuda.current_device() == device.index:
-        return _lib.check(function(*args, torch.cuda.current_stream(device).cuda_stream))
-    with torch.cuda.device(device):
-        return _lib.check(function(*args, torch.cuda.current_stream(device).cuda_stream))
+        rc = function(*args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = function(*args, _raw_stream(device.index))
+    if rc:
+        _lib.check(rc)
 
 
 def _int32(name, x, shape):
@@ -143,59 +132,72 @@ def paged_plan(context_lens, new_lens, block_tables, *, page_size, num_pages, to
             raise ValueError("free_pages must be a list of page numbers")
         _int32("free_pages", free_pages, (free_pages.shape[0],))
         # an empty list too is a list: no request gets a new page
-        free_count, free = free_pages.shape[0], _lib.ptr(free_pages) if free_pages.numel() else _lib.ptr(new_lens)
+        free_count = free_pages.shape[0]
+        free = free_pages.data_ptr() if free_count else new_lens.data_ptr()
+    plan = PagedPlan()
+    plan.block_tables, plan.page_size, plan.num_pages = block_tables, int(page_size), int(num_pages)
+    plan.requests, plan.tokens, plan.device = requests, tokens, device
     width = block_tables.shape[1]
-    max_new = tokens if max_new is None else int(max_new)
-    max_context = min(width * int(page_size), 2**31 - 1) if max_context is None else int(max_context)
+    plan.max_new = tokens if max_new is None else int(max_new)
+    plan.max_context = min(width * plan.page_size, 2**31 - 1) if max_context is None else int(max_context)
     # one allocation for the small tensors: slots (int64) first, then the int32 ones
     sizes = (2 * max(tokens, 1), requests + 1, requests, requests, requests, max(tokens, 1), 1, 1)
-    slots, starts, rows, context, status, positions, used, needed = torch.empty(
-        sum(sizes), dtype=torch.int32, device=device).split(sizes)
-    slots = slots.view(torch.int64)
-    _call(device, _lib.load().smx_paged_plan, requests, width, page_size, num_pages, tokens, max_new, max_context,
-          _lib.ptr(context_lens), _lib.ptr(new_lens), _lib.ptr(block_tables), block_tables.stride(0), free, free_count,
-          _lib.ptr(starts), _lib.ptr(rows), _lib.ptr(context), _lib.ptr(positions), _lib.ptr(slots), _lib.ptr(status),
-          _lib.ptr(used))
-    return PagedPlan(starts, rows, context, status, positions, slots, used, needed, block_tables, int(page_size),
-                     int(num_pages), max_new, max_context)
+    memory = torch.empty(sum(sizes), dtype=torch.int32, device=device)
+    (slots, plan.starts, plan.rows, plan.context, plan.status, plan.positions, plan.pages_used,
+     plan.pages_needed) = memory.split_with_sizes(sizes)
+    plan.slots = slots.view(torch.int64)
+    at = plan._slots = memory.data_ptr()
+    starts = at + 4 * sizes[0]
+    rows = starts + 4 * sizes[1]
+    context = rows + 4 * requests
+    status = context + 4 * requests
+    positions = plan._positions = status + 4 * requests
+    tables, stride = block_tables.data_ptr(), block_tables.stride(0)
+    _call(device, _lib.load().smx_paged_plan, requests, width, plan.page_size, plan.num_pages, tokens, plan.max_new,
+          plan.max_context, context_lens.data_ptr(), new_lens.data_ptr(), tables, stride, free, free_count, starts,
+          rows, context, positions, at, status, positions + 4 * sizes[5])
+    plan._step = _lib.SmxPagedStep(requests, tokens, plan.max_new, tables, stride, starts, rows, context, positions)
+    return plan
 
 
 def _cache(k_cache, v_cache, plan):
     """The cache's description for the library; ``plan`` fixes its pages."""
-    device = plan.device
     for name, x in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _check_device(name, x, device)
-        if x.dim() != 4 or x.dtype != torch.bfloat16:
+        _check_device(name, x, plan.device)
+        if x.dtype != torch.bfloat16 or x.dim() != 4:
             raise ValueError(f"{name} must be a bf16 tensor [pages, page_size, kv_heads, head_dim], got {x.dtype} "
                              f"{tuple(x.shape)}")
-    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+    strides = k_cache.stride()
+    if k_cache.shape != v_cache.shape or strides != v_cache.stride():
         raise ValueError("k_cache and v_cache must have the same shape and strides")
     pages, page_size, kv_heads, head_dim = k_cache.shape
     if page_size != plan.page_size or pages != plan.num_pages:
         raise ValueError(f"the plan is of {plan.num_pages} pages of {plan.page_size} tokens, the cache of {pages} of "
                          f"{page_size}")
-    if k_cache.stride(3) != 1:
+    if strides[3] != 1:
         raise ValueError("cache heads must be contiguous runs")
-    return _lib.SmxPagedCache(k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride()[:3], pages, page_size,
-                              kv_heads, head_dim)
+    return _lib.SmxPagedCache(k_cache.data_ptr(), v_cache.data_ptr(), strides[0], strides[1], strides[2], pages,
+                              page_size, kv_heads, head_dim)
 
 
 def _heads(name, x, plan, heads, head_dim, lay_out=True):
     """Head rows ``[tokens, heads, head_dim]`` for the library; rows that it cannot take as they lie
     (not 16-byte aligned runs) are laid out first, or refused."""
     _check_device(name, x, plan.device)
-    if x.dtype != torch.bfloat16 or x.dim() != 3 or x.shape[0] != plan.tokens or x.shape[2] != head_dim \
-            or (heads is not None and x.shape[1] != heads):
+    shape = x.shape
+    if x.dtype != torch.bfloat16 or len(shape) != 3 or shape[0] != plan.tokens or shape[2] != head_dim \
+            or (heads is not None and shape[1] != heads):
         raise ValueError(f"{name} must be a bf16 tensor of shape {(plan.tokens, heads or 'heads', head_dim)}, got "
-                         f"{x.dtype} {tuple(x.shape)}")
+                         f"{x.dtype} {tuple(shape)}")
+    token, head, unit = x.stride()
     # the stride of a dimension of one is no stride: nothing steps over it
-    token, head = x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0
-    if x.stride(2) != 1 or token % 8 or head % 8 or x.data_ptr() % 16:
+    token, head, at = token if shape[0] > 1 else 0, head if shape[1] > 1 else 0, x.data_ptr()
+    if unit != 1 or token % 8 or head % 8 or at % 16:
         if not lay_out:
             raise ValueError(f"{name} rows must be 16-byte aligned runs")
         x = x.clone(memory_format=torch.contiguous_format)
-        token, head = x.shape[1] * head_dim, head_dim
-    return x, _lib.SmxHeads(x.data_ptr(), token, head, x.shape[1])
+        token, head, at = shape[1] * head_dim, head_dim, x.data_ptr()
+    return x, _lib.SmxHeads(at, token, head, shape[1])
 
 
 def _no_gradients(*tensors):
@@ -266,8 +268,8 @@ def paged_write(k, v, k_cache, v_cache, plan, *, q=None, rope_cos=None, rope_sin
         dtypes |= _lib.SMX_PAGED_Q_SCALE_F32
     if k_scale is not None and k_scale.dtype == torch.float32:
         dtypes |= _lib.SMX_PAGED_K_SCALE_F32
-    _call(plan.device, _lib.load().smx_paged_write, cache, plan.tokens, _lib.ptr(plan.positions), _lib.ptr(plan.slots),
-          q_rows, k_rows, v_rows, _lib.ptr(rope_cos), _lib.ptr(rope_sin), rope_rows, rope_stride, _lib.ptr(q_scale),
+    _call(plan.device, _lib.load().smx_paged_write, cache, plan.tokens, plan._positions, plan._slots, q_rows,
+          k_rows, v_rows, _lib.ptr(rope_cos), _lib.ptr(rope_sin), rope_rows, rope_stride, _lib.ptr(q_scale),
           _lib.ptr(k_scale), dtypes, float(eps), _lib.ptr(out))
     return out
 
@@ -306,11 +308,8 @@ def paged_attention(q, k_cache, v_cache, plan, *, scale=None, window=None, out=N
     if zero_rows:
         out = torch.empty(q.shape, dtype=torch.bfloat16, device=plan.device)
     _, out_rows = _heads("out", out, plan, q.shape[1], head_dim, lay_out=False)
-    step = _lib.SmxPagedStep(plan.requests, plan.tokens, plan.max_new, plan.block_tables.data_ptr(),
-                             plan.block_tables.stride(0), plan.starts.data_ptr(), plan.rows.data_ptr(),
-                             plan.context.data_ptr(), plan.positions.data_ptr())
     need = _workspace_bytes(plan.device, head_dim)
     workspace = torch.empty(need, dtype=torch.uint8, device=plan.device)
-    _call(plan.device, _lib.load().smx_paged_attention, cache, step, q_rows, out_rows, float(scale), window, zero_rows,
-          _lib.ptr(workspace), need)
+    _call(plan.device, _lib.load().smx_paged_attention, cache, plan._step, q_rows, out_rows, float(scale), window,
+          zero_rows, workspace.data_ptr(), need)
     return out
