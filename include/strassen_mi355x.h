@@ -488,14 +488,16 @@ int smx_paged_attention_workspace_bytes(int32_t head_dim, int64_t* bytes);
  * tiles of the gate half and of the up half in turn; an even number of tiles, padded
  * with scale 0), k in tiles of 128 (padded likewise).
  *   codes: per column tile and k tile 64 lanes of four words; word s of lane l holds
- *     column l % 16, k = 32 s + 8 (l / 16) + j, j = 0 .. 7, at bit 16 (j % 2) + 4 (j / 2);
- *   scales: per column tile, group (of 32, 64 or 128) and column one word: the bf16
- *     scale in the upper half, bf16(-(16 + zero)) in the lower.
+ *     column l % 16, k = 32 s + 8 (l / 16) + j, j = 0 .. 7, from bit 16 (j % 2) + 4 (j / 2) + 3
+ *     on (the last, from bit 31, goes on at bit 0);
+ *   scales: per column tile, k tile, column and group (of 32, 64 or 128) of the k tile one
+ *     word: the bf16 scale in the upper half, bf16(-(16 + zero)) in the lower.
+ * zeros 0: every zero point is 8 (the lower halves are not read).
  */
 typedef struct smx_int4_weight {
   const void *codes, *scales;
   int64_t k, n;
-  int32_t group, swiglu;
+  int32_t group, swiglu, zeros;
 } smx_int4_weight;
 
 /*
@@ -506,7 +508,10 @@ typedef struct smx_int4_weight {
  * An infinity in x makes its row NaN. Asynchronous on stream.
  */
 int smx_int4_matmul(const smx_int4_weight* w, int64_t m, const void* x, int64_t ldx, int32_t epilogue,
-                    const void* extra, int64_t lde, int32_t extra_f32, void* out, int64_t ldo, void* stream);
+                    const void* extra, int64_t lde, int32_t extra_f32, void* out, int64_t ldo, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+/* Device memory that the call needs (16-byte aligned, overwritten; 0: none), on the current device. */
+int smx_int4_workspace_bytes(const smx_int4_weight* w, int64_t m, int64_t* bytes);
 
 /* Message of the last failing call on this thread ("" if none). */
 const char* smx_last_error(void);

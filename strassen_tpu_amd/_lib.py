@@ -68,7 +68,8 @@ SMX_PAGED_ROPE_F32 = 4
 EXPORTS = ("smx_gemm", "smx_gemm_noalloc", "smx_gemm_workspace_bytes", "smx_matmul", "smx_matmul_workspace_bytes", "smx_matmul_plan",
            "smx_tile_requirements", "smx_packed_bytes", "smx_pack_operand", "smx_pack_rhs_transposed", "smx_norm_residual_add", "smx_rms_norm",
            "smx_row_squares", "smx_scale_rows", "smx_qk_norm_rope", "smx_paged_plan", "smx_paged_write",
-           "smx_paged_attention", "smx_paged_attention_workspace_bytes", "smx_int4_matmul", "smx_last_error", "smx_version")
+           "smx_paged_attention", "smx_paged_attention_workspace_bytes", "smx_int4_matmul",
+           "smx_int4_workspace_bytes", "smx_last_error", "smx_version")
 
 
 class SmxGemmDesc(ctypes.Structure):
@@ -114,7 +115,7 @@ class SmxPagedStep(ctypes.Structure):
 
 class SmxInt4Weight(ctypes.Structure):
     _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("k", ctypes.c_int64), ("n", ctypes.c_int64),
-                ("group", ctypes.c_int32), ("swiglu", ctypes.c_int32)]
+                ("group", ctypes.c_int32), ("swiglu", ctypes.c_int32), ("zeros", ctypes.c_int32)]
 
 
 _lib = None
@@ -175,8 +176,10 @@ def load():
     lib.smx_paged_attention.restype = ctypes.c_int
     lib.smx_paged_attention_workspace_bytes.argtypes = [i32, ctypes.POINTER(i64)]
     lib.smx_paged_attention_workspace_bytes.restype = ctypes.c_int
-    lib.smx_int4_matmul.argtypes = [ctypes.POINTER(SmxInt4Weight), i64, vp, i64, i32, vp, i64, i32, vp, i64, vp]
+    lib.smx_int4_matmul.argtypes = [ctypes.POINTER(SmxInt4Weight), i64, vp, i64, i32, vp, i64, i32, vp, i64, vp, i64, vp]
     lib.smx_int4_matmul.restype = ctypes.c_int
+    lib.smx_int4_workspace_bytes.argtypes = [ctypes.POINTER(SmxInt4Weight), i64, ctypes.POINTER(i64)]
+    lib.smx_int4_workspace_bytes.restype = ctypes.c_int
     lib.smx_last_error.argtypes = []
     lib.smx_last_error.restype = ctypes.c_char_p
     lib.smx_version.argtypes = []

@@ -127,7 +127,7 @@ _SPLIT = re.compile(r"gemm_splitILi(\d+)ELi(\d+)ELb(\d)E")
 _PM = re.compile(r"gemm_pmILi(\d+)ELi(\d+)EE")
 _STREAM = re.compile(r"gemm_streamILi(\d+)E")
 _PACKED = re.compile(r"gemm_packedILi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)ELb(\d)E")
-_SERVING = re.compile(r"(paged_attend|paged_join|int4_matmul)")
+_SERVING = re.compile(r"(paged_attend|paged_join|int4_few|int4_tiled)")
 _QUAD_CUBIC_PARTIAL = 1
 PARTIAL_SCRATCH_CAP = 1024
 

@@ -9,6 +9,8 @@ zero point 0 .. 15 per group of 32, 64 or 128 consecutive k and column.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -23,10 +25,23 @@ _EPILOGUES = (None, "swiglu", "residual_add", "bias_add")
 class Int4Operand:
     """A weight laid out by ``int4_weight_layout``."""
 
-    def __init__(self, codes, scales, k, n, group, swiglu):
+    def __init__(self, codes, scales, k, n, group, swiglu, zeros):
         self.codes, self.scales = codes, scales
         self.k, self.n, self.group, self.swiglu = k, n, group, swiglu
-        self.desc = _lib.SmxInt4Weight(codes.data_ptr(), scales.data_ptr(), k, n, group, int(swiglu))
+        self.desc = _lib.SmxInt4Weight(codes.data_ptr(), scales.data_ptr(), k, n, group, int(swiglu), int(zeros))
+        self._workspace = {}  # bytes by number of rows, up to 64 of them
+
+    def workspace_bytes(self, m):
+        """Device memory that a product of ``m`` rows needs."""
+        need = self._workspace.get(m)
+        if need is None:
+            value = ctypes.c_int64()
+            with torch.cuda.device(self.device):
+                _lib.check(_lib.load().smx_int4_workspace_bytes(self.desc, m, ctypes.byref(value)))
+            need = value.value
+            if m <= 64:
+                self._workspace[m] = need
+        return need
 
     @property
     def shape(self):
@@ -101,16 +116,21 @@ def int4_weight_layout(codes, scales, zeros=None, *, group, epilogue=None):
     tiled = tiled.view(k_tiles, 4, 4, 8, -1, 16)
     words = torch.zeros(k_tiles, 4, 4, tiled.shape[4], 16, dtype=torch.int32, device=codes.device)
     for j in range(8):
-        words |= tiled[:, :, :, j].to(torch.int32) << (16 * (j % 2) + 4 * (j // 2))
+        at = 16 * (j % 2) + 4 * (j // 2) + 3
+        part = tiled[:, :, :, j].to(torch.int32)
+        # the last pair's upper code wraps around: its lowest bit at 31, the others at 0 .. 2
+        words |= part << at if at < 29 else (part << 31) | (part >> 1)
     words = words.permute(3, 0, 2, 4, 1).contiguous()  # [tiles, k_tiles, quad, column, word]
     # -(16 + zero) is a bf16 number: sign, exponent of 16, four mantissa bits
     zero = torch.full(shape, 8, dtype=torch.int32, device=codes.device) if zeros is None else zeros.to(torch.int32)
     pairs = (scales.contiguous().view(torch.int16).to(torch.int32) << 16) | (0xC180 | zero << 3)
     pairs = _tiles(pairs, swiglu)  # [groups, tiles, 16]
-    missing = k_tiles * (128 // group) - shape[0]
+    per_tile = 128 // group
+    missing = k_tiles * per_tile - shape[0]
     if missing:
         pairs = torch.nn.functional.pad(pairs, (0, 0, 0, 0, 0, missing))
-    return Int4Operand(words, pairs.permute(1, 0, 2).contiguous(), k, n, group, swiglu)
+    pairs = pairs.unflatten(0, (k_tiles, per_tile)).permute(2, 0, 3, 1).contiguous()  # [tiles, k_tiles, column, group]
+    return Int4Operand(words, pairs, k, n, group, swiglu, zeros is not None)
 
 
 def int4_matmul(x, w, *, epilogue=None, residual=None, bias=None):
@@ -152,9 +172,11 @@ def int4_matmul(x, w, *, epilogue=None, residual=None, bias=None):
     if not m:
         return out
     row = x.stride(0) if m > 1 else k  # a single row has no stride
-    if x.stride(1) != 1 or row % 8 or row < k or x.data_ptr() % 16:
+    if x.stride(1) != 1 or row % 8 or row < k or row > 1 << 24 or x.data_ptr() % 16:
         x, row = x.clone(memory_format=torch.contiguous_format), k
+    need = w.workspace_bytes(m)
+    workspace = torch.empty(need, dtype=torch.uint8, device=w.device) if need else None
     _call(w.device, _lib.load().smx_int4_matmul, w.desc, m, _lib.ptr(x), row, _lib.SMX_EPI[epilogue],
           _lib.ptr(extra), max(extra.stride(0), n) if residual is not None else 0,
-          int(extra is not None and extra.dtype == torch.float32), _lib.ptr(out), n)
+          int(extra is not None and extra.dtype == torch.float32), _lib.ptr(out), n, _lib.ptr(workspace), need)
     return out

@@ -46,7 +46,7 @@ def test_int4_layout(k, n, group, swiglu):
     half = n // 2
     tiles = 2 * -(-half // 16) if swiglu else 2 * -(-n // 32)
     assert w.codes.shape == (tiles, -(-k // 128), 4, 16, 4)
-    assert w.scales.shape == (tiles, -(-k // 128) * (128 // group), 16)
+    assert w.scales.shape == (tiles, -(-k // 128), 16, 128 // group)
     words = w.codes.to(torch.int64) & 0xffffffff
     pairs = w.scales.to(torch.int64) & 0xffffffff
     for tile in range(tiles):
@@ -60,9 +60,10 @@ def test_int4_layout(k, n, group, swiglu):
                 word = int(words[tile, kk // 128, kk % 32 // 8, c, kk % 128 // 32])
                 j = kk % 8
                 want = int(codes[kk, column]) if column is not None and kk < k else 0
-                assert word >> (16 * (j % 2) + 4 * (j // 2)) & 15 == want
+                at = 16 * (j % 2) + 4 * (j // 2) + 3
+                assert (word | word << 32) >> at & 15 == want
             for gr in range(k // group):
-                pair = int(pairs[tile, gr, c])
+                pair = int(pairs[tile, gr * group // 128, c, gr % (128 // group)])
                 as_bf16 = lambda bits: torch.tensor([bits - (bits >> 15 << 16)], dtype=torch.int16).view(torch.bfloat16)
                 if column is None:
                     assert pair == 0
@@ -152,14 +153,14 @@ def test_write_refusals(change):
 
 
 def _int4(w=None, m=4, x=P, ldx=256, epilogue=0, extra=None, lde=0, f32=0, out=P, ldo=64):
-    w = w or _lib.SmxInt4Weight(P, P, 256, 64, 128, 0)
-    return _lib.load().smx_int4_matmul(w, m, x, ldx, epilogue, extra, lde, f32, out, ldo, None)
+    w = w or _lib.SmxInt4Weight(P, P, 256, 64, 128, 0, 1)
+    return _lib.load().smx_int4_matmul(w, m, x, ldx, epilogue, extra, lde, f32, out, ldo, None, 0, None)
 
 
 @pytest.mark.parametrize("change", [
-    {"w": _lib.SmxInt4Weight(None, P, 256, 64, 128, 0)}, {"w": _lib.SmxInt4Weight(P, P + 4, 256, 64, 128, 0)},
-    {"w": _lib.SmxInt4Weight(P, P, 240, 64, 128, 0)}, {"w": _lib.SmxInt4Weight(P, P, 256, 64, 96, 0)},
-    {"w": _lib.SmxInt4Weight(P, P, 256, 64, 128, 1)}, {"w": _lib.SmxInt4Weight(P, P, 256, 63, 128, 1), "epilogue": 1}, {"m": 0},
+    {"w": _lib.SmxInt4Weight(None, P, 256, 64, 128, 0, 1)}, {"w": _lib.SmxInt4Weight(P, P + 4, 256, 64, 128, 0)},
+    {"w": _lib.SmxInt4Weight(P, P, 240, 64, 128, 0, 1)}, {"w": _lib.SmxInt4Weight(P, P, 256, 64, 96, 0)},
+    {"w": _lib.SmxInt4Weight(P, P, 256, 64, 128, 1, 1)}, {"w": _lib.SmxInt4Weight(P, P, 256, 63, 128, 1), "epilogue": 1}, {"m": 0},
     {"x": P + 2}, {"ldx": 255}, {"ldx": 248}, {"epilogue": 1}, {"epilogue": 4}, {"epilogue": 5}, {"epilogue": 2}, {"extra": P},
     {"epilogue": 2, "extra": P, "lde": 63}, {"ldo": 63}, {"out": P + 4}, {"out": None}])
 def test_int4_refusals(change):
