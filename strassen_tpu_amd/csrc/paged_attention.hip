@@ -78,6 +78,14 @@ struct Request {
       : context(p.context[b]), fresh(p.rows[b]), per_tile(p.tile_tokens), window(p.window) {
     tiles = (fresh + per_tile - 1) / per_tile;
   }
+  // The request that a whole wave works on: its lengths in scalar registers, on which the
+  // page buffers' descriptors depend.
+  __device__ static Request uniform(const AttentionArgs& p, int b) {
+    Request r(p, b);
+    r.context = __builtin_amdgcn_readfirstlane(r.context), r.fresh = __builtin_amdgcn_readfirstlane(r.fresh);
+    r.tiles = __builtin_amdgcn_readfirstlane(r.tiles);
+    return r;
+  }
   __device__ int first(int t) const {
     return window ? max(0, context + t * per_tile - window + 1) / kKeys : 0;
   }
@@ -112,6 +120,11 @@ __device__ __forceinline__ int64_t wave_sum(int64_t x) {
   return x;
 }
 
+__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, lane) |
+         (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
+}
+
 // Inclusive sum of x over a wave's lanes.
 __device__ __forceinline__ int64_t wave_scan(int64_t x) {
 #pragma unroll
@@ -120,11 +133,6 @@ __device__ __forceinline__ int64_t wave_scan(int64_t x) {
     if ((int)(threadIdx.x & 63) >= d) x += y;
   }
   return x;
-}
-
-__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
-  return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, lane) |
-         (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
 }
 
 // Finds the workgroup's span (kWaves waves, uniform result). Consecutive spans lie
@@ -143,6 +151,7 @@ __device__ bool find_span(const AttentionArgs& p, Span* s) {
     __syncthreads();
     total = 0;
     for (int w = 0; w < kWaves; ++w) total += waves[w];
+    total = lane_value(total, 0);
   }
   const int64_t everything = total * p.kv_heads;
   s->each = max((int64_t)p.min_span, (everything + gridDim.x - 1) / gridDim.x);
@@ -151,7 +160,7 @@ __device__ bool find_span(const AttentionArgs& p, Span* s) {
   if ((blockIdx.x >> 3) >= per_xcd || s->worker >= spans) return false;
   s->begin = (int64_t)s->worker * s->each;
   s->left = min(s->each, everything - s->begin);
-  s->head = (int)(s->begin / total);
+  s->head = __builtin_amdgcn_readfirstlane((int)(s->begin / total));
   const int64_t at = s->begin - (int64_t)s->head * total;
 
   int64_t base = 0, rest = 0;
@@ -186,9 +195,9 @@ __device__ bool find_span(const AttentionArgs& p, Span* s) {
   if constexpr (kWaves > 1) {
     __syncthreads();
     s->request = __builtin_amdgcn_readfirstlane(found);
-    rest = found_rest;
+    rest = lane_value(found_rest, 0);
   }
-  const Request<kKeys> r(p, s->request);
+  const auto r = Request<kKeys>::uniform(p, s->request);
   int low = 0, high = r.tiles;  // the last tile with before(tile) <= rest
   while (high - low > 1) {
     const int mid = (low + high) >> 1;
@@ -206,7 +215,7 @@ __device__ __forceinline__ void next_item(const AttentionArgs& p, Span* s, int t
   s->tile = 0;
   do {
     if (++s->request == p.requests) s->request = 0, ++s->head;
-  } while (p.rows[s->request] <= 0);
+  } while (__builtin_amdgcn_readfirstlane(p.rows[s->request]) <= 0);
 }
 
 // Rows that belong to no request are zeroed on the way.
@@ -268,7 +277,9 @@ struct Lanes {
       const bool held = (uint32_t)page < (uint32_t)p.num_pages;
       const int64_t at =
           ((int64_t)(held ? page : 0) * p.page_stride + (int64_t)(first & ((1 << p.page_shift) - 1)) * p.slot_stride) * 2;
-      const int rows = held ? max(0, min(8, length - first)) : 0;
+      // (the clamp is a vector instruction; the descriptor has to be scalar, or every lane's
+      // is compared in a loop around the DMA)
+      const int rows = __builtin_amdgcn_readfirstlane(held ? max(0, min(8, length - first)) : 0);
       const uint32_t bytes = (uint32_t)rows * (uint32_t)p.slot_stride * 2;
       const auto from_k = packed::panel_rsrc(k + at, bytes), from_v = packed::panel_rsrc(v + at, bytes);
 #pragma unroll
@@ -483,7 +494,7 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
   const Lanes<D, 16> lanes(p.slot_stride);
 
   while (s.left > 0) {
-    const Request<kKeys> r(p, s.request);
+    const auto r = Request<kKeys>::uniform(p, s.request);
     const int tile_first = r.first(s.tile), tile_count = r.count(s.tile);
     const int count = (int)min((int64_t)(tile_count - s.skip), s.left);
     const int from = tile_first + s.skip;
@@ -582,7 +593,7 @@ __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
   const Lanes<D, kKeys> lanes(p.slot_stride);
 
   while (s.left > 0) {
-    const Request<kKeys> r(p, s.request);
+    const auto r = Request<kKeys>::uniform(p, s.request);
     const int tile_first = r.first(s.tile), tile_count = r.count(s.tile);
     const int count = (int)min((int64_t)(tile_count - s.skip), s.left);
     const int from = tile_first + s.skip;
