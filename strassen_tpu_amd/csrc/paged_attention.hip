@@ -291,41 +291,62 @@ struct Lanes {
   }
 };
 
-// V^T fragments of 16 keys: for each block of 32 columns, lane l's 8 values of column
-// l % 32 by two transposing LDS reads (4 keys each; lane group l / 16 reads 4
+// V^T fragments of 32 keys (two MFMA steps): for each block of 32 columns, lane l's 8 values of
+// column l % 32 by two transposing LDS reads (4 keys each; lane group l / 16 reads 4
 // rows of 16 columns). `at`: LDS address of the block's first read. Written as one asm
 // block with its wait: before the builtin of this read the compiler waits for every
 // DMA in flight, the next step's too.
 template <int D, int kOffset>
-__device__ __forceinline__ void read_values(bf16x8 (&v)[D / 32], const uint32_t (&at)[D / 32]) {
-  u32x2 a[D / 32], b[D / 32];
+__device__ __forceinline__ void read_values(bf16x8 (&v)[2][D / 32], const uint32_t (&at)[D / 32]) {
+  constexpr int kRow = 2 * D;
+  u32x2 r[2][D / 32][2];
   if constexpr (D == 128) {
     asm volatile(
-        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %0, %16 offset:%20\n\t"
+        "ds_read_b64_tr_b16 %1, %16 offset:%21\n\t"
+        "ds_read_b64_tr_b16 %2, %17 offset:%20\n\t"
+        "ds_read_b64_tr_b16 %3, %17 offset:%21\n\t"
+        "ds_read_b64_tr_b16 %4, %18 offset:%20\n\t"
+        "ds_read_b64_tr_b16 %5, %18 offset:%21\n\t"
+        "ds_read_b64_tr_b16 %6, %19 offset:%20\n\t"
+        "ds_read_b64_tr_b16 %7, %19 offset:%21\n\t"
+        "ds_read_b64_tr_b16 %8, %16 offset:%22\n\t"
+        "ds_read_b64_tr_b16 %9, %16 offset:%23\n\t"
+        "ds_read_b64_tr_b16 %10, %17 offset:%22\n\t"
+        "ds_read_b64_tr_b16 %11, %17 offset:%23\n\t"
+        "ds_read_b64_tr_b16 %12, %18 offset:%22\n\t"
+        "ds_read_b64_tr_b16 %13, %18 offset:%23\n\t"
+        "ds_read_b64_tr_b16 %14, %19 offset:%22\n\t"
+        "ds_read_b64_tr_b16 %15, %19 offset:%23\n\t"
         "s_waitcnt lgkmcnt(0)"
-        : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]), "=&v"(b[2]), "=&v"(a[3]), "=&v"(b[3])
-        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(kOffset), "n"(kOffset + 8 * 2 * D)
+        : "=&v"(r[0][0][0]), "=&v"(r[0][0][1]), "=&v"(r[0][1][0]), "=&v"(r[0][1][1]), "=&v"(r[0][2][0]),
+          "=&v"(r[0][2][1]), "=&v"(r[0][3][0]), "=&v"(r[0][3][1]), "=&v"(r[1][0][0]), "=&v"(r[1][0][1]),
+          "=&v"(r[1][1][0]), "=&v"(r[1][1][1]), "=&v"(r[1][2][0]), "=&v"(r[1][2][1]), "=&v"(r[1][3][0]),
+          "=&v"(r[1][3][1])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(kOffset), "n"(kOffset + 8 * kRow), "n"(kOffset + 16 * kRow),
+          "n"(kOffset + 24 * kRow)
         : "memory");
   } else {
     asm volatile(
-        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
-        "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
-        "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
-        "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %0, %8 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
+        "ds_read_b64_tr_b16 %2, %9 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %3, %9 offset:%11\n\t"
+        "ds_read_b64_tr_b16 %4, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %5, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %6, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
         "s_waitcnt lgkmcnt(0)"
-        : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1])
-        : "v"(at[0]), "v"(at[1]), "n"(kOffset), "n"(kOffset + 8 * 2 * D)
+        : "=&v"(r[0][0][0]), "=&v"(r[0][0][1]), "=&v"(r[0][1][0]), "=&v"(r[0][1][1]), "=&v"(r[1][0][0]),
+          "=&v"(r[1][0][1]), "=&v"(r[1][1][0]), "=&v"(r[1][1][1])
+        : "v"(at[0]), "v"(at[1]), "n"(kOffset), "n"(kOffset + 8 * kRow), "n"(kOffset + 16 * kRow), "n"(kOffset + 24 * kRow)
         : "memory");
   }
 #pragma unroll
-  for (int x = 0; x < D / 32; ++x) v[x] = __builtin_bit_cast(bf16x8, u32x4{a[x][0], a[x][1], b[x][0], b[x][1]});
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+      v[t][x] = __builtin_bit_cast(bf16x8, u32x4{r[t][x][0][0], r[t][x][0][1], r[t][x][1][0], r[t][x][1][1]});
 }
 
 __device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
@@ -367,13 +388,29 @@ __device__ __forceinline__ void attend(Rows<D>& r, const bf16x8 (&q)[D / 16], co
   for (int x = 0; x < kBlocks; ++x)
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[x][e] = 0.f;
+  // All of the step's keys on their way before the first MFMA (one at a time they cost its latency each).
+  bf16x8 k[D / 16][kBlocks];
 #pragma unroll
   for (int t = 0; t < D / 16; ++t)
 #pragma unroll
-    for (int x = 0; x < kBlocks; ++x) {
-      const bf16x8 k = packed::ld_frag(keys + (32 * x + (lane & 31)) * T::kRow + 16 * T::key_chunk(2 * t + half, lane & 31));
-      s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[t], s[x], 0, 0, 0);
-    }
+    for (int x = 0; x < kBlocks; ++x)
+      k[t][x] = packed::ld_frag(keys + (32 * x + (lane & 31)) * T::kRow + 16 * T::key_chunk(2 * t + half, lane & 31));
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+    for (int x = 0; x < kBlocks; ++x) s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[t][x], q[t], s[x], 0, 0, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  // The values too, behind the MFMAs: lane group lane / 16 reads rows 4 half .. + 3 of 16
+  // columns; the lane's row and piece there.
+  const int row = 4 * half + ((lane & 15) >> 2), piece = lane & 3, side = (lane >> 4) & 1;
+  uint32_t at[D / 32];
+#pragma unroll
+  for (int x = 0; x < D / 32; ++x)
+    at[x] = lds_address(values) + row * T::kRow + 16 * T::value_chunk(2 * (2 * x + side), row) + 8 * piece;
+  bf16x8 v[kBlocks][2][D / 32];
+  read_values<D, 0>(v[0], at);
+  if constexpr (kBlocks == 2) read_values<D, 32 * T::kRow>(v[kBlocks - 1], at);
   if (masked) {
     // key - first key of the step = 32 x + 8 (e / 4) + 4 half + e % 4; `rel` is the
     // row's position less the step's first key
@@ -421,25 +458,11 @@ __device__ __forceinline__ void attend(Rows<D>& r, const bf16x8 (&q)[D / 16], co
       w[2 * x + h] = __builtin_bit_cast(bf16x8, b);
     }
   }
-  // Lane group lane / 16 reads rows 4 half .. + 3 of 16 columns: lane's row and piece there.
-  const int row = 4 * half + ((lane & 15) >> 2), piece = lane & 3, side = (lane >> 4) & 1;
-  uint32_t at[D / 32];
 #pragma unroll
-  for (int x = 0; x < D / 32; ++x)
-    at[x] = lds_address(values) + row * T::kRow + 16 * T::value_chunk(2 * (2 * x + side), row) + 8 * piece;
-  auto product = [&](auto step) __attribute__((always_inline)) {
-    constexpr int t = decltype(step)::value;
-    bf16x8 v[D / 32];
-    read_values<D, 16 * t * T::kRow>(v, at);
+  for (int t = 0; t < 2 * kBlocks; ++t)
 #pragma unroll
-    for (int x = 0; x < D / 32; ++x) r.o[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[x], w[t], r.o[x], 0, 0, 0);
-  };
-  product(std::integral_constant<int, 0>{});
-  product(std::integral_constant<int, 1>{});
-  if constexpr (kBlocks == 2) {
-    product(std::integral_constant<int, 2>{});
-    product(std::integral_constant<int, 3>{});
-  }
+    for (int x = 0; x < D / 32; ++x)
+      r.o[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[t / 2][t % 2][x], w[t], r.o[x], 0, 0, 0);
 }
 
 // A tile's output or partial sums. kWaves row groups of 32 in a tile. Partial layout per
@@ -545,6 +568,9 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
         const uint8_t* const at = lds + (i & 1) * 2 * kTileBytes;
         attend<D, 2>(o, q, at, at + kTileBytes, p.scale, masked, position - key0, p.window, now);
       }
+      // one set of registers for the output whether the step was the wave's or not (else it is copied)
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) asm volatile("" : "+v"(o.o[x]));
     }
 
     const bool whole = count == tile_count;
