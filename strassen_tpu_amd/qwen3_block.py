@@ -21,6 +21,11 @@ fused epilogue (the reference's ``cubic_matmul`` takes none), SwiGLU and the
 residual adds as torch ops, and q, k and v on hipBLASLt with torch's norms
 and RoPE. Weights are random-init (there is no network to fetch
 checkpoints); a caller may supply real ones through ``BlockWeights``.
+
+``ServingBlock`` and ``block_step`` run the same block as a serving step: requests of
+ragged lengths append new tokens to a paged key/value cache (``paged.py``), which
+the reference's layer does not have. Their ``"int4"`` arm keeps the projections in
+4 bits (``int4.py``).
 """
 
 from __future__ import annotations
@@ -31,15 +36,18 @@ import torch
 from torch.utils._python_dispatch import _get_current_dispatch_mode
 
 from . import _lib
+from .int4 import int4_matmul, int4_quantize, int4_weight_layout
 from .layouts import (rope_layout_tables, rope_layout_to_heads, rope_scale_layout, rope_weight_layout,
                       swiglu_weight_layout)
 from .packing import cubic_weight_layout, pack_activation, strassen_weight_layout
+from .paged import paged_attention, paged_write
 from .strassen import cubic_matmul, strassen_matmul
 
 __all__ = ["Qwen3Dims", "QWEN3_32B", "BlockWeights", "PreparedBlock", "rms_norm", "apply_rope", "rope_values",
-           "attention", "block_forward", "ARMS"]
+           "attention", "block_forward", "ARMS", "ServingBlock", "block_step", "SERVING_ARMS"]
 
 ARMS = ("strassen", "cubic", "hipblaslt", "cubic_unfused")
+SERVING_ARMS = ("strassen", "cubic", "int4")
 
 
 @dataclasses.dataclass(frozen=True)
@@ -270,3 +278,62 @@ def block_forward(x, block):
     normalized = _row_rms_norm(residual, w.mlp_norm, d.eps)
     activated = block.gemm(normalized, block.gate_up, epilogue="swiglu")
     return block.gemm(activated, block.mlp_down, epilogue="residual_add", residual=residual)
+
+
+class ServingBlock:
+    """A block's weights laid out for ``block_step``, built once and kept on the device.
+
+    The query, key and value projections are one product. ``arm`` "strassen" and "cubic" pack
+    the weights for tiles of ``(bn, bk)`` columns and K; "int4" quantises them in groups of
+    ``group`` (``int4_quantize``). ``max_context`` positions have RoPE tables."""
+
+    def __init__(self, weights, dims, arm, *, max_context, tile=(1024, 512), group=128):
+        if arm not in SERVING_ARMS:
+            raise ValueError(f"unknown arm {arm!r}; expected one of {SERVING_ARMS}")
+        self.weights, self.dims, self.arm, self.tile = weights, dims, arm, tuple(tile)
+        self.max_context = int(max_context)
+        self.cos, self.sin = rope_values(self.max_context, dims.head_dim, dims.theta, weights.query.device)
+        qkv = torch.cat((weights.query, weights.key, weights.value), dim=1)
+        if arm == "int4":
+            def pack(w, epilogue=None):
+                codes, scales, zeros = int4_quantize(w, group)
+                return int4_weight_layout(codes, scales, zeros, group=group, epilogue=epilogue)
+
+            self.gate_up = pack(weights.gate_up, "swiglu")
+        else:
+            bn, bk = self.tile
+            layout = strassen_weight_layout if arm == "strassen" else cubic_weight_layout
+
+            def pack(w):
+                return layout(w, bn, bk)
+
+            self.gate_up = pack(swiglu_weight_layout(weights.gate_up, bn))
+        self.qkv, self.attention_output, self.mlp_down = (
+            pack(w) for w in (qkv, weights.attention_output, weights.mlp_down))
+
+    def product(self, x, w, **kw):
+        if self.arm == "int4":
+            return int4_matmul(x, w, **kw)
+        # the largest row tile that the step's rows fill whole
+        bm = next((m for m in (1024, 512, 256) if x.shape[0] % m == 0), 16)
+        matmul = strassen_matmul if self.arm == "strassen" else cubic_matmul
+        return matmul(x, w, bm=bm, bn=self.tile[0], bk=self.tile[1], **kw)
+
+
+def block_step(x, block, k_cache, v_cache, plan, *, window=None):
+    """One serving step through a decoder block: ``x [plan.tokens, hidden]`` bf16 -> same
+    shape, the new tokens' keys and values stored in the layer's cache and attended to
+    together with those before them (``paged_plan``, ``paged_write``, ``paged_attention``).
+    The "strassen" and "cubic" arms take tokens in whole sixteens (the plan may have padding
+    rows). Rows of no admitted request pass through as rows of their own and touch no cache."""
+    d, w = block.dims, block.weights
+    normalized = _row_rms_norm(x, w.attention_norm, d.eps)
+    heads = block.product(normalized, block.qkv).view(plan.tokens, d.heads + 2 * d.kv_heads, d.head_dim)
+    query, key, value = heads.split((d.heads, d.kv_heads, d.kv_heads), dim=1)
+    query = paged_write(key, value, k_cache, v_cache, plan, q=query, rope_cos=block.cos, rope_sin=block.sin,
+                        q_scale=w.query_norm, k_scale=w.key_norm, eps=d.eps)
+    attended = paged_attention(query, k_cache, v_cache, plan, window=window).flatten(1)
+    residual = block.product(attended, block.attention_output, epilogue="residual_add", residual=x)
+    normalized = _row_rms_norm(residual, w.mlp_norm, d.eps)
+    activated = block.product(normalized, block.gate_up, epilogue="swiglu")
+    return block.product(activated, block.mlp_down, epilogue="residual_add", residual=residual)

@@ -64,6 +64,31 @@ def test_int4_matmul(m, k, n, group, zeros):
         assert torch.equal(smx.int4_matmul(view, laid), got)
 
 
+# each way the kernels run: x in LDS in eight and sixteen waves, more than half of LDS, x by wave; streamed
+# x of 16, 32 and 64 rows, K whole and in shares
+@pytest.mark.parametrize("m,k,n,group,epilogue", [
+    (1, 128, 32832, 128, None), (2, 256, 32900, 64, "swiglu"), (1, 8320, 34, 64, "swiglu"), (12, 5120, 70, 128, "residual_add"),
+    (16, 5120, 98, 32, "swiglu"), (15, 6016, 100, 64, "residual_add"), (16, 12800, 40, 128, "bias_add"), (9, 12832, 66, 32, "swiglu"),
+    (32, 2048, 98, 128, "swiglu"), (31, 12800, 1030, 64, "residual_add"), (32, 512, 96, 128, "swiglu"),
+    (61, 6400, 10300, 128, "swiglu"), (64, 25600, 2750, 64, "residual_add"), (128, 5152, 13200, 32, None)])
+def test_int4_launches(m, k, n, group, epilogue):
+    codes, scales, zero, w, spread, g = weight(k, n, group, True)
+    laid = smx.int4_weight_layout(codes, scales, zero, group=group, epilogue="swiglu" if epilogue == "swiglu" else None)
+    x = torch.randn(m, k, device=DEV, generator=g).to(torch.bfloat16)
+    extra = torch.randn(*((n,) if epilogue == "bias_add" else (m, n)), device=DEV, generator=g).to(torch.bfloat16)
+    options = {"residual_add": {"residual": extra}, "bias_add": {"bias": extra}}.get(epilogue, {})
+
+    def finish(y):
+        if epilogue == "swiglu":
+            gate, up = y.chunk(2, -1)
+            return gate * torch.sigmoid(gate) * up
+        return y + extra.double() if options else y
+
+    got = smx.int4_matmul(x, laid, epilogue=epilogue, **options)
+    check(got, x, w, spread, finish)
+    assert torch.equal(smx.int4_matmul(x, laid, epilogue=epilogue, **options), got)
+
+
 def test_int4_matmul_is_exact_on_whole_numbers():
     """Codes, zeros, scales of 1 and whole x: every sum is exact in FP32."""
     codes, _, zero, _, _, g = weight(640, 48, 64, True)
