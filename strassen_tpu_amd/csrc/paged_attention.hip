@@ -43,7 +43,8 @@ struct AttentionArgs {
   int64_t table_stride;
   const int32_t *starts, *rows, *context, *positions;
   int32_t requests, tokens, group, kv_heads, page_shift, num_pages, window, tile_tokens, zero_rows, min_span;
-  float scale;  // times log2 e
+  float scale;      // times log2 e
+  float per_group;  // 1 / group
   float* partial;
   int32_t* records;
 };
@@ -69,20 +70,27 @@ __device__ int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
   return sum;
 }
 
-// The row tiles of one request and the key tiles (of kKeys keys) that each sees.
-template <int kKeys>
+// A plan's lengths, read through the scalar cache where the index is a wave's.
+__device__ __forceinline__ int32_t scalar_at(const int32_t* p, int i) {
+  return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p)[i];
+}
+
+// The row tiles of one request and the key tiles (of kKeys keys) that each sees. An item (one of
+// them) counts kItem units of work before its key tiles, for its start and end: queries to load,
+// the first keys to wait for, the result to store.
+template <int kKeys, int kItem>
 struct Request {
   int32_t context, fresh, per_tile, window, tiles;
 
-  __device__ Request(const AttentionArgs& p, int b)
-      : context(p.context[b]), fresh(p.rows[b]), per_tile(p.tile_tokens), window(p.window) {
+  __device__ Request(const AttentionArgs& p, int32_t context_, int32_t fresh_)
+      : context(context_), fresh(fresh_), per_tile(p.tile_tokens), window(p.window) {
     tiles = (fresh + per_tile - 1) / per_tile;
   }
+  __device__ Request(const AttentionArgs& p, int b) : Request(p, p.context[b], p.rows[b]) {}
   // The request that a whole wave works on: its lengths in scalar registers, on which the
   // page buffers' descriptors depend.
   __device__ static Request uniform(const AttentionArgs& p, int b) {
-    Request r(p, b);
-    r.context = __builtin_amdgcn_readfirstlane(r.context), r.fresh = __builtin_amdgcn_readfirstlane(r.fresh);
+    Request r(p, scalar_at(p.context, b), scalar_at(p.rows, b));
     r.tiles = __builtin_amdgcn_readfirstlane(r.tiles);
     return r;
   }
@@ -91,10 +99,10 @@ struct Request {
   }
   __device__ int last(int t) const { return (context + min(fresh, (t + 1) * per_tile) + kKeys - 1) / kKeys; }
   __device__ int count(int t) const { return last(t) - first(t); }
-  // Key tiles of the row tiles before t < tiles.
+  // Units of the row tiles before t < tiles.
   __device__ int64_t before(int t) const {
     if (!t) return 0;
-    int64_t sum = floor_sum(t, kKeys, per_tile, context + per_tile + kKeys - 1);
+    int64_t sum = (int64_t)t * kItem + floor_sum(t, kKeys, per_tile, context + per_tile + kKeys - 1);
     if (window) {
       const int x = context - window + 1;  // first(s) = max(0, x + s per_tile) / kKeys
       const int skip = x >= 0 ? 0 : (-x + per_tile - 1) / per_tile;
@@ -102,16 +110,35 @@ struct Request {
     }
     return sum;
   }
-  __device__ int64_t all() const { return fresh > 0 ? before(tiles - 1) + count(tiles - 1) : 0; }
+  __device__ int64_t all() const { return fresh > 0 ? before(tiles - 1) + kItem + count(tiles - 1) : 0; }
 };
 
-// A workgroup's span of the key tiles, and the item in which it begins.
+// A workgroup's span of the units, and the item in which it begins.
 struct Span {
-  int64_t left;         // key tiles to do
-  int64_t each;         // key tiles of a span
+  int64_t left;         // units to do
+  int64_t each;         // units of a span
   int64_t begin;        // of this one, over all key/value heads
   int32_t worker;       // which span this is
-  int32_t head, request, tile, skip;  // skip: key tiles of that item done by others
+  int32_t head, request, tile, skip;  // skip: units of that item that lie in spans before
+};
+
+// The span's part of one item: its first step (key tile), its steps and units.
+template <int kKeys, int kItem>
+struct Part {
+  Request<kKeys, kItem> r;
+  int head, request, tile;
+  int from, count, tile_count;  // steps of the part, and of the whole item
+  int units, rest;              // of the part; of the item behind it
+  bool begins;                  // no span before has steps of the item
+
+  __device__ __forceinline__ Part(const AttentionArgs& p, const Span& s)
+      : r(Request<kKeys, kItem>::uniform(p, s.request)), head(s.head), request(s.request), tile(s.tile) {
+    tile_count = r.count(tile);
+    units = (int)min((int64_t)(tile_count + kItem - s.skip), s.left);
+    rest = tile_count + kItem - s.skip - units;
+    const int before = max(0, s.skip - kItem), upto = max(0, s.skip + units - kItem);
+    from = r.first(tile) + before, count = upto - before, begins = before == 0;
+  }
 };
 
 __device__ __forceinline__ int64_t wave_sum(int64_t x) {
@@ -123,6 +150,15 @@ __device__ __forceinline__ int64_t wave_sum(int64_t x) {
 __device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
   return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, lane) |
          (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
+}
+
+// a / b for 0 <= a < 2^52 and 0 < b, through the floating-point reciprocal (the integer
+// division is ten times as long).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  int64_t q = (int64_t)((double)a / (double)b);
+  if (q * b > a) --q;
+  if ((q + 1) * b <= a) ++q;
+  return q;
 }
 
 // Inclusive sum of x over a wave's lanes.
@@ -137,57 +173,52 @@ __device__ __forceinline__ int64_t wave_scan(int64_t x) {
 
 // Finds the workgroup's span (kWaves waves, uniform result). Consecutive spans lie
 // on one XCD, whose L2 then serves one key/value head's pages at a time.
-template <int kKeys, int kWaves>
+template <int kKeys, int kItem, int kWaves>
 __device__ bool find_span(const AttentionArgs& p, Span* s) {
   constexpr int kThreads = 64 * kWaves;
   __shared__ int64_t waves[kWaves], found_rest;
   __shared__ int32_t found;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t total = 0;
-  for (int b = threadIdx.x; b < p.requests; b += kThreads) total += Request<kKeys>(p, b).all();
-  total = lane_value(wave_scan(total), 63);
-  if constexpr (kWaves > 1) {
-    if (lane == 0) waves[wave] = total;
+  // Inclusive sum over the workgroup of this thread's request among kThreads of them.
+  int64_t mine = 0, upto = 0;
+  auto scan = [&](int first) -> int64_t {
+    const int b = first + (int)threadIdx.x;
+    mine = b < p.requests ? Request<kKeys, kItem>(p, b).all() : 0;
+    upto = wave_scan(mine);
+    if constexpr (kWaves == 1) return lane_value(upto, 63);
     __syncthreads();
-    total = 0;
-    for (int w = 0; w < kWaves; ++w) total += waves[w];
-    total = lane_value(total, 0);
-  }
+    if (lane == 63) waves[wave] = upto;
+    __syncthreads();
+    int64_t all = 0;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) upto += waves[w];
+      all += waves[w];
+    }
+    return lane_value(all, 0);
+  };
+  int64_t total = 0;
+  for (int first = 0; first < p.requests; first += kThreads) total += scan(first);
   const int64_t everything = total * p.kv_heads;
-  s->each = max((int64_t)p.min_span, (everything + gridDim.x - 1) / gridDim.x);
-  const int64_t spans = (everything + s->each - 1) / s->each, per_xcd = (spans + 7) / 8;
+  s->each = max((int64_t)p.min_span, quotient(everything + gridDim.x - 1, gridDim.x));
+  const int64_t spans = quotient(everything + s->each - 1, s->each), per_xcd = (spans + 7) / 8;
   s->worker = (int)((blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3));
   if ((blockIdx.x >> 3) >= per_xcd || s->worker >= spans) return false;
   s->begin = (int64_t)s->worker * s->each;
   s->left = min(s->each, everything - s->begin);
-  s->head = __builtin_amdgcn_readfirstlane((int)(s->begin / total));
+  s->head = __builtin_amdgcn_readfirstlane((int)quotient(s->begin, total));
   const int64_t at = s->begin - (int64_t)s->head * total;
 
   int64_t base = 0, rest = 0;
   for (int first = 0; first < p.requests; first += kThreads) {
-    const int b = first + (int)threadIdx.x;
-    const int64_t mine = b < p.requests ? Request<kKeys>(p, b).all() : 0;
-    int64_t upto = wave_scan(mine), all;
+    // (the sums of a single round are still there)
+    const int64_t all = p.requests <= kThreads ? total : scan(first);
+    const bool here = at >= base + upto - mine && at < base + upto;
     if constexpr (kWaves > 1) {
-      __syncthreads();
-      if (lane == 63) waves[wave] = upto;
-      __syncthreads();
-      all = 0;
-      for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) upto += waves[w];
-        all += waves[w];
-      }
-    } else {
-      all = lane_value(upto, 63);
-    }
-    upto += base;
-    const bool here = at >= upto - mine && at < upto;
-    if constexpr (kWaves > 1) {
-      if (here) found = b, found_rest = at - (upto - mine);
+      if (here) found = first + (int)threadIdx.x, found_rest = at - (base + upto - mine);
     } else if (const uint64_t who = __ballot(here)) {
       const int l = __builtin_ctzll(who);
       s->request = first + l;
-      rest = at - lane_value(upto - mine, l);
+      rest = at - (base + lane_value(upto - mine, l));
     }
     base += all;
     if (at < base) break;  // uniform
@@ -197,7 +228,7 @@ __device__ bool find_span(const AttentionArgs& p, Span* s) {
     s->request = __builtin_amdgcn_readfirstlane(found);
     rest = lane_value(found_rest, 0);
   }
-  const auto r = Request<kKeys>::uniform(p, s->request);
+  const auto r = Request<kKeys, kItem>::uniform(p, s->request);
   int low = 0, high = r.tiles;  // the last tile with before(tile) <= rest
   while (high - low > 1) {
     const int mid = (low + high) >> 1;
@@ -215,10 +246,15 @@ __device__ __forceinline__ void next_item(const AttentionArgs& p, Span* s, int t
   s->tile = 0;
   do {
     if (++s->request == p.requests) s->request = 0, ++s->head;
-  } while (__builtin_amdgcn_readfirstlane(p.rows[s->request]) <= 0);
+  } while (scalar_at(p.rows, s->request) <= 0);
 }
 
-// Rows that belong to no request are zeroed on the way.
+// Row r of a tile belongs to its token r / group; exact for rows below 2^12.
+__device__ __forceinline__ int row_token(int row, const AttentionArgs& p) {
+  return (int)(((float)row + 0.5f) * p.per_group);
+}
+
+// Rows that belong to no request are zeroed behind the work.
 template <int D, int kThreads>
 __device__ __forceinline__ void clear_rows(const AttentionArgs& p) {
   if (!p.zero_rows) return;
@@ -415,15 +451,21 @@ __device__ __forceinline__ void attend(Rows<D>& r, const bf16x8 (&q)[D / 16], co
     // key - first key of the step = 32 x + 8 (e / 4) + 4 half + e % 4; `rel` is the
     // row's position less the step's first key
     const int mine = rel - 4 * half;
-    const uint64_t bits = held >> (4 * half);
 #pragma unroll
     for (int x = 0; x < kBlocks; ++x)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int key = 32 * x + 8 * (e >> 2) + (e & 3);
-        const bool ok = key <= mine && (!window || key > mine - window) && ((bits >> key) & 1);
-        s[x][e] = ok ? s[x][e] : -INFINITY;
-      }
+      for (int e = 0; e < 16; ++e) s[x][e] = 32 * x + 8 * (e >> 2) + (e & 3) <= mine ? s[x][e] : -INFINITY;
+    if (window || held != (kBlocks == 2 ? ~0ull : 0xffffffffull)) {
+      const int oldest = window ? mine - window : -(1 << 30);
+      const uint64_t bits = held >> (4 * half);
+#pragma unroll
+      for (int x = 0; x < kBlocks; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = 32 * x + 8 * (e >> 2) + (e & 3);
+          s[x][e] = key > oldest && ((bits >> key) & 1) ? s[x][e] : -INFINITY;
+        }
+    }
   }
   float top = s[0][0];
 #pragma unroll
@@ -503,100 +545,137 @@ __device__ __forceinline__ float inverse_of(float sum) { return sum > 0.f ? 1.f 
 template <int D>
 __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
   using T = Tile<D>;
-  constexpr int kKeys = 64;
+  constexpr int kKeys = 64, kItem = 3;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   constexpr int kTileBytes = kKeys * T::kRow;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
 
-  clear_rows<D, 256>(p);
   Record* const record = reinterpret_cast<Record*>(p.records) + blockIdx.x;
   if (threadIdx.x == 0) record->others = 0;
   Span s;
-  if (!find_span<kKeys, 4>(p, &s)) return;
+  if (!find_span<kKeys, kItem, 4>(p, &s)) return clear_rows<D, 256>(p);
 
   const Lanes<D, 16> lanes(p.slot_stride);
 
-  while (s.left > 0) {
-    const auto r = Request<kKeys>::uniform(p, s.request);
-    const int tile_first = r.first(s.tile), tile_count = r.count(s.tile);
-    const int count = (int)min((int64_t)(tile_count - s.skip), s.left);
-    const int from = tile_first + s.skip;
-    const int tile_tokens = min(r.per_tile, r.fresh - s.tile * r.per_tile), tile_rows = tile_tokens * p.group;
-    const int row = min(32 * wave + (lane & 31), tile_rows - 1);
-    const int local = s.tile * r.per_tile + row / p.group, head = s.head * p.group + row % p.group;
-    const int64_t token = p.starts[s.request] + local;
-    const int position = r.context + local;
-    const int length = r.context + r.fresh;
-    // positions of the wave's first and last row
-    const int low = __builtin_amdgcn_readfirstlane(position);
-    const int high = __builtin_amdgcn_readlane(position, 31);
-    const bool active = 32 * wave < tile_rows;  // rows of its own
-    const int32_t* const table = p.tables + s.request * p.table_stride;
-
-    bf16x8 q[D / 16];
-    const uint16_t* const q_row = p.q + token * p.q_token + head * p.q_head + 8 * half;
+  using Part = Part<kKeys, kItem>;
+  // lane l's page of a step: that of its key 64 step + l
+  auto pages_of = [&](const Part& w, int step) __attribute__((always_inline)) {
+    const int key = min(step * kKeys + lane, w.r.context + w.r.fresh - 1);
+    return p.tables[w.request * p.table_stride + (key >> p.page_shift)];
+  };
+  auto fetch = [&](const Part& w, int step, int pages, int buffer) __attribute__((always_inline)) {
+    uint8_t* const to = lds + buffer * 2 * kTileBytes + 16 * wave * T::kRow;
+    lanes.fetch(p, w.head, step * kKeys + 16 * wave, w.r.context + w.r.fresh, pages, 16 * wave, to, to + kTileBytes);
+  };
+  auto held_of = [&](int pages) __attribute__((always_inline)) { return __ballot((uint32_t)pages < (uint32_t)p.num_pages); };
+  // this lane's row of an item: its token within the request and its query head
+  auto row_of = [&](const Part& w, int* local, int* head) __attribute__((always_inline)) {
+    const int rows = min(w.r.per_tile, w.r.fresh - w.tile * w.r.per_tile) * p.group;
+    const int row = min(32 * wave + (lane & 31), rows - 1), token = row_token(row, p);
+    *local = w.tile * w.r.per_tile + token, *head = w.head * p.group + row - token * p.group;
+    return rows;
+  };
+  bf16x8 q[D / 16];
+  auto load_q = [&](const Part& w) __attribute__((always_inline)) {
+    int local, head;
+    row_of(w, &local, &head);
+    const int64_t token = scalar_at(p.starts, w.request) + local;
+    const uint16_t* const from = p.q + token * p.q_token + head * p.q_head + 8 * half;
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) q[t] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q_row + 16 * t));
+    for (int t = 0; t < D / 16; ++t) q[t] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(from + 16 * t));
+  };
 
-    Rows<D> o;
-    o.clear();
-    // lane l's page of a step: that of its key 64 step + l
-    auto pages_of = [&](int step) __attribute__((always_inline)) {
-      return table[min(step * kKeys + lane, length - 1) >> p.page_shift];
-    };
-    auto fetch = [&](int step, int pages, int buffer) __attribute__((always_inline)) {
-      uint8_t* const to = lds + buffer * 2 * kTileBytes + 16 * wave * T::kRow;
-      lanes.fetch(p, s.head, step * kKeys + 16 * wave, length, pages, 16 * wave, to, to + kTileBytes);
-    };
-    int pages = pages_of(from);
-    uint64_t held = __ballot((uint32_t)pages < (uint32_t)p.num_pages);
-    packed::stage_barrier<0>();  // the item before is done with the buffers
-    fetch(from, pages, 0);
-    int next_pages = pages_of(from + 1);
-    for (int i = 0; i < count; ++i) {
-      const int step = from + i;
-      packed::stage_barrier<0>();
-      const uint64_t now = held;
-      if (i + 1 < count) {
-        held = __ballot((uint32_t)next_pages < (uint32_t)p.num_pages);
-        fetch(step + 1, next_pages, (i + 1) & 1);
-        next_pages = pages_of(step + 2);
-      }
-      const int key0 = step * kKeys;
-      if (active && key0 <= high && (!p.window || key0 + kKeys - 1 > low - p.window)) {
-        const bool masked = key0 + kKeys - 1 > low || (p.window && key0 <= high - p.window) || now != ~0ull;
-        const uint8_t* const at = lds + (i & 1) * 2 * kTileBytes;
-        attend<D, 2>(o, q, at, at + kTileBytes, p.scale, masked, position - key0, p.window, now);
-      }
-      // one set of registers for the output whether the step was the wave's or not (else it is copied)
-#pragma unroll
-      for (int x = 0; x < D / 32; ++x) asm volatile("" : "+v"(o.o[x]));
+  // One stream of steps over all parts: while a step is computed the next one's DMAs are on
+  // their way, whichever part it belongs to, and the pages of the one after that are looked up.
+  // A part may end before its first step (all of its units lie before them): it is passed over.
+  auto next_part = [&]() __attribute__((always_inline)) {
+    Part w(p, s);
+    while (!w.count && s.left > w.units) {
+      s.left -= w.units;
+      next_item(p, &s, w.r.tiles);
+      w = Part(p, s);
     }
-
-    const bool whole = count == tile_count;
-    const float sum = o.sum + other_half(o.sum);
-    if (whole) {
-      store_rows<D>(p, o.o, inverse_of(sum), 32 * wave + (lane & 31) < tile_rows, token, head);
-    } else {
-      float* const to = p.partial + (2 * (int64_t)s.worker + (s.skip == 0)) * kPartialFloats<D>;
+    return w;
+  };
+  Part part = next_part(), next = part;
+  if (part.count) {
+    int pages = pages_of(part, part.from);
+    uint64_t held = held_of(pages);
+    load_q(part);
+    fetch(part, part.from, pages, 0);
+    if (part.count > 1) pages = pages_of(part, part.from + 1);
+    int buffer = 0;
+    for (;;) {
+      int local, head;
+      const int tile_rows = row_of(part, &local, &head);
+      const int position = part.r.context + local;
+      // positions of the wave's first and last row
+      const int low = __builtin_amdgcn_readfirstlane(position), high = __builtin_amdgcn_readlane(position, 31);
+      const bool active = 32 * wave < tile_rows;  // rows of its own
+      bool more = s.left > part.units;
+      Rows<D> o;
+      o.clear();
+      for (int i = 0; i < part.count; ++i) {
+        const int step = part.from + i;
+        packed::stage_barrier<0>();
+        const uint64_t now = held;
+        const bool ends = i + 1 == part.count;
+        if (more && (ends ? part.count == 1 : i + 2 == part.count)) {
+          s.left -= part.units;
+          next_item(p, &s, part.r.tiles);
+          next = next_part();
+          more = next.count > 0;
+          if (more && ends) pages = pages_of(next, next.from);
+        }
+        if (!ends) {
+          held = held_of(pages);
+          fetch(part, step + 1, pages, buffer ^ 1);
+          if (i + 2 < part.count)
+            pages = pages_of(part, step + 2);
+          else if (more)
+            pages = pages_of(next, next.from);
+        } else if (more) {
+          held = held_of(pages);
+          fetch(next, next.from, pages, buffer ^ 1);
+          if (next.count > 1) pages = pages_of(next, next.from + 1);
+        }
+        const int key0 = step * kKeys;
+        if (active && key0 <= high && (!p.window || key0 + kKeys - 1 > low - p.window)) {
+          const bool masked = key0 + kKeys - 1 > low || (p.window && key0 <= high - p.window) || now != ~0ull;
+          const uint8_t* const at = lds + buffer * 2 * kTileBytes;
+          attend<D, 2>(o, q, at, at + kTileBytes, p.scale, masked, position - key0, p.window, now);
+        }
+        buffer ^= 1;
+        // one set of registers for the output whether the step was the wave's or not (else it is copied)
 #pragma unroll
-      for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          reinterpret_cast<f32x4*>(to)[(4 * x + e) * 256 + threadIdx.x] =
-              f32x4{o.o[x][4 * e], o.o[x][4 * e + 1], o.o[x][4 * e + 2], o.o[x][4 * e + 3]};
-      to[256 * (D / 2) + threadIdx.x] = o.top;
-      to[256 * (D / 2 + 1) + threadIdx.x] = sum;
-      if (s.skip == 0 && threadIdx.x == 0) {
-        record->worker = s.worker, record->head = s.head, record->request = s.request, record->tile = s.tile;
-        // the item goes on for tile_count - count key tiles in the spans behind this one
-        record->others = (int)((tile_count - count + s.each - 1) / s.each);
+        for (int x = 0; x < D / 32; ++x) asm volatile("" : "+v"(o.o[x]));
       }
+      if (more) load_q(next);
+
+      const float sum = o.sum + other_half(o.sum);
+      if (part.count == part.tile_count) {
+        store_rows<D>(p, o.o, inverse_of(sum), 32 * wave + (lane & 31) < tile_rows, scalar_at(p.starts, part.request) + local, head);
+      } else {
+        float* const to = p.partial + (2 * (int64_t)s.worker + part.begins) * kPartialFloats<D>;
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            reinterpret_cast<f32x4*>(to)[(4 * x + e) * 256 + threadIdx.x] =
+                f32x4{o.o[x][4 * e], o.o[x][4 * e + 1], o.o[x][4 * e + 2], o.o[x][4 * e + 3]};
+        to[256 * (D / 2) + threadIdx.x] = o.top;
+        to[256 * (D / 2 + 1) + threadIdx.x] = sum;
+        if (part.begins && threadIdx.x == 0) {
+          record->worker = s.worker, record->head = part.head, record->request = part.request, record->tile = part.tile;
+          // the item goes on in the spans behind this one
+          record->others = (int)quotient(part.rest + s.each - 1, s.each);
+        }
+      }
+      if (!more) break;
+      part = next;
     }
-    s.left -= count;
-    if (s.left <= 0) break;
-    next_item(p, &s, r.tiles);
   }
+  clear_rows<D, 256>(p);
 }
 
 // Steps of few rows (decoding): a workgroup is one wave with 32 rows a tile, which streams 32
@@ -606,31 +685,35 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
 template <int D>
 __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
   using T = Tile<D>;
-  constexpr int kKeys = 32, kDmas = kKeys / T::kDmaRows, kTileBytes = kKeys * T::kRow;
+  constexpr int kKeys = 32, kItem = 1, kDmas = kKeys / T::kDmaRows, kTileBytes = kKeys * T::kRow;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x, half = lane >> 5;
 
-  clear_rows<D, 64>(p);
   Record* const record = reinterpret_cast<Record*>(p.records) + blockIdx.x;
   if (lane == 0) record->others = 0;
   Span s;
-  if (!find_span<kKeys, 1>(p, &s)) return;
+  if (!find_span<kKeys, kItem, 1>(p, &s)) return clear_rows<D, 64>(p);
 
   const Lanes<D, kKeys> lanes(p.slot_stride);
 
   while (s.left > 0) {
-    const auto r = Request<kKeys>::uniform(p, s.request);
-    const int tile_first = r.first(s.tile), tile_count = r.count(s.tile);
-    const int count = (int)min((int64_t)(tile_count - s.skip), s.left);
-    const int from = tile_first + s.skip;
-    const int tile_rows = min(r.per_tile, r.fresh - s.tile * r.per_tile) * p.group;
-    const int row = min(lane & 31, tile_rows - 1);
-    const int local = s.tile * r.per_tile + row / p.group, head = s.head * p.group + row % p.group;
-    const int64_t token = p.starts[s.request] + local;
+    const Part<kKeys, kItem> part(p, s);
+    const auto& r = part.r;
+    const int count = part.count, from = part.from;
+    if (!count) {  // all of its units lie before its first step
+      s.left -= part.units;
+      if (s.left <= 0) break;
+      next_item(p, &s, r.tiles);
+      continue;
+    }
+    const int tile_rows = min(r.per_tile, r.fresh - part.tile * r.per_tile) * p.group;
+    const int row = min(lane & 31, tile_rows - 1), in = row_token(row, p);
+    const int local = part.tile * r.per_tile + in, head = part.head * p.group + row - in * p.group;
+    const int64_t token = scalar_at(p.starts, part.request) + local;
     const int position = r.context + local, length = r.context + r.fresh;
     const int low = __builtin_amdgcn_readfirstlane(position), high = __builtin_amdgcn_readlane(position, 31);
     const bool valid = (lane & 31) < tile_rows;
-    const int32_t* const table = p.tables + s.request * p.table_stride;
+    const int32_t* const table = p.tables + part.request * p.table_stride;
 
     // lane l's page of a step: that of its key l % 32 of the step
     auto pages_of = [&](int step) __attribute__((always_inline)) {
@@ -671,10 +754,10 @@ __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
     }
 
     const float sum = o.sum + other_half(o.sum);
-    if (count == tile_count) {
+    if (count == part.tile_count) {
       store_rows<D>(p, o.o, inverse_of(sum), valid, token, head);
     } else {
-      float* const to = p.partial + (2 * (int64_t)s.worker + (s.skip == 0)) * kFewPartialFloats<D>;
+      float* const to = p.partial + (2 * (int64_t)s.worker + part.begins) * kFewPartialFloats<D>;
       if (valid) {
 #pragma unroll
         for (int x = 0; x < D / 32; ++x)
@@ -687,17 +770,18 @@ __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
           to[32 * D + 32 + row] = sum;
         }
       }
-      if (s.skip == 0 && lane == 0) {
-        record->worker = s.worker, record->head = s.head, record->request = s.request, record->tile = s.tile;
-        record->others = (int)((tile_count - count + s.each - 1) / s.each);
+      if (part.begins && lane == 0) {
+        record->worker = s.worker, record->head = part.head, record->request = part.request, record->tile = part.tile;
+        record->others = (int)quotient(part.rest + s.each - 1, s.each);
       }
     }
-    s.left -= count;
+    s.left -= part.units;
     if (s.left <= 0) break;
     next_item(p, &s, r.tiles);
   }
   // no DMA outlives the wave
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  clear_rows<D, 64>(p);
 }
 
 // Adds up the partial sums of paged_attend_few: a workgroup per record, a thread per
@@ -872,8 +956,9 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
   const bool few = few_rows(step->max_new, p.group);
   const int blocks = workgroups(cus, few);
   p.tile_tokens = (few ? 32 : 128) / p.group;
-  p.min_span = few ? 4 : 2;
+  p.min_span = few ? 3 : 5;
   p.scale = scale * 1.44269504088896341f;
+  p.per_group = 1.f / p.group;
   p.records = (int32_t*)workspace;
   p.partial = (float*)((char*)workspace + blocks * kRecordBytes);
   return cache->head_dim == 128 ? launch_attention<128>(p, few, blocks, (hipStream_t)stream)
