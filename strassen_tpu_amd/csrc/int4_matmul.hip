@@ -263,12 +263,13 @@ __global__ __launch_bounds__(kWaves * 64) void int4_few(Int4Args p) {
 // column tiles each, times kWays that take the K tiles of a stage, one each. All share the stage's
 // rows of x in LDS (brought by DMA, kRing stages around); a row's 16-byte chunks are XORed with
 // its low bits, so that 8 rows of one chunk lie on different banks. Codes go to registers. A K
-// tile is a chain of MFMAs and vector work that fills a quarter to half of a SIMD: the
-// ways overlap it (with one way, 64 workgroups took 18.4 us for 16 rows of a 5120 x 8192
-// weight, whatever was in flight). blockIdx: columns, shares of K, row blocks.
+// tile is a chain of MFMAs and vector work that fills a quarter to half of a SIMD, which the
+// ways overlap; two of them leave room for two workgroups a CU (16 rows of a 5120 x
+// 51200 weight: 32.0 us, with four ways 34.7; 61 rows: 57, with one way 81). blockIdx: columns, shares
+// of K, row blocks.
 template <int kRows>
 struct Ring {
-  static constexpr int kWays = kRows == 4 ? 2 : 4, kRing = kRows == 1 ? 4 : 3;
+  static constexpr int kWays = 2, kRing = kRows == 1 ? 4 : 3;
   static constexpr int kThreads = 256 * kWays, kTileBytes = kRows * 4096, kStage = kWays * kTileBytes;
   static constexpr int kDmas = kRows;      // a wave's for one stage, of 1 KB
   static constexpr int kLoads = 4 + kDmas;  // and its codes and scales
@@ -424,20 +425,20 @@ Int4Plan int4_plan(int64_t m, int64_t k_tiles, int64_t tiles, bool gated, int cu
       return plan;
     }
     // Short K and no more columns than that: each wave its own x (16 rows, 5120 x 8192: 9.6,
-    // int4_tiled 13.0; but 25600 x 5120: 31 and 21.7)
+    // int4_tiled 11.8; but 25600 x 5120: 31 and 21.2)
     if (k_tiles <= 64 && tiles <= 4 * cus) {
       plan.waves = 8, plan.cols = 2;
       return plan;
     }
   }
-  // 64 rows a workgroup read and widen the weight once for all of them (61 rows, 5120 x 51200: 60, with
-  // 32 rows 76); small weights have the workgroups rather (5120 x 1024: 11.1 and 9.8).
+  // 64 rows a workgroup read and widen the weight once for all of them (61 rows, 5120 x 51200: 57, with
+  // 32 rows 70); small weights have the workgroups rather (5120 x 8192: 17.5 and 15.8).
   plan.rows = m <= 16 ? 1 : m <= 32 || tiles * k_tiles <= 128 * cus ? 2 : 4;
   const int64_t blocks = (tiles + 7) / 8 * ((m + 16 * plan.rows - 1) / (16 * plan.rows));
   // K in shares of whole stages, up to a workgroup a CU (more only make more sums to join); a
-  // weight of two stages is not worth the second launch
-  const int64_t stage = plan.rows == 4 ? 2 : 4, stages = (k_tiles + stage - 1) / stage;
-  const int64_t shares = stages <= 2 ? 1 : max((int64_t)1, min(cus / blocks, stages));
+  // weight of four stages is not worth the second launch
+  const int64_t stage = 2, stages = (k_tiles + stage - 1) / stage;
+  const int64_t shares = stages <= 4 ? 1 : max((int64_t)1, min(cus / blocks, stages));
   const int64_t each = (stages + shares - 1) / shares;
   plan.share = (int)(each * stage);
   plan.shares = (int)((stages + each - 1) / each);
@@ -470,7 +471,7 @@ int launch_int4(const Int4Plan& plan, Int4Args p, hipStream_t s) {
   const dim3 grid((unsigned)((p.tiles + 7) / 8), (unsigned)plan.shares, (unsigned)((p.m + 16 * plan.rows - 1) / (16 * plan.rows)));
   auto kern = plan.rows == 1 ? int4_tiled<1, kGroups, kZeros> : plan.rows == 2 ? int4_tiled<2, kGroups, kZeros> : int4_tiled<4, kGroups, kZeros>;
   const int lds = plan.rows == 1 ? Ring<1>::kLds : plan.rows == 2 ? Ring<2>::kLds : Ring<4>::kLds;
-  if (int rc = launch_int4_kernel(kern, grid, plan.rows == 4 ? 512 : 1024, lds, p, s)) return rc;
+  if (int rc = launch_int4_kernel(kern, grid, 512, lds, p, s)) return rc;
   if (plan.shares == 1) return SMX_OK;
   const int64_t items = (int64_t)p.m * p.tiles * (p.epilogue == SMX_EPI_SWIGLU ? 2 : 4);
   hipLaunchKernelGGL(int4_join, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, p, plan.shares);

@@ -26,7 +26,7 @@ class Int4Operand:
     """A weight laid out by ``int4_weight_layout``."""
 
     def __init__(self, codes, scales, k, n, group, swiglu, zeros):
-        self.codes, self.scales = codes, scales
+        self.codes, self.scales, self.device = codes, scales, codes.device
         self.k, self.n, self.group, self.swiglu = k, n, group, swiglu
         self.desc = _lib.SmxInt4Weight(codes.data_ptr(), scales.data_ptr(), k, n, group, int(swiglu), int(zeros))
         self._workspace = {}  # bytes by number of rows, up to 64 of them
@@ -46,10 +46,6 @@ class Int4Operand:
     @property
     def shape(self):
         return self.k, self.n
-
-    @property
-    def device(self):
-        return self.codes.device
 
     def __repr__(self):
         return f"Int4Operand(k={self.k}, n={self.n}, group={self.group}, swiglu={self.swiglu})"
@@ -168,14 +164,14 @@ def int4_matmul(x, w, *, epilogue=None, residual=None, bias=None):
             extra = extra.float()
         if not (extra.stride(-1) == 1 or n == 1) or (extra.dim() == 2 and extra.stride(0) < n):
             extra = extra.clone(memory_format=torch.contiguous_format)
-    out = torch.empty((m, n), dtype=torch.bfloat16, device=w.device)
+    out = x.new_empty((m, n))
     if not m:
         return out
     row = x.stride(0) if m > 1 else k  # a single row has no stride
     if x.stride(1) != 1 or row % 8 or row < k or row > 1 << 24 or x.data_ptr() % 16:
         x, row = x.clone(memory_format=torch.contiguous_format), k
     need = w.workspace_bytes(m)
-    workspace = torch.empty(need, dtype=torch.uint8, device=w.device) if need else None
+    workspace = w.codes.new_empty(need // 4) if need else None
     _call(w.device, _lib.load().smx_int4_matmul, w.desc, m, _lib.ptr(x), row, _lib.SMX_EPI[epilogue],
           _lib.ptr(extra), max(extra.stride(0), n) if residual is not None else 0,
           int(extra is not None and extra.dtype == torch.float32), _lib.ptr(out), n, _lib.ptr(workspace), need)

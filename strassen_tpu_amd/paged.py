@@ -65,10 +65,11 @@ class PagedPlan:
 def _check_device(name, x, device=None):
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(x).__name__}")
-    if not x.is_cuda:
-        raise ValueError(f"the gfx950 kernel needs tensors on the HIP device (got {name} on {x.device})")
-    if device is not None and x.device != device:
-        raise ValueError(f"{name} is on {x.device}, the call on {device}")
+    if device is None or x.device != device:
+        if not x.is_cuda:
+            raise ValueError(f"the gfx950 kernel needs tensors on the HIP device (got {name} on {x.device})")
+        if device is not None:
+            raise ValueError(f"{name} is on {x.device}, the call on {device}")
 
 
 # The stream's handle itself: torch.cuda.current_stream makes an object of it first, which takes as long as
@@ -142,7 +143,7 @@ def paged_plan(context_lens, new_lens, block_tables, *, page_size, num_pages, to
     plan.max_context = min(width * plan.page_size, 2**31 - 1) if max_context is None else int(max_context)
     # one allocation for the small tensors: slots (int64) first, then the int32 ones
     sizes = (2 * max(tokens, 1), requests + 1, requests, requests, requests, max(tokens, 1), 1, 1)
-    memory = torch.empty(sum(sizes), dtype=torch.int32, device=device)
+    memory = context_lens.new_empty(sum(sizes))
     (slots, plan.starts, plan.rows, plan.context, plan.status, plan.positions, plan.pages_used,
      plan.pages_needed) = memory.split_with_sizes(sizes)
     plan.slots = slots.view(torch.int64)
@@ -201,8 +202,10 @@ def _heads(name, x, plan, heads, head_dim, lay_out=True):
 
 
 def _no_gradients(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("serving operators record no gradients: call them under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("serving operators record no gradients: call them under torch.no_grad()")
 
 
 def _scale(name, x, plan, head_dim):
@@ -247,7 +250,7 @@ def paged_write(k, v, k_cache, v_cache, plan, *, q=None, rope_cos=None, rope_sin
             raise ValueError("q_scale= without q=")
     else:
         q, q_rows = _heads("q", q, plan, None, head_dim)
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=plan.device)
+        out = q.new_empty(q.shape)
     dtypes = rope_rows = rope_stride = 0
     if rope_cos is not None:
         for name, x in (("rope_cos", rope_cos), ("rope_sin", rope_sin)):
@@ -306,7 +309,7 @@ def paged_attention(q, k_cache, v_cache, plan, *, scale=None, window=None, out=N
         raise ValueError(f"window must be a positive number of tokens, got {window!r}")
     zero_rows = out is None
     if zero_rows:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=plan.device)
+        out = q.new_empty(q.shape)
     _, out_rows = _heads("out", out, plan, q.shape[1], head_dim, lay_out=False)
     need = _workspace_bytes(plan.device, head_dim)
     workspace = torch.empty(need, dtype=torch.uint8, device=plan.device)
