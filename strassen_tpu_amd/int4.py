@@ -139,6 +139,7 @@ def int4_matmul(x, w, *, epilogue=None, residual=None, bias=None):
     if not isinstance(w, Int4Operand):
         raise TypeError("w must be an Int4Operand (int4_weight_layout)")
     _no_gradients(x, residual, bias)
+    _check_device("x", x)
     _check_device("x", x, w.device)
     if x.dtype != torch.bfloat16 or x.dim() != 2:
         raise ValueError(f"x must be a bf16 matrix, got {x.dtype} {tuple(x.shape)}")
