@@ -61,6 +61,7 @@ SMX_QK_OUT_F32 = 4
 
 SMX_PAGED_MAX_REQUESTS = 8192
 SMX_PAGED_MAX_TOKENS = 1 << 20
+SMX_PAGED_MAX_CONTEXT = 1 << 30
 SMX_PAGED_Q_SCALE_F32 = 1
 SMX_PAGED_K_SCALE_F32 = 2
 SMX_PAGED_ROPE_F32 = 4

@@ -952,7 +952,8 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
   p.requests = step->requests, p.tokens = step->tokens;
   p.kv_heads = cache->kv_heads, p.group = q->heads / cache->kv_heads;
   p.page_shift = __builtin_ctz(cache->page_size), p.num_pages = cache->num_pages;
-  p.window = window, p.zero_rows = zero_rows;
+  p.window = window < SMX_PAGED_MAX_CONTEXT ? window : 0;  // wider than any request: none
+  p.zero_rows = zero_rows;
   const bool few = few_rows(step->max_new, p.group);
   const int blocks = workgroups(cus, few);
   p.tile_tokens = (few ? 32 : 128) / p.group;

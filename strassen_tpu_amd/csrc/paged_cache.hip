@@ -308,9 +308,10 @@ int smx_paged_plan(int32_t requests, int32_t width, int32_t page_size, int32_t n
   if (width <= 0 || num_pages <= 0 || (int64_t)num_pages * page_size > INT32_MAX)
     return fail(SMX_ERR_INVALID, "empty or too large table or cache (width=%d, num_pages=%d)", width, num_pages);
   if (table_stride < width) return fail(SMX_ERR_INVALID, "table_stride must be at least the table's width");
-  if (max_new < 0 || max_context < 0 || (int64_t)max_context > (int64_t)width * page_size)
-    return fail(SMX_ERR_INVALID, "max_context=%d: the block tables hold %lld tokens a request", max_context,
-                (long long)width * page_size);
+  if (max_new < 0 || max_context < 0 || (int64_t)max_context > (int64_t)width * page_size ||
+      max_context > SMX_PAGED_MAX_CONTEXT)
+    return fail(SMX_ERR_INVALID, "max_new=%d, max_context=%d: the block tables hold %lld tokens a request, at most %d count",
+                max_new, max_context, (long long)width * page_size, SMX_PAGED_MAX_CONTEXT);
   if (free_count < 0 || (free_count > 0 && !free_pages)) return fail(SMX_ERR_INVALID, "free_count without a list");
   if (!context_lens || !new_lens || !block_tables || !starts || !rows || !context || !positions || !slots ||
       !status || !pages)

@@ -140,7 +140,7 @@ def paged_plan(context_lens, new_lens, block_tables, *, page_size, num_pages, to
     plan.requests, plan.tokens, plan.device = requests, tokens, device
     width = block_tables.shape[1]
     plan.max_new = tokens if max_new is None else int(max_new)
-    plan.max_context = min(width * plan.page_size, 2**31 - 1) if max_context is None else int(max_context)
+    plan.max_context = min(width * plan.page_size, _lib.SMX_PAGED_MAX_CONTEXT) if max_context is None else int(max_context)
     # one allocation for the small tensors: slots (int64) first, then the int32 ones
     sizes = (2 * max(tokens, 1), requests + 1, requests, requests, requests, max(tokens, 1), 1, 1)
     memory = context_lens.new_empty(sum(sizes))
@@ -168,10 +168,18 @@ def _cache(k_cache, v_cache, plan):
         if x.dtype != torch.bfloat16 or x.dim() != 4:
             raise ValueError(f"{name} must be a bf16 tensor [pages, page_size, kv_heads, head_dim], got {x.dtype} "
                              f"{tuple(x.shape)}")
-    strides = k_cache.stride()
-    if k_cache.shape != v_cache.shape or strides != v_cache.stride():
+    shape = k_cache.shape
+    if v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must have the same shape and strides")
-    pages, page_size, kv_heads, head_dim = k_cache.shape
+    strides = k_cache.stride()
+    if 1 in shape:  # the stride of a dimension of one is no stride: nothing steps over it
+        strides, other = (tuple(s if n > 1 else shape[3] for s, n in zip(x.stride(), shape[:3])) + x.stride()[3:]
+                          for x in (k_cache, v_cache))
+    else:
+        other = v_cache.stride()
+    if strides != other:
+        raise ValueError("k_cache and v_cache must have the same shape and strides")
+    pages, page_size, kv_heads, head_dim = shape
     if page_size != plan.page_size or pages != plan.num_pages:
         raise ValueError(f"the plan is of {plan.num_pages} pages of {plan.page_size} tokens, the cache of {pages} of "
                          f"{page_size}")
@@ -293,7 +301,9 @@ def paged_attention(q, k_cache, v_cache, plan, *, scale=None, window=None, out=N
 
     Softmax in FP32; its weights are rounded to bf16 for the product with the values, and
     the result once. Keys of table entries that are no page of the cache are not seen; a row
-    that sees none is zero. Rows of no admitted request are zero in a new result, and left as they
+    that sees none is zero. A request's values must be finite up to its last token: one that is
+    not spoils rows of the step that do not see it, too. (Nothing behind that token is
+    read.) Rows of no admitted request are zero in a new result, and left as they
     were in ``out`` (bf16 ``[tokens, heads, head_dim]``, rows 16-byte aligned)."""
     _no_gradients(q, k_cache, v_cache, out)
     cache = _cache(k_cache, v_cache, plan)

@@ -259,6 +259,44 @@ def test_attention_leaves_out_pages_that_are_not_in_the_cache(max_new):
     assert not got[2:5].any()
 
 
+@pytest.mark.parametrize("new_high,max_new", [(1, 1), (3, 4), (3, None)])
+@pytest.mark.parametrize("window", [None, 40])
+def test_attention_of_many_requests(new_high, max_new, window):
+    """More requests than a workgroup looks at in one round, some of them idle."""
+    generator = torch.Generator().manual_seed(7)
+    requests = 700
+    context = torch.randint(0, 150, (requests,), generator=generator).tolist()
+    new = torch.randint(0, new_high + 1, (requests,), generator=generator).tolist()
+    plan, k, v, keys, values, g = make_step(context, new, page=16, kv_heads=1, dim=64, pad=1)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=16, num_pages=plan.num_pages,
+                          tokens=plan.tokens, max_new=max_new)
+    q = torch.randn(plan.tokens, 4, 64, device=DEV, generator=g).to(torch.bfloat16)
+    want, size = attend64(q, keys, values, context, new, window)
+    check_attention(smx.paged_attention(q, k, v, plan, window=window), want, size)
+
+
+@pytest.mark.parametrize("heads,kv_heads,max_new", [(8, 8, 32), (32, 1, 1), (6, 2, 10), (64, 2, 1)])
+@pytest.mark.parametrize("window", [None, 1, 2**31 - 1])
+def test_attention_of_few_rows(heads, kv_heads, max_new, window):
+    """Steps whose rows fill a tile of 32, nearly fill it or hold one token in it."""
+    context, new = [600, 0, 33, 64], [max_new, max_new, 1, max(1, max_new // 2)]
+    plan, k, v, keys, values, g = make_step(context, new, page=8, kv_heads=kv_heads, dim=128, pad=2)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=8, num_pages=plan.num_pages,
+                          tokens=plan.tokens, max_new=max_new)
+    q = torch.randn(plan.tokens, heads, 128, device=DEV, generator=g).to(torch.bfloat16)
+    want, size = attend64(q, keys, values, context, new, window)
+    check_attention(smx.paged_attention(q, k, v, plan, window=window), want, size)
+
+
+def test_one_page_one_head_views():
+    """Dimensions of one, whose strides mean nothing."""
+    plan, k, v, keys, values, g = make_step([3], [2], page=8, kv_heads=1, dim=64, spare=0)
+    q = torch.randn(2, 1, 64, device=DEV, generator=g).to(torch.bfloat16)
+    want, size = attend64(q, keys, values, [3], [2], None)
+    odd = [x.as_strided((1, 8, 1, 64), s) for x, s in ((k, (0, 64, 3, 1)), (v, (7, 64, 512, 1)))]
+    check_attention(smx.paged_attention(q.as_strided((2, 1, 64), (64, 5, 1)), *odd, plan), want, size)
+
+
 def test_attention_scale_and_out():
     context, new = [70, 12], [9, 1]
     plan, k, v, keys, values, g = make_step(context, new, page=16, kv_heads=2, dim=64, pad=6)

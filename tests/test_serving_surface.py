@@ -94,7 +94,8 @@ def _plan(**kw):
 @pytest.mark.parametrize("change", [
     {"requests": 0}, {"requests": 8193}, {"tokens": 0}, {"tokens": (1 << 20) + 1}, {"page_size": 24}, {"page_size": 4},
     {"page_size": 8192}, {"width": 0}, {"num_pages": 0}, {"num_pages": 1 << 30}, {"stride": 3}, {"max_new": -1},
-    {"max_context": 65}, {"max_context": -1}, {"count": -1}, {"free": None}, {"context": None}, {"slots": None}])
+    {"max_context": 65}, {"max_context": -1},
+    {"max_context": (1 << 30) + 1, "width": 1 << 27, "stride": 1 << 27}, {"count": -1}, {"free": None}, {"context": None}, {"slots": None}])
 def test_plan_refusals(change):
     assert _plan(**change) == _lib.SMX_ERR_INVALID
     assert _lib.last_error()
