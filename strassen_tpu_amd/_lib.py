@@ -189,6 +189,26 @@ def load():
     return lib
 
 
+_host = None
+
+
+def host():
+    """The host side of the serving operators (``csrc/serving_host.cpp``), bound to the library."""
+    global _host
+    if _host is None:
+        lib = load()
+        try:
+            from . import _serving
+        except ImportError as e:
+            raise RuntimeError(f"the serving operators' host module is missing or does not load ({e}): build it with "
+                               "`python -m strassen_tpu_amd.build`") from e
+        _serving.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "smx_paged_plan", "smx_paged_write", "smx_paged_attention", "smx_paged_attention_workspace_bytes",
+            "smx_int4_matmul", "smx_int4_workspace_bytes", "smx_last_error")), torch._C._cuda_getCurrentRawStream)
+        _host = _serving
+    return _host
+
+
 def last_error():
     return load().smx_last_error().decode("utf-8", "replace")
 

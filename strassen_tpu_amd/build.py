@@ -5,7 +5,9 @@ translation unit (``csrc/strassen_gemm.hip``), the six units that
 instantiate the GEMM kernels (``csrc/gemm_*.hip``) and the three of the serving
 operators (``csrc/paged_*.hip``, ``csrc/int4_matmul.hip``) with hipcc, in parallel,
 checks each unit's device assembly, and links ``libstrassen_mi355x.so`` next
-to this file. hipcc cross-compiles for gfx950 without a GPU.
+to this file. hipcc cross-compiles for gfx950 without a GPU. The serving operators' host side
+(``csrc/serving_host.cpp``, a Python extension module on torch's tensors) is compiled with the
+host compiler to ``_serving.so``.
 """
 
 from __future__ import annotations
@@ -16,6 +18,7 @@ from concurrent.futures import ThreadPoolExecutor
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -24,6 +27,7 @@ SOURCES = tuple(os.path.join(HERE, "csrc", name) for name in (
     "strassen_gemm.hip", "gemm_strassen.hip", "gemm_strassen_thin.hip", "gemm_strassen_pm.hip", "gemm_cubic.hip",
     "gemm_cubic_thin.hip", "gemm_stream.hip", "paged_cache.hip", "paged_attention.hip", "int4_matmul.hip"))
 LIBRARY = os.path.join(HERE, "libstrassen_mi355x.so")
+HOST_SOURCE, HOST_MODULE = os.path.join(HERE, "csrc", "serving_host.cpp"), os.path.join(HERE, "_serving.so")
 INCLUDE = os.path.join(REPO, "include")
 
 
@@ -48,6 +52,20 @@ def compile_command(source, output, extra=()):
         # Packed FP32 VALU ops (v_pk_add_f32 and friends) stay disabled.
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-I", INCLUDE, *extra, source, "-o", output,
+    ]
+
+
+def host_command(output):
+    """Host compiler's command for the serving operators' host module. Torch's libraries are found through
+    the process that has loaded torch before."""
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    return [
+        os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-Wall", "-fPIC", "-shared", "-fvisibility=hidden",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+        "-isystem", os.path.join(root, "include"), "-I", sysconfig.get_paths()["include"], HOST_SOURCE, "-o", output,
+        "-L", os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
     ]
 
 
@@ -186,7 +204,12 @@ def build(verbose=False, jobs=None):
     with tempfile.TemporaryDirectory() as scratch:
         dirs = [os.path.join(scratch, f"unit{i}") for i in range(len(SOURCES))]
         with ThreadPoolExecutor(max_workers=jobs) as pool:
+            host = pool.submit(subprocess.run, host_command(HOST_MODULE + ".tmp"), capture_output=True, text=True)
             units = list(pool.map(_compile_unit, SOURCES, dirs))
+        if host.result().returncode != 0:
+            raise RuntimeError("host module failed:\n" + host.result().stderr)
+        if verbose and host.result().stderr.strip():
+            print(host.result().stderr, file=sys.stderr)
         checked = gemms = 0
         for source, (_, text, stderr) in zip(SOURCES, units):
             if verbose and stderr.strip():
@@ -207,6 +230,7 @@ def build(verbose=False, jobs=None):
             raise RuntimeError("link failed:\n" + " ".join(cmd) + "\n" + result.stderr)
     if verbose:
         print(f"verified {checked} inline-asm MFMA kernels and the scratch of {gemms} GEMM kernels", file=sys.stderr)
+    os.replace(HOST_MODULE + ".tmp", HOST_MODULE)
     os.replace(tmp, LIBRARY)
     return LIBRARY
 

@@ -9,12 +9,9 @@ zero point 0 .. 15 per group of 32, 64 or 128 consecutive k and column.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
-from .paged import _call, _check_device, _no_gradients
 
 __all__ = ["Int4Operand", "int4_quantize", "int4_weight_layout", "int4_matmul"]
 
@@ -27,21 +24,7 @@ class Int4Operand:
 
     def __init__(self, codes, scales, k, n, group, swiglu, zeros):
         self.codes, self.scales, self.device = codes, scales, codes.device
-        self.k, self.n, self.group, self.swiglu = k, n, group, swiglu
-        self.desc = _lib.SmxInt4Weight(codes.data_ptr(), scales.data_ptr(), k, n, group, int(swiglu), int(zeros))
-        self._workspace = {}  # bytes by number of rows, up to 64 of them
-
-    def workspace_bytes(self, m):
-        """Device memory that a product of ``m`` rows needs."""
-        need = self._workspace.get(m)
-        if need is None:
-            value = ctypes.c_int64()
-            with torch.cuda.device(self.device):
-                _lib.check(_lib.load().smx_int4_workspace_bytes(self.desc, m, ctypes.byref(value)))
-            need = value.value
-            if m <= 64:
-                self._workspace[m] = need
-        return need
+        self.k, self.n, self.group, self.swiglu, self.zeros = k, n, group, swiglu, zeros
 
     @property
     def shape(self):
@@ -138,42 +121,9 @@ def int4_matmul(x, w, *, epilogue=None, residual=None, bias=None):
     with an infinity is NaN in the result."""
     if not isinstance(w, Int4Operand):
         raise TypeError("w must be an Int4Operand (int4_weight_layout)")
-    _no_gradients(x, residual, bias)
-    _check_device("x", x)
-    _check_device("x", x, w.device)
-    if x.dtype != torch.bfloat16 or x.dim() != 2:
-        raise ValueError(f"x must be a bf16 matrix, got {x.dtype} {tuple(x.shape)}")
-    m, k = x.shape
-    if k != w.k:
-        raise ValueError(f"inner dimensions disagree: {k} vs {w.k}")
     if epilogue not in _EPILOGUES:
         raise ValueError(f"unknown epilogue {epilogue!r}; choose 'swiglu', 'residual_add' or 'bias_add'")
     if (epilogue == "swiglu") != w.swiglu:
         raise ValueError(f"{w!r} is {'' if w.swiglu else 'not '}laid out for swiglu")
-    if (epilogue == "residual_add") != (residual is not None):
-        raise ValueError("residual= goes with the residual_add epilogue")
-    if (epilogue == "bias_add") != (bias is not None):
-        raise ValueError("bias= goes with the bias_add epilogue")
-    n = w.n // 2 if w.swiglu else w.n
-    extra = residual if residual is not None else bias
-    if extra is not None:
-        _check_device("residual" if residual is not None else "bias", extra, w.device)
-        shape = (m, n) if residual is not None else (n,)
-        if tuple(extra.shape) != shape:
-            raise ValueError(f"{epilogue} operand shape {tuple(extra.shape)} != {shape}")
-        if extra.dtype not in (torch.bfloat16, torch.float32):
-            extra = extra.float()
-        if not (extra.stride(-1) == 1 or n == 1) or (extra.dim() == 2 and extra.stride(0) < n):
-            extra = extra.clone(memory_format=torch.contiguous_format)
-    out = x.new_empty((m, n))
-    if not m:
-        return out
-    row = x.stride(0) if m > 1 else k  # a single row has no stride
-    if x.stride(1) != 1 or row % 8 or row < k or row > 1 << 24 or x.data_ptr() % 16:
-        x, row = x.clone(memory_format=torch.contiguous_format), k
-    need = w.workspace_bytes(m)
-    workspace = w.codes.new_empty(need // 4) if need else None
-    _call(w.device, _lib.load().smx_int4_matmul, w.desc, m, _lib.ptr(x), row, _lib.SMX_EPI[epilogue],
-          _lib.ptr(extra), max(extra.stride(0), n) if residual is not None else 0,
-          int(extra is not None and extra.dtype == torch.float32), _lib.ptr(out), n, _lib.ptr(workspace), need)
-    return out
+    return _lib.host().int4(x, w.codes, w.scales, w.k, w.n, w.group, w.swiglu, w.zeros, _lib.SMX_EPI[epilogue], residual,
+                            bias)
