@@ -472,9 +472,8 @@ int smx_paged_write(const smx_paged_cache* cache, int32_t tokens, const int32_t*
  * values already: the row at position p of its request sees that request's keys j <= p, and with
  * window > 0 only those with j > p - window. Query head h reads key/value head
  * h / (heads / kv_heads). softmax(scale q k) in FP32, its weights rounded to bf16 for the
- * product with the values, one bf16 rounding of the result. A key's values must be finite
- * for the rows of the same request that do not see it as well (their weight of 0 times
- * an infinity or NaN is NaN); slots behind a request's last token are not read. Keys of pages that are
+ * product with the values, one bf16 rounding of the result. Infinities and NaN
+ * reach the rows that see them only; slots behind a request's last token are not read. Keys of pages that are
  * not in the cache (0 .. num_pages - 1) are not seen, and a row that sees none is zero. Rows of no
  * request stay as they are, or become zero with zero_rows. The workspace
  * (smx_paged_attention_workspace_bytes, for the current device) is overwritten.

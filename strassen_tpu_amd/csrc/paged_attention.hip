@@ -129,7 +129,7 @@ struct Part {
   int head, request, tile;
   int from, count, tile_count;  // steps of the part, and of the whole item
   int units, rest;              // of the part; of the item behind it
-  bool begins;                  // no span before has steps of the item
+  int begins;                   // 1: no span before has steps of the item
 
   __device__ __forceinline__ Part(const AttentionArgs& p, const Span& s)
       : r(Request<kKeys, kItem>::uniform(p, s.request)), head(s.head), request(s.request), tile(s.tile) {
@@ -137,7 +137,7 @@ struct Part {
     units = (int)min((int64_t)(tile_count + kItem - s.skip), s.left);
     rest = tile_count + kItem - s.skip - units;
     const int before = max(0, s.skip - kItem), upto = max(0, s.skip + units - kItem);
-    from = r.first(tile) + before, count = upto - before, begins = before == 0;
+    from = r.first(tile) + before, count = upto - before, begins = __builtin_amdgcn_readfirstlane(before == 0);
   }
 };
 
@@ -410,8 +410,84 @@ __device__ __forceinline__ float other_half(float x) {
   return (threadIdx.x & 32) ? __uint_as_float(r[0]) : __uint_as_float(r[1]);
 }
 
-// One step: the wave's 32 rows against 32 kBlocks keys in LDS. `seen` is called for
-// score registers only if kMask. The maximum that the exponentials are taken against
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// Whether a step's values hold an infinity or a NaN, in any lane.
+template <int kBlocks, int kColumns>
+__device__ __forceinline__ bool any_not_finite(const bf16x8 (&v)[kBlocks][2][kColumns]) {
+  u16x2 most = {0, 0};
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int x = 0; x < kColumns; ++x) {
+        const u32x4 words = __builtin_bit_cast(u32x4, v[b][h][x]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, words[i] & 0x7fff7fffu));
+      }
+  return __any(max(most[0], most[1]) >= 0x7f80);
+}
+
+// A step that masks keys and whose values are not all finite: a product alone would give 0 * inf = NaN
+// to the rows that do not see them. Every +inf and NaN (sign 0), every -inf and NaN (sign 1) that a row
+// weighs adds a product beyond FP32's range to its column, which is that infinity (both: NaN), and the
+// values themselves become zero.
+template <int D, int kBlocks>
+__device__ __forceinline__ void add_not_finite(f32x16 (&o)[D / 32], bf16x8 (&v)[kBlocks][2][D / 32],
+                                               const bf16x8 (&w)[2 * kBlocks]) {
+  // two values a register; 0 or 1 for no and yes (asm: constants loaded here, not held by the whole kernel)
+  uint32_t weight = 0x43804380u, ones = 0x10001u, largest[2] = {0x7f7f7f7fu, 0xff7fff7fu};
+  asm volatile("" : "+s"(weight), "+s"(ones), "+s"(largest[0]), "+s"(largest[1]));
+  const uint32_t finite = largest[0];
+  const u16x2 one = __builtin_bit_cast(u16x2, ones), most = __builtin_bit_cast(u16x2, finite);
+#pragma unroll
+  for (int t = 0; t < 2 * kBlocks; ++t) {
+    // (elements are copied before they are reinterpreted: a bit cast of a vector's element takes its first)
+    const u32x4 weights = __builtin_bit_cast(u32x4, w[t]);
+    u32x4 large;  // 2^8 for every weight above zero
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t two = weights[i];
+      large[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, two), one) *
+                                                  __builtin_bit_cast(u16x2, weight));
+    }
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) {
+      u32x4 words = __builtin_bit_cast(u32x4, v[t / 2][t % 2][x]), bad;
+#pragma unroll
+      for (int sign = 0; sign < 2; ++sign) {
+        asm volatile("" : "+v"(words));  // nothing shared with any_not_finite and between signs, for want of registers
+        const uint32_t value = largest[sign];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t two = words[i], sizes = two & 0x7fff7fffu;
+          const u16x2 beyond = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, sizes), most);  // 1: inf, more: NaN
+          u16x2 side = __builtin_bit_cast(u16x2, two) >> (uint16_t)15;
+          if (!sign) side = one - side;
+          const u16x2 hit = __builtin_elementwise_min(beyond >> (uint16_t)1 | side, one) * __builtin_elementwise_min(beyond, one);
+          bad[i] = __builtin_bit_cast(uint32_t, hit * __builtin_bit_cast(u16x2, value));
+        }
+        o[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, bad), __builtin_bit_cast(bf16x8, large),
+                                                       o[x], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t two = words[i];
+        asm volatile("" : "+v"(two));
+        const uint32_t sizes = two & 0x7fff7fffu;
+        const u16x2 beyond = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, sizes), most);
+        words[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, two) * (one - __builtin_elementwise_min(beyond, one)));
+      }
+      v[t / 2][t % 2][x] = __builtin_bit_cast(bf16x8, words);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+// One step: the wave's 32 rows against 32 kBlocks keys in LDS. The maximum that the exponentials are taken against
 // moves only once it is exceeded by 2^8, so that most steps rescale nothing; sums
 // stay below 2^8 times their number of keys.
 template <int D, int kBlocks>
@@ -500,6 +576,7 @@ __device__ __forceinline__ void attend(Rows<D>& r, const bf16x8 (&q)[D / 16], co
       w[2 * x + h] = __builtin_bit_cast(bf16x8, b);
     }
   }
+  if (masked && any_not_finite(v)) add_not_finite<D, kBlocks>(r.o, v, w);
 #pragma unroll
   for (int t = 0; t < 2 * kBlocks; ++t)
 #pragma unroll
@@ -520,7 +597,9 @@ constexpr int kFewPartialFloats = 32 * (D + 2);
 template <int D>
 __device__ __forceinline__ void store_rows(const AttentionArgs& p, const f32x16 (&o)[D / 32], float inverse, bool valid,
                                            int64_t token, int head) {
-  const int half = (threadIdx.x & 63) >> 5;
+  int thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));  // (offsets are made here, not held by the whole kernel)
+  const int half = thread >> 5 & 1;
   uint16_t* const to = p.out + token * p.out_token + head * p.out_head;
 #pragma unroll
   for (int x = 0; x < D / 32; ++x)
@@ -580,7 +659,9 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
     int local, head;
     row_of(w, &local, &head);
     const int64_t token = scalar_at(p.starts, w.request) + local;
-    const uint16_t* const from = p.q + token * p.q_token + head * p.q_head + 8 * half;
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));  // (the offset is made here, not held by the whole kernel)
+    const uint16_t* const from = p.q + token * p.q_token + head * p.q_head + 8 * (thread >> 5 & 1);
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) q[t] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(from + 16 * t));
   };
@@ -612,7 +693,7 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
       // positions of the wave's first and last row
       const int low = __builtin_amdgcn_readfirstlane(position), high = __builtin_amdgcn_readlane(position, 31);
       const bool active = 32 * wave < tile_rows;  // rows of its own
-      bool more = s.left > part.units;
+      int more = __builtin_amdgcn_readfirstlane(s.left > part.units);  // another part follows
       Rows<D> o;
       o.clear();
       for (int i = 0; i < part.count; ++i) {
@@ -624,7 +705,7 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
           s.left -= part.units;
           next_item(p, &s, part.r.tiles);
           next = next_part();
-          more = next.count > 0;
+          more = __builtin_amdgcn_readfirstlane(next.count > 0);
           if (more && ends) pages = pages_of(next, next.from);
         }
         if (!ends) {
@@ -657,18 +738,22 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
         store_rows<D>(p, o.o, inverse_of(sum), 32 * wave + (lane & 31) < tile_rows, scalar_at(p.starts, part.request) + local, head);
       } else {
         float* const to = p.partial + (2 * (int64_t)s.worker + part.begins) * kPartialFloats<D>;
+        int thread = threadIdx.x;
+        asm volatile("" : "+v"(thread));  // (nor are these addresses)
 #pragma unroll
         for (int x = 0; x < D / 32; ++x)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            reinterpret_cast<f32x4*>(to)[(4 * x + e) * 256 + threadIdx.x] =
+            reinterpret_cast<f32x4*>(to)[(4 * x + e) * 256 + thread] =
                 f32x4{o.o[x][4 * e], o.o[x][4 * e + 1], o.o[x][4 * e + 2], o.o[x][4 * e + 3]};
-        to[256 * (D / 2) + threadIdx.x] = o.top;
-        to[256 * (D / 2 + 1) + threadIdx.x] = sum;
+        to[256 * (D / 2) + thread] = o.top;
+        to[256 * (D / 2 + 1) + thread] = sum;
         if (part.begins && threadIdx.x == 0) {
           record->worker = s.worker, record->head = part.head, record->request = part.request, record->tile = part.tile;
           // the item goes on in the spans behind this one
-          record->others = (int)quotient(part.rest + s.each - 1, s.each);
+          int64_t each = s.each;
+          asm volatile("" : "+s"(each));  // (its floating-point form is made here, not held by the whole kernel)
+          record->others = (int)quotient(part.rest + each - 1, each);
         }
       }
       if (!more) break;
@@ -680,7 +765,7 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
 
 // Steps of few rows (decoding): a workgroup is one wave with 32 rows a tile, which streams 32
 // keys a step through its own two buffers, so that no barrier joins it to others and
-// five of them (LDS: 32 KB each at head_dim 128) keep up to 160 KB of a CU's reads in
+// four of them (32 KB of LDS each at head_dim 128) keep up to 128 KB of a CU's reads in
 // flight. Rows are few: what bounds it is the cache's bytes.
 template <int D>
 __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
@@ -870,8 +955,8 @@ __global__ __launch_bounds__(256) void paged_join(AttentionArgs p) {
   store_rows<D>(p, o, inverse_of(sum), at < tile_rows, token, record.head * p.group + row % p.group);
 }
 
-// Workgroups of a launch, a multiple of the 8 XCDs: as many as a CU's LDS holds (two of paged_attend;
-// five of paged_attend_few, its registers would allow eight).
+// Workgroups of a launch, a multiple of the 8 XCDs: as many as a CU holds (two of paged_attend, by its
+// LDS; four of paged_attend_few, by its registers).
 int workgroups(int cus, bool few) { return ((few ? 4 : 2) * cus + 7) / 8 * 8; }
 
 constexpr int64_t kRecordBytes = sizeof(Record);

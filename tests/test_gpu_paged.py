@@ -288,6 +288,50 @@ def test_attention_of_few_rows(heads, kv_heads, max_new, window):
     check_attention(smx.paged_attention(q, k, v, plan, window=window), want, size)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("context,new,max_new,window", [
+    ([40, 0, 300], [1, 1, 1], 1, 16),  # behind the window, in the step's first keys
+    ([30, 5, 200], [4, 3, 4], 4, None), ([30, 5, 200], [4, 3, 4], 4, 8),  # tokens of the step that come later
+    ([0, 100], [150, 70], None, None), ([90, 700], [150, 70], None, 33),
+])
+def test_attention_of_rows_that_do_not_see_an_infinity_or_nan(dim, context, new, max_new, window):
+    """Infinities and NaN among a request's values, and NaN among its keys, reach the rows that see them and no
+    others."""
+    page, kv_heads, heads = 8, 2, 4
+    plan, k, v, keys, values, g = make_step(context, new, page=page, kv_heads=kv_heads, dim=dim)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=page, num_pages=plan.num_pages,
+                          tokens=plan.tokens, max_new=max_new)
+    q = torch.randn(plan.tokens, heads, dim, device=DEV, generator=g).to(torch.bfloat16)
+    for b, (c, n) in enumerate(zip(context, new)):
+        odd = [(0, 0, math.inf), (max(0, c - 9), 3, math.nan), (c + n // 2, 5, -math.inf), (c + n - 1, 40, math.inf),
+               (c + n - 1, 5, math.inf), (c + n - 1, 41, -math.inf), (c, 63, math.nan)]
+        for at, column, value in odd:
+            page_at = plan.block_tables[b, at // page]
+            v[page_at, at % page, 1, column] = value
+            values[b][at, 1, column] = value
+        k[plan.block_tables[b, (c + n - 1) // page], (c + n - 1) % page, 0, 7] = math.nan
+        keys[b][c + n - 1, 0, 7] = math.nan
+    finite = [x.masked_fill(~x.isfinite(), 0.0) for x in values]
+    got = smx.paged_attention(q, k, v, plan, window=window).double()
+    want, size = attend64(q, [x.nan_to_num(0.0) for x in keys], finite, context, new, window)
+    row = 0
+    for b, (c, n) in enumerate(zip(context, new)):
+        key, own = torch.arange(c + n, device=DEV), torch.arange(c, c + n, device=DEV)[:, None]
+        sees = ((key <= own) & (key > own - (window or 1 << 30))).double()
+        value = values[b][:, 1]
+        up, down = (sees @ ((value == way) | value.isnan()).double() > 0 for way in (math.inf, -math.inf))
+        part = want[row:row + n, 2:]  # the second key/value head's query heads
+        part[up[:, None].expand_as(part)] = math.inf
+        part[down[:, None].expand_as(part)] = -math.inf
+        part[(up & down)[:, None].expand_as(part)] = math.nan
+        want[row + n - 1, :2] = math.nan  # the last row alone sees the key
+        row += n
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got == math.inf, want == math.inf) and torch.equal(got == -math.inf, want == -math.inf)
+    here = want.isfinite()
+    check_attention(got[here], want[here], size[here])
+
+
 def test_one_page_one_head_views():
     """Dimensions of one, whose strides mean nothing."""
     plan, k, v, keys, values, g = make_step([3], [2], page=8, kv_heads=1, dim=64, spare=0)
