@@ -44,7 +44,8 @@ struct AttentionArgs {
   const int32_t *starts, *rows, *context, *positions;
   int32_t requests, tokens, group, kv_heads, page_shift, num_pages, window, tile_tokens, zero_rows, min_span;
   float scale;      // times log2 e
-  float per_group;  // 1 / group
+  float per_group;       // 1 / group
+  double per_workgroup;  // 1 / workgroups
   float* partial;
   int32_t* records;
 };
@@ -86,11 +87,10 @@ struct Request {
       : context(context_), fresh(fresh_), per_tile(p.tile_tokens), window(p.window) {
     tiles = (fresh + per_tile - 1) / per_tile;
   }
-  __device__ Request(const AttentionArgs& p, int b) : Request(p, p.context[b], p.rows[b]) {}
   // The request that a whole wave works on: its lengths in scalar registers, on which the
   // page buffers' descriptors depend.
-  __device__ static Request uniform(const AttentionArgs& p, int b) {
-    Request r(p, scalar_at(p.context, b), scalar_at(p.rows, b));
+  __device__ static Request uniform(const AttentionArgs& p, int32_t context_, int32_t fresh_) {
+    Request r(p, context_, fresh_);
     r.tiles = __builtin_amdgcn_readfirstlane(r.tiles);
     return r;
   }
@@ -120,6 +120,7 @@ struct Span {
   int64_t begin;        // of this one, over all key/value heads
   int32_t worker;       // which span this is
   int32_t head, request, tile, skip;  // skip: units of that item that lie in spans before
+  int32_t context, fresh;             // of that request
 };
 
 // The span's part of one item: its first step (key tile), its steps and units.
@@ -132,7 +133,7 @@ struct Part {
   int begins;                   // 1: no span before has steps of the item
 
   __device__ __forceinline__ Part(const AttentionArgs& p, const Span& s)
-      : r(Request<kKeys, kItem>::uniform(p, s.request)), head(s.head), request(s.request), tile(s.tile) {
+      : r(Request<kKeys, kItem>::uniform(p, s.context, s.fresh)), head(s.head), request(s.request), tile(s.tile) {
     tile_count = r.count(tile);
     units = (int)min((int64_t)(tile_count + kItem - s.skip), s.left);
     rest = tile_count + kItem - s.skip - units;
@@ -141,33 +142,37 @@ struct Part {
   }
 };
 
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  return x;
-}
-
 __device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
   return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, lane) |
          (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
 }
 
-// a / b for 0 <= a < 2^52 and 0 < b, through the floating-point reciprocal (the integer
-// division is ten times as long).
+// a / b for 0 <= a, 0 < b and a quotient below 2^19, of which the reciprocal of b misses less
+// than one (the integer division is ten times as long).
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  int64_t q = (int64_t)((double)a / (double)b);
+  int64_t q = (int64_t)((float)a * __builtin_amdgcn_rcpf((float)b));
   if (q * b > a) --q;
   if ((q + 1) * b <= a) ++q;
   return q;
 }
 
-// Inclusive sum of x over a wave's lanes.
+// x of the lanes that kControl names, zero where there are none.
+template <int kControl, int kRows>
+__device__ __forceinline__ int64_t moved(int64_t x) {
+  const uint32_t low = __builtin_amdgcn_update_dpp(0, (int)x, kControl, kRows, 15, false);
+  const uint32_t high = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), kControl, kRows, 15, false);
+  return (int64_t)((uint64_t)high << 32 | low);
+}
+
+// Inclusive sum of x over a wave's lanes: within rows of 16 lanes, then a row's last value
+// to the next row, and the lower half's to the upper.
 __device__ __forceinline__ int64_t wave_scan(int64_t x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t y = __shfl_up(x, d);
-    if ((int)(threadIdx.x & 63) >= d) x += y;
-  }
+  x += moved<0x111, 15>(x);
+  x += moved<0x112, 15>(x);
+  x += moved<0x114, 15>(x);
+  x += moved<0x118, 15>(x);
+  x += moved<0x142, 10>(x);
+  x += moved<0x143, 12>(x);
   return x;
 }
 
@@ -177,13 +182,16 @@ template <int kKeys, int kItem, int kWaves>
 __device__ bool find_span(const AttentionArgs& p, Span* s) {
   constexpr int kThreads = 64 * kWaves;
   __shared__ int64_t waves[kWaves], found_rest;
-  __shared__ int32_t found;
+  __shared__ int32_t found[3];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // Inclusive sum over the workgroup of this thread's request among kThreads of them.
   int64_t mine = 0, upto = 0;
+  int32_t context = 0, fresh = 0;
   auto scan = [&](int first) -> int64_t {
     const int b = first + (int)threadIdx.x;
-    mine = b < p.requests ? Request<kKeys, kItem>(p, b).all() : 0;
+    const bool here = b < p.requests;
+    context = here ? p.context[b] : 0, fresh = here ? p.rows[b] : 0;
+    mine = Request<kKeys, kItem>(p, context, fresh).all();
     upto = wave_scan(mine);
     if constexpr (kWaves == 1) return lane_value(upto, 63);
     __syncthreads();
@@ -199,7 +207,9 @@ __device__ bool find_span(const AttentionArgs& p, Span* s) {
   int64_t total = 0;
   for (int first = 0; first < p.requests; first += kThreads) total += scan(first);
   const int64_t everything = total * p.kv_heads;
-  s->each = max((int64_t)p.min_span, quotient(everything + gridDim.x - 1, gridDim.x));
+  int64_t each = (int64_t)((double)everything * p.per_workgroup);  // (at most one short)
+  while (each * gridDim.x < everything) ++each;
+  s->each = max((int64_t)p.min_span, each);
   const int64_t spans = quotient(everything + s->each - 1, s->each), per_xcd = (spans + 7) / 8;
   s->worker = (int)((blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3));
   if ((blockIdx.x >> 3) >= per_xcd || s->worker >= spans) return false;
@@ -214,10 +224,14 @@ __device__ bool find_span(const AttentionArgs& p, Span* s) {
     const int64_t all = p.requests <= kThreads ? total : scan(first);
     const bool here = at >= base + upto - mine && at < base + upto;
     if constexpr (kWaves > 1) {
-      if (here) found = first + (int)threadIdx.x, found_rest = at - (base + upto - mine);
+      if (here) {
+        found[0] = first + (int)threadIdx.x, found[1] = context, found[2] = fresh;
+        found_rest = at - (base + upto - mine);
+      }
     } else if (const uint64_t who = __ballot(here)) {
       const int l = __builtin_ctzll(who);
       s->request = first + l;
+      s->context = __builtin_amdgcn_readlane(context, l), s->fresh = __builtin_amdgcn_readlane(fresh, l);
       rest = at - (base + lane_value(upto - mine, l));
     }
     base += all;
@@ -225,10 +239,11 @@ __device__ bool find_span(const AttentionArgs& p, Span* s) {
   }
   if constexpr (kWaves > 1) {
     __syncthreads();
-    s->request = __builtin_amdgcn_readfirstlane(found);
+    s->request = __builtin_amdgcn_readfirstlane(found[0]);
+    s->context = __builtin_amdgcn_readfirstlane(found[1]), s->fresh = __builtin_amdgcn_readfirstlane(found[2]);
     rest = lane_value(found_rest, 0);
   }
-  const auto r = Request<kKeys, kItem>::uniform(p, s->request);
+  const auto r = Request<kKeys, kItem>::uniform(p, s->context, s->fresh);
   int low = 0, high = r.tiles;  // the last tile with before(tile) <= rest
   while (high - low > 1) {
     const int mid = (low + high) >> 1;
@@ -246,7 +261,9 @@ __device__ __forceinline__ void next_item(const AttentionArgs& p, Span* s, int t
   s->tile = 0;
   do {
     if (++s->request == p.requests) s->request = 0, ++s->head;
-  } while (scalar_at(p.rows, s->request) <= 0);
+    s->fresh = scalar_at(p.rows, s->request);
+  } while (s->fresh <= 0);
+  s->context = scalar_at(p.context, s->request);
 }
 
 // Row r of a tile belongs to its token r / group; exact for rows below 2^12.
@@ -299,29 +316,49 @@ struct Lanes {
     }
   }
 
+  // The DMAs of the eight rows of group g, whose first lies at byte `from` of the cache.
+  __device__ __forceinline__ void fetch_group(const AttentionArgs& p, int g, int64_t from, uint32_t bytes, uint8_t* keys,
+                                              uint8_t* values) const {
+    const auto from_k = packed::panel_rsrc(reinterpret_cast<const uint8_t*>(p.k) + from, bytes);
+    const auto from_v = packed::panel_rsrc(reinterpret_cast<const uint8_t*>(p.v) + from, bytes);
+#pragma unroll
+    for (int i = g * kPer8; i < (g + 1) * kPer8; ++i) {
+      packed::dma_frag(from_k, key[i], 0, keys + i * T::kDmaRows * T::kRow);
+      packed::dma_frag(from_v, value[i], 0, values + i * T::kDmaRows * T::kRow);
+    }
+  }
+
   // Starts the DMAs of rows key0 .. key0 + kRows - 1 of a head to LDS. A page holds whole
   // groups of eight rows: each group is one buffer, whose rows behind `length`, and
   // all of whose rows if its page is not in the cache, read as zeros. Lane
   // lane0 + r of `pages` holds row r's page.
+  // kByLane: every lane works out its row's address, and a group reads its lane's. That is a third of
+  // the instructions, for a wave alone on its SIMD (1000 keys, one row: 13.4 us, else 14.4); where waves share
+  // it, scalar instructions run beside the others' vector ones (8192 rows: 1220 us, by lane 1275).
+  template <bool kByLane>
   __device__ __forceinline__ void fetch(const AttentionArgs& p, int head, int key0, int length, int pages, int lane0,
                                         uint8_t* keys, uint8_t* values) const {
-    const uint8_t* const k = reinterpret_cast<const uint8_t*>(p.k + head * p.head_stride);
-    const uint8_t* const v = reinterpret_cast<const uint8_t*>(p.v + head * p.head_stride);
+    if constexpr (kByLane) {
+      const int row = key0 - lane0 + (int)(threadIdx.x & 63);
+      const bool held = (uint32_t)pages < (uint32_t)p.num_pages;
+      const uint64_t at = 2 * ((uint64_t)(uint32_t)(held ? pages : 0) * (uint32_t)p.page_stride +
+                               (uint64_t)(uint32_t)(row & ((1 << p.page_shift) - 1)) * (uint32_t)p.slot_stride +
+                               (uint64_t)(uint32_t)head * (uint32_t)p.head_stride);
+      const uint32_t bytes = held ? (uint32_t)max(0, min(8, length - row)) * (uint32_t)p.slot_stride * 2 : 0u;
 #pragma unroll
-    for (int g = 0; g < kRows / 8; ++g) {
-      const int first = key0 + 8 * g, page = __builtin_amdgcn_readlane(pages, lane0 + 8 * g);
-      const bool held = (uint32_t)page < (uint32_t)p.num_pages;
-      const int64_t at =
-          ((int64_t)(held ? page : 0) * p.page_stride + (int64_t)(first & ((1 << p.page_shift) - 1)) * p.slot_stride) * 2;
-      // (the clamp is a vector instruction; the descriptor has to be scalar, or every lane's
-      // is compared in a loop around the DMA)
-      const int rows = __builtin_amdgcn_readfirstlane(held ? max(0, min(8, length - first)) : 0);
-      const uint32_t bytes = (uint32_t)rows * (uint32_t)p.slot_stride * 2;
-      const auto from_k = packed::panel_rsrc(k + at, bytes), from_v = packed::panel_rsrc(v + at, bytes);
+      for (int g = 0; g < kRows / 8; ++g)
+        fetch_group(p, g, lane_value((int64_t)at, lane0 + 8 * g), __builtin_amdgcn_readlane((int)bytes, lane0 + 8 * g), keys, values);
+    } else {
 #pragma unroll
-      for (int i = g * kPer8; i < (g + 1) * kPer8; ++i) {
-        packed::dma_frag(from_k, key[i], 0, keys + i * T::kDmaRows * T::kRow);
-        packed::dma_frag(from_v, value[i], 0, values + i * T::kDmaRows * T::kRow);
+      for (int g = 0; g < kRows / 8; ++g) {
+        const int first = key0 + 8 * g, page = __builtin_amdgcn_readlane(pages, lane0 + 8 * g);
+        const bool held = (uint32_t)page < (uint32_t)p.num_pages;
+        const int64_t at = (int64_t)(held ? page : 0) * p.page_stride + (int64_t)(first & ((1 << p.page_shift) - 1)) * p.slot_stride +
+                           head * p.head_stride;
+        // (the clamp is a vector instruction; the descriptor has to be scalar, or every lane's
+        // is compared in a loop around the DMA)
+        const int rows = __builtin_amdgcn_readfirstlane(held ? max(0, min(8, length - first)) : 0);
+        fetch_group(p, g, 2 * at, (uint32_t)rows * (uint32_t)p.slot_stride * 2, keys, values);
       }
     }
   }
@@ -644,13 +681,15 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
   };
   auto fetch = [&](const Part& w, int step, int pages, int buffer) __attribute__((always_inline)) {
     uint8_t* const to = lds + buffer * 2 * kTileBytes + 16 * wave * T::kRow;
-    lanes.fetch(p, w.head, step * kKeys + 16 * wave, w.r.context + w.r.fresh, pages, 16 * wave, to, to + kTileBytes);
+    lanes.template fetch<false>(p, w.head, step * kKeys + 16 * wave, w.r.context + w.r.fresh, pages, 16 * wave, to, to + kTileBytes);
   };
   auto held_of = [&](int pages) __attribute__((always_inline)) { return __ballot((uint32_t)pages < (uint32_t)p.num_pages); };
   // this lane's row of an item: its token within the request and its query head
   auto row_of = [&](const Part& w, int* local, int* head) __attribute__((always_inline)) {
     const int rows = min(w.r.per_tile, w.r.fresh - w.tile * w.r.per_tile) * p.group;
-    const int row = min(32 * wave + (lane & 31), rows - 1), token = row_token(row, p);
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));  // (made here, not held by the whole kernel)
+    const int row = min((thread >> 1 & ~31) + (thread & 31), rows - 1), token = row_token(row, p);
     *local = w.tile * w.r.per_tile + token, *head = w.head * p.group + row - token * p.group;
     return rows;
   };
@@ -808,7 +847,7 @@ __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
     // number of operations in flight stays the same.
     auto fetch = [&](int i, int pages) __attribute__((always_inline)) {
       uint8_t* const to = lds + (i & 1) * 2 * kTileBytes;
-      lanes.fetch(p, s.head, (from + i) * kKeys, i < count ? length : 0, pages, 0, to, to + kTileBytes);
+      lanes.template fetch<true>(p, s.head, (from + i) * kKeys, i < count ? length : 0, pages, 0, to, to + kTileBytes);
     };
     int pages = pages_of(from), next = pages_of(from + 1);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the item before: its last fetches and stores
@@ -1045,6 +1084,7 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
   p.min_span = few ? 3 : 5;
   p.scale = scale * 1.44269504088896341f;
   p.per_group = 1.f / p.group;
+  p.per_workgroup = 1. / blocks;
   p.records = (int32_t*)workspace;
   p.partial = (float*)((char*)workspace + blocks * kRecordBytes);
   return cache->head_dim == 128 ? launch_attention<128>(p, few, blocks, (hipStream_t)stream)

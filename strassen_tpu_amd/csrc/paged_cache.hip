@@ -278,6 +278,8 @@ int paged_layout(const smx_paged_cache* c) {
   if (c->slot_stride < c->head_dim || c->slot_stride > (1 << 26) || c->page_stride < c->head_dim ||
       c->head_stride < c->head_dim)
     return fail(SMX_ERR_INVALID, "cache strides must be at least head_dim and its slots at most 2^26 elements apart");
+  if (c->page_stride > INT32_MAX || c->head_stride > INT32_MAX)
+    return fail(SMX_ERR_UNSUPPORTED, "pages and heads may be at most 2^31 - 1 elements apart");
   return SMX_OK;
 }
 
