@@ -325,7 +325,12 @@ __global__ __launch_bounds__(Ring<kRows>::kThreads) void int4_tiled(Int4Args p) 
 
   const int stages = (last - first + kWays - 1) / kWays;
 #pragma unroll
-  for (int d = 0; d < kRing - 1; ++d) load(s[d], d, d);
+  for (int d = 0; d < kRing - 1; ++d) {
+    load(s[d], d, d);
+    // the waits below count operations: none of a stage may be moved behind the next one's
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  }
   for (int i = 0; i < stages; i += kRing) {
 #pragma unroll
     for (int d = 0; d < kRing; ++d) {

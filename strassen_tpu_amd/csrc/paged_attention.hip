@@ -856,10 +856,17 @@ __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) q[t] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q_row + 16 * t));
     uint32_t held = (uint32_t)__ballot((uint32_t)pages < (uint32_t)p.num_pages);
+    // The loop's waits count operations: none of those behind the first fetch may be moved before its end.
+    auto in_order = []() __attribute__((always_inline)) {
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
     fetch(0, pages);
+    in_order();
     int after = pages_of(from + 2);
     uint32_t next_held = (uint32_t)__ballot((uint32_t)next < (uint32_t)p.num_pages);
     fetch(1, next);
+    in_order();
 
     Rows<D> o;
     o.clear();

@@ -275,6 +275,24 @@ def test_attention_of_many_requests(new_high, max_new, window):
     check_attention(smx.paged_attention(q, k, v, plan, window=window), want, size)
 
 
+@pytest.mark.parametrize("heads,kv_heads,max_new", [(64, 8, 1), (8, 2, 4), (16, 2, 16)])
+def test_attention_gives_the_same_bits_again(heads, kv_heads, max_new):
+    """Many spans that begin and end within requests, their keys from memory: nothing is used before it has arrived."""
+    context = [(b * 997) % 4000 + 1 for b in range(48)]
+    new = [1 + b % max_new for b in range(48)]
+    plan, k, v, keys, values, g = make_step(context, new, page=16, kv_heads=kv_heads, dim=128)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=16, num_pages=plan.num_pages,
+                          tokens=plan.tokens, max_new=max_new)
+    q = torch.randn(plan.tokens, heads, 128, device=DEV, generator=g).to(torch.bfloat16)
+    want, size = attend64(q, keys, values, context, new, None)
+    got = smx.paged_attention(q, k, v, plan)
+    check_attention(got, want, size)
+    other = torch.empty(1 << 28, device=DEV)
+    for _ in range(12):
+        other.zero_()  # leaves nothing of the cache in the caches
+        assert torch.equal(smx.paged_attention(q, k, v, plan), got)
+
+
 @pytest.mark.parametrize("heads,kv_heads,max_new", [(8, 8, 32), (32, 1, 1), (6, 2, 10), (64, 2, 1)])
 @pytest.mark.parametrize("window", [None, 1, 2**31 - 1])
 def test_attention_of_few_rows(heads, kv_heads, max_new, window):
