@@ -405,8 +405,8 @@ int smx_qk_norm_rope(int64_t m, int64_t n, const float* x, int64_t ldx, const vo
 #define SMX_PAGED_ROPE_F32 4
 
 /* bf16 keys and values of one layer: [num_pages, page_size, kv_heads, head_dim], any strides
- * (in elements) whose head rows are 16-byte aligned runs, the same for both. Powers of two
- * from 8 to 4096 as page_size, head_dim 64 or 128. */
+ * (in elements) whose head rows are 16-byte aligned runs, the same for both: pages and heads at most
+ * 2^31 - 1 elements apart, slots 2^26. Powers of two from 8 to 4096 as page_size, head_dim 64 or 128. */
 typedef struct smx_paged_cache {
   void *k, *v;
   int64_t page_stride, slot_stride, head_stride;

@@ -120,7 +120,9 @@ template <int kRows, int kCols, int kGroups, bool kZeros>
 __device__ __forceinline__ void multiply(f32x4 (&acc)[kCols][kRows], const Codes<kCols>& s, const u32x4 (&x)[kRows][4],
                                          const Widen& widen) {
   constexpr int kSteps = 4 / kGroups;  // MFMA steps of 32 in a group
-  const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80});
+  // sum: of x against ones, or without zero points against -24 = -(16 + 8), from which the products start
+  constexpr uint32_t kOnes = kZeros ? 0x3f803f80 : 0xc1c0c1c0;
+  const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes});
   auto group = [&](auto index) __attribute__((always_inline)) {
     constexpr int g = decltype(index)::value;
     f32x4 sum[kRows];
@@ -135,7 +137,7 @@ __device__ __forceinline__ void multiply(f32x4 (&acc)[kCols][kRows], const Codes
     for (int c = 0; c < kCols; ++c) {
       f32x4 part[kRows];
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) part[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int r = 0; r < kRows; ++r) part[r] = kZeros ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[r];
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) {
         const bf16x8 a = widen(s.codes[c][g * kSteps + t]);
@@ -144,13 +146,17 @@ __device__ __forceinline__ void multiply(f32x4 (&acc)[kCols][kRows], const Codes
           part[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, x[r][g * kSteps + t]), part[r], 0, 0, 0);
       }
       const f32x4 scale = quad_columns<kGroups, g>(hi_f32(s.scales[c]));
-      f32x4 zero = {-24.f, -24.f, -24.f, -24.f};
-      if constexpr (kZeros) zero = quad_columns<kGroups, g>(lo_f32(s.scales[c]));
+      if constexpr (kZeros) {
+        const f32x4 zero = quad_columns<kGroups, g>(lo_f32(s.scales[c]));
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) part[r][i] = __builtin_fmaf(zero[i], sum[r][i], part[r][i]);
+      }
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          acc[c][r][i] = __builtin_fmaf(scale[i], __builtin_fmaf(zero[i], sum[r][i], part[r][i]), acc[c][r][i]);
+        for (int i = 0; i < 4; ++i) acc[c][r][i] = __builtin_fmaf(scale[i], part[r][i], acc[c][r][i]);
     }
   };
   group(std::integral_constant<int, 0>{});

@@ -113,7 +113,7 @@ def _heads(heads=8, data=P, token=1024, head=128):
 
 
 BAD_CACHES = [{"k": None}, {"v": P + 8}, {"page_stride": 12}, {"slot_stride": 100}, {"slot_stride": 64}, {"head_stride": 8},
-              {"num_pages": 0}, {"page_size": 12}, {"kv_heads": 0}, {"head_dim": 96}, {"slot_stride": 1 << 27},
+              {"num_pages": 0}, {"page_size": 12}, {"kv_heads": 0}, {"head_dim": 96}, {"slot_stride": 1 << 27}, {"page_stride": 1 << 31}, {"head_stride": 1 << 31},
               {"num_pages": 1 << 28}]
 
 
