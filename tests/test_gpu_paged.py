@@ -370,6 +370,31 @@ def test_attention_scale_and_out():
     assert (out[10:] == 7).all()  # rows behind the last request stay
 
 
+@pytest.mark.parametrize("max_new", [None, 2])
+def test_attention_in_place_of_the_queries(max_new):
+    """Each row is read before it is written, also those of requests that several workgroups share."""
+    context, new = [5000, 12, 700], [2, 1, 2]
+    plan, k, v, keys, values, g = make_step(context, new, page=16, kv_heads=2, dim=128)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=16, num_pages=plan.num_pages,
+                          tokens=plan.tokens, max_new=max_new)
+    q = torch.randn(plan.tokens, 16, 128, device=DEV, generator=g).to(torch.bfloat16)
+    want = smx.paged_attention(q, k, v, plan)
+    assert smx.paged_attention(q, k, v, plan, out=q) is q
+    assert torch.equal(q, want)
+
+
+def test_attention_of_a_long_prompt():
+    """100,000 rows of one request, whose tiles' counts pass 16 bits, against sampled rows."""
+    new, page, heads = 100_000, 64, 2
+    plan, k, v, keys, values, g = make_step([0], [new], page=page, kv_heads=1, dim=64)
+    q = torch.randn(new, heads, 64, device=DEV, generator=g).to(torch.bfloat16)
+    got = smx.paged_attention(q, k, v, plan)
+    for row in (0, 1, 63, 64, 4095, 31337, 65535, 65536, new - 2, new - 1):
+        want, size = attend64(q[row:row + 1], [keys[0][:row + 1]], [values[0][:row + 1]], [row], [1], None)
+        check_attention(got[row:row + 1], want, size)
+    assert got.isfinite().all()
+
+
 def test_attention_of_requests_that_are_not_admitted():
     """Their rows are zero, the others' as if alone."""
     plan, k, v, keys, values, g = make_step([20, 30, 4], [3, 5, 2], page=8, kv_heads=2, dim=64, pad=1)
@@ -576,6 +601,7 @@ def test_refusals():
             ({"k_cache": k[:2], "v_cache": v[:2]}, "pages"), ({"scale": 0.0}, "scale"), ({"scale": math.inf}, "scale"),
             ({"window": 0}, "window"), ({"window": -3}, "window"), ({"out": q.float()}, "bf16"),
             ({"out": torch.empty(4, 8, 130, dtype=torch.bfloat16, device=DEV)[..., 1:129]}, "aligned"),
+            ({"out": torch.empty(1, 8, 128, dtype=torch.bfloat16, device=DEV).expand(4, 8, 128)}, "on each other"),
             ({"q": q.cpu()}, "HIP device"), ({"q": q.clone().requires_grad_()}, "gradients")):
         with pytest.raises(ValueError, match=message):
             smx.paged_attention(**{**good, **change})
