@@ -629,30 +629,32 @@ constexpr int kPartialFloats = 256 * (D / 2 + 2);
 template <int D>
 constexpr int kFewPartialFloats = 32 * (D + 2);
 
-// Rows of 32 D-wide outputs to memory: lane l of half h holds columns 8 (e / 4) + 4 h ..
-// of block x; two lanes exchange halves so that each stores 16 bytes.
+// One block of 32 columns of 32 rows to memory, `to` the lane's row there: lane l of half h holds columns
+// 8 (e / 4) + 4 h ..; two lanes exchange halves so that each stores 16 bytes.
+__device__ __forceinline__ void store_block(uint16_t* to, const f32x16& o, float inverse, bool valid, int half) {
+#pragma unroll
+  for (int e = 0; e < 16; e += 8) {
+    // columns 4 h .. of groups e / 4 (mine if half 0) and e / 4 + 1 (mine if half 1)
+    const uint32_t a0 = pack_bf16(o[e] * inverse, o[e + 1] * inverse);
+    const uint32_t a1 = pack_bf16(o[e + 2] * inverse, o[e + 3] * inverse);
+    const uint32_t b0 = pack_bf16(o[e + 4] * inverse, o[e + 5] * inverse);
+    const uint32_t b1 = pack_bf16(o[e + 6] * inverse, o[e + 7] * inverse);
+    // swap: a's upper half with b's lower half
+    const auto r0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+    const auto r1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+    const u32x4 v = {r0[0], r1[0], r0[1], r1[1]};
+    if (valid) *reinterpret_cast<u32x4*>(to + 8 * ((e >> 2) + half)) = v;
+  }
+}
+
 template <int D>
 __device__ __forceinline__ void store_rows(const AttentionArgs& p, const f32x16 (&o)[D / 32], float inverse, bool valid,
                                            int64_t token, int head) {
   int thread = threadIdx.x;
   asm volatile("" : "+v"(thread));  // (offsets are made here, not held by the whole kernel)
-  const int half = thread >> 5 & 1;
   uint16_t* const to = p.out + token * p.out_token + head * p.out_head;
 #pragma unroll
-  for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-    for (int e = 0; e < 16; e += 8) {
-      // columns 4 h .. of groups e / 4 (mine if half 0) and e / 4 + 1 (mine if half 1)
-      const uint32_t a0 = pack_bf16(o[x][e] * inverse, o[x][e + 1] * inverse);
-      const uint32_t a1 = pack_bf16(o[x][e + 2] * inverse, o[x][e + 3] * inverse);
-      const uint32_t b0 = pack_bf16(o[x][e + 4] * inverse, o[x][e + 5] * inverse);
-      const uint32_t b1 = pack_bf16(o[x][e + 6] * inverse, o[x][e + 7] * inverse);
-      // swap: a's upper half with b's lower half
-      const auto r0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
-      const auto r1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
-      const u32x4 v = {r0[0], r1[0], r0[1], r1[1]};
-      if (valid) *reinterpret_cast<u32x4*>(to + 32 * x + 8 * ((e >> 2) + half)) = v;
-    }
+  for (int x = 0; x < D / 32; ++x) store_block(to + 32 * x, o[x], inverse, valid, thread >> 5 & 1);
 }
 
 __device__ __forceinline__ float inverse_of(float sum) { return sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum; }
@@ -972,41 +974,38 @@ __global__ __launch_bounds__(1024) void paged_join_few(AttentionArgs p) {
       make_uint2(pack_bf16(value[0] * inverse, value[1] * inverse), pack_bf16(value[2] * inverse, value[3] * inverse));
 }
 
-// Adds up the partial sums of the items that spans cut: one workgroup per
-// record, its threads in the layout that paged_attend wrote them in.
+// Adds up the partial sums of the items that spans cut, four parts at a time: one workgroup per
+// record, 256 threads in the layout that paged_attend wrote them in for each block of 32 columns (200 rows of four heads on 3000
+// keys, 14 items of about eleven parts: 28.7 us with the attention before it; 256 threads in all, part by part: 43).
 template <int D>
-__global__ __launch_bounds__(256) void paged_join(AttentionArgs p) {
+__global__ __launch_bounds__(8 * D) void paged_join(AttentionArgs p) {
   const Record record = reinterpret_cast<const Record*>(p.records)[blockIdx.x];
   if (record.others <= 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  auto slot = [&](int i) { return p.partial + (2 * (int64_t)(record.worker + i) + (i == 0)) * kPartialFloats<D>; };
-  float top = -INFINITY;
-  for (int i = 0; i <= record.others; ++i) top = fmaxf(top, slot(i)[256 * (D / 2) + threadIdx.x]);
-  f32x16 o[D / 32];
+  const int thread = threadIdx.x & 255, x = threadIdx.x >> 8, lane = threadIdx.x & 63, wave = thread >> 6;
+  f32x16 o;
 #pragma unroll
-  for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[x][e] = 0.f;
-  float sum = 0.f;
+  for (int e = 0; e < 16; ++e) o[e] = 0.f;
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
   for (int i = 0; i <= record.others; ++i) {
-    const float* const from = slot(i);
-    const float mine = from[256 * (D / 2) + threadIdx.x];
-    const float factor = mine == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - top);
-    sum += from[256 * (D / 2 + 1) + threadIdx.x] * factor;
+    const float* const from = p.partial + (2 * (int64_t)(record.worker + i) + (i == 0)) * kPartialFloats<D>;
+    const float mine = from[256 * (D / 2) + thread], part = from[256 * (D / 2 + 1) + thread];
+    f32x4 v[4];
 #pragma unroll
-    for (int x = 0; x < D / 32; ++x)
+    for (int e = 0; e < 4; ++e) v[e] = reinterpret_cast<const f32x4*>(from)[(4 * x + e) * 256 + thread];
+    const float next = fmaxf(top, mine), ref = next == -INFINITY ? 0.f : next;
+    const float keep = __builtin_amdgcn_exp2f(top - ref), add = __builtin_amdgcn_exp2f(mine - ref);
+    top = next;
+    sum = sum * keep + part * add;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const f32x4 v = reinterpret_cast<const f32x4*>(from)[(4 * x + e) * 256 + threadIdx.x];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[x][4 * e + j] += v[j] * factor;
-      }
+    for (int e = 0; e < 16; ++e) o[e] = o[e] * keep + v[e >> 2][e & 3] * add;
   }
   const int fresh = p.rows[record.request];
   const int tile_rows = min(p.tile_tokens, fresh - record.tile * p.tile_tokens) * p.group;
   const int at = 32 * wave + (lane & 31), row = min(at, tile_rows - 1);
   const int64_t token = p.starts[record.request] + record.tile * p.tile_tokens + row / p.group;
-  store_rows<D>(p, o, inverse_of(sum), at < tile_rows, token, record.head * p.group + row % p.group);
+  store_block(p.out + token * p.out_token + (record.head * p.group + row % p.group) * p.out_head + 32 * x, o, inverse_of(sum),
+              at < tile_rows, lane >> 5);
 }
 
 // Workgroups of a launch, a multiple of the 8 XCDs: as many as a CU holds (two of paged_attend, by its
@@ -1033,7 +1032,7 @@ int launch_attention(AttentionArgs& p, bool few, unsigned blocks, hipStream_t st
   if (e != hipSuccess) return fail(SMX_ERR_LAUNCH, "hipFuncSetAttribute: %s", hipGetErrorString(e));
   hipLaunchKernelGGL(kern, dim3(blocks), dim3(few ? 64 : 256), lds, stream, p);
   if (int rc = check_launch()) return rc;
-  hipLaunchKernelGGL(few ? paged_join_few<D> : paged_join<D>, dim3(blocks), dim3(few ? 1024 : 256), 0, stream, p);
+  hipLaunchKernelGGL(few ? paged_join_few<D> : paged_join<D>, dim3(blocks), dim3(few ? 1024 : 8 * D), 0, stream, p);
   return check_launch();
 }
 
@@ -1096,7 +1095,7 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
   const bool few = few_rows(step->max_new, p.group);
   const int blocks = workgroups(cus, few);
   p.tile_tokens = (few ? 32 : 128) / p.group;
-  p.min_span = few ? 3 : 5;
+  p.min_span = few ? 2 : 5;
   p.scale = scale * 1.44269504088896341f;
   p.per_group = 1.f / p.group;
   p.per_workgroup = 1. / blocks;
