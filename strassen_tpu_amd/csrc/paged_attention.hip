@@ -980,14 +980,17 @@ __global__ __launch_bounds__(1024) void paged_join_few(AttentionArgs p) {
       make_uint2(pack_bf16(value[0] * inverse, value[1] * inverse), pack_bf16(value[2] * inverse, value[3] * inverse));
 }
 
-// Adds up the partial sums of the items that spans cut, four parts at a time: one workgroup per
-// record, 256 threads in the layout that paged_attend wrote them in for each block of 32 columns (200 rows of four heads on 3000
-// keys, 14 items of about eleven parts: 28.7 us with the attention before it; 256 threads in all, part by part: 43).
+constexpr int kJoinThreads = 256;
+
+// Adds up the partial sums of the items that spans cut, four parts at a time: D / 32 workgroups per
+// record, 256 threads in the layout that paged_attend wrote them in for each block of 32 columns. 200 rows of
+// four heads on 3000 keys, 14 items of about eleven parts: 27.0 us with the attention before it (one workgroup
+// with all threads: 28.4; one of 256 threads, part by part: 43).
 template <int D>
-__global__ __launch_bounds__(8 * D) void paged_join(AttentionArgs p) {
+__global__ __launch_bounds__(kJoinThreads) void paged_join(AttentionArgs p) {
   const Record record = reinterpret_cast<const Record*>(p.records)[blockIdx.x];
   if (record.others <= 0) return;
-  const int thread = threadIdx.x & 255, x = threadIdx.x >> 8, lane = threadIdx.x & 63, wave = thread >> 6;
+  const int thread = threadIdx.x, x = blockIdx.y, lane = thread & 63, wave = thread >> 6;
   f32x16 o;
 #pragma unroll
   for (int e = 0; e < 16; ++e) o[e] = 0.f;
@@ -1038,7 +1041,8 @@ int launch_attention(AttentionArgs& p, bool few, unsigned blocks, hipStream_t st
   if (e != hipSuccess) return fail(SMX_ERR_LAUNCH, "hipFuncSetAttribute: %s", hipGetErrorString(e));
   hipLaunchKernelGGL(kern, dim3(blocks), dim3(few ? 64 : 256), lds, stream, p);
   if (int rc = check_launch()) return rc;
-  hipLaunchKernelGGL(few ? paged_join_few<D> : paged_join<D>, dim3(blocks), dim3(few ? 1024 : 8 * D), 0, stream, p);
+  hipLaunchKernelGGL(few ? paged_join_few<D> : paged_join<D>, dim3(blocks, few ? 1 : D / 32),
+                     dim3(few ? 1024 : kJoinThreads), 0, stream, p);
   return check_launch();
 }
 
