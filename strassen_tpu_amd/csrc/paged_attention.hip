@@ -682,8 +682,8 @@ __device__ __forceinline__ float inverse_of(float sum) { return sum > 0.f ? 1.f 
 // 16384 cached ones: 1.33 ms, 0.88 PFLOP/s. Matrix cores, vector units and LDS are each busy 40 to 44% of the time
 // (one workgroup a CU: 2.0 ms): two waves a SIMD do not cover each other's way from a step's keys to
 // its output, and registers and LDS hold no third. Without the exponentials 9% less, without the
-// values' reads nothing. Scores of the next step beside the weights of this one, in the same wave: 209 registers
-// at head_dim 64, 1.2 ms for 8192 tokens where this takes 0.9.
+// values' reads nothing. Scores of the next step beside the weights of this one, in the same wave: 1.50 ms (247
+// registers); the next step's first keys read before its DMAs are started: 64 registers too many.
 template <int D>
 __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
   using T = Tile<D>;
@@ -833,8 +833,8 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
 // four of them (32 KB of LDS each at head_dim 128) keep up to 128 KB of a CU's reads in
 // flight. Rows are few: what bounds it is the cache's bytes: 64 requests, 260,000 cached tokens of 4 KB, 198 us
 // and 7 in paged_join_few (5.2 TB/s); four of 131,000 tokens 367 and 9 (5.7). Short caches are
-// bound by latency: 1000 tokens 10 us, of which 1.7 pass until the span is found, 1.5 until the first
-// loads are on their way, 1.2 each of three steps.
+// bound by latency: 1000 tokens 9 us, of which 1.6 pass until the span is found, 1.4 until the first
+// loads are on their way, 1.2 in a step.
 template <int D>
 __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
   using T = Tile<D>;
@@ -1118,6 +1118,9 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
   const bool few = few_rows(step->max_new, p.group);
   const int blocks = workgroups(cus, few);
   p.tile_tokens = (few ? 32 : 128) / p.group;
+  // Units of a span at least, so that few partial sums are joined: an item's start and one step of 32 keys (one row on
+  // 1000 keys 12.4 us; with two steps 13.1, three 15.4), two of 64 (two requests of 60 rows on 1000: 25.4; one
+  // 27.4, three 26.0).
   p.min_span = few ? 2 : 5;
   p.scale = scale * 1.44269504088896341f;
   p.per_group = 1.f / p.group;
