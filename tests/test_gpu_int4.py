@@ -47,6 +47,20 @@ SHAPES = [(1, 32, 1, 32), (1, 128, 16, 128), (3, 96, 33, 32), (16, 192, 40, 64),
           (33, 1024, 2047, 64), (64, 640, 96, 128), (65, 1056, 250, 32), (130, 384, 31, 128), (2, 25600, 48, 128)]
 
 
+@pytest.mark.parametrize("m,k,n,group", [(1, 25600, 1024, 128), (16, 5120, 20000, 32), (16, 25600, 512, 64), (61, 5120, 2048, 32)])
+def test_int4_gives_the_same_bits_again(m, k, n, group):
+    """Weights from memory: nothing is used before it has arrived."""
+    codes, scales, zero, w, spread, g = weight(k, n, group, True)
+    laid = smx.int4_weight_layout(codes, scales, zero, group=group)
+    x = torch.randn(m, k, device=DEV, generator=g).to(torch.bfloat16)
+    got = smx.int4_matmul(x, laid)
+    check(got, x, w, spread)
+    other = torch.empty(1 << 28, device=DEV)
+    for _ in range(12):
+        other.zero_()  # leaves nothing of the weight in the caches
+        assert torch.equal(smx.int4_matmul(x, laid), got)
+
+
 @pytest.mark.parametrize("m,k,n,group", SHAPES)
 @pytest.mark.parametrize("zeros", [True, False])
 def test_int4_matmul(m, k, n, group, zeros):
