@@ -28,8 +28,6 @@
 namespace smx {
 namespace {
 
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
 struct Int4Args {
   const uint16_t* x;
   int64_t ldx;
@@ -79,14 +77,10 @@ __device__ __forceinline__ f32x4 quad_columns(float x) {
 }
 
 // One K tile's codes and scales of a wave's kCols column tiles.
-template <int kCols, int kGroups, bool kZeros>
+template <int kCols>
 struct Codes {
-  // Zero points of several groups a tile are subtracted by a matrix instruction each (multiply)
-  static constexpr bool kByColumn = kZeros && kGroups > 1;
-  static constexpr int kLoads = (kByColumn ? 3 : 2) * kCols;
   u32x4 codes[kCols];
-  uint32_t scales[kCols];                          // lane j of a quad's 16: column j / kGroups % 4, group j % kGroups
-  uint32_t columns[kCols][kByColumn ? kGroups : 1];  // the same words: lane l < 16 all groups of column l, others zeros
+  uint32_t scales[kCols];  // lane j of a quad's 16: column j / kGroups % 4, group j % kGroups
 };
 
 // A wave's column tiles as buffers that end with their last K tile: later ones load
@@ -95,7 +89,7 @@ struct Codes {
 template <int kCols, int kGroups>
 struct Columns {
   __amdgpu_buffer_rsrc_t codes[kCols], scales[kCols];
-  uint32_t code_at, scale_at, column_at;
+  uint32_t code_at, scale_at;
   int k_tiles;
 
   __device__ __forceinline__ Columns(const Int4Args& p, int64_t tile0) : k_tiles(p.k_tiles) {
@@ -110,26 +104,14 @@ struct Columns {
     }
     code_at = lane * 16;
     scale_at = ((lane >> 4) * 4 * kGroups + (lane & (4 * kGroups - 1))) * 4;
-    column_at = lane < 16 ? lane * 4 * kGroups : 1u << 30;  // behind every buffer of scales
   }
 
-  template <bool kZeros>
-  __device__ __forceinline__ void load(Codes<kCols, kGroups, kZeros>& s, int at) const {
+  __device__ __forceinline__ void load(Codes<kCols>& s, int at) const {
     const int kt = min(at, k_tiles);
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
       s.codes[c] = __builtin_amdgcn_raw_buffer_load_b128(codes[c], code_at, kt * 1024, 2);  // 2: non-temporal
       s.scales[c] = __builtin_amdgcn_raw_buffer_load_b32(scales[c], scale_at, kt * (64 * kGroups), 2);
-      if constexpr (Codes<kCols, kGroups, kZeros>::kByColumn) {
-        if constexpr (kGroups == 4) {
-          const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(scales[c], column_at, kt * (64 * kGroups), 2);
-#pragma unroll
-          for (int g = 0; g < 4; ++g) s.columns[c][g] = v[g];
-        } else {
-          const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(scales[c], column_at, kt * (64 * kGroups), 2);
-          s.columns[c][0] = v[0], s.columns[c][1] = v[1];
-        }
-      }
     }
   }
 };
@@ -137,7 +119,7 @@ struct Columns {
 // acc += one K tile. x[r][t]: 16 rows of step t (32 of k) as the MFMA's B operand, lane l
 // holding row l % 16, k = 8 (l / 16) .. + 7; acc[c][r]: lane l's columns 4 (l / 16) .. + 3 of row l % 16.
 template <int kRows, int kCols, int kGroups, bool kZeros>
-__device__ __forceinline__ void multiply(f32x4 (&acc)[kCols][kRows], const Codes<kCols, kGroups, kZeros>& s, const u32x4 (&x)[kRows][4],
+__device__ __forceinline__ void multiply(f32x4 (&acc)[kCols][kRows], const Codes<kCols>& s, const u32x4 (&x)[kRows][4],
                                          const Widen& widen) {
   constexpr int kSteps = 4 / kGroups;  // MFMA steps of 32 in a group
   // sum: of x against ones, or without zero points against -24 = -(16 + 8), from which the products start
@@ -166,12 +148,7 @@ __device__ __forceinline__ void multiply(f32x4 (&acc)[kCols][kRows], const Codes
           part[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, x[r][g * kSteps + t]), part[r], 0, 0, 0);
       }
       const f32x4 scale = quad_columns<kGroups, g>(hi_f32(s.scales[c]));
-      if constexpr (Codes<kCols, kGroups, kZeros>::kByColumn) {
-        // column (lane l < 16) times sum (row l % 16), in FP32; the other lanes' three products are with zeros
-        const float zero = lo_f32(s.columns[c][g]);
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) part[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(zero, sum[r][0], part[r], 0, 0, 0);
-      } else if constexpr (kZeros) {
+      if constexpr (kZeros) {
         const f32x4 zero = quad_columns<kGroups, g>(lo_f32(s.scales[c]));
 #pragma unroll
         for (int r = 0; r < kRows; ++r)
@@ -227,7 +204,7 @@ __global__ __launch_bounds__(kWaves * 64) void int4_few(Int4Args p) {
   f32x4 acc[kCols][1];
 #pragma unroll
   for (int c = 0; c < kCols; ++c) acc[c][0] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Codes<kCols, kGroups, kZeros> s[2];
+  Codes<kCols> s[2];
   columns.load(s[0], wave);
   columns.load(s[1], wave + kWaves);
 
@@ -303,6 +280,7 @@ struct Ring {
   static constexpr int kWays = 2, kRing = kRows == 1 ? 4 : 3;
   static constexpr int kThreads = 256 * kWays, kTileBytes = kRows * 4096, kStage = kWays * kTileBytes;
   static constexpr int kDmas = kRows;      // a wave's for one stage, of 1 KB
+  static constexpr int kLoads = 4 + kDmas;  // and its codes and scales
   static constexpr int kLds = kRing * kStage > kWays * 8 * kRows * 1024 ? kRing * kStage : kWays * 8 * kRows * 1024;
 };
 
@@ -330,10 +308,10 @@ __global__ __launch_bounds__(Ring<kRows>::kThreads) void int4_tiled(Int4Args p) 
     x_chunk[d] = (lane & 15) ^ (row & 15);
     x_at[d] = row < rows ? (uint32_t)(row * p.ldx) * 2 + 16 * x_chunk[d] : ~0u;
   }
-  Codes<2, kGroups, kZeros> s[kRing];
+  Codes<2> s[kRing];
   // K tiles behind the share's last are loaded as those behind the weight's: as zeros, without
   // memory traffic.
-  auto load = [&](Codes<2, kGroups, kZeros>& codes, int slot, int stage) __attribute__((always_inline)) {
+  auto load = [&](Codes<2>& codes, int slot, int stage) __attribute__((always_inline)) {
     const int begin = first + stage * kWays;
     columns.load(codes, begin + way < last ? begin + way : p.k_tiles);
 #pragma unroll
@@ -367,7 +345,7 @@ __global__ __launch_bounds__(Ring<kRows>::kThreads) void int4_tiled(Int4Args p) 
       if (i + d >= stages) break;
       // This stage's loads are done, kRing - 2 stages' are on their way; then everybody's, and the
       // stage before has been multiplied: its slot is free.
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((kRing - 2) * (Codes<2, kGroups, kZeros>::kLoads + R::kDmas)) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((kRing - 2) * R::kLoads) : "memory");
       constexpr int kFree = kRing - 1;
       load(s[(d + kFree) % kRing], (d + kFree) % kRing, i + d + kFree);
       u32x4 x[kRows][4];
