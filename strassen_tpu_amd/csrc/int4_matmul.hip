@@ -464,8 +464,10 @@ int64_t int4_workspace(const Int4Plan& plan, int64_t m, int64_t tiles) {
 
 template <class K>
 int launch_int4_kernel(K kern, dim3 grid, int threads, int lds, const Int4Args& p, hipStream_t stream) {
-  hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (e != hipSuccess) return fail(SMX_ERR_LAUNCH, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+  if (lds > 48 * 1024) {
+    hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return fail(SMX_ERR_LAUNCH, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+  }
   hipLaunchKernelGGL(kern, grid, dim3(threads), lds, stream, p);
   return check_launch();
 }

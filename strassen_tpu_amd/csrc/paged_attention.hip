@@ -1050,8 +1050,10 @@ template <int D>
 int launch_attention(AttentionArgs& p, bool few, unsigned blocks, hipStream_t stream) {
   auto kern = few ? paged_attend_few<D> : paged_attend<D>;
   const int lds = (few ? 4 * 32 : 4 * 64) * 2 * D;
-  hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (e != hipSuccess) return fail(SMX_ERR_LAUNCH, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+  if (lds > 48 * 1024) {
+    hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return fail(SMX_ERR_LAUNCH, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+  }
   hipLaunchKernelGGL(kern, dim3(blocks), dim3(few ? 64 : 256), lds, stream, p);
   if (int rc = check_launch()) return rc;
   hipLaunchKernelGGL(few ? paged_join_few<D> : paged_join<D>, dim3(blocks, few ? 1 : D / 32),

@@ -195,12 +195,17 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t) {
     Tensor parts[8];
     int32_t* at[8];
     int64_t from = 0;
+    int32_t* const base = memory.mutable_data_ptr<int32_t>();
     for (int i = 0; i < 8; ++i) {
-      parts[i] = memory.narrow(0, from, sizes[i]);
-      at[i] = memory.mutable_data_ptr<int32_t>() + from;
+      // a view of the memory, made directly (narrow() and view() take 3 us for the eight)
+      parts[i] = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(memory.storage()), memory.key_set(),
+                                                          c10::scalarTypeToTypeMeta(i ? at::kInt : at::kLong));
+      c10::TensorImpl* const view = parts[i].unsafeGetTensorImpl();
+      view->set_storage_offset(memory.storage_offset() + from);  // the int64 one lies at the front
+      view->set_sizes_contiguous({i ? sizes[i] : tokens});
+      at[i] = base + from;
       from += sizes[i];
     }
-    parts[0] = parts[0].view(at::kLong);
     auto* p = new Plan{tables, memory, device, page_size, num_pages, max_context, reinterpret_cast<int64_t*>(at[0]), {}};
     PyObject* const capsule = PyCapsule_New(p, kPlan, [](PyObject* c) {
       delete static_cast<Plan*>(PyCapsule_GetPointer(c, kPlan));
