@@ -6,6 +6,7 @@
 #pragma once
 
 #include "common.hpp"
+#include "overlap.hpp"
 
 namespace smx {
 
@@ -17,6 +18,14 @@ int device_cus(int* cus);
 
 // Checks the description of a paged cache (paged_cache.hip).
 int paged_layout(const smx_paged_cache* c);
+
+// The head rows of a paged cache's keys or values, and of a step's tokens.
+inline Runs cache_runs(const smx_paged_cache& c, const void* at) {
+  return Runs{at, c.head_dim, {{c.num_pages, c.page_stride}, {c.page_size, c.slot_stride}, {c.kv_heads, c.head_stride}}};
+}
+inline Runs head_runs(const smx_heads& x, int64_t tokens, int64_t head_dim) {
+  return Runs{x.data, head_dim, {{tokens, x.token_stride}, {x.heads, x.head_stride}, {1, 0}}};
+}
 
 inline int check_launch() {
   hipError_t e = hipGetLastError();

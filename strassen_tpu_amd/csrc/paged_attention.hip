@@ -1098,6 +1098,14 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
     if ((uintptr_t)x->data % 16 || x->token_stride % 8 || x->head_stride % 8 || x->token_stride < 0 ||
         x->head_stride < 0)
       return fail(SMX_ERR_INVALID, "head rows must be 16-byte aligned");
+  // A workgroup stores its rows while others load theirs: no row of out may be another's, nor a query of
+  // another row, nor a key or value.
+  const Runs from = head_runs(*q, step->tokens, cache->head_dim), to = head_runs(*out, step->tokens, cache->head_dim);
+  if (!lie_apart(to)) return fail(SMX_ERR_INVALID, "out holds rows that lie on each other");
+  if (!same_runs(from, to) && meet(from, to))
+    return fail(SMX_ERR_INVALID, "out must be the queries themselves or share no memory with them");
+  for (const void* x : {cache->k, cache->v})
+    if (meet(cache_runs(*cache, x), to)) return fail(SMX_ERR_INVALID, "out must share no memory with the cache");
   if (!(scale > 0.f) || !(scale < INFINITY)) return fail(SMX_ERR_INVALID, "scale must be positive and finite");
   if (window < 0) return fail(SMX_ERR_INVALID, "window must not be negative (0: none)");
   int cus = 0;

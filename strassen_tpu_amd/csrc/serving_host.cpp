@@ -5,7 +5,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 
@@ -374,7 +373,6 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t) {
       rows = smx_heads{out.mutable_data_ptr(), q.heads * head_dim, head_dim, q.heads};
     } else {
       rows = heads_of(a[6], "out", plan, q.heads, head_dim, nullptr);
-      if (at::has_internal_overlap(tensor(a[6], "out")) == at::MemOverlap::Yes) refuse("out holds rows that lie on each other");
     }
     int64_t need = 0;
     check(lib.attention_bytes((int32_t)head_dim, &need));

@@ -1,0 +1,52 @@
+"""Calls of the serving operators at the edge of what they take, on the GPU: what is refused, and
+results where lengths, values and layouts are odd."""
+
+import math
+
+import pytest
+import torch
+
+import strassen_tpu_amd as smx
+from test_gpu_paged import attend64, check_attention, i32, make_step
+from test_gpu_parity import DEV, say
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _announce(request):
+    say(f"\n[gpu] {request.node.nodeid}")
+    yield
+    torch.cuda.synchronize()
+
+
+def bf16(*shape, g=None):
+    return torch.randn(*shape, device=DEV, generator=g).to(torch.bfloat16)
+
+
+def test_attention_refuses_results_that_overlap():
+    plan, k, v, *_, g = make_step([9], [4], page=8, kv_heads=2, dim=128)
+    rows = bf16(5, 8, 128, g=g)
+    flat = bf16(5 * 8 * 128, g=g)
+    for q, out, message in (
+            (rows[:4], rows[1:], "queries"), (rows[1:], rows[:4], "queries"),
+            (rows[:4, :4], rows[:4, 2:6], "queries"),
+            (rows[:4], flat.as_strided((4, 8, 128), (512, 128, 1)), "on each other"),
+            (rows[:4, :2], k.flatten(0, 1)[:4], "cache"), (rows[:4, :2], v.flatten(0, 1)[8:12], "cache")):
+        with pytest.raises(ValueError, match=message):
+            smx.paged_attention(q, k, v, plan, out=out)
+
+
+@pytest.mark.parametrize("max_new", [None, 1])
+def test_attention_into_columns_beside_the_queries(max_new):
+    """Queries and result interleaved in one tensor's memory, row by row, share none of it."""
+    context, new = [3000, 12, 90], [1, 1, 1]
+    plan, k, v, keys, values, g = make_step(context, new, page=16, kv_heads=2, dim=128, pad=2)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=16, num_pages=plan.num_pages,
+                          tokens=plan.tokens, max_new=max_new)
+    both = bf16(plan.tokens, 16, 128, g=g)
+    want, size = attend64(both[:, :8], keys, values, context, new, None)
+    kept = both.clone()
+    smx.paged_attention(both[:, :8], k, v, plan, out=both[:, 8:])
+    check_attention(both[:3, 8:], want[:3], size[:3])
+    assert torch.equal(both[:, :8], kept[:, :8]) and torch.equal(both[3:], kept[3:])
