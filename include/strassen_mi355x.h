@@ -460,7 +460,8 @@ int smx_paged_plan(int32_t requests, int32_t width, int32_t page_size, int32_t n
  * (dense [tokens, heads, head_dim], rows of position -1 zero), are RMS-normalised over
  * head_dim (q_scale, k_scale [head_dim]) and rotated by their positions (rope_cos,
  * rope_sin: row `position`, head_dim / 2 values), in FP32 with one rounding.
- * q and q_out, scales and tables may be NULL. Asynchronous on stream.
+ * q and q_out, scales and tables may be NULL. The cache's rows lie apart from each other, keys from
+ * values, and share no memory with the heads; nor does q_out, unless it is q (dense). Asynchronous on stream.
  */
 int smx_paged_write(const smx_paged_cache* cache, int32_t tokens, const int32_t* positions, const int64_t* slots,
                     const smx_heads* q, const smx_heads* k, const smx_heads* v, const void* rope_cos,

@@ -355,6 +355,20 @@ int smx_paged_write(const smx_paged_cache* cache, int32_t tokens, const int32_t*
   if (dtypes & ~(SMX_PAGED_Q_SCALE_F32 | SMX_PAGED_K_SCALE_F32 | SMX_PAGED_ROPE_F32))
     return fail(SMX_ERR_INVALID, "unknown dtype bits 0x%x", dtypes);
   if (!(eps >= 0.f)) return fail(SMX_ERR_INVALID, "eps must not be negative");
+  // Heads are stored while others are loaded: no stored row may be another's, nor one that is read.
+  const Runs keys = cache_runs(*cache, cache->k), values = cache_runs(*cache, cache->v);
+  if (!lie_apart(keys)) return fail(SMX_ERR_INVALID, "the cache holds rows that lie on each other");
+  if (meet(keys, values)) return fail(SMX_ERR_INVALID, "keys and values must share no memory of the cache");
+  smx_heads result = has_q ? *q : *k;
+  result.data = q_out, result.head_stride = cache->head_dim, result.token_stride = (int64_t)result.heads * cache->head_dim;
+  const Runs to = head_runs(result, tokens, cache->head_dim);
+  for (const smx_heads* x : {has_q ? q : k, k, v}) {
+    const Runs from = head_runs(*x, tokens, cache->head_dim);
+    if (meet(from, keys) || meet(from, values)) return fail(SMX_ERR_INVALID, "the heads must share no memory with the cache");
+    if (has_q && meet(from, to) && !(x == q && same_runs(from, to)))
+      return fail(SMX_ERR_INVALID, "q_out must be the queries themselves or share no memory with the heads");
+  }
+  if (has_q && (meet(to, keys) || meet(to, values))) return fail(SMX_ERR_INVALID, "q_out must share no memory with the cache");
   WriteArgs w{};
   if (has_q) w.q = (const uint16_t*)q->data, w.q_token = q->token_stride, w.q_head = q->head_stride, w.heads = q->heads;
   w.k = (const uint16_t*)k->data, w.k_token = k->token_stride, w.k_head = k->head_stride;

@@ -94,7 +94,8 @@ def paged_write(k, v, k_cache, v_cache, plan, *, q=None, rope_cos=None, rope_sin
     the first half is read), bf16 or float32. All of it is computed in FP32 and rounded to
     bf16 once. Heads that come normalised and rotated from the ``qk_norm_rope``
     epilogue are stored without these. Rows of no admitted request are not stored and
-    zero in the result."""
+    zero in the result. The heads share no memory with the cache, nor the cache's keys and values with each
+    other."""
     return _lib.host().write(k, v, k_cache, v_cache, plan._native, q, rope_cos, rope_sin, q_scale, k_scale, eps)
 
 

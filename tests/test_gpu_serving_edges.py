@@ -50,3 +50,23 @@ def test_attention_into_columns_beside_the_queries(max_new):
     smx.paged_attention(both[:, :8], k, v, plan, out=both[:, 8:])
     check_attention(both[:3, 8:], want[:3], size[:3])
     assert torch.equal(both[:, :8], kept[:, :8]) and torch.equal(both[3:], kept[3:])
+
+
+def test_write_refuses_overlaps():
+    plan, k, v, *_, g = make_step([9], [4], page=8, kv_heads=2, dim=128)
+    heads, rows = bf16(4, 2, 128, g=g), k.flatten(0, 1)
+    for args, message in (((heads, heads, k, k), "keys and values"), ((rows[:4], heads, k, v), "heads must share"),
+                          ((heads, v.flatten(0, 1)[3:7], k, v), "heads must share")):
+        with pytest.raises(ValueError, match=message):
+            smx.paged_write(*args, plan)
+    with pytest.raises(ValueError, match="heads must share"):
+        smx.paged_write(heads, heads, k, v, plan, q=rows[8:12])
+    near = torch.zeros(k.numel(), dtype=torch.bfloat16, device=DEV).as_strided(k.shape, (k.stride(0) - 128, *k.stride()[1:]))
+    with pytest.raises(ValueError, match="each other"):
+        smx.paged_write(heads, heads, near, torch.zeros_like(k).as_strided(k.shape, near.stride()), plan)
+    # one tensor for both, heads outside the page's tokens: no row of one is a row of the other
+    both = torch.zeros(k.shape[0], 2, 2, 8, 128, dtype=torch.bfloat16, device=DEV)
+    apart = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    smx.paged_write(heads, heads, *apart, plan)
+    at = plan.slots // 8, plan.slots % 8
+    assert all(torch.equal(x[at], heads) for x in apart) and int(both.count_nonzero()) == 2 * int(heads.count_nonzero())

@@ -7,7 +7,7 @@ import subprocess
 import pytest
 
 from strassen_tpu_amd import _lib
-from test_serving_surface import P, _attention, _cache, _heads
+from test_serving_surface import P, _attention, _cache, _heads, _write
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -61,3 +61,26 @@ def test_attention_takes_results_beside_the_queries(q, out):
     """Refused for the workspace or, without a GPU, for the device, not for what they overlap."""
     rc, said = _message(_attention(q=q, out=out, cache=_cache(k=FAR, v=FAR + (1 << 24)), workspace=P))
     assert rc != _lib.SMX_OK and not any(x in said for x in ("queries", "each other", "share")), said
+
+
+PAGE = 16 * 2 * 128  # elements of the test cache's page
+
+
+@pytest.mark.parametrize("change,message", [
+    # pages, slots and heads nearer to each other than they are long
+    (dict(cache=_cache(k=Q, v=OUT, page_stride=PAGE - 128)), "each other"),
+    (dict(cache=_cache(k=Q, v=OUT, slot_stride=128)), "each other"),
+    (dict(cache=_cache(k=Q, v=OUT, page_stride=128, slot_stride=128)), "each other"),
+    # keys and values: the same, one slot, one head, half a head apart; interleaved pages of another size
+    (dict(cache=_cache(k=Q, v=Q)), "keys and values"), (dict(cache=_cache(k=Q, v=Q + 2 * 256)), "keys and values"),
+    (dict(cache=_cache(k=Q + 2 * 128, v=Q)), "keys and values"), (dict(cache=_cache(k=Q, v=Q + 128)), "keys and values"),
+    (dict(cache=_cache(k=Q, v=Q + 2 * (PAGE - 128), page_stride=2 * PAGE)), "keys and values"),
+    # heads read from the cache, a result within it or over the heads
+    (dict(k=_heads(2, data=Q, token=256)), "heads must share"), (dict(v=_heads(2, data=OUT + 512, token=256)), "heads must share"),
+    (dict(q=_heads(data=Q), out=FAR), "heads must share"), (dict(q=_heads(data=FAR), out=OUT + 2 * PAGE), "q_out must share"),
+    (dict(q=_heads(data=FAR), out=FAR + 2 * 1024), "q_out must be"), (dict(q=_heads(data=FAR, token=2048), out=FAR), "q_out must be"),
+    (dict(q=_heads(data=FAR), k=_heads(2, data=FAR + (1 << 20)), out=FAR + (1 << 20)), "q_out must be"),
+])
+def test_write_refuses_overlaps(change, message):
+    rc, said = _message(_write(**{"cache": _cache(k=Q, v=OUT), **change}))
+    assert rc == _lib.SMX_ERR_INVALID and message in said, said
