@@ -435,7 +435,7 @@ typedef struct smx_paged_step {
  * requests are consecutive rows 0 .. tokens - 1 of the step, padding rows behind
  * them. With a free list, request b takes ceil((c + n) / page_size) - ceil(c / page_size)
  * pages from free_pages in request order, and its entries in
- * block_tables [requests, width] are filled in; without one (NULL) the tables must
+ * block_tables [requests, width], which share no memory with the other lists, are filled in; without one (NULL) the tables must
  * hold every page already. Out:
  *   starts [requests + 1]: first row of each request;
  *   rows, context, status [requests]: new and context tokens of the requests that are

@@ -74,6 +74,17 @@ inline bool meet(const Runs& x, const Runs& y) {
   return !alike || !lie_apart(a) || meet_at(a, 2, (from_b - from_a) / 2);
 }
 
+// Whether `count` values from `list` on share memory with the rows of a table of `size`-byte values
+// (rows at least `width` apart, from each first value on).
+inline bool list_meets_table(const void* list, int64_t count, const void* table, int64_t rows, int64_t width,
+                             int64_t stride, int64_t size) {
+  const int64_t from = (intptr_t)list - (intptr_t)table, to = from + count * size, row = stride * size;
+  if (count <= 0) return false;
+  // the first row that ends behind the list's start
+  const int64_t first = from < width * size ? 0 : (from - width * size) / row + 1;
+  return first < rows && first * row < to;
+}
+
 // The same elements at the same indices.
 inline bool same_runs(const Runs& x, const Runs& y) {
   bool same = x.at == y.at && x.width == y.width;

@@ -313,6 +313,16 @@ int smx_paged_plan(int32_t requests, int32_t width, int32_t page_size, int32_t n
   if (!context_lens || !new_lens || !block_tables || !starts || !rows || !context || !positions || !slots ||
       !status || !pages)
     return fail(SMX_ERR_INVALID, "null pointer");
+  if (free_pages) {
+    // entries are filled in while other workgroups read the lists
+    const struct {
+      const void* list;
+      int64_t count;
+    } lists[] = {{context_lens, requests}, {new_lens, requests}, {free_pages, free_count}};
+    for (const auto& l : lists)
+      if (list_meets_table(l.list, l.count, block_tables, requests, width, table_stride, 4))
+        return fail(SMX_ERR_INVALID, "block_tables must share no memory with the lengths and free_pages");
+  }
   PlanArgs p{context_lens, new_lens, block_tables, table_stride, free_pages, starts, rows, context, positions,
              status, pages, slots, requests, width, __builtin_ctz(page_size), num_pages, tokens, max_new,
              max_context, free_count};

@@ -63,8 +63,8 @@ def paged_plan(context_lens, new_lens, block_tables, *, page_size, num_pages, to
     ``block_tables`` int32 ``[requests, width]`` names each request's pages. With
     ``free_pages`` (int32, distinct page numbers) the requests take the pages that they
     need, ``ceil((context + new) / page_size) - ceil(context / page_size)`` each, from its front in
-    request order, and their entries are written into ``block_tables``; without,
-    every page must be there already. ``tokens`` is the step's number of rows
+    request order, and their entries are written into ``block_tables`` (which shares no memory
+    with the other arguments); without, every page must be there already. ``tokens`` is the step's number of rows
     (the new tokens and any padding behind them); ``max_new`` and ``max_context``
     bound the new tokens of a request and its tokens in all, where a program knows
     them (default: ``tokens``, and what the tables hold).

@@ -55,6 +55,19 @@ int main() {
             for (const auto* e : elements(other)) met = met || set.count(e);
             if (met && !smx::meet(a, other)) return printf("missed another layout\n"), 1;
           }
+  // lists among the rows of tables
+  for (int64_t rows = 1; rows <= 3; ++rows)
+    for (int64_t width = 1; width <= 4; ++width)
+      for (int64_t stride = width; stride <= width + 3; ++stride)
+        for (int64_t count = 0; count <= 5; ++count)
+          for (int64_t at = -8; at <= rows * stride + 2; ++at) {
+            bool met = false;
+            for (int64_t r = 0; r < rows; ++r)
+              for (int64_t e = at; e < at + count; ++e) met = met || (e >= r * stride && e < r * stride + width);
+            const auto* table = (const int32_t*)memory + 64;
+            if (smx::list_meets_table(table + at, count, table, rows, width, stride, 4) != met)
+              return printf("table of %ld rows of %ld, %ld apart, list of %ld at %ld\n", rows, width, stride, count, at), 1;
+          }
   // the layouts of heads lie apart: rows of tokens, heads outside tokens, columns of a wider product, one run
   const int64_t heads[][4] = {{16, 512, 4, 128}, {16, 128, 4, 2048}, {16, 768, 4, 128}, {1, 0, 1, 0}, {1, 5, 4, 128}};
   for (const auto& h : heads)

@@ -70,3 +70,15 @@ def test_write_refuses_overlaps():
     smx.paged_write(heads, heads, *apart, plan)
     at = plan.slots // 8, plan.slots % 8
     assert all(torch.equal(x[at], heads) for x in apart) and int(both.count_nonzero()) == 2 * int(heads.count_nonzero())
+
+
+def test_plan_refuses_tables_over_its_lists():
+    lens, tables = i32([1, 2]), i32([[0, -1, 9, 9], [1, -1, 9, 9]])
+    good = dict(page_size=8, num_pages=4, tokens=5, free_pages=i32([2, 3]))
+    for args, change in (((lens, lens, tables), {"free_pages": tables[1]}), ((tables[0, :2], lens, tables), {}),
+                         ((lens, tables.view(-1)[3:5], tables), {})):
+        with pytest.raises(ValueError, match="block_tables"):
+            smx.paged_plan(*args, **{**good, **change})
+    # a list between the rows of narrower tables, and tables that are only read
+    assert smx.paged_plan(lens, lens, tables[:, :2], **{**good, "free_pages": tables[0, 2:]}).status.tolist() == [0, 0]
+    assert smx.paged_plan(lens, lens, tables, **{**good, "free_pages": None}).status.tolist() == [0, 0]

@@ -7,7 +7,7 @@ import subprocess
 import pytest
 
 from strassen_tpu_amd import _lib
-from test_serving_surface import P, _attention, _cache, _heads, _write
+from test_serving_surface import P, _attention, _cache, _heads, _plan, _write
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -84,3 +84,11 @@ PAGE = 16 * 2 * 128  # elements of the test cache's page
 def test_write_refuses_overlaps(change, message):
     rc, said = _message(_write(**{"cache": _cache(k=Q, v=OUT), **change}))
     assert rc == _lib.SMX_ERR_INVALID and message in said, said
+
+
+@pytest.mark.parametrize("change", [{"context": FAR}, {"fresh": FAR + 28}, {"free": FAR - 8}, {"free": FAR + 4 * 8 + 12},
+                                    {"context": FAR - 4}])
+def test_plan_refuses_tables_over_its_lists(change):
+    lists = dict(context=Q, fresh=Q + 64, free=OUT, tables=FAR, stride=8)
+    rc, said = _message(_plan(**{**lists, **change}))
+    assert rc == _lib.SMX_ERR_INVALID and "block_tables" in said, said
