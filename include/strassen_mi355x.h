@@ -420,7 +420,7 @@ typedef struct smx_heads {
   int32_t heads;
 } smx_heads;
 
-/* What smx_paged_attention reads of a plan (device pointers). */
+/* What smx_paged_attention reads of a plan (device pointers); sizes and max_new are the plan's. */
 typedef struct smx_paged_step {
   int32_t requests, tokens, max_new;
   const int32_t* block_tables;

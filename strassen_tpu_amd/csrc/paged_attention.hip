@@ -1043,8 +1043,9 @@ int64_t workspace_of(int cus, int head_dim) {
 }
 
 // Requests whose new rows fill one tile of 32 at most take the kernel for few rows: its waves
-// share no work, so a tile of four times the rows reads the cache four times less.
-bool few_rows(int64_t max_new, int group) { return max_new * group <= 32; }
+// share no work, so a tile of four times the rows reads the cache four times less. A step without new rows
+// counts as one row a request: a tile holds a token at least.
+bool few_rows(int64_t max_new, int group) { return (max_new > 1 ? max_new : 1) * group <= 32; }
 
 template <int D>
 int launch_attention(AttentionArgs& p, bool few, unsigned blocks, hipStream_t stream) {

@@ -82,3 +82,17 @@ def test_plan_refuses_tables_over_its_lists():
     # a list between the rows of narrower tables, and tables that are only read
     assert smx.paged_plan(lens, lens, tables[:, :2], **{**good, "free_pages": tables[0, 2:]}).status.tolist() == [0, 0]
     assert smx.paged_plan(lens, lens, tables, **{**good, "free_pages": None}).status.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(64, 1), (128, 1), (8, 2)])
+def test_attention_of_a_plan_without_new_tokens(heads, kv_heads):
+    """max_new=0: every request sits the step out, whatever the number of query heads to a tile of rows."""
+    context = [30, 0, 7]
+    plan, k, v, *_, g = make_step(context, [0, 0, 0], page=8, kv_heads=kv_heads, dim=128, pad=5)
+    plan = smx.paged_plan(i32(context), i32([0, 0, 0]), plan.block_tables, page_size=8, num_pages=plan.num_pages,
+                          tokens=5, max_new=0)
+    assert plan.status.tolist() == [smx.PAGED_OK] * 3
+    q = bf16(plan.tokens, heads, 128, g=g)
+    assert not smx.paged_attention(q, k, v, plan).any()
+    out = torch.full_like(q, 7.0)
+    assert (smx.paged_attention(q, k, v, plan, out=out) == 7).all()
