@@ -385,19 +385,32 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t) {
   });
 }
 
+// One of the two tensors of a weight laid out for int4_matmul.
+void laid_out_for(const Tensor& t, const char* name, const at::Device& device, int64_t numel) {
+  if (t.scalar_type() != at::kInt || t.device() != device || !t.is_contiguous() || t.numel() != numel)
+    refuse(name, " is not that of int4_weight_layout (", numel, " contiguous int32 values on ", device, "), got ", shape_of(t), " on ",
+           t.device());
+}
+
 // (x, codes, scales, k, n, group, swiglu, zeros, epilogue, residual, bias) -> the product
 PyObject* int4(PyObject*, PyObject* const* a, Py_ssize_t) {
   return guarded([&]() -> PyObject* {
     no_gradients({a[0], a[9], a[10]});
-    const Tensor& codes = THPVariable_Unpack(a[1]);
+    const Tensor &codes = tensor(a[1], "w.codes"), &scales = tensor(a[2], "w.scales");
     const at::Device device = codes.device();
     const Tensor* x = &on_device(a[0], "x");
     on_device(a[0], "x", device);
-    const int64_t k = PyLong_AsLongLong(a[3]), width = PyLong_AsLongLong(a[4]);
+    // The operand's fields are a program's to change: its memory is what the kernels will read of it
+    const int64_t k = integer(a[3], "w.k", 1, 1 << 22), width = integer(a[4], "w.n", 1, 1 << 24);
+    const int64_t group = integer(a[5], "w.group", 32, 128);
+    const int32_t swiglu = (int32_t)integer(a[6], "w.swiglu", 0, 1), zeros = (int32_t)integer(a[7], "w.zeros", 0, 1);
+    if (128 % group) refuse("w.group must be 32, 64 or 128, got ", group);
+    const int64_t k_tiles = (k + 127) / 128, columns = swiglu ? 2 * ((width / 2 + 15) / 16) : 2 * ((width + 31) / 32);
+    laid_out_for(codes, "w.codes", device, columns * k_tiles * 256);
+    laid_out_for(scales, "w.scales", device, columns * k_tiles * 16 * (128 / group));
     const int32_t epilogue = (int32_t)PyLong_AsLong(a[8]);
-    const smx_int4_weight w{codes.data_ptr(), THPVariable_Unpack(a[2]).data_ptr(), k, width, (int32_t)PyLong_AsLong(a[5]),
-                            (int32_t)PyLong_AsLong(a[6]), (int32_t)PyLong_AsLong(a[7])};
     if (PyErr_Occurred()) throw Raised();
+    const smx_int4_weight w{codes.data_ptr(), scales.data_ptr(), k, width, (int32_t)group, swiglu, zeros};
     if (x->scalar_type() != at::kBFloat16 || x->dim() != 2) refuse("x must be a bf16 matrix, got ", shape_of(*x));
     const int64_t m = x->size(0), n = w.swiglu ? width / 2 : width;
     if (x->size(1) != k) refuse("inner dimensions disagree: ", x->size(1), " vs ", k);

@@ -20,7 +20,8 @@ _EPILOGUES = (None, "swiglu", "residual_add", "bias_add")
 
 
 class Int4Operand:
-    """A weight laid out by ``int4_weight_layout``."""
+    """A weight laid out by ``int4_weight_layout``: int32 tensors ``codes`` and ``scales`` on one device. A call
+    refuses one whose tensors are not of the size, type or device that its other fields say."""
 
     def __init__(self, codes, scales, k, n, group, swiglu, zeros):
         self.codes, self.scales, self.device = codes, scales, codes.device

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import strassen_tpu_amd as smx
+from test_gpu_int4 import check, weight
 from test_gpu_paged import attend64, check_attention, i32, make_step
 from test_gpu_parity import DEV, say
 
@@ -96,3 +97,22 @@ def test_attention_of_a_plan_without_new_tokens(heads, kv_heads):
     assert not smx.paged_attention(q, k, v, plan).any()
     out = torch.full_like(q, 7.0)
     assert (smx.paged_attention(q, k, v, plan, out=out) == 7).all()
+
+
+def test_int4_operands_that_do_not_hold_what_they_say():
+    """Fields and tensors changed by hand: sizes that the kernels would read past are refused before a launch."""
+    codes, scales, zero, w, spread, g = weight(256, 70, 64, True)
+    good = smx.int4_weight_layout(codes, scales, zero, group=64)
+    x = bf16(3, 256, g=g)
+    for change, message in (
+            ({"codes": good.codes[:-1]}, "w.codes"), ({"codes": good.codes.float()}, "w.codes"), ({"codes": good.codes.cpu()}, "on"),
+            ({"codes": good.codes.transpose(0, 1)}, "w.codes"), ({"scales": good.scales[:, :1]}, "w.scales"),
+            ({"scales": good.scales.short()}, "w.scales"), ({"scales": good.scales.cpu()}, "w.scales"), ({"n": 97}, "w.codes"),
+            ({"n": 0}, "w.n"), ({"n": 1 << 40}, "w.n"), ({"k": 288}, "w.codes"), ({"k": -32}, "w.k"), ({"group": 32}, "w.scales"),
+            ({"group": 96}, "w.group"), ({"group": 0}, "w.group")):
+        fields = {f: getattr(good, f) for f in ("codes", "scales", "k", "n", "group", "swiglu", "zeros")}
+        made = smx.Int4Operand(**{**fields, **change})
+        with pytest.raises(ValueError, match=message):
+            smx.int4_matmul(x, made)
+    made = smx.Int4Operand(good.codes.clone(), good.scales.flatten(), 256, 70, 64, False, True)  # by hand, but right
+    check(smx.int4_matmul(x, made), x, w, spread)

@@ -5,9 +5,11 @@ import shutil
 import subprocess
 
 import pytest
+import torch
 
+import strassen_tpu_amd as smx
 from strassen_tpu_amd import _lib
-from test_serving_surface import P, _attention, _cache, _heads, _plan, _write
+from test_serving_surface import P, _attention, _cache, _heads, _plan, _weight, _write
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -92,3 +94,11 @@ def test_plan_refuses_tables_over_its_lists(change):
     lists = dict(context=Q, fresh=Q + 64, free=OUT, tables=FAR, stride=8)
     rc, said = _message(_plan(**{**lists, **change}))
     assert rc == _lib.SMX_ERR_INVALID and "block_tables" in said, said
+
+
+@pytest.mark.parametrize("field", ["codes", "scales"])
+def test_int4_operands_that_hold_no_tensors(field):
+    w = smx.int4_weight_layout(*_weight(), group=128)
+    setattr(w, field, [1, 2])
+    with pytest.raises(TypeError, match=f"w.{field} must be a tensor"):
+        smx.int4_matmul(torch.zeros(1, 128, dtype=torch.bfloat16), w)
