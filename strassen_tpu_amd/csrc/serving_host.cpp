@@ -303,7 +303,7 @@ const void* scale_of(PyObject* o, const char* name, const Plan& plan, int64_t he
 // (k, v, k_cache, v_cache, plan, q, rope_cos, rope_sin, q_scale, k_scale, eps) -> q' or None
 PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t) {
   return guarded([&]() -> PyObject* {
-    no_gradients({a[0], a[1], a[2], a[3], a[5]});
+    no_gradients({a[0], a[1], a[2], a[3], a[5], a[6], a[7], a[8], a[9]});
     const Plan& plan = plan_of(a[4]);
     const smx_paged_cache cache = cache_of(a[2], a[3], plan);
     const int64_t head_dim = cache.head_dim;

@@ -116,3 +116,23 @@ def test_int4_operands_that_do_not_hold_what_they_say():
             smx.int4_matmul(x, made)
     made = smx.Int4Operand(good.codes.clone(), good.scales.flatten(), 256, 70, 64, False, True)  # by hand, but right
     check(smx.int4_matmul(x, made), x, w, spread)
+
+
+def write_inputs(g):
+    """A plan, its cache and every tensor that paged_write takes."""
+    plan, k_cache, v_cache, *_ = make_step([9], [4], page=8, kv_heads=2, dim=128)
+    angle = torch.rand(plan.max_context, 64, device=DEV, generator=g)
+    return plan, dict(k=bf16(4, 2, 128, g=g), v=bf16(4, 2, 128, g=g), k_cache=k_cache, v_cache=v_cache, q=bf16(4, 8, 128, g=g),
+                      rope_cos=angle.cos(), rope_sin=angle.sin(), q_scale=bf16(128, g=g), k_scale=bf16(128, g=g))
+
+
+def test_write_refuses_gradients_of_all_its_tensors():
+    """Norm weights, a model's parameters, among them; without gradients to record they are taken."""
+    plan, good = write_inputs(torch.Generator(device=DEV).manual_seed(1))
+    want = smx.paged_write(plan=plan, **good)
+    for name in good:
+        args = {**good, name: good[name].clone().requires_grad_()}
+        with pytest.raises(ValueError, match="gradients"):
+            smx.paged_write(plan=plan, **args)
+        with torch.no_grad():
+            assert torch.equal(smx.paged_write(plan=plan, **args), want)
