@@ -5,8 +5,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
-#include <c10/core/GradMode.h>
 
 #include <cmath>
 #include <sstream>
@@ -93,10 +93,16 @@ const Tensor& on_device(PyObject* o, const char* name, const at::Device& device)
 bool given(PyObject* o) { return o != Py_None; }
 
 void no_gradients(std::initializer_list<PyObject*> tensors) {
-  if (!c10::GradMode::is_enabled()) return;
-  for (PyObject* const o : tensors)
-    if (given(o) && THPVariable_Check(o) && THPVariable_Unpack(o).requires_grad())
+  const c10::AutogradState& state = c10::AutogradState::get_tls_state();
+  const bool backward = state.get_grad_mode(), forward = state.get_fw_grad_mode();
+  for (PyObject* const o : tensors) {
+    if (!given(o) || !THPVariable_Check(o)) continue;
+    const Tensor& t = THPVariable_Unpack(o);
+    if (backward && t.requires_grad())
       refuse("serving operators record no gradients: call them under torch.no_grad()");
+    if (forward && t._fw_grad(0).defined())  // (torch has one level of forward-mode tangents)
+      refuse("serving operators carry no forward-mode gradients: unpack the dual tensor first");
+  }
 }
 
 int64_t integer(PyObject* o, const char* name, int64_t low, int64_t high) {

@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import strassen_tpu_amd as smx
 from test_gpu_int4 import check, weight
@@ -136,3 +137,27 @@ def test_write_refuses_gradients_of_all_its_tensors():
             smx.paged_write(plan=plan, **args)
         with torch.no_grad():
             assert torch.equal(smx.paged_write(plan=plan, **args), want)
+
+
+def test_tangents_are_refused():
+    """Forward-mode gradients, which torch.no_grad() leaves on."""
+    plan, good = write_inputs(torch.Generator(device=DEV).manual_seed(2))
+    codes, scales, zero, *_, g = weight(128, 40, 128, True)
+    w = smx.int4_weight_layout(codes, scales, zero, group=128)
+    x, bias, residual = bf16(4, 128, g=g), bf16(40, g=g), bf16(4, 40, g=g)
+    q, k, v = (good[n] for n in ("q", "k_cache", "v_cache"))
+    with forward_ad.dual_level(), torch.no_grad():
+        def dual(t):
+            return forward_ad.make_dual(t.clone(), torch.ones_like(t))
+
+        calls = [lambda n=n: smx.paged_write(plan=plan, **{**good, n: dual(good[n])}) for n in good]
+        calls += [lambda: smx.paged_attention(dual(q), k, v, plan), lambda: smx.paged_attention(q, dual(k), v, plan),
+                  lambda: smx.paged_attention(q, k, dual(v), plan), lambda: smx.paged_attention(q, k, v, plan, out=dual(q)),
+                  lambda: smx.int4_matmul(dual(x), w),
+                  lambda: smx.int4_matmul(x, w, epilogue="bias_add", bias=dual(bias)),
+                  lambda: smx.int4_matmul(x, w, epilogue="residual_add", residual=dual(residual))]
+        for call in calls:
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        smx.paged_attention(smx.paged_write(plan=plan, **good), k, v, plan)
+        smx.int4_matmul(forward_ad.unpack_dual(dual(x)).primal, w)
