@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <cmath>
 #include <sstream>
@@ -72,10 +73,31 @@ std::string shape_of(const Tensor& t) {
   return s.str();
 }
 
+// Tensors whose memory is not what they stand for: fake and other dispatching types, batched and
+// differentiated ones of torch.func, views that negate when they are read, sparse layouts.
+bool plain(const Tensor& t) {
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet kOthers({DispatchKey::Python, DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper,
+                                         DispatchKey::Batched, DispatchKey::Functionalize, DispatchKey::Conjugate,
+                                         DispatchKey::Negative, DispatchKey::ZeroTensor});
+  return t.layout() == at::kStrided && !t.key_set().has_any(kOthers);
+}
+
 const Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o))
     throw Refused(std::string(name) + " must be a tensor, got " + Py_TYPE(o)->tp_name, PyExc_TypeError);
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!plain(t)) refuse(name, " must be a plain strided tensor, the kernels read its memory (got ", Py_TYPE(o)->tp_name, ")");
+  return t;
+}
+
+// A call that is traced would run once, on the tensors at hand, and be missing from what is traced.
+void not_traced() {
+  using c10::impl::TorchDispatchModeKey;
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  if (!c10::impl::dispatch_mode_enabled()) return;
+  for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+    if (Modes::get_mode(mode)) refuse("serving operators cannot be traced (", c10::impl::to_string(mode), " mode)");
 }
 
 const Tensor& on_device(PyObject* o, const char* name) {
@@ -121,6 +143,7 @@ double real(PyObject* o) {
 template <class F>
 PyObject* guarded(F f) {
   try {
+    not_traced();
     const at::AutoDispatchBelowADInplaceOrView below;  // nothing here records gradients
     return f();
   } catch (const Raised&) {

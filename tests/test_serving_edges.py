@@ -102,3 +102,43 @@ def test_int4_operands_that_hold_no_tensors(field):
     setattr(w, field, [1, 2])
     with pytest.raises(TypeError, match=f"w.{field} must be a tensor"):
         smx.int4_matmul(torch.zeros(1, 128, dtype=torch.bfloat16), w)
+
+
+def _serving_calls(lens, tables, x, w):
+    yield lambda: smx.paged_plan(lens, lens, tables, page_size=16, num_pages=1, tokens=1)
+    yield lambda: smx.int4_matmul(x, w)
+
+
+def test_tensors_without_memory_of_their_own_are_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    w = smx.int4_weight_layout(*_weight(), group=128)
+    with FakeTensorMode():
+        fake = (torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(1, 1, dtype=torch.int32, device="cuda"),
+                torch.zeros(1, 128, dtype=torch.bfloat16, device="cuda"))
+    for call in _serving_calls(*fake, w):
+        with pytest.raises(ValueError, match="plain strided tensor"):
+            call()
+    real = torch.zeros(1, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="plain strided tensor"):
+        smx.int4_matmul(torch._neg_view(real), w)
+    with pytest.raises(ValueError, match="plain strided tensor"):
+        smx.int4_matmul(real.to_sparse(), w)
+    for transform in (lambda f: torch.vmap(f), lambda f: lambda x: torch.func.vjp(f, x),
+                      lambda f: lambda x: torch.func.jvp(f, (x,), (x,))):
+        with pytest.raises(ValueError, match="plain strided tensor|gradients"):
+            transform(lambda x: smx.int4_matmul(x, w))(real[None])
+
+
+def test_traced_calls_are_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    lens, tables = torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32)
+    x, w = torch.zeros(1, 128, dtype=torch.bfloat16), smx.int4_weight_layout(*_weight(), group=128)
+    for call in _serving_calls(lens, tables, x, w):
+        with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(ValueError, match="traced"):
+            call()
+    for mode in ("real", "fake"):
+        with pytest.raises(ValueError, match="traced"):
+            make_fx(lambda x: smx.int4_matmul(x, w), tracing_mode=mode)(x)
