@@ -676,7 +676,22 @@ __device__ __forceinline__ void store_rows(const AttentionArgs& p, const f32x16 
   for (int x = 0; x < D / 32; ++x) store_block(to + 32 * x, o[x], inverse, valid, thread >> 5 & 1);
 }
 
-__device__ __forceinline__ float inverse_of(float sum) { return sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum; }
+// Whether the row at `position` of a request sees any key: a page from its window's first on is in the cache.
+__device__ __forceinline__ bool sees_a_key(const AttentionArgs& p, int request, int position) {
+  const int32_t* const table = p.tables + request * p.table_stride;
+  const int first = p.window ? max(0, position - p.window + 1) >> p.page_shift : 0;
+  for (int i = position >> p.page_shift; i >= first; --i)
+    if ((uint32_t)table[i] < (uint32_t)p.num_pages) return true;
+  return false;
+}
+
+// What a row's values are multiplied with. Its largest weight is 1, so that a sum is zero only without one: a row
+// that sees no key is zero, and one all of whose scores are -inf is NaN. Only then is the table looked through.
+__device__ __forceinline__ float inverse_of(float sum, const AttentionArgs& p, int request, int position) {
+  float inverse = sum > 0.f ? 1.f / sum : sum;
+  if (__any(sum == 0.f) && sum == 0.f && sees_a_key(p, request, position)) inverse = NAN;
+  return inverse;
+}
 
 // 128 rows a tile (four waves of 32), 64 keys a step, keys and values double buffered. 2048 tokens of 64 heads on
 // 16384 cached ones: 1.33 ms, 0.88 PFLOP/s. Matrix cores, vector units and LDS are each busy 40 to 44% of the time
@@ -800,7 +815,8 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
 
       const float sum = o.sum + other_half(o.sum);
       if (part.count == part.tile_count) {
-        store_rows<D>(p, o.o, inverse_of(sum), 32 * wave + (lane & 31) < tile_rows, scalar_at(p.starts, part.request) + local, head);
+        store_rows<D>(p, o.o, inverse_of(sum, p, part.request, position), 32 * wave + (lane & 31) < tile_rows,
+                      scalar_at(p.starts, part.request) + local, head);
       } else {
         float* const to = p.partial + (2 * (int64_t)s.worker + part.begins) * kPartialFloats<D>;
         int thread = threadIdx.x;
@@ -915,7 +931,7 @@ __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
 
     const float sum = o.sum + other_half(o.sum);
     if (count == part.tile_count) {
-      store_rows<D>(p, o.o, inverse_of(sum), valid, token, head);
+      store_rows<D>(p, o.o, inverse_of(sum, p, part.request, position), valid, token, head);
     } else {
       float* const to = p.partial + (2 * (int64_t)s.worker + part.begins) * kFewPartialFloats<D>;
       if (valid) {
@@ -987,8 +1003,9 @@ __global__ __launch_bounds__(1024) void paged_join_few(AttentionArgs p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) value[j] = value[j] * keep + values[at][j] * add;
   }
-  const float inverse = inverse_of(total);
-  const int64_t token = p.starts[record.request] + record.tile * p.tile_tokens + row / p.group;
+  const int local = record.tile * p.tile_tokens + row / p.group;
+  const float inverse = inverse_of(total, p, record.request, p.context[record.request] + local);
+  const int64_t token = p.starts[record.request] + local;
   *reinterpret_cast<uint2*>(p.out + token * p.out_token + (record.head * p.group + row % p.group) * p.out_head + column) =
       make_uint2(pack_bf16(value[0] * inverse, value[1] * inverse), pack_bf16(value[2] * inverse, value[3] * inverse));
 }
@@ -1025,9 +1042,10 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join(AttentionArgs p) {
   const int fresh = p.rows[record.request];
   const int tile_rows = min(p.tile_tokens, fresh - record.tile * p.tile_tokens) * p.group;
   const int at = 32 * wave + (lane & 31), row = min(at, tile_rows - 1);
-  const int64_t token = p.starts[record.request] + record.tile * p.tile_tokens + row / p.group;
-  store_block(p.out + token * p.out_token + (record.head * p.group + row % p.group) * p.out_head + 32 * x, o, inverse_of(sum),
-              at < tile_rows, lane >> 5);
+  const int local = record.tile * p.tile_tokens + row / p.group;
+  const int64_t token = p.starts[record.request] + local;
+  store_block(p.out + token * p.out_token + (record.head * p.group + row % p.group) * p.out_head + 32 * x, o,
+              inverse_of(sum, p, record.request, p.context[record.request] + local), at < tile_rows, lane >> 5);
 }
 
 // Workgroups of a launch, a multiple of the 8 XCDs: as many as a CU holds (two of paged_attend, by its

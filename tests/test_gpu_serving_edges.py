@@ -161,3 +161,61 @@ def test_tangents_are_refused():
                 call()
         smx.paged_attention(smx.paged_write(plan=plan, **good), k, v, plan)
         smx.int4_matmul(forward_ad.unpack_dual(dual(x)).primal, w)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("context,new,max_new,window", [
+    ([0, 20, 9000], [1, 1, 1], 1, None), ([5, 0, 3000], [3, 4, 1], 4, 1), ([0, 40, 6000], [150, 70, 9], None, None),
+    ([90, 700], [150, 70], None, 33)])
+def test_attention_of_infinite_scores(dim, context, new, max_new, window):
+    """Infinities among the keys. A score of -inf weighs nothing beside others; a row that sees no other score is NaN
+    (not the zero of a row that sees no key), and so is one that sees a score of +inf."""
+    page, kv_heads, heads = 8, 3, 6
+    plan, k, v, keys, values, g = make_step(context, new, page=page, kv_heads=kv_heads, dim=dim, pad=2)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=page, num_pages=plan.num_pages,
+                          tokens=plan.tokens, max_new=max_new)
+    q = bf16(plan.tokens, heads, dim, g=g)
+    q[:, :, 5] = q[:, :, 5].abs() + 1  # the sign of the infinity is the score's
+    for b, (c, n) in enumerate(zip(context, new)):
+        at = torch.arange(c + n, device=DEV)
+        rows = plan.block_tables[b].long()[at // page], at % page
+        odd = torch.zeros(c + n, kv_heads, device=DEV)
+        odd[::3, 0] = -math.inf  # every third, the first among them
+        odd[:c + (n + 1) // 2, 1] = -math.inf  # all that the first half of the rows see
+        odd[c + n // 2, 2] = math.inf
+        column = torch.where(odd != 0, odd, k[(*rows, slice(None), 5)].float())
+        k[(*rows, slice(None), 5)] = column.to(torch.bfloat16)
+        keys[b][:, :, 5] = column.double()
+    want, size, row = torch.zeros(q.shape, dtype=torch.float64, device=DEV), torch.zeros(q.shape, dtype=torch.float64, device=DEV), 0
+    for b, (c, n) in enumerate(zip(context, new)):
+        key, own = torch.arange(c + n, device=DEV), torch.arange(c, c + n, device=DEV)[:, None]
+        hidden = (key > own) | (key <= own - (window or 1 << 30))
+        for h in range(heads):
+            # elementwise, not by a library product, whose sums of infinities are its own affair
+            s = (q[row:row + n, h, None].double() * keys[b][None, :, h // 2]).sum(-1) * dim ** -0.5
+            w = torch.softmax(s.masked_fill(hidden, -math.inf), dim=-1)
+            want[row:row + n, h], size[row:row + n, h] = w @ values[b][:, h // 2], w @ values[b][:, h // 2].abs()
+        row += n
+    got = smx.paged_attention(q, k, v, plan, window=window)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert want.isnan().any() and not want[row:].any()
+    here = ~want.isnan()
+    check_attention(got[here], want[here], size[here])
+
+
+@pytest.mark.parametrize("max_new", [None, 2])
+def test_attention_of_a_row_that_sees_infinite_scores_and_missing_pages(max_new):
+    """Rows whose pages are all missing are zero, those that see one key of score -inf among missing pages NaN."""
+    context, new, page = [40, 16], [2, 2], 8
+    plan, k, v, *_, g = make_step(context, new, page=page, kv_heads=1, dim=128)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=page, num_pages=plan.num_pages,
+                          tokens=plan.tokens, max_new=max_new)
+    q = bf16(4, 2, 128, g=g).abs() + 1
+    k.copy_(torch.where(k.isnan(), k, torch.full_like(k, -math.inf)))
+    plan.block_tables[0], plan.block_tables[1, 1:] = -1, plan.num_pages
+    for window in (None, 12):
+        got = smx.paged_attention(q, k, v, plan, window=window)
+        assert not got[:2].any()
+        # positions 16 and 17 of the second request see keys 5 .. and 6 .. of the page that is there
+        assert got[2:].isnan().all()
+    assert not smx.paged_attention(q, k, v, plan, window=8).any()
