@@ -488,26 +488,28 @@ __device__ __forceinline__ bool any_not_finite(const bf16x8 (&v)[kBlocks][2][kCo
 
 // A step that masks keys and whose values are not all finite: a product alone would give 0 * inf = NaN
 // to the rows that do not see them. Every +inf and NaN (sign 0), every -inf and NaN (sign 1) that a row
-// weighs adds a product beyond FP32's range to its column, which is that infinity (both: NaN), and the
-// values themselves become zero.
+// sees, however small its weight, adds a product beyond FP32's range to its column, which is that infinity
+// (both: NaN), and the values themselves become zero. The row sees the step's keys after `oldest` up to `newest`
+// (both less 4 half) whose bit in `held` (shifted so too) is set.
 template <int D, int kBlocks>
-__device__ __forceinline__ void add_not_finite(f32x16 (&o)[D / 32], bf16x8 (&v)[kBlocks][2][D / 32],
-                                               const bf16x8 (&w)[2 * kBlocks]) {
+__device__ __forceinline__ void add_not_finite(f32x16 (&o)[D / 32], bf16x8 (&v)[kBlocks][2][D / 32], int oldest, int newest,
+                                               uint64_t held) {
   // two values a register; 0 or 1 for no and yes (asm: constants loaded here, not held by the whole kernel)
-  uint32_t weight = 0x43804380u, ones = 0x10001u, largest[2] = {0x7f7f7f7fu, 0xff7fff7fu};
+  uint32_t weight = 0x4380u, ones = 0x10001u, largest[2] = {0x7f7f7f7fu, 0xff7fff7fu};
   asm volatile("" : "+s"(weight), "+s"(ones), "+s"(largest[0]), "+s"(largest[1]));
   const uint32_t finite = largest[0];
   const u16x2 one = __builtin_bit_cast(u16x2, ones), most = __builtin_bit_cast(u16x2, finite);
 #pragma unroll
   for (int t = 0; t < 2 * kBlocks; ++t) {
-    // (elements are copied before they are reinterpreted: a bit cast of a vector's element takes its first)
-    const u32x4 weights = __builtin_bit_cast(u32x4, w[t]);
-    u32x4 large;  // 2^8 for every weight above zero
+    u32x4 large;  // 2^8 for every key that the row sees
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t two = weights[i];
-      large[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, two), one) *
-                                                  __builtin_bit_cast(u16x2, weight));
+      large[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int e = 8 * (t % 2) + 2 * i + j, key = 32 * (t / 2) + 8 * (e >> 2) + (e & 3);
+        large[i] |= key <= newest && key > oldest && ((held >> key) & 1) ? weight << 16 * j : 0;
+      }
     }
 #pragma unroll
     for (int x = 0; x < D / 32; ++x) {
@@ -518,6 +520,7 @@ __device__ __forceinline__ void add_not_finite(f32x16 (&o)[D / 32], bf16x8 (&v)[
         const uint32_t value = largest[sign];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+          // (copied before it is reinterpreted: a bit cast of a vector's element takes its first)
           const uint32_t two = words[i], sizes = two & 0x7fff7fffu;
           const u16x2 beyond = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, sizes), most);  // 1: inf, more: NaN
           u16x2 side = __builtin_bit_cast(u16x2, two) >> (uint16_t)15;
@@ -632,7 +635,8 @@ __device__ __forceinline__ void attend(Rows<D>& r, const bf16x8 (&q)[D / 16], co
       w[2 * x + h] = __builtin_bit_cast(bf16x8, b);
     }
   }
-  if (masked && any_not_finite(v)) add_not_finite<D, kBlocks>(r.o, v, w);
+  if (masked && any_not_finite(v))
+    add_not_finite<D, kBlocks>(r.o, v, window ? rel - 4 * half - window : -(1 << 30), rel - 4 * half, held >> (4 * half));
 #pragma unroll
   for (int t = 0; t < 2 * kBlocks; ++t)
 #pragma unroll

@@ -219,3 +219,29 @@ def test_attention_of_a_row_that_sees_infinite_scores_and_missing_pages(max_new)
         # positions 16 and 17 of the second request see keys 5 .. and 6 .. of the page that is there
         assert got[2:].isnan().all()
     assert not smx.paged_attention(q, k, v, plan, window=8).any()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("context,new,max_new,window", [
+    ([3, 41, 2000], [1, 1, 1], 1, None), ([30, 5, 200], [4, 3, 4], 4, 8), ([0, 100], [150, 70], None, None),
+    ([90, 700], [150, 70], None, 33)])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_attention_of_infinities_whose_weight_is_nothing(dim, context, new, max_new, window, value):
+    """A key 300 below the others, whose weight FP32 does not hold: an infinity or NaN of its value reaches the rows
+    that see it all the same, in steps that mask keys and in others, and no other row."""
+    page, heads = 8, 4
+    plan, k, v, keys, values, g = make_step(context, new, page=page, kv_heads=1, dim=dim)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=page, num_pages=plan.num_pages,
+                          tokens=plan.tokens, max_new=max_new)
+    q = bf16(plan.tokens, heads, dim, g=g)
+    q[:, :, 5] = 2.0
+    reached, row = torch.zeros(plan.tokens, dtype=torch.bool, device=DEV), 0
+    for b, (c, n) in enumerate(zip(context, new)):
+        own = torch.arange(c, c + n, device=DEV)
+        for at in {max(0, c - 2), max(0, c + n // 2 - 1)}:
+            page_at = plan.block_tables[b, at // page]
+            k[page_at, at % page, 0, 5], v[page_at, at % page, 0, 17] = -2400.0 * (dim / 64) ** 0.5, value
+            reached[row:row + n] |= (at <= own) & (at > own - (window or 1 << 30))
+        row += n
+    got = smx.paged_attention(q, k, v, plan, window=window)[:, :, 17]
+    assert (~got.isfinite()).eq(reached[:, None]).all() and reached.any()
