@@ -397,7 +397,8 @@ int smx_qk_norm_rope(int64_t m, int64_t n, const float* x, int64_t ldx, const vo
 #define SMX_PAGED_BAD_LENGTH 1   /* a negative length, over max_new new tokens or past max_context */
 #define SMX_PAGED_OUT_OF_ROWS 2  /* its rows end behind the step's last */
 #define SMX_PAGED_OUT_OF_PAGES 3 /* the free list does not hold the pages it needs */
-#define SMX_PAGED_BAD_PAGE 4     /* the page its context ends in is not one of the cache */
+#define SMX_PAGED_BAD_PAGE 4     /* the page its context ends in, or without a free list one that its new tokens
+                                    need, is not one of the cache */
 
 /* dtype bits of smx_paged_write: float32 scales and RoPE tables (else bf16). */
 #define SMX_PAGED_Q_SCALE_F32 1
@@ -434,14 +435,15 @@ typedef struct smx_paged_step {
  * context_lens[b] tokens in the cache and appends new_lens[b]; the new tokens of all
  * requests are consecutive rows 0 .. tokens - 1 of the step, padding rows behind
  * them. With a free list, request b takes ceil((c + n) / page_size) - ceil(c / page_size)
- * pages from free_pages in request order, and its entries in
+ * pages from free_pages (numbers of the cache's pages, each once) in request order, and its entries in
  * block_tables [requests, width], which share no memory with the other lists, are filled in; without one (NULL) the tables must
  * hold every page already. Out:
  *   starts [requests + 1]: first row of each request;
  *   rows, context, status [requests]: new and context tokens of the requests that are
  *     admitted (0 for others), and SMX_PAGED_* for each;
  *   positions [tokens]: position in its request, -1 for rows of no admitted request;
- *   slots [tokens]: page * page_size + offset, -1 where there is no such page;
+ *   slots [tokens]: page * page_size + offset, -1 for rows of no admitted request and where the free list gave
+ *     a number that is no page of the cache;
  *   pages [2]: how many of free_pages were taken, from its front; and how many the
  *     requests up to the last admitted one need together, admitted or not (more than are free
  *     once they ran out).

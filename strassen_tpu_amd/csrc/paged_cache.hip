@@ -44,6 +44,27 @@ __device__ int32_t block_scan(int32_t x, int32_t* waves, int32_t* total) {
   return x + before;
 }
 
+// Whether entries first .. last of a request's table, for the lanes of a wave with `wanted`, are all pages of the
+// cache. A lane looks at its own request's entries where they are few; the long lists of a prompt are
+// looked through by the whole wave, one request after another. All lanes take part.
+__device__ bool pages_there(const PlanArgs& p, bool wanted, const int32_t* table, int32_t first, int32_t last) {
+  constexpr int32_t kOwn = 4;
+  bool there = true;
+  const bool few = last - first < kOwn;
+  if (wanted && few)
+    for (int32_t i = first; i <= last; ++i) there &= (uint32_t)table[i] < (uint32_t)p.num_pages;
+  for (uint64_t left = __ballot(wanted && !few); left; left &= left - 1) {
+    const int who = __builtin_ctzll(left), lane = threadIdx.x & 63;
+    const auto* const theirs = (const int32_t*)__shfl((int64_t)(uintptr_t)table, who);
+    const int32_t from = __shfl(first, who), to = __shfl(last, who);
+    bool all = true;
+#pragma unroll 4
+    for (int32_t i = from + lane; i <= to; i += 64) all &= (uint32_t)theirs[i] < (uint32_t)p.num_pages;
+    if (!__all(all) && lane == who) there = false;
+  }
+  return there;
+}
+
 // Every workgroup scans the requests for itself (a few thousand integers, in
 // cache after the first) and lays out its own tokens, so that one launch does
 // without a second one behind it: with c the context, n the new tokens and P
@@ -79,11 +100,13 @@ __global__ __launch_bounds__(1024) void paged_plan(PlanArgs p) {
       status = SMX_PAGED_BAD_LENGTH;
     } else if (n > 0 && start + n > p.tokens) {
       status = SMX_PAGED_OUT_OF_ROWS;
-    } else if (n > 0 && (c & mask)) {
-      // the first new token joins the page that the context ends in
-      const int32_t page = p.tables[b * p.table_stride + (c >> p.page_shift)];
-      if ((uint32_t)page >= (uint32_t)p.num_pages) status = SMX_PAGED_BAD_PAGE;
     }
+    // The new tokens' pages that have to be there: that which the context ends in, which the first one joins, and
+    // without a free list all of them.
+    const bool joins = status == SMX_PAGED_OK && n > 0 && ((c & mask) || !p.free_pages);
+    const int32_t page0 = (int32_t)(c >> p.page_shift);
+    const int32_t page1 = joins && !p.free_pages ? (int32_t)((c + n - 1) >> p.page_shift) : page0;
+    if (!pages_there(p, joins, p.tables + b * p.table_stride, page0, page1)) status = SMX_PAGED_BAD_PAGE;
     const int64_t held = (c + mask) >> p.page_shift;
     const int64_t need =
         here && p.free_pages && status == SMX_PAGED_OK && n > 0 ? ((c + n + mask) >> p.page_shift) - held : 0;

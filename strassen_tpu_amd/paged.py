@@ -39,8 +39,8 @@ class PagedPlan:
       requests that are not admitted.
     * ``status`` int32 [requests]: ``PAGED_OK`` or why a request is not admitted.
     * ``positions`` int32 [tokens]: each row's position, -1 for rows of no admitted request.
-    * ``slots`` int64 [tokens]: ``page * page_size + offset`` of each row, -1 where
-      there is no page.
+    * ``slots`` int64 [tokens]: ``page * page_size + offset`` of each row, -1 for rows of no admitted
+      request, and where the free list gave a number that is no page of the cache.
     * ``pages_used`` int32 [1]: how many free pages were taken, from the list's front.
     * ``pages_needed`` int32 [1]: how many the requests up to the last admitted one need together,
       admitted or not; more than the list holds once it ran out.
@@ -61,7 +61,7 @@ def paged_plan(context_lens, new_lens, block_tables, *, page_size, num_pages, to
     tokens and appends ``new_lens[b]`` (0: it sits the step out).
 
     ``block_tables`` int32 ``[requests, width]`` names each request's pages. With
-    ``free_pages`` (int32, distinct page numbers) the requests take the pages that they
+    ``free_pages`` (int32, distinct numbers of the cache's pages) the requests take the pages that they
     need, ``ceil((context + new) / page_size) - ceil(context / page_size)`` each, from its front in
     request order, and their entries are written into ``block_tables`` (which shares no memory
     with the other arguments); without, every page must be there already. ``tokens`` is the step's number of rows
@@ -69,8 +69,9 @@ def paged_plan(context_lens, new_lens, block_tables, *, page_size, num_pages, to
     bound the new tokens of a request and its tokens in all, where a program knows
     them (default: ``tokens``, and what the tables hold).
 
-    A request whose lengths break these bounds, whose rows do not fit or whose pages ran
-    out is not admitted: ``status`` says why, its table stays as it was, nothing of it is
+    A request whose lengths break these bounds, whose rows do not fit, whose pages ran
+    out, or whose table does not name the page that its context ends in (without ``free_pages``: any
+    page that its new tokens go to) is not admitted: ``status`` says why, its table stays as it was, nothing of it is
     written and its rows of an attention are zero. Its rows keep their place. A request that
     needs no new page is admitted though others before it ran out.
     """

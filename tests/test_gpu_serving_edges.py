@@ -245,3 +245,39 @@ def test_attention_of_infinities_whose_weight_is_nothing(dim, context, new, max_
         row += n
     got = smx.paged_attention(q, k, v, plan, window=window)[:, :, 17]
     assert (~got.isfinite()).eq(reached[:, None]).all() and reached.any()
+
+
+@pytest.mark.parametrize("requests,page,most,tokens", [(5, 8, 70, 400), (70, 8, 40, 4000), (1500, 16, 70, 60000), (3, 8, 9000, 30000)])
+def test_plan_without_a_free_list_looks_at_every_page_of_the_new_tokens(requests, page, most, tokens):
+    """Missing entries among the pages that the new tokens go to, a few or thousands of a request, keep it out; entries
+    before and behind them do not matter."""
+    g = torch.Generator().manual_seed(requests)
+    context = torch.randint(0, 60, (requests,), generator=g)
+    new = torch.randint(0, most, (requests,), generator=g)
+    context[0], new[0] = 2 * page, page  # whole pages
+    width = int(((context + new + page - 1) // page).max()) + 1
+    pages = requests * width
+    tables = torch.randperm(pages, generator=g).view(requests, width)
+    first, last = context // page, (context + new - 1) // page
+    at = torch.arange(width)[None]
+    tables[(at < first[:, None]) | (at > last[:, None])] = -1  # what no new token goes to
+    bad = torch.rand(requests, generator=g) < 0.5
+    bad[0] = False
+    where = first + (torch.rand(requests, generator=g) * (last - first + 1)).long()
+    where[1], where[2] = first[1], last[2]
+    odd = torch.tensor([-1, pages, 2**31 - 1, -2**31])[torch.arange(requests) % 4]
+    spoilt = bad & (new > 0)
+    tables[spoilt, where[spoilt]] = odd[spoilt]
+    plan = smx.paged_plan(i32(context.tolist()), i32(new.tolist()), i32(tables.tolist()), page_size=page, num_pages=pages,
+                          tokens=tokens)
+    starts = torch.cat((torch.zeros(1, dtype=torch.int64), new.cumsum(0)))
+    assert int(starts[-1]) <= tokens and spoilt.any()
+    assert plan.status.tolist() == torch.where(spoilt, smx.PAGED_BAD_PAGE, smx.PAGED_OK).tolist()
+    assert plan.rows.tolist() == torch.where(spoilt, 0, new).tolist() and plan.starts.tolist() == starts.tolist()
+    slots = torch.full((tokens,), -1)
+    for b in range(requests):
+        if not spoilt[b]:
+            key = torch.arange(int(context[b]), int(context[b] + new[b]))
+            slots[starts[b]:starts[b + 1]] = tables[b][key // page] * page + key % page
+    assert plan.slots.tolist() == slots.tolist()  # no row of an admitted request without a place
+    assert torch.equal(plan.positions >= 0, plan.slots >= 0)
