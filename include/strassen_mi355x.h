@@ -511,7 +511,8 @@ typedef struct smx_int4_weight {
  * SMX_EPI_NONE; SMX_EPI_SWIGLU (out [m, n / 2] = silu(gate) up, a weight laid out for
  * it); SMX_EPI_RESIDUAL_ADD and SMX_EPI_BIAS_ADD (extra [m, n] or [n], bf16, or float32 with
  * extra_f32). k % 32 == 0. Meant for few rows: every 64 rows read the weight again.
- * An infinity in x makes its row NaN. Asynchronous on stream.
+ * An infinity in x makes its row NaN, and finite values beyond 2^115 may: sums of up to 31 |x| over a group
+ * are formed in FP32 before its scale. Asynchronous on stream.
  */
 int smx_int4_matmul(const smx_int4_weight* w, int64_t m, const void* x, int64_t ldx, int32_t epilogue,
                     const void* extra, int64_t lde, int32_t extra_f32, void* out, int64_t ldo, void* workspace,

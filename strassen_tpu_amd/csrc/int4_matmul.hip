@@ -7,7 +7,8 @@
 // half an and-or. Per group
 //   sum_k x_k (q_k - z) = sum_k x_k (16 + q_k) - (16 + z) sum_k x_k,
 // whose second sum is one more MFMA, against ones, shared by all columns of the wave, and
-// the group's scale multiplies the FP32 sum of both: no product is rounded before the end. Without zero
+// the group's scale multiplies the FP32 sum of both: no product is rounded before the end. (Both sums
+// stay below 128 * 31 |x| < 2^127 for |x| up to 2^115; larger values may overflow.) Without zero
 // points (z = 8) that MFMA is against -24 and the products start from its result (61 rows of a 5120 x
 // 8192 weight in groups of 32: 18.8 us, with the multiply-adds 20.6).
 //

@@ -119,7 +119,8 @@ def int4_matmul(x, w, *, epilogue=None, residual=None, bias=None):
     "swiglu" (``silu(gate) * up``), "residual_add" (``residual [M, N]``) and "bias_add"
     (``bias [N]``), in FP32 with one rounding; the weight is used exactly as its codes, scales
     and zeros say. Meant for decode steps: every 64 rows read the weight again. A row of ``x``
-    with an infinity is NaN in the result."""
+    with an infinity is NaN in the result; one with finite values beyond 2^115 (4e34) may be, however small the
+    scales: 31 times a group's ``|x|`` is summed in FP32 before its scale."""
     if not isinstance(w, Int4Operand):
         raise TypeError("w must be an Int4Operand (int4_weight_layout)")
     if epilogue not in _EPILOGUES:

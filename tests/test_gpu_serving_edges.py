@@ -281,3 +281,17 @@ def test_plan_without_a_free_list_looks_at_every_page_of_the_new_tokens(requests
             slots[starts[b]:starts[b + 1]] = tables[b][key // page] * page + key % page
     assert plan.slots.tolist() == slots.tolist()  # no row of an admitted request without a place
     assert torch.equal(plan.positions >= 0, plan.slots >= 0)
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("m,zeros", [(1, True), (20, True), (61, False)])
+def test_int4_of_the_largest_values(group, m, zeros):
+    """|x| up to 2^115 times scales that bring the sums back: 128 terms of 31 |x| stay below 2^127."""
+    codes, scales, zero, w, spread, g = weight(512, 70, group, zeros)
+    scales = (scales.float() * 2.0 ** -118).to(torch.bfloat16)  # some of them subnormal, with fewer bits
+    spread = scales.double().repeat_interleave(group, 0)
+    w = (codes.double() - (8 if zero is None else zero.double().repeat_interleave(group, 0))) * spread
+    laid = smx.int4_weight_layout(codes, scales, zero, group=group)
+    x = bf16(m, 512, g=g).sign() * 2.0 ** 115  # of one size: the sums are as large as they get
+    x[0] = x[0].abs()  # without cancellation
+    check(smx.int4_matmul(x, laid), x, w, spread.abs())
