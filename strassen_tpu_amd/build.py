@@ -20,6 +20,7 @@ import subprocess
 import sys
 import sysconfig
 import tempfile
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
@@ -197,19 +198,41 @@ def _compile_unit(source, workdir):
         return obj, f.read(), stderr
 
 
+def _compile_host(output):
+    """Compiles the host module to `output`; returns (whether it did, the compiler's messages)."""
+    try:
+        result = subprocess.run(host_command(output), capture_output=True, text=True)
+    except OSError as e:  # no host compiler
+        return False, str(e)
+    return result.returncode == 0, result.stderr
+
+
+def _install_host(built, messages):
+    """Puts the host module in its place. Without one (no host compiler, or no headers of torch or Python) the
+    library serves everything but the serving operators, which then say what is missing: a module
+    of another build is not left beside it."""
+    if built:
+        os.replace(HOST_MODULE + ".tmp", HOST_MODULE)
+        return
+    for path in (HOST_MODULE, HOST_MODULE + ".tmp"):
+        if os.path.exists(path):
+            os.remove(path)
+    warnings.warn("the serving operators' host module was not built, the library was:\n" + messages, RuntimeWarning, stacklevel=3)
+
+
 def build(verbose=False, jobs=None):
-    """Compile the library; returns its path. Always recompiles."""
+    """Compile the library, and the serving operators' host module where the host can; returns the library's
+    path. Always recompiles."""
     tmp = LIBRARY + ".tmp"
     jobs = jobs or min(len(SOURCES), os.cpu_count() or 1)
     with tempfile.TemporaryDirectory() as scratch:
         dirs = [os.path.join(scratch, f"unit{i}") for i in range(len(SOURCES))]
         with ThreadPoolExecutor(max_workers=jobs) as pool:
-            host = pool.submit(subprocess.run, host_command(HOST_MODULE + ".tmp"), capture_output=True, text=True)
+            host = pool.submit(_compile_host, HOST_MODULE + ".tmp")
             units = list(pool.map(_compile_unit, SOURCES, dirs))
-        if host.result().returncode != 0:
-            raise RuntimeError("host module failed:\n" + host.result().stderr)
-        if verbose and host.result().stderr.strip():
-            print(host.result().stderr, file=sys.stderr)
+        built, messages = host.result()
+        if verbose and built and messages.strip():
+            print(messages, file=sys.stderr)
         checked = gemms = 0
         for source, (_, text, stderr) in zip(SOURCES, units):
             if verbose and stderr.strip():
@@ -230,8 +253,8 @@ def build(verbose=False, jobs=None):
             raise RuntimeError("link failed:\n" + " ".join(cmd) + "\n" + result.stderr)
     if verbose:
         print(f"verified {checked} inline-asm MFMA kernels and the scratch of {gemms} GEMM kernels", file=sys.stderr)
-    os.replace(HOST_MODULE + ".tmp", HOST_MODULE)
     os.replace(tmp, LIBRARY)
+    _install_host(built, messages)
     return LIBRARY
 
 

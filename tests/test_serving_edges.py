@@ -142,3 +142,34 @@ def test_traced_calls_are_refused():
     for mode in ("real", "fake"):
         with pytest.raises(ValueError, match="traced"):
             make_fx(lambda x: smx.int4_matmul(x, w), tracing_mode=mode)(x)
+
+
+def _headers_without_torch(build, monkeypatch, tmp_path):
+    command = build.host_command
+    monkeypatch.setattr(build, "host_command", lambda output: [x for x in command(output) if not x.endswith("torch/include")])
+
+
+def _no_compiler(build, monkeypatch, tmp_path):
+    monkeypatch.setenv("CXX", str(tmp_path / "no-such-compiler"))
+
+
+@pytest.mark.parametrize("missing", [_no_compiler, _headers_without_torch])
+def test_library_is_built_without_the_host_module(missing, monkeypatch, tmp_path):
+    """No host compiler, or no headers of torch: the library is put in place, a host module of another build is not
+    left beside it, and the build says so."""
+    from strassen_tpu_amd import build
+
+    library, module = tmp_path / "library.so", tmp_path / "_serving.so"
+    library.write_text("old"), module.write_text("old")
+    monkeypatch.setattr(build, "LIBRARY", str(library))
+    monkeypatch.setattr(build, "HOST_MODULE", str(module))
+    # the device units' part of the build, whose compiler is not what is missing
+    monkeypatch.setattr(build, "_compile_unit", lambda source, workdir: (source, "", ""))
+    monkeypatch.setattr(build, "verify_inline_asm_kernels", lambda text: 1)
+    monkeypatch.setattr(build, "verify_kernel_scratch", lambda text, require=True: 1)
+    monkeypatch.setattr(build, "link_command", lambda objects, output: ["cp", objects[0], output])
+    missing(build, monkeypatch, tmp_path)
+    with pytest.warns(RuntimeWarning, match="host module was not built"):
+        assert build.build() == str(library)
+    assert library.read_text() == open(build.SOURCES[0]).read()
+    assert not module.exists() and not (tmp_path / "_serving.so.tmp").exists()
