@@ -295,3 +295,74 @@ def test_int4_of_the_largest_values(group, m, zeros):
     x = bf16(m, 512, g=g).sign() * 2.0 ** 115  # of one size: the sums are as large as they get
     x[0] = x[0].abs()  # without cancellation
     check(smx.int4_matmul(x, laid), x, w, spread.abs())
+
+
+def counted_cache(context, new, *, page, kv_heads, dim, seed, max_new=None):
+    """A plan, and a cache whose values are whole numbers in a few units: with queries of zero every key weighs 1, so
+    that a row's sums are exact in FP32 and its result is their mean, rounded once. Also the requests' values
+    summed up to each position [context + new, kv_heads, dim]."""
+    plan, k, v, keys, values, g = make_step(context, new, page=page, kv_heads=kv_heads, dim=dim, seed=seed)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=page, num_pages=plan.num_pages,
+                          tokens=plan.tokens, max_new=max_new)
+    sums = []
+    for b, (c, n) in enumerate(zip(context, new)):
+        at = torch.arange(c + n, device=DEV)
+        whole = torch.randint(-8, 9, (c + n, kv_heads, dim), device=DEV, generator=g).double()
+        v[plan.block_tables[b].long()[at // page], at % page] = whole.to(torch.bfloat16)
+        sums.append(whole.cumsum(0))
+    return plan, k, v, sums
+
+
+def check_means(got, sums, context, new, window, steps):
+    """Every row's mean over the keys that it sees, to one rounding (and the reciprocal's): a step of keys left out,
+    counted twice or taken from elsewhere moves a row's 64 or more columns by several times that."""
+    row = 0
+    for (c, n), total in zip(zip(context, new), sums):
+        own = torch.arange(c, c + n, device=DEV)
+        seen = torch.clamp(own + 1, max=window or 1 << 30)
+        before = torch.where((own >= seen)[:, None, None], total[(own - seen).clamp(min=0)], 0.0)
+        want = (total[own] - before) / seen[:, None, None]
+        mine = got[row:row + n].double().unflatten(1, (total.shape[1], -1))
+        bound = (2.0 ** -8 + 2.0 ** -22) * want.abs()[:, :, None]
+        assert ((mine - want[:, :, None]).abs() <= bound).all()
+        # what the bound can tell, for the last row: any one step of its keys left out
+        first, last = int(own[-1] - seen[-1]) // steps + 1, int(own[-1]) // steps
+        ends = total[torch.arange(first + 1, max(first + 1, last), device=DEV) * steps - 1]  # (none of a short one)
+        lost = want[-1] - (want[-1] * seen[-1] - ends.diff(dim=0)) / (seen[-1] - steps)
+        assert (lost.abs() > 2 * bound[-1, :, 0]).flatten(1).any(1).all()
+        row += n
+
+
+@pytest.mark.parametrize("context,new,kv_heads,group,dim,max_new,window", [
+    ([131000], [1], 1, 8, 128, 1, None), ([131071, 5, 70001, 129], [1, 1, 1, 1], 2, 4, 64, 1, None),
+    ([131000, 3000], [4, 3], 1, 8, 128, 4, None), ([131000, 65536], [1, 1], 2, 8, 128, 1, 70000),
+    ([131000], [40], 1, 4, 128, None, None), ([131071, 9, 40000], [1, 1, 300], 2, 8, 64, None, None),
+    ([131000, 65530], [200, 33], 1, 4, 64, None, 70000), ([1_000_000], [1], 1, 2, 128, 1, None)])
+def test_attention_counts_every_key_of_long_contexts(context, new, kv_heads, group, dim, max_new, window):
+    plan, k, v, sums = counted_cache(context, new, page=64, kv_heads=kv_heads, dim=dim, seed=11, max_new=max_new)
+    q = torch.zeros(plan.tokens, kv_heads * group, dim, dtype=torch.bfloat16, device=DEV)
+    check_means(smx.paged_attention(q, k, v, plan, window=window), sums, context, new, window, 32 if max_new else 64)
+
+
+@pytest.mark.parametrize("window", [None, 20000])
+def test_attention_counts_every_key_of_a_long_prompt(window):
+    """All of 100,000 rows, whose tiles' counts of steps pass 16 bits."""
+    plan, k, v, sums = counted_cache([0], [100_000], page=64, kv_heads=1, dim=64, seed=12)
+    q = torch.zeros(plan.tokens, 2, 64, dtype=torch.bfloat16, device=DEV)
+    check_means(smx.paged_attention(q, k, v, plan, window=window), sums, [0], [100_000], window, 64)
+
+
+@pytest.mark.parametrize("context,new,max_new,dim", [([131000, 20], [1, 1], 1, 128), ([131072], [1], 1, 64),
+                                                    ([131000, 20], [30, 1], None, 128)])
+def test_attention_of_131000_keys(context, new, max_new, dim):
+    """Weights and result are rounded to bf16, each by half a step at most evenly spread, 2^-8 / 3^0.5 in the mean:
+    2^-8 (2 / 3)^0.5 = 3.2e-3 of a row's norm together, over 64 or more columns seldom more than a third above it. A
+    step of 32 keys less would be (32 / 131000)^0.5 = 1.6e-2."""
+    plan, k, v, keys, values, g = make_step(context, new, page=16, kv_heads=2, dim=dim, seed=13)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=16, num_pages=plan.num_pages,
+                          tokens=plan.tokens, max_new=max_new)
+    q = bf16(plan.tokens, 8, dim, g=g)
+    want, size = attend64(q, keys, values, context, new, None)
+    got = smx.paged_attention(q, k, v, plan)
+    check_attention(got, want, size)
+    assert ((got.double() - want).norm(dim=-1) <= 5e-3 * want.norm(dim=-1)).all()
