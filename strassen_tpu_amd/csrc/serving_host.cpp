@@ -91,6 +91,11 @@ const Tensor& tensor(PyObject* o, const char* name) {
   return t;
 }
 
+// The call wrote to t: a backward pass that kept its values finds out.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // A call that is traced would run once, on the tensors at hand, and be missing from what is traced.
 void not_traced() {
   using c10::impl::TorchDispatchModeKey;
@@ -249,6 +254,7 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t) {
       check(lib.plan((int32_t)std::min<int64_t>(requests, INT32_MAX), (int32_t)width, (int32_t)page_size, (int32_t)num_pages,
                      (int32_t)tokens, (int32_t)max_new, (int32_t)max_context, context, fresh, entries, stride, free,
                      (int32_t)free_count, at[1], at[2], at[3], at[5], p->slots, at[4], at[6], stream_of(device)));
+      if (free) written(tables);
       PyObject* const result = PyTuple_New(12);
       if (!result) throw Raised();
       PyTuple_SET_ITEM(result, 0, capsule);
@@ -373,6 +379,7 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t) {
     check(lib.write(&cache, plan.step.tokens, plan.step.positions, plan.slots, out.defined() ? &q : nullptr, &k, &v, cos, sin,
                     rope_rows, rope_stride, q_scale, k_scale, dtypes, (float)real(a[10]),
                     out.defined() ? out.mutable_data_ptr() : nullptr, stream_of(plan.device)));
+    for (PyObject* const o : {a[2], a[3]}) written(tensor(o, "cache"));
     if (!out.defined()) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
   });
@@ -409,6 +416,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t) {
     check(lib.attention(&cache, &plan.step, &q, &rows, (float)scale, (int32_t)window, own, workspace.mutable_data_ptr(), need,
                         stream_of(plan.device)));
     if (own) return THPVariable_Wrap(std::move(out));
+    written(tensor(a[6], "out"));
     Py_INCREF(a[6]);
     return a[6];
   });

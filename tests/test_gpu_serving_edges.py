@@ -366,3 +366,29 @@ def test_attention_of_131000_keys(context, new, max_new, dim):
     got = smx.paged_attention(q, k, v, plan)
     check_attention(got, want, size)
     assert ((got.double() - want).norm(dim=-1) <= 5e-3 * want.norm(dim=-1)).all()
+
+
+def test_backward_passes_find_out_what_was_written():
+    """Values kept for a backward pass that a call overwrites are an error there, not another gradient."""
+    plan, good = write_inputs(torch.Generator(device=DEV).manual_seed(3))
+    k_cache, v_cache, q = good["k_cache"], good["v_cache"], good["q"]
+    out, tables = torch.zeros_like(q), i32([[0, 1, -1]])
+    lens = i32([9])
+    for kept, call in ((k_cache, lambda: smx.paged_write(plan=plan, **good)), (v_cache, lambda: smx.paged_write(plan=plan, **good)),
+                       (out, lambda: smx.paged_attention(q, k_cache, v_cache, plan, out=out)),
+                       (tables, lambda: smx.paged_plan(lens, lens, tables, page_size=8, num_pages=4, tokens=9, free_pages=i32([3])))):
+        factor = torch.ones((), device=DEV, requires_grad=True)
+        loss = (factor * kept).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    assert tables.tolist() == [[0, 1, 3]]
+    before = tables._version, k_cache._version, q._version
+    smx.paged_plan(lens, lens, tables, page_size=8, num_pages=4, tokens=9)  # read only
+    smx.paged_attention(q, k_cache, v_cache, plan)
+    assert before == (tables._version, k_cache._version, q._version)
+    with torch.inference_mode():
+        cache = [torch.zeros_like(k_cache) for _ in range(2)]
+    with torch.no_grad():  # tensors of inference mode, which count no versions
+        smx.paged_write(good["k"], good["v"], *cache, plan)
+    assert torch.equal(cache[0][plan.slots // 8, plan.slots % 8], good["k"])
