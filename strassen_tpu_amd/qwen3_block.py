@@ -325,8 +325,12 @@ def block_step(x, block, k_cache, v_cache, plan, *, window=None):
     shape, the new tokens' keys and values stored in the layer's cache and attended to
     together with those before them (``paged_plan``, ``paged_write``, ``paged_attention``).
     The "strassen" and "cubic" arms take tokens in whole sixteens (the plan may have padding
-    rows). Rows of no admitted request pass through as rows of their own and touch no cache."""
+    rows). Rows of no admitted request touch no cache and no other row. "strassen", whose products combine rows
+    (an infinity or NaN in one admitted row reaches others of its tile), takes them as zero; in the other arms
+    they pass through as rows of their own."""
     d, w = block.dims, block.weights
+    if block.arm == "strassen":
+        x = x.masked_fill((plan.positions < 0)[:, None], 0)
     normalized = _row_rms_norm(x, w.attention_norm, d.eps)
     heads = block.product(normalized, block.qkv).view(plan.tokens, d.heads + 2 * d.kv_heads, d.head_dim)
     query, key, value = heads.split((d.heads, d.kv_heads, d.kv_heads), dim=1)
