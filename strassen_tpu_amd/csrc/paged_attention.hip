@@ -1129,7 +1129,9 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
     return fail(SMX_ERR_INVALID, "out must be the queries themselves or share no memory with them");
   for (const void* x : {cache->k, cache->v})
     if (meet(cache_runs(*cache, x), to)) return fail(SMX_ERR_INVALID, "out must share no memory with the cache");
-  if (!(scale > 0.f) || !(scale < INFINITY)) return fail(SMX_ERR_INVALID, "scale must be positive and finite");
+  constexpr float kLog2E = 1.44269504088896341f;  // (the kernels' exponentials are powers of two)
+  if (!(scale > 0.f) || !(scale * kLog2E < INFINITY))
+    return fail(SMX_ERR_INVALID, "scale must be positive and finite, also times log2 e");
   if (window < 0) return fail(SMX_ERR_INVALID, "window must not be negative (0: none)");
   int cus = 0;
   if (int rc = device_cus(&cus)) return rc;
@@ -1155,7 +1157,7 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
   // 1000 keys 12.4 us; with two steps 13.1, three 15.4), two of 64 (two requests of 60 rows on 1000: 25.4; one
   // 27.4, three 26.0).
   p.min_span = few ? 2 : 5;
-  p.scale = scale * 1.44269504088896341f;
+  p.scale = scale * kLog2E;
   p.per_group = 1.f / p.group;
   p.per_workgroup = 1. / blocks;
   p.records = (int32_t*)workspace;

@@ -173,3 +173,12 @@ def test_library_is_built_without_the_host_module(missing, monkeypatch, tmp_path
         assert build.build() == str(library)
     assert library.read_text() == open(build.SOURCES[0]).read()
     assert not module.exists() and not (tmp_path / "_serving.so.tmp").exists()
+
+
+def test_attention_refuses_a_scale_that_overflows():
+    """The largest scales times log2 e are infinite, and an infinity times a score of zero NaN."""
+    for scale in (3e38, 2.36e38, float("inf")):
+        rc, said = _message(_attention(scale=scale, q=_heads(data=Q), out=_heads(data=OUT), cache=_cache(k=FAR, v=FAR + (1 << 24))))
+        assert rc == _lib.SMX_ERR_INVALID and "scale" in said, said
+    rc, said = _message(_attention(scale=2.35e38, q=_heads(data=Q), out=_heads(data=OUT), cache=_cache(k=FAR, v=FAR + (1 << 24))))
+    assert "scale" not in said, said
