@@ -477,7 +477,8 @@ int smx_paged_write(const smx_paged_cache* cache, int32_t tokens, const int32_t*
  * h / (heads / kv_heads). softmax(scale q k) in FP32, its weights rounded to bf16 for the
  * product with the values, one bf16 rounding of the result. Infinities and NaN
  * reach the rows that see them only; slots behind a request's last token are not read. Keys of pages that are
- * not in the cache (0 .. num_pages - 1) are not seen, and a row that sees none is zero. Rows of no
+ * not in the cache (0 .. num_pages - 1) are not seen, and a row that sees none is zero (one whose scores are
+ * all -inf is NaN). Rows of no
  * request stay as they are, or become zero with zero_rows. out's rows lie apart from each other and
  * share no memory with the cache, nor with q unless they are q's (same address and strides). The workspace
  * (smx_paged_attention_workspace_bytes, for the current device) is overwritten.

@@ -24,6 +24,8 @@
 // prompts, alone or mixed, fill the chip alike. An item cut by a span's end leaves
 // partial sums in the workspace that paged_join adds up. Counts of tiles have closed
 // forms, so every workgroup finds its span by itself, from the lengths on the device.
+#include <cfloat>
+
 #include "kernel_packed.hpp"
 #include "launch.hpp"
 
@@ -450,7 +452,7 @@ __device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
 template <int D>
 struct Rows {
   f32x16 o[D / 32];
-  float top, sum;  // the reference maximum (scores times scale); this lane's share of the sum
+  float top, sum;  // the reference maximum (scores times scale; -inf: no key was seen); this lane's share of the sum
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -582,6 +584,7 @@ __device__ __forceinline__ void attend(Rows<D>& r, const bf16x8 (&q)[D / 16], co
   bf16x8 v[kBlocks][2][D / 32];
   read_values<D, 0>(v[0], at);
   if constexpr (kBlocks == 2) read_values<D, 32 * T::kRow>(v[kBlocks - 1], at);
+  float lowest = -FLT_MAX;
   if (masked) {
     // key - first key of the step = 32 x + 8 (e / 4) + 4 half + e % 4; `rel` is the
     // row's position less the step's first key
@@ -601,13 +604,19 @@ __device__ __forceinline__ void attend(Rows<D>& r, const bf16x8 (&q)[D / 16], co
           s[x][e] = key > oldest && ((bits >> key) & 1) ? s[x][e] : -INFINITY;
         }
     }
+    // the bits of the keys that the row sees
+    const int newest = min(rel, 32 * kBlocks - 1), before = window ? min(rel - window, 63) : -1;
+    uint64_t sees = newest >= 0 ? held & ~0ull >> (63 - newest) : 0;
+    if (before >= 0) sees &= ~(~0ull >> (63 - before));
+    if (!sees) lowest = -INFINITY;
   }
   float top = s[0][0];
 #pragma unroll
   for (int x = 0; x < kBlocks; ++x)
 #pragma unroll
     for (int e = 0; e < 16; ++e) top = fmaxf(top, s[x][e]);
-  top = fmaxf(top, other_half(top)) * scale;
+  // (a maximum of -inf is left to rows that see no key)
+  top = fmaxf(fmaxf(top, other_half(top)) * scale, lowest);
   if (__any(top > r.top + 8.f)) {
     const float next = fmaxf(r.top, top);
     const float factor = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(r.top - next);
@@ -680,21 +689,10 @@ __device__ __forceinline__ void store_rows(const AttentionArgs& p, const f32x16 
   for (int x = 0; x < D / 32; ++x) store_block(to + 32 * x, o[x], inverse, valid, thread >> 5 & 1);
 }
 
-// Whether the row at `position` of a request sees any key: a page from its window's first on is in the cache.
-__device__ __forceinline__ bool sees_a_key(const AttentionArgs& p, int request, int position) {
-  const int32_t* const table = p.tables + request * p.table_stride;
-  const int first = p.window ? max(0, position - p.window + 1) >> p.page_shift : 0;
-  for (int i = position >> p.page_shift; i >= first; --i)
-    if ((uint32_t)table[i] < (uint32_t)p.num_pages) return true;
-  return false;
-}
-
 // What a row's values are multiplied with. Its largest weight is 1, so that a sum is zero only without one: a row
-// that sees no key is zero, and one all of whose scores are -inf is NaN. Only then is the table looked through.
-__device__ __forceinline__ float inverse_of(float sum, const AttentionArgs& p, int request, int position) {
-  float inverse = sum > 0.f ? 1.f / sum : sum;
-  if (__any(sum == 0.f) && sum == 0.f && sees_a_key(p, request, position)) inverse = NAN;
-  return inverse;
+// that sees no key (its maximum is still -inf) is zero, and one all of whose scores are -inf is NaN.
+__device__ __forceinline__ float inverse_of(float sum, float top) {
+  return sum > 0.f ? 1.f / sum : sum == 0.f && top > -INFINITY ? NAN : sum;
 }
 
 // 128 rows a tile (four waves of 32), 64 keys a step, keys and values double buffered. 2048 tokens of 64 heads on
@@ -819,7 +817,7 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
 
       const float sum = o.sum + other_half(o.sum);
       if (part.count == part.tile_count) {
-        store_rows<D>(p, o.o, inverse_of(sum, p, part.request, position), 32 * wave + (lane & 31) < tile_rows,
+        store_rows<D>(p, o.o, inverse_of(sum, o.top), 32 * wave + (lane & 31) < tile_rows,
                       scalar_at(p.starts, part.request) + local, head);
       } else {
         float* const to = p.partial + (2 * (int64_t)s.worker + part.begins) * kPartialFloats<D>;
@@ -935,7 +933,7 @@ __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
 
     const float sum = o.sum + other_half(o.sum);
     if (count == part.tile_count) {
-      store_rows<D>(p, o.o, inverse_of(sum, p, part.request, position), valid, token, head);
+      store_rows<D>(p, o.o, inverse_of(sum, o.top), valid, token, head);
     } else {
       float* const to = p.partial + (2 * (int64_t)s.worker + part.begins) * kFewPartialFloats<D>;
       if (valid) {
@@ -1007,9 +1005,8 @@ __global__ __launch_bounds__(1024) void paged_join_few(AttentionArgs p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) value[j] = value[j] * keep + values[at][j] * add;
   }
-  const int local = record.tile * p.tile_tokens + row / p.group;
-  const float inverse = inverse_of(total, p, record.request, p.context[record.request] + local);
-  const int64_t token = p.starts[record.request] + local;
+  const float inverse = inverse_of(total, top);
+  const int64_t token = p.starts[record.request] + record.tile * p.tile_tokens + row / p.group;
   *reinterpret_cast<uint2*>(p.out + token * p.out_token + (record.head * p.group + row % p.group) * p.out_head + column) =
       make_uint2(pack_bf16(value[0] * inverse, value[1] * inverse), pack_bf16(value[2] * inverse, value[3] * inverse));
 }
@@ -1046,10 +1043,9 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join(AttentionArgs p) {
   const int fresh = p.rows[record.request];
   const int tile_rows = min(p.tile_tokens, fresh - record.tile * p.tile_tokens) * p.group;
   const int at = 32 * wave + (lane & 31), row = min(at, tile_rows - 1);
-  const int local = record.tile * p.tile_tokens + row / p.group;
-  const int64_t token = p.starts[record.request] + local;
+  const int64_t token = p.starts[record.request] + record.tile * p.tile_tokens + row / p.group;
   store_block(p.out + token * p.out_token + (record.head * p.group + row % p.group) * p.out_head + 32 * x, o,
-              inverse_of(sum, p, record.request, p.context[record.request] + local), at < tile_rows, lane >> 5);
+              inverse_of(sum, top), at < tile_rows, lane >> 5);
 }
 
 // Workgroups of a launch, a multiple of the 8 XCDs: as many as a CU holds (two of paged_attend, by its
