@@ -696,7 +696,7 @@ __device__ __forceinline__ float inverse_of(float sum, float top) {
 }
 
 // 128 rows a tile (four waves of 32), 64 keys a step, keys and values double buffered. 2048 tokens of 64 heads on
-// 16384 cached ones: 1.33 ms, 0.88 PFLOP/s. Matrix cores, vector units and LDS are each busy 40 to 44% of the time
+// 16384 cached ones: 1.32 ms, 0.89 PFLOP/s. Matrix cores, vector units and LDS are each busy 41 to 44% of the time
 // (one workgroup a CU: 2.0 ms): two waves a SIMD do not cover each other's way from a step's keys to
 // its output, and registers and LDS hold no third. Without the exponentials 9% less, without the
 // values' reads nothing. Scores of the next step beside the weights of this one, in the same wave: 1.50 ms (247
@@ -849,7 +849,7 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
 // Steps of few rows (decoding): a workgroup is one wave with 32 rows a tile, which streams 32
 // keys a step through its own two buffers, so that no barrier joins it to others and
 // four of them (32 KB of LDS each at head_dim 128) keep up to 128 KB of a CU's reads in
-// flight. Rows are few: what bounds it is the cache's bytes: 64 requests, 260,000 cached tokens of 4 KB, 198 us
+// flight. Rows are few: what bounds it is the cache's bytes: 64 requests, 260,000 cached tokens of 4 KB, 197 us
 // and 7 in paged_join_few (5.2 TB/s); four of 131,000 tokens 367 and 9 (5.7). Short caches are
 // bound by latency: 1000 tokens 9 us, of which 1.6 pass until the span is found, 1.4 until the first
 // loads are on their way, 1.2 in a step.

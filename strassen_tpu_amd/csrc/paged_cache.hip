@@ -72,8 +72,8 @@ __device__ bool pages_there(const PlanArgs& p, bool wanted, const int32_t* table
 // needs ceil((c + n) / P) - ceil(c / P) new pages, taken from the free list in
 // request order. LDS: [requests + 1] row starts, then [requests] offsets into the
 // free list (-1: not admitted). What bounds it is latency: one load of
-// the lengths, two scans, one dependent load per token: 4.2 us at 16 requests,
-// 11.1 us at 2048 (13.0 with 64-bit scans).
+// the lengths, two scans, one dependent load per token: 4.4 us at 16 requests,
+// 11.7 us at 2048 (13.0 with 64-bit scans).
 __global__ __launch_bounds__(1024) void paged_plan(PlanArgs p) {
   extern __shared__ int32_t plan_lds[];
   __shared__ int32_t waves[16], most[32];

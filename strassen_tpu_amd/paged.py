@@ -67,7 +67,8 @@ def paged_plan(context_lens, new_lens, block_tables, *, page_size, num_pages, to
     with the other arguments); without, every page must be there already. ``tokens`` is the step's number of rows
     (the new tokens and any padding behind them); ``max_new`` and ``max_context``
     bound the new tokens of a request and its tokens in all, where a program knows
-    them (default: ``tokens``, and what the tables hold).
+    them (default: ``tokens``, and what the tables hold). ``paged_attention`` picks its kernel by ``max_new``:
+    say 1 of a decode step, which else runs in the tiles of a prompt (64 requests: 248 us, not 205).
 
     A request whose lengths break these bounds, whose rows do not fit, whose pages ran
     out, or whose table does not name the page that its context ends in (without ``free_pages``: any
