@@ -436,8 +436,8 @@ typedef struct smx_paged_step {
  * requests are consecutive rows 0 .. tokens - 1 of the step, padding rows behind
  * them. With a free list, request b takes ceil((c + n) / page_size) - ceil(c / page_size)
  * pages from free_pages (numbers of the cache's pages, each once) in request order, and its entries in
- * block_tables [requests, width], which share no memory with the other lists, are filled in; without one (NULL) the tables must
- * hold every page already. Out:
+ * block_tables [requests, width], which share no memory with the other lists, are filled in; without one
+ * (NULL) the tables must hold every page already. Out:
  *   starts [requests + 1]: first row of each request;
  *   rows, context, status [requests]: new and context tokens of the requests that are
  *     admitted (0 for others), and SMX_PAGED_* for each;
@@ -478,10 +478,9 @@ int smx_paged_write(const smx_paged_cache* cache, int32_t tokens, const int32_t*
  * product with the values, one bf16 rounding of the result. Infinities and NaN
  * reach the rows that see them only; slots behind a request's last token are not read. Keys of pages that are
  * not in the cache (0 .. num_pages - 1) are not seen, and a row that sees none is zero (one whose scores are
- * all -inf is NaN). Rows of no
- * request stay as they are, or become zero with zero_rows. out's rows lie apart from each other and
- * share no memory with the cache, nor with q unless they are q's (same address and strides). The workspace
- * (smx_paged_attention_workspace_bytes, for the current device) is overwritten.
+ * all -inf is NaN). Rows of no request stay as they are, or become zero with zero_rows. out's rows lie apart
+ * from each other and share no memory with the cache, nor with q unless they are q's (same address and
+ * strides). The workspace (smx_paged_attention_workspace_bytes, for the current device) is overwritten.
  * Asynchronous on stream.
  */
 int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step, const smx_heads* q,
@@ -513,7 +512,8 @@ typedef struct smx_int4_weight {
  * it); SMX_EPI_RESIDUAL_ADD and SMX_EPI_BIAS_ADD (extra [m, n] or [n], bf16, or float32 with
  * extra_f32). k % 32 == 0. Meant for few rows: every 64 rows read the weight again.
  * An infinity in x makes its row NaN, and finite values beyond 2^115 may: sums of up to 31 |x| over a group
- * are formed in FP32 before its scale. Asynchronous on stream.
+ * are formed in FP32 before its scale. out shares no memory with x or the weight, and with extra only where it
+ * is extra (same address and row length). Asynchronous on stream.
  */
 int smx_int4_matmul(const smx_int4_weight* w, int64_t m, const void* x, int64_t ldx, int32_t epilogue,
                     const void* extra, int64_t lde, int32_t extra_f32, void* out, int64_t ldo, void* workspace,

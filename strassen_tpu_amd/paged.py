@@ -109,8 +109,8 @@ def paged_attention(q, k_cache, v_cache, plan, *, scale=None, window=None, out=N
 
     Softmax in FP32; its weights are rounded to bf16 for the product with the values, and
     the result once. Keys of table entries that are no page of the cache are not seen; a row
-    that sees none is zero. Infinities and NaN in the cache reach the rows that see them
-    and no others. Rows of no admitted request are zero in a new result, and left as they
+    that sees none is zero (one all of whose scores are -inf is NaN). Infinities and NaN in the cache
+    reach the rows that see them and no others. Rows of no admitted request are zero in a new result, and left as they
     were in ``out`` (bf16 ``[tokens, heads, head_dim]``, rows 16-byte aligned). ``out`` may be ``q``; else its rows
     share memory neither with each other nor with ``q`` or the cache."""
     return _lib.host().attention(q, k_cache, v_cache, plan._native, scale, window, out)
