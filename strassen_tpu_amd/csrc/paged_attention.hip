@@ -696,7 +696,7 @@ __device__ __forceinline__ float inverse_of(float sum, float top) {
 }
 
 // 128 rows a tile (four waves of 32), 64 keys a step, keys and values double buffered. 2048 tokens of 64 heads on
-// 16384 cached ones: 1.32 ms, 0.89 PFLOP/s. Matrix cores, vector units and LDS are each busy 41 to 44% of the time
+// 16384 cached ones: 1.30 ms, 0.90 PFLOP/s. Matrix cores, vector units and LDS are each busy 41 to 44% of the time
 // (one workgroup a CU: 2.0 ms): two waves a SIMD do not cover each other's way from a step's keys to
 // its output, and registers and LDS hold no third. Without the exponentials 9% less, without the
 // values' reads nothing. Scores of the next step beside the weights of this one, in the same wave: 1.50 ms (247
