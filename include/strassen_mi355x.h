@@ -41,7 +41,7 @@
 extern "C" {
 #endif
 
-#define SMX_VERSION 15
+#define SMX_VERSION 16
 
 /* Status codes. */
 #define SMX_OK 0
@@ -487,6 +487,89 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
                         const smx_heads* out, float scale, int32_t window, int32_t zero_rows, void* workspace,
                         int64_t workspace_bytes, void* stream);
 int smx_paged_attention_workspace_bytes(int32_t head_dim, int64_t* bytes);
+/* The same, and lse [tokens, heads] (float32, dense, of memory of its own): the logarithm of each row's sum of
+ * exponentials, -inf for a row that sees no key or whose scores are all -inf. Rows of no request are left as they
+ * are. NULL: none. */
+int smx_paged_attention_lse(const smx_paged_cache* cache, const smx_paged_step* step, const smx_heads* q,
+                            const smx_heads* out, float scale, int32_t window, int32_t zero_rows, float* lse,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The attention weight that cached keys receive in a step, summed into key_weights [num_pages, kv_heads,
+ * page_size] (float32, dense, 16-byte aligned): to the slot of key j of a request, for each key/value head,
+ * the sum over the request's rows that see j, and the head's query heads, of exp(scale q k_j - lse) is added; the step's own
+ * keys start from zero. lse is that of smx_paged_attention_lse for the same queries, scale and window. Scores and sums in
+ * FP32; the same call gives the same bits. Slots that no admitted request's keys lie in are left as they are, and so are
+ * those of pages that are not in the cache. The cache's values are not read (v may be k). Requests share no pages.
+ * key_weights shares no memory with the keys, the queries and lse. The workspace
+ * (smx_paged_key_weights_workspace_bytes, for the current device) is overwritten. Asynchronous on stream.
+ */
+int smx_paged_key_weights(const smx_paged_cache* cache, const smx_paged_step* step, const smx_heads* q, const float* lse,
+                          float scale, int32_t window, float* key_weights, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+int smx_paged_key_weights_workspace_bytes(int64_t* bytes);
+
+/*
+ * Cuts the caches of requests down: of the n = context_lens[b] tokens of a request, n > keep, each key/value
+ * head keeps the last min(recent, keep) and of those before them the ones of the largest key_weights (ties: the
+ * lowest index; NaN counts as the largest). Keys, values and weights of the survivors end up at the request's indices 0 ..
+ * keep - 1: a survivor among the first need = keep - min(recent, keep) stays, the j-th evicted place among them
+ * takes the j-th survivor from behind, and the recent ones follow in their order. What lies at keep and behind is left as it
+ * was. keep is keep_lens[b] where keep_lens is not NULL. lens [requests] becomes keep, or n where nothing is cut: n <= keep,
+ * n over max_context, a negative length, or a page of the request that is not in the cache. block_tables is not
+ * changed: the pages behind the last kept token are the caller's to reuse. Requests share no pages. The cache's rows lie apart
+ * from each other and from key_weights. workspace: smx_paged_evict_workspace_bytes, with the same keep (-1 with
+ * keep_lens) and max_context, which bounds the contexts and is at most width * page_size. Asynchronous on stream.
+ */
+int smx_paged_evict(const smx_paged_cache* cache, float* key_weights, int32_t requests, int32_t width,
+                    const int32_t* context_lens, const int32_t* block_tables, int64_t table_stride,
+                    const int32_t* keep_lens, int32_t keep, int32_t recent, int32_t max_context, int32_t* lens,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+int smx_paged_evict_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t keep, int32_t max_context, int64_t* bytes);
+
+/* flags of smx_rotary: float32 heads, norm, frequencies (else bf16, bf16, float64), int64 positions (else
+ * int32), pairs of neighbours (else of the rotated part's halves). */
+#define SMX_ROTARY_F32 1
+#define SMX_ROTARY_NORM_F32 2
+#define SMX_ROTARY_FREQUENCIES_F32 4
+#define SMX_ROTARY_POSITIONS_I64 8
+#define SMX_ROTARY_INTERLEAVED 16
+
+/*
+ * Rotary positions: the first rotary_dim values of every head row (tokens, heads and strides as in x and out, in elements
+ * of the heads' type) are rotated, pair i by the angle positions[token] * frequencies[i], and multiplied by
+ * amplitude; the values behind them are copied. With norm [head_dim] the whole head is RMS-normalised and scaled first.
+ * Angles are reduced in 64 bits, the rest is FP32 with one rounding. Rows of negative position are left as they are in
+ * out, or become zero with zero_rows. out is x (same address and strides) or shares no memory with it; its rows lie apart from
+ * each other. head_dim 2 to 1024. Asynchronous on stream.
+ */
+int smx_rotary(int32_t tokens, int32_t head_dim, int32_t rotary_dim, const smx_heads* x, const smx_heads* out,
+               const void* positions, const void* frequencies, const void* norm, int32_t flags, float amplitude,
+               float eps, int32_t zero_rows, void* stream);
+
+/* flags of smx_verify_drafts: bf16 probabilities (else float32), int64 tokens (else int32). */
+#define SMX_VERIFY_BF16 1
+#define SMX_VERIFY_TOKENS_I64 2
+#define SMX_VERIFY_MAX_VOCAB (1 << 28)
+
+/*
+ * Verification of drafted tokens. Rows are those of a step's plan (starts, rows and positions are read; the request's rows are
+ * its last token and then its drafts): tokens [step tokens] are the rows' tokens, row i of target [step tokens, vocab]
+ * holds the probabilities of the token behind row i, row i of draft those that this token was drawn from
+ * (draft NULL: it was not drawn, its own probability counts as 1 and all others as 0). The draft x behind row i is accepted
+ * if target[i][x] > 0 and accept[i] * draft[i][x] < target[i][x], and no draft before it was refused. The token behind the last
+ * accepted one is drawn from max(target - draft, 0) of its row if a draft was refused there (from target where that
+ * is zero everywhere), else from target: the first token whose running sum exceeds sample[request] times the whole sum (the last
+ * of any probability if there is none). Probabilities that are no positive finite numbers count as zero, a draft outside the
+ * vocabulary is refused; products and sums in 64 bits. Out: counts [requests], the accepted drafts and one (0 for a request
+ * without rows); out [step tokens], from each request's first row on its accepted drafts, the drawn token (-1 if its
+ * row holds no probability at all) and -1. workspace: smx_verify_workspace_bytes. Asynchronous on stream.
+ */
+int smx_verify_drafts(const smx_paged_step* step, int32_t vocab, const void* target, int64_t target_row,
+                      const void* draft, int64_t draft_row, const void* tokens, const float* accept,
+                      const float* sample, int32_t flags, void* out, int32_t* counts, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+int smx_verify_workspace_bytes(int32_t requests, int32_t vocab, int64_t* bytes);
 
 /*
  * A [k, n] weight of 4-bit codes with a scale and a zero point per group of k and column:

@@ -24,8 +24,10 @@ from .strassen import PlainWeightPackWarning  # noqa: F401
 from .tuning import tuned_matmul  # noqa: F401
 from .paged import (  # noqa: F401
     PAGED_BAD_LENGTH, PAGED_BAD_PAGE, PAGED_OK, PAGED_OUT_OF_PAGES, PAGED_OUT_OF_ROWS, PagedPlan, paged_attention,
-    paged_plan, paged_write,
+    paged_evict, paged_key_weights, paged_plan, paged_write,
 )
+from .rotary import ROTARY_SCALINGS, rotary, rotary_frequencies  # noqa: F401
+from .verify import verify_drafts  # noqa: F401
 from .int4 import Int4Operand, int4_matmul, int4_quantize, int4_weight_layout  # noqa: F401
 
 __version__ = "0.5.0"

@@ -65,11 +65,21 @@ SMX_PAGED_MAX_CONTEXT = 1 << 30
 SMX_PAGED_Q_SCALE_F32 = 1
 SMX_PAGED_K_SCALE_F32 = 2
 SMX_PAGED_ROPE_F32 = 4
+SMX_ROTARY_F32 = 1
+SMX_ROTARY_NORM_F32 = 2
+SMX_ROTARY_FREQUENCIES_F32 = 4
+SMX_ROTARY_POSITIONS_I64 = 8
+SMX_ROTARY_INTERLEAVED = 16
+SMX_VERIFY_BF16 = 1
+SMX_VERIFY_TOKENS_I64 = 2
+SMX_VERIFY_MAX_VOCAB = 1 << 28
 
 EXPORTS = ("smx_gemm", "smx_gemm_noalloc", "smx_gemm_workspace_bytes", "smx_matmul", "smx_matmul_workspace_bytes", "smx_matmul_plan",
            "smx_tile_requirements", "smx_packed_bytes", "smx_pack_operand", "smx_pack_rhs_transposed", "smx_norm_residual_add", "smx_rms_norm",
            "smx_row_squares", "smx_scale_rows", "smx_qk_norm_rope", "smx_paged_plan", "smx_paged_write",
-           "smx_paged_attention", "smx_paged_attention_workspace_bytes", "smx_int4_matmul",
+           "smx_paged_attention", "smx_paged_attention_lse", "smx_paged_attention_workspace_bytes", "smx_paged_key_weights",
+           "smx_paged_key_weights_workspace_bytes", "smx_paged_evict", "smx_paged_evict_workspace_bytes", "smx_rotary",
+           "smx_verify_drafts", "smx_verify_workspace_bytes", "smx_int4_matmul",
            "smx_int4_workspace_bytes", "smx_last_error", "smx_version")
 
 
@@ -177,6 +187,22 @@ def load():
     lib.smx_paged_attention.restype = ctypes.c_int
     lib.smx_paged_attention_workspace_bytes.argtypes = [i32, ctypes.POINTER(i64)]
     lib.smx_paged_attention_workspace_bytes.restype = ctypes.c_int
+    lib.smx_paged_attention_lse.argtypes = [cache, step, heads, heads, f32, i32, i32, vp, vp, i64, vp]
+    lib.smx_paged_attention_lse.restype = ctypes.c_int
+    lib.smx_paged_key_weights.argtypes = [cache, step, heads, vp, f32, i32, vp, vp, i64, vp]
+    lib.smx_paged_key_weights.restype = ctypes.c_int
+    lib.smx_paged_key_weights_workspace_bytes.argtypes = [ctypes.POINTER(i64)]
+    lib.smx_paged_key_weights_workspace_bytes.restype = ctypes.c_int
+    lib.smx_paged_evict.argtypes = [cache, vp, i32, i32, vp, vp, i64, vp, i32, i32, i32, vp, vp, i64, vp]
+    lib.smx_paged_evict.restype = ctypes.c_int
+    lib.smx_paged_evict_workspace_bytes.argtypes = [i32, i32, i32, i32, ctypes.POINTER(i64)]
+    lib.smx_paged_evict_workspace_bytes.restype = ctypes.c_int
+    lib.smx_rotary.argtypes = [i32, i32, i32, heads, heads, vp, vp, vp, i32, f32, f32, i32, vp]
+    lib.smx_rotary.restype = ctypes.c_int
+    lib.smx_verify_drafts.argtypes = [step, i32, vp, i64, vp, i64, vp, vp, vp, i32, vp, vp, vp, i64, vp]
+    lib.smx_verify_drafts.restype = ctypes.c_int
+    lib.smx_verify_workspace_bytes.argtypes = [i32, i32, ctypes.POINTER(i64)]
+    lib.smx_verify_workspace_bytes.restype = ctypes.c_int
     lib.smx_int4_matmul.argtypes = [ctypes.POINTER(SmxInt4Weight), i64, vp, i64, i32, vp, i64, i32, vp, i64, vp, i64, vp]
     lib.smx_int4_matmul.restype = ctypes.c_int
     lib.smx_int4_workspace_bytes.argtypes = [ctypes.POINTER(SmxInt4Weight), i64, ctypes.POINTER(i64)]
@@ -203,7 +229,9 @@ def host():
             raise RuntimeError(f"the serving operators' host module is missing or does not load ({e}): build it with "
                                "`python -m strassen_tpu_amd.build`") from e
         _serving.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-            "smx_paged_plan", "smx_paged_write", "smx_paged_attention", "smx_paged_attention_workspace_bytes",
+            "smx_paged_plan", "smx_paged_write", "smx_paged_attention_lse", "smx_paged_attention_workspace_bytes",
+            "smx_paged_key_weights", "smx_paged_key_weights_workspace_bytes", "smx_paged_evict",
+            "smx_paged_evict_workspace_bytes", "smx_rotary", "smx_verify_drafts", "smx_verify_workspace_bytes",
             "smx_int4_matmul", "smx_int4_workspace_bytes", "smx_last_error")), torch._C._cuda_getCurrentRawStream)
         _host = _serving
     return _host

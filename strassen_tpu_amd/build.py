@@ -2,8 +2,8 @@
 
 ``python -m strassen_tpu_amd.build`` (or ``build()``) compiles the C ABI's
 translation unit (``csrc/strassen_gemm.hip``), the six units that
-instantiate the GEMM kernels (``csrc/gemm_*.hip``) and the three of the serving
-operators (``csrc/paged_*.hip``, ``csrc/int4_matmul.hip``) with hipcc, in parallel,
+instantiate the GEMM kernels (``csrc/gemm_*.hip``) and those of the serving
+operators (``csrc/paged_*.hip``, ``csrc/rotary.hip``, ``csrc/verify.hip``, ``csrc/int4_matmul.hip``) with hipcc, in parallel,
 checks each unit's device assembly, and links ``libstrassen_mi355x.so`` next
 to this file. hipcc cross-compiles for gfx950 without a GPU. The serving operators' host side
 (``csrc/serving_host.cpp``, a Python extension module on torch's tensors) is compiled with the
@@ -26,7 +26,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
 SOURCES = tuple(os.path.join(HERE, "csrc", name) for name in (
     "strassen_gemm.hip", "gemm_strassen.hip", "gemm_strassen_thin.hip", "gemm_strassen_pm.hip", "gemm_cubic.hip",
-    "gemm_cubic_thin.hip", "gemm_stream.hip", "paged_cache.hip", "paged_attention.hip", "int4_matmul.hip"))
+    "gemm_cubic_thin.hip", "gemm_stream.hip", "paged_cache.hip", "paged_attention.hip", "paged_weights.hip",
+    "paged_evict.hip", "rotary.hip", "verify.hip", "int4_matmul.hip"))
 LIBRARY = os.path.join(HERE, "libstrassen_mi355x.so")
 HOST_SOURCE, HOST_MODULE = os.path.join(HERE, "csrc", "serving_host.cpp"), os.path.join(HERE, "_serving.so")
 INCLUDE = os.path.join(REPO, "include")
@@ -146,7 +147,7 @@ _SPLIT = re.compile(r"gemm_splitILi(\d+)ELi(\d+)ELb(\d)E")
 _PM = re.compile(r"gemm_pmILi(\d+)ELi(\d+)EE")
 _STREAM = re.compile(r"gemm_streamILi(\d+)E")
 _PACKED = re.compile(r"gemm_packedILi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)ELb(\d)E")
-_SERVING = re.compile(r"(paged_attend|paged_join|int4_few|int4_tiled)")
+_SERVING = re.compile(r"(paged_attend|paged_join|key_weights|evict_|rotary_|verify_|int4_few|int4_tiled)")
 _QUAD_CUBIC_PARTIAL = 1
 PARTIAL_SCRATCH_CAP = 1024
 
@@ -244,7 +245,8 @@ def build(verbose=False, jobs=None):
             # operators', whose registers are held to the same limit).
             unit = os.path.basename(source)
             kernel_unit = unit not in ("strassen_gemm.hip", "paged_cache.hip")
-            if kernel_unit and unit not in ("gemm_stream.hip", "paged_attention.hip", "int4_matmul.hip"):
+            if kernel_unit and unit not in ("gemm_stream.hip", "paged_attention.hip", "paged_weights.hip", "paged_evict.hip",
+                                                "rotary.hip", "verify.hip", "int4_matmul.hip"):
                 checked += verify_inline_asm_kernels(text)
             gemms += verify_kernel_scratch(text, require=kernel_unit)
         cmd = link_command([obj for obj, _, _ in units], tmp)

@@ -28,6 +28,7 @@
 
 #include "kernel_packed.hpp"
 #include "launch.hpp"
+#include "paged_spans.hpp"
 
 namespace smx {
 
@@ -50,6 +51,7 @@ struct AttentionArgs {
   double per_workgroup;  // 1 / workgroups
   float* partial;
   int32_t* records;
+  float* lse;  // [tokens, heads] or null: the logarithm of each row's sum of exponentials
 };
 
 // What paged_join needs to know of an item that workgroup w begins and others
@@ -84,11 +86,6 @@ __device__ __forceinline__ int64_t floor_sum(uint32_t n, uint32_t a, uint32_t b)
     top = a * n + b;
   }
   return sum;
-}
-
-// A plan's lengths, read through the scalar cache where the index is a wave's.
-__device__ __forceinline__ int32_t scalar_at(const int32_t* p, int i) {
-  return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)p)[i];
 }
 
 // The row tiles of one request and the key tiles (of kKeys keys) that each sees. An item (one of
@@ -128,16 +125,6 @@ struct Request {
   __device__ int64_t all() const { return fresh > 0 ? before(tiles - 1) + kItem + count(tiles - 1) : 0; }
 };
 
-// A workgroup's span of the units, and the item in which it begins.
-struct Span {
-  int64_t left;         // units to do
-  int64_t each;         // units of a span
-  int64_t begin;        // of this one, over all key/value heads
-  int32_t worker;       // which span this is
-  int32_t head, request, tile, skip;  // skip: units of that item that lie in spans before
-  int32_t context, fresh;             // of that request
-};
-
 // The span's part of one item: its first step (key tile), its steps and units.
 template <int kKeys, int kItem>
 struct Part {
@@ -156,136 +143,6 @@ struct Part {
     from = r.first(tile) + before, count = upto - before, begins = __builtin_amdgcn_readfirstlane(before == 0);
   }
 };
-
-__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
-  return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, lane) |
-         (int64_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
-}
-
-// a / b for 0 <= a, 0 < b and a quotient below 2^19, of which the reciprocal of b misses less
-// than one (the integer division is ten times as long).
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  int64_t q = (int64_t)((float)a * __builtin_amdgcn_rcpf((float)b));
-  if (q * b > a) --q;
-  if ((q + 1) * b <= a) ++q;
-  return q;
-}
-
-// x of the lanes that kControl names, zero where there are none.
-template <int kControl, int kRows>
-__device__ __forceinline__ int64_t moved(int64_t x) {
-  const uint32_t low = __builtin_amdgcn_update_dpp(0, (int)x, kControl, kRows, 15, false);
-  const uint32_t high = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), kControl, kRows, 15, false);
-  return (int64_t)((uint64_t)high << 32 | low);
-}
-
-// Inclusive sum of x over a wave's lanes: within rows of 16 lanes, then a row's last value
-// to the next row, and the lower half's to the upper.
-__device__ __forceinline__ int64_t wave_scan(int64_t x) {
-  x += moved<0x111, 15>(x);
-  x += moved<0x112, 15>(x);
-  x += moved<0x114, 15>(x);
-  x += moved<0x118, 15>(x);
-  x += moved<0x142, 10>(x);
-  x += moved<0x143, 12>(x);
-  return x;
-}
-
-// Finds the workgroup's span (kWaves waves, uniform result). Consecutive spans lie
-// on one XCD, whose L2 then serves one key/value head's pages at a time.
-template <int kKeys, int kItem, int kWaves>
-__device__ bool find_span(const AttentionArgs& p, Span* s) {
-  constexpr int kThreads = 64 * kWaves;
-  __shared__ int64_t waves[kWaves], found_rest;
-  __shared__ int32_t found[3];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // Inclusive sum over the workgroup of this thread's request among kThreads of them.
-  int64_t mine = 0, upto = 0;
-  int32_t context = 0, fresh = 0;
-  auto scan = [&](int first) -> int64_t {
-    const int b = first + (int)threadIdx.x;
-    const bool here = b < p.requests;
-    context = here ? p.context[b] : 0, fresh = here ? p.rows[b] : 0;
-    mine = Request<kKeys, kItem>(p, context, fresh).all();
-    upto = wave_scan(mine);
-    if constexpr (kWaves == 1) return lane_value(upto, 63);
-    __syncthreads();
-    if (lane == 63) waves[wave] = upto;
-    __syncthreads();
-    int64_t all = 0;
-    for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) upto += waves[w];
-      all += waves[w];
-    }
-    return lane_value(all, 0);
-  };
-  int64_t total = 0;
-  for (int first = 0; first < p.requests; first += kThreads) total += scan(first);
-  const int64_t everything = total * p.kv_heads;
-  int64_t each = (int64_t)((double)everything * p.per_workgroup);  // (at most one short)
-  while (each * gridDim.x < everything) ++each;
-  s->each = max((int64_t)p.min_span, each);
-  const int64_t spans = quotient(everything + s->each - 1, s->each), per_xcd = (spans + 7) / 8;
-  s->worker = (int)((blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3));
-  if ((blockIdx.x >> 3) >= per_xcd || s->worker >= spans) return false;
-  s->begin = (int64_t)s->worker * s->each;
-  s->left = min(s->each, everything - s->begin);
-  s->head = __builtin_amdgcn_readfirstlane((int)quotient(s->begin, total));
-  const int64_t at = s->begin - (int64_t)s->head * total;
-
-  int64_t base = 0, rest = 0;
-  for (int first = 0; first < p.requests; first += kThreads) {
-    // (the sums of a single round are still there)
-    const int64_t all = p.requests <= kThreads ? total : scan(first);
-    const bool here = at >= base + upto - mine && at < base + upto;
-    if constexpr (kWaves > 1) {
-      if (here) {
-        found[0] = first + (int)threadIdx.x, found[1] = context, found[2] = fresh;
-        found_rest = at - (base + upto - mine);
-      }
-    } else if (const uint64_t who = __ballot(here)) {
-      const int l = __builtin_ctzll(who);
-      s->request = first + l;
-      s->context = __builtin_amdgcn_readlane(context, l), s->fresh = __builtin_amdgcn_readlane(fresh, l);
-      rest = at - (base + lane_value(upto - mine, l));
-    }
-    base += all;
-    if (at < base) break;  // uniform
-  }
-  if constexpr (kWaves > 1) {
-    __syncthreads();
-    s->request = __builtin_amdgcn_readfirstlane(found[0]);
-    s->context = __builtin_amdgcn_readfirstlane(found[1]), s->fresh = __builtin_amdgcn_readfirstlane(found[2]);
-    rest = lane_value(found_rest, 0);
-  }
-  const auto r = Request<kKeys, kItem>::uniform(p, s->context, s->fresh);
-  // The last tile with before(tile) <= rest: a lane each for 64 of them, evenly apart (500 rows
-  // on 100 keys: 32.8 us, one after another 34.6).
-  int low = 0, high = r.tiles;
-  int64_t skipped = 0;  // before(low)
-  while (high - low > 1) {
-    const int width = (high - low + 63) >> 6, tile = low + lane * width;
-    const int64_t sum = r.before(min(tile, high - 1));
-    const int last = 63 - __builtin_clzll(__ballot(tile < high && sum <= rest));
-    skipped = lane_value(sum, last);
-    low += last * width, high = min(high, low + width);
-  }
-  s->tile = __builtin_amdgcn_readfirstlane(low);
-  s->skip = __builtin_amdgcn_readfirstlane((int)(rest - skipped));
-  return true;
-}
-
-// On to the next item with rows.
-__device__ __forceinline__ void next_item(const AttentionArgs& p, Span* s, int tiles) {
-  s->skip = 0;
-  if (++s->tile < tiles) return;
-  s->tile = 0;
-  do {
-    if (++s->request == p.requests) s->request = 0, ++s->head;
-    s->fresh = scalar_at(p.rows, s->request);
-  } while (s->fresh <= 0);
-  s->context = scalar_at(p.context, s->request);
-}
 
 // Row r of a tile belongs to its token r / group; exact for rows below 2^12.
 __device__ __forceinline__ int row_token(int row, const AttentionArgs& p) {
@@ -462,11 +319,6 @@ struct Rows {
     top = -INFINITY, sum = 0.f;
   }
 };
-
-__device__ __forceinline__ float other_half(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return (threadIdx.x & 32) ? __uint_as_float(r[0]) : __uint_as_float(r[1]);
-}
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
@@ -695,6 +547,12 @@ __device__ __forceinline__ float inverse_of(float sum, float top) {
   return sum > 0.f ? 1.f / sum : sum == 0.f && top > -INFINITY ? NAN : sum;
 }
 
+// The logarithm of a row's sum of exponentials; -inf where there is none.
+__device__ __forceinline__ void store_lse(const AttentionArgs& p, int64_t token, int head, float top, float sum) {
+  constexpr float kLn2 = 0.693147180559945309f;
+  p.lse[token * ((int64_t)p.group * p.kv_heads) + head] = sum > 0.f || sum != sum ? (top + __builtin_amdgcn_logf(sum)) * kLn2 : -INFINITY;
+}
+
 // 128 rows a tile (four waves of 32), 64 keys a step, keys and values double buffered. 2048 tokens of 64 heads on
 // 16384 cached ones: 1.30 ms, 0.90 PFLOP/s. Matrix cores, vector units and LDS are each busy 41 to 44% of the time
 // (one workgroup a CU: 2.0 ms): two waves a SIMD do not cover each other's way from a step's keys to
@@ -712,7 +570,7 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
   Record* const record = reinterpret_cast<Record*>(p.records) + blockIdx.x;
   if (threadIdx.x == 0) record->others = 0;
   Span s;
-  if (!find_span<kKeys, kItem, 4>(p, &s)) return clear_rows<D, 256>(p);
+  if (!find_span<Request<kKeys, kItem>, 4>(p, &s)) return clear_rows<D, 256>(p);
 
   const Lanes<D, 16> lanes(p.slot_stride);
 
@@ -817,8 +675,9 @@ __global__ __launch_bounds__(256, 2) void paged_attend(AttentionArgs p) {
 
       const float sum = o.sum + other_half(o.sum);
       if (part.count == part.tile_count) {
-        store_rows<D>(p, o.o, inverse_of(sum, o.top), 32 * wave + (lane & 31) < tile_rows,
-                      scalar_at(p.starts, part.request) + local, head);
+        const int64_t token = scalar_at(p.starts, part.request) + local;
+        store_rows<D>(p, o.o, inverse_of(sum, o.top), 32 * wave + (lane & 31) < tile_rows, token, head);
+        if (p.lse && !half && 32 * wave + (lane & 31) < tile_rows) store_lse(p, token, head, o.top, sum);
       } else {
         float* const to = p.partial + (2 * (int64_t)s.worker + part.begins) * kPartialFloats<D>;
         int thread = threadIdx.x;
@@ -863,7 +722,7 @@ __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
   Record* const record = reinterpret_cast<Record*>(p.records) + blockIdx.x;
   if (lane == 0) record->others = 0;
   Span s;
-  if (!find_span<kKeys, kItem, 1>(p, &s)) return clear_rows<D, 64>(p);
+  if (!find_span<Request<kKeys, kItem>, 1>(p, &s)) return clear_rows<D, 64>(p);
 
   const Lanes<D, kKeys> lanes(p.slot_stride);
 
@@ -934,6 +793,7 @@ __global__ __launch_bounds__(64) void paged_attend_few(AttentionArgs p) {
     const float sum = o.sum + other_half(o.sum);
     if (count == part.tile_count) {
       store_rows<D>(p, o.o, inverse_of(sum, o.top), valid, token, head);
+      if (p.lse && valid && !half) store_lse(p, token, head, o.top, sum);
     } else {
       float* const to = p.partial + (2 * (int64_t)s.worker + part.begins) * kFewPartialFloats<D>;
       if (valid) {
@@ -1009,6 +869,7 @@ __global__ __launch_bounds__(1024) void paged_join_few(AttentionArgs p) {
   const int64_t token = p.starts[record.request] + record.tile * p.tile_tokens + row / p.group;
   *reinterpret_cast<uint2*>(p.out + token * p.out_token + (record.head * p.group + row % p.group) * p.out_head + column) =
       make_uint2(pack_bf16(value[0] * inverse, value[1] * inverse), pack_bf16(value[2] * inverse, value[3] * inverse));
+  if (p.lse && !column) store_lse(p, token, record.head * p.group + row % p.group, top, total);
 }
 
 constexpr int kJoinThreads = 256;
@@ -1046,6 +907,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join(AttentionArgs p) {
   const int64_t token = p.starts[record.request] + record.tile * p.tile_tokens + row / p.group;
   store_block(p.out + token * p.out_token + (record.head * p.group + row % p.group) * p.out_head + 32 * x, o,
               inverse_of(sum, top), at < tile_rows, lane >> 5);
+  if (p.lse && x == 0 && lane < 32 && at < tile_rows) store_lse(p, token, record.head * p.group + row % p.group, top, sum);
 }
 
 // Workgroups of a launch, a multiple of the 8 XCDs: as many as a CU holds (two of paged_attend, by its
@@ -1100,6 +962,12 @@ int smx_paged_attention_workspace_bytes(int32_t head_dim, int64_t* bytes) {
 int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step, const smx_heads* q,
                         const smx_heads* out, float scale, int32_t window, int32_t zero_rows, void* workspace,
                         int64_t workspace_bytes, void* stream) {
+  return smx_paged_attention_lse(cache, step, q, out, scale, window, zero_rows, nullptr, workspace, workspace_bytes, stream);
+}
+
+int smx_paged_attention_lse(const smx_paged_cache* cache, const smx_paged_step* step, const smx_heads* q,
+                            const smx_heads* out, float scale, int32_t window, int32_t zero_rows, float* lse,
+                            void* workspace, int64_t workspace_bytes, void* stream) {
   smx::fail(SMX_OK, "%s", "");
   if (int rc = paged_layout(cache)) return rc;
   if (!step || !step->block_tables || !step->starts || !step->rows || !step->context || !step->positions || !q ||
@@ -1125,6 +993,12 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
     return fail(SMX_ERR_INVALID, "out must be the queries themselves or share no memory with them");
   for (const void* x : {cache->k, cache->v})
     if (meet(cache_runs(*cache, x), to)) return fail(SMX_ERR_INVALID, "out must share no memory with the cache");
+  if (lse) {
+    const Runs sums{lse, 2 * (int64_t)step->tokens * q->heads, {{1, 0}, {1, 0}, {1, 0}}};  // (in units of 2 bytes)
+    if ((uintptr_t)lse % 4 || meet(sums, from) || meet(sums, to) || meet(sums, cache_runs(*cache, cache->k)) ||
+        meet(sums, cache_runs(*cache, cache->v)))
+      return fail(SMX_ERR_INVALID, "lse must be aligned and share no memory with the queries, out or the cache");
+  }
   constexpr float kLog2E = 1.44269504088896341f;  // (the kernels' exponentials are powers of two)
   if (!(scale > 0.f) || !(scale * kLog2E < INFINITY))
     return fail(SMX_ERR_INVALID, "scale must be positive and finite, also times log2 e");
@@ -1158,6 +1032,7 @@ int smx_paged_attention(const smx_paged_cache* cache, const smx_paged_step* step
   p.per_workgroup = 1. / blocks;
   p.records = (int32_t*)workspace;
   p.partial = (float*)((char*)workspace + blocks * kRecordBytes);
+  p.lse = lse;
   return cache->head_dim == 128 ? launch_attention<128>(p, few, blocks, (hipStream_t)stream)
                                 : launch_attention<64>(p, few, blocks, (hipStream_t)stream);
 }

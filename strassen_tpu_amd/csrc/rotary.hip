@@ -1,0 +1,274 @@
+// Rotary positions (smx_rotary): pairs of a head's values turned by an angle that grows with the row's
+// position, the head RMS-normalised before if asked.
+//
+// Mathematics. Pair i of a head at position p turns by p f_i: (a, b) -> A (a cos - b sin, b cos + a sin), (a, b) the
+// values (i, i + half) or (2 i, 2 i + 1) of the head's first 2 half, the values behind them as they are. The
+// norm is x / sqrt(mean x^2 + eps) w over the whole head. FP32 throughout, one rounding at the store.
+//
+// Angles. p f_i in FP32 is off by a hundredth of a radian at a position of 10^5, so turns p f_i / (2 pi) are formed in
+// 64 bits, less whole quarters, and the rest, at most an eighth of a turn, is exact to FP32's last bit. All heads
+// of a row share its angles: a workgroup works them out once, in LDS.
+#include "launch.hpp"
+
+namespace smx {
+namespace {
+
+struct RotaryArgs {
+  const void *x, *positions, *frequencies, *norm;
+  void* out;
+  int64_t x_token, x_head, out_token, out_head;
+  int32_t tokens, heads, dim, half, flags, zero_rows, per_block;
+  float amplitude, eps;
+};
+
+constexpr int kMaxDim = 1024, kMaxRows = 8;
+
+// The positions of the workgroup's rows, and the factors of each one's pairs: LDS [rows][half] cos, then sin.
+__device__ __forceinline__ void turns(const RotaryArgs& p, int64_t row0, int rows, float* cos, float* sin) {
+  for (int i = threadIdx.x; i < rows * p.half; i += blockDim.x) {
+    const int row = i / p.half, pair = i - row * p.half;
+    const int64_t at = row0 + row;
+    const double position = p.flags & SMX_ROTARY_POSITIONS_I64 ? (double)((const int64_t*)p.positions)[at]
+                                                               : (double)((const int32_t*)p.positions)[at];
+    const double f = p.flags & SMX_ROTARY_FREQUENCIES_F32 ? (double)((const float*)p.frequencies)[pair]
+                                                          : ((const double*)p.frequencies)[pair];
+    const double turn = position * f * 0.15915494309189533577;  // 1 / (2 pi)
+    const double quarters = rint(turn * 4);
+    const float rest = (float)(turn - quarters * 0.25);
+    // which quarter: quarters mod 4, in 64 bits (a float's turn may pass 2^31)
+    const int quarter = (int)(quarters - 4 * floor(quarters * 0.25));
+    float s, c;
+    sincospif(2 * rest, &s, &c);
+    const float a = quarter & 1 ? s : c, b = quarter & 1 ? c : s;
+    cos[i] = p.amplitude * (quarter == 1 || quarter == 2 ? -a : a);
+    sin[i] = p.amplitude * (quarter >= 2 ? -b : b);
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ bool covered(const RotaryArgs& p, int64_t row) {
+  return p.flags & SMX_ROTARY_POSITIONS_I64 ? ((const int64_t*)p.positions)[row] >= 0
+                                            : ((const int32_t*)p.positions)[row] >= 0;
+}
+
+template <bool kF32>
+__device__ __forceinline__ F8 load8(const void* p, int64_t at) {
+  if constexpr (!kF32) return unpack8(*reinterpret_cast<const u32x4*>((const uint16_t*)p + at));
+  F8 r;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const f32x4 v = reinterpret_cast<const f32x4*>((const float*)p + at)[j];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[4 * j + i] = v[i];
+  }
+  return r;
+}
+
+template <bool kF32>
+__device__ __forceinline__ void store8(void* p, int64_t at, const F8& x) {
+  if constexpr (kF32) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      reinterpret_cast<f32x4*>((float*)p + at)[j] = f32x4{x.v[4 * j], x.v[4 * j + 1], x.v[4 * j + 2], x.v[4 * j + 3]};
+  } else {
+    *reinterpret_cast<u32x4*>((uint16_t*)p + at) = pack8(x);
+  }
+}
+
+// Heads whose values fall into aligned runs of eight: a lane takes two of them, eight pairs (or sixteen values
+// that stay as they are), and goes from head to head. Bound by memory.
+template <bool kF32, bool kInterleaved, bool kNorm>
+__global__ __launch_bounds__(256) void rotary_runs(RotaryArgs p) {
+  extern __shared__ __attribute__((aligned(16))) float rotary_lds[];
+  const int64_t row0 = (int64_t)blockIdx.x * p.per_block;
+  const int rows = (int)min((int64_t)p.per_block, p.tokens - row0);
+  float* const cos = rotary_lds;
+  float* const sin = cos + p.per_block * p.half;
+  turns(p, row0, rows, cos, sin);
+
+  const int lanes = (p.dim + 15) / 16, slots = 256 / lanes;
+  const int slot = (int)threadIdx.x / lanes, lane = (int)threadIdx.x - slot * lanes;
+  if (slot >= slots) return;  // (with a norm 256 is a multiple of lanes)
+  const bool turned = 8 * lane < p.half;
+  const int first = !turned ? 2 * p.half + 16 * (lane - p.half / 8) : kInterleaved ? 16 * lane : 8 * lane;
+  const int second = !turned || kInterleaved ? first + 8 : p.half + first;
+  const bool two = second < p.dim;
+  int row = 0, head = slot;
+  while (head >= p.heads) head -= p.heads, ++row;
+  F8 wa, wb;
+  if constexpr (kNorm) {
+    if (p.flags & SMX_ROTARY_NORM_F32) {
+      wa = load8<true>(p.norm, first), wb = load8<true>(p.norm, second);
+    } else {
+      wa = load8<false>(p.norm, first), wb = load8<false>(p.norm, second);
+    }
+  }
+  while (row < rows) {
+    const int64_t token = row0 + row;
+    const int64_t to = token * p.out_token + head * p.out_head;
+    if (covered(p, token)) {
+      const int64_t from = token * p.x_token + head * p.x_head;
+      F8 a = load8<kF32>(p.x, from + first), b;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b.v[i] = 0.f;
+      if (two) b = load8<kF32>(p.x, from + second);
+      if constexpr (kNorm) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += a.v[i] * a.v[i] + b.v[i] * b.v[i];
+        for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor(sum, d);  // a head's lanes stay together in the loop
+        const float r = 1.0f / sqrtf(sum / p.dim + p.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a.v[i] = a.v[i] * r * wa.v[i], b.v[i] = b.v[i] * r * wb.v[i];
+      }
+      if (turned) {
+        const f32x4* const c = reinterpret_cast<const f32x4*>(cos + row * p.half + 8 * lane);
+        const f32x4* const s = reinterpret_cast<const f32x4*>(sin + row * p.half + 8 * lane);
+        const f32x4 cs[2] = {c[0], c[1]}, sn[2] = {s[0], s[1]};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float& x = !kInterleaved ? a.v[i] : i < 4 ? a.v[2 * i] : b.v[2 * i - 8];
+          float& y = !kInterleaved ? b.v[i] : i < 4 ? a.v[2 * i + 1] : b.v[2 * i - 7];
+          const float u = x, v = y, cv = cs[i >> 2][i & 3], sv = sn[i >> 2][i & 3];
+          x = u * cv - v * sv;
+          y = v * cv + u * sv;
+        }
+      }
+      store8<kF32>(p.out, to + first, a);
+      if (two) store8<kF32>(p.out, to + second, b);
+    } else if (p.zero_rows) {
+      F8 zero;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) zero.v[i] = 0.f;
+      store8<kF32>(p.out, to + first, zero);
+      if (two) store8<kF32>(p.out, to + second, zero);
+    }
+    head += slots;
+    while (head >= p.heads) head -= p.heads, ++row;
+  }
+}
+
+// Any other head: a wave takes a head, value by value.
+template <bool kF32>
+__global__ __launch_bounds__(256) void rotary_values(RotaryArgs p) {
+  extern __shared__ __attribute__((aligned(16))) float rotary_lds[];
+  const int64_t token = blockIdx.x;
+  float* const cos = rotary_lds;
+  float* const sin = cos + p.half;
+  turns(p, token, 1, cos, sin);
+  const int lane = threadIdx.x & 63;
+  const bool here = covered(p, token), wide = p.flags & SMX_ROTARY_INTERLEAVED;
+  if (!here && !p.zero_rows) return;
+  auto load = [&](int64_t at) { return kF32 ? ((const float*)p.x)[at] : bf16_to_f32(((const uint16_t*)p.x)[at]); };
+  auto store = [&](int64_t at, float v) {
+    if (kF32)
+      ((float*)p.out)[at] = v;
+    else
+      ((uint16_t*)p.out)[at] = f32_to_bf16(v);
+  };
+  for (int head = threadIdx.x >> 6; head < p.heads; head += 4) {
+    const int64_t from = token * p.x_token + head * p.x_head, to = token * p.out_token + head * p.out_head;
+    float r = 1.f;
+    if (p.norm && here) {
+      float sum = 0.f;
+      for (int i = lane; i < p.dim; i += 64) {
+        const float v = load(from + i);
+        sum += v * v;
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+      r = 1.0f / sqrtf(sum / p.dim + p.eps);
+    }
+    auto value = [&](int i) {
+      if (!here) return 0.f;
+      const float v = load(from + i);
+      if (!p.norm) return v;
+      return v * r * (p.flags & SMX_ROTARY_NORM_F32 ? ((const float*)p.norm)[i] : bf16_to_f32(((const uint16_t*)p.norm)[i]));
+    };
+    for (int i = lane; i < p.half; i += 64) {
+      const int a = wide ? 2 * i : i, b = wide ? 2 * i + 1 : i + p.half;
+      const float u = value(a), v = value(b);
+      store(to + a, here ? u * cos[i] - v * sin[i] : 0.f);
+      store(to + b, here ? v * cos[i] + u * sin[i] : 0.f);
+    }
+    for (int i = 2 * p.half + lane; i < p.dim; i += 64) store(to + i, value(i));
+  }
+}
+
+template <bool kF32, bool kInterleaved>
+auto runs_kernel(bool norm) {
+  return norm ? rotary_runs<kF32, kInterleaved, true> : rotary_runs<kF32, kInterleaved, false>;
+}
+
+// Overlap checks count in two-byte units.
+Runs runs_of(const smx_heads& x, int64_t tokens, int64_t dim, int units) {
+  smx_heads y = x;
+  y.token_stride *= units, y.head_stride *= units;
+  return head_runs(y, tokens, dim * units);
+}
+
+}  // namespace
+}  // namespace smx
+
+using namespace smx;
+
+extern "C" {
+
+int smx_rotary(int32_t tokens, int32_t head_dim, int32_t rotary_dim, const smx_heads* x, const smx_heads* out,
+               const void* positions, const void* frequencies, const void* norm, int32_t flags, float amplitude,
+               float eps, int32_t zero_rows, void* stream) {
+  smx::fail(SMX_OK, "%s", "");
+  if (!x || !x->data || !out || !out->data || !positions || !frequencies) return fail(SMX_ERR_INVALID, "null pointer");
+  if (tokens <= 0 || tokens > SMX_PAGED_MAX_TOKENS)
+    return fail(SMX_ERR_INVALID, "1 to %d tokens, got %d", SMX_PAGED_MAX_TOKENS, tokens);
+  if (x->heads <= 0 || x->heads > 65535 || out->heads != x->heads)
+    return fail(SMX_ERR_INVALID, "1 to 65535 heads, as many out of the call as in (%d, %d)", x->heads, out->heads);
+  if (head_dim < 2 || head_dim > kMaxDim) return fail(SMX_ERR_UNSUPPORTED, "head_dim must be 2 to %d, got %d", kMaxDim, head_dim);
+  if (rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2)
+    return fail(SMX_ERR_INVALID, "an even number of values, at most head_dim=%d, are rotated, got %d", head_dim, rotary_dim);
+  constexpr int32_t kFlags = SMX_ROTARY_F32 | SMX_ROTARY_NORM_F32 | SMX_ROTARY_FREQUENCIES_F32 | SMX_ROTARY_POSITIONS_I64 |
+                             SMX_ROTARY_INTERLEAVED;
+  if (flags & ~kFlags) return fail(SMX_ERR_INVALID, "unknown flags 0x%x", flags);
+  if (!(amplitude >= -3e38f && amplitude <= 3e38f)) return fail(SMX_ERR_INVALID, "amplitude must be finite");
+  if (!(eps >= 0.f)) return fail(SMX_ERR_INVALID, "eps must not be negative");
+  const int size = flags & SMX_ROTARY_F32 ? 4 : 2;
+  for (const smx_heads* h : {x, out})
+    if ((uintptr_t)h->data % size || h->token_stride < 0 || h->head_stride < 0)
+      return fail(SMX_ERR_INVALID, "misaligned heads or negative strides");
+  const auto misaligned = [](const void* q, int bytes) { return (uintptr_t)q % bytes != 0; };
+  if (misaligned(positions, flags & SMX_ROTARY_POSITIONS_I64 ? 8 : 4) ||
+      misaligned(frequencies, flags & SMX_ROTARY_FREQUENCIES_F32 ? 4 : 8) || misaligned(norm, flags & SMX_ROTARY_NORM_F32 ? 4 : 2))
+    return fail(SMX_ERR_INVALID, "misaligned positions, frequencies or norm");
+  // Heads are stored while others are loaded.
+  const Runs from = runs_of(*x, tokens, head_dim, size / 2), to = runs_of(*out, tokens, head_dim, size / 2);
+  if (!lie_apart(to)) return fail(SMX_ERR_INVALID, "out holds rows that lie on each other");
+  if (!same_runs(from, to) && meet(from, to))
+    return fail(SMX_ERR_INVALID, "out must be x itself or share no memory with it");
+  RotaryArgs p{};
+  p.x = x->data, p.out = out->data, p.positions = positions, p.frequencies = frequencies, p.norm = norm;
+  p.x_token = x->token_stride, p.x_head = x->head_stride, p.out_token = out->token_stride, p.out_head = out->head_stride;
+  p.tokens = tokens, p.heads = x->heads, p.dim = head_dim, p.half = rotary_dim / 2, p.flags = flags;
+  p.zero_rows = zero_rows, p.amplitude = amplitude, p.eps = eps;
+  const int run = 16 / size;  // values of 16 bytes
+  bool aligned = p.half % 8 == 0 && head_dim % 8 == 0 && !misaligned(norm, 16);
+  for (const smx_heads* h : {x, out}) aligned = aligned && !misaligned(h->data, 16) && h->token_stride % run == 0 && h->head_stride % run == 0;
+  // a norm's sum goes over the lanes of a head, a power of two of them
+  if (norm) aligned = aligned && head_dim % 16 == 0 && !(head_dim & (head_dim - 1));
+  if (!aligned) {
+    p.per_block = 1;
+    hipLaunchKernelGGL(flags & SMX_ROTARY_F32 ? rotary_values<true> : rotary_values<false>, dim3((unsigned)tokens), dim3(256),
+                       2 * p.half * 4, (hipStream_t)stream, p);
+    return check_launch();
+  }
+  // Rows of a workgroup: several where enough workgroups remain to fill the chip.
+  p.per_block = tokens >= 4096 ? 4 : tokens >= 2048 ? 2 : 1;
+  const unsigned blocks = (unsigned)((tokens + p.per_block - 1) / p.per_block);
+  const int lds = 2 * p.per_block * p.half * 4;
+  const bool wide = flags & SMX_ROTARY_INTERLEAVED;
+  auto kern = flags & SMX_ROTARY_F32 ? (wide ? runs_kernel<true, true>(norm) : runs_kernel<true, false>(norm))
+                                     : (wide ? runs_kernel<false, true>(norm) : runs_kernel<false, false>(norm));
+  hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), lds, (hipStream_t)stream, p);
+  return check_launch();
+}
+
+}  // extern "C"

@@ -1,5 +1,5 @@
-// Host side of the serving operators: argument checks, result tensors and the library calls of paged.py and
-// int4.py. Those calls last a few microseconds on the device; checked and marshalled in Python they took 13
+// Host side of the serving operators: argument checks, result tensors and the library calls of paged.py,
+// rotary.py, verify.py and int4.py. Those calls last a few microseconds on the device; checked and marshalled in Python they took 13
 // to 15 microseconds of the host. A Python extension module on torch's tensors, no device code; the C
 // ABI's entry points are handed over by address.
 #include <torch/csrc/autograd/python_variable.h>
@@ -39,8 +39,15 @@ struct Raised {};
 struct Library {
   decltype(&smx_paged_plan) plan;
   decltype(&smx_paged_write) write;
-  decltype(&smx_paged_attention) attention;
+  decltype(&smx_paged_attention_lse) attention;
   decltype(&smx_paged_attention_workspace_bytes) attention_bytes;
+  decltype(&smx_paged_key_weights) weights;
+  decltype(&smx_paged_key_weights_workspace_bytes) weights_bytes;
+  decltype(&smx_paged_evict) evict;
+  decltype(&smx_paged_evict_workspace_bytes) evict_bytes;
+  decltype(&smx_rotary) rotary;
+  decltype(&smx_verify_drafts) verify;
+  decltype(&smx_verify_workspace_bytes) verify_bytes;
   decltype(&smx_int4_matmul) int4;
   decltype(&smx_int4_workspace_bytes) int4_bytes;
   decltype(&smx_last_error) error;
@@ -188,6 +195,13 @@ int32_t* int32_list(const Tensor& t, const char* name, int64_t length) {
   return t.mutable_data_ptr<int32_t>();
 }
 
+const int32_t* table_rows(const Tensor& tables, int64_t requests) {
+  if (tables.scalar_type() != at::kInt || tables.dim() != 2 || tables.size(0) != requests || !tables.size(1) ||
+      (tables.size(1) > 1 && tables.stride(1) != 1) || (requests > 1 && tables.stride(0) < tables.size(1)))
+    refuse("block_tables must be int32 [", requests, ", width] with rows apart from each other, got ", shape_of(tables));
+  return tables.const_data_ptr<int32_t>();
+}
+
 // (context_lens, new_lens, block_tables, page_size, num_pages, tokens, free_pages, max_new, max_context) ->
 // (capsule, requests, max_new, max_context, starts, rows, context, status, positions, slots, used, needed)
 PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t) {
@@ -199,9 +213,7 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t) {
     const int32_t* const context = int32_list(context_lens, "context_lens", requests);
     const int32_t* const fresh = int32_list(on_device(a[1], "new_lens", device), "new_lens", requests);
     const Tensor& tables = on_device(a[2], "block_tables", device);
-    if (tables.scalar_type() != at::kInt || tables.dim() != 2 || tables.size(0) != requests || !tables.size(1) ||
-        (tables.size(1) > 1 && tables.stride(1) != 1) || (requests > 1 && tables.stride(0) < tables.size(1)))
-      refuse("block_tables must be int32 [", requests, ", width] with rows apart from each other, got ", shape_of(tables));
+    table_rows(tables, requests);
     const int64_t page_size = integer(a[3], "page_size", INT32_MIN, INT32_MAX);
     const int64_t num_pages = integer(a[4], "num_pages", INT32_MIN, INT32_MAX);
     const int64_t tokens = integer(a[5], "tokens", 1, SMX_PAGED_MAX_TOKENS);
@@ -274,9 +286,8 @@ PyObject* plan(PyObject*, PyObject* const* a, Py_ssize_t) {
 // Caches and heads
 // ---------------------------------------------------------------------------
 
-smx_paged_cache cache_of(PyObject* k_object, PyObject* v_object, const Plan& plan) {
-  const Tensor& k = on_device(k_object, "k_cache", plan.device);
-  const Tensor& v = on_device(v_object, "v_cache", plan.device);
+// A cache's layout; of a plan's sizes where one is given.
+smx_paged_cache cache_layout(const Tensor& k, const Tensor& v, const Plan* plan) {
   for (const Tensor* x : {&k, &v})
     if (x->scalar_type() != at::kBFloat16 || x->dim() != 4)
       refuse(x == &k ? "k_cache" : "v_cache", " must be a bf16 tensor [pages, page_size, kv_heads, head_dim], got ", shape_of(*x));
@@ -287,12 +298,17 @@ smx_paged_cache cache_of(PyObject* k_object, PyObject* v_object, const Plan& pla
     strides[i] = k.size(i) == 1 ? k.size(3) : k.stride(i);
     if (k.size(i) != 1 && k.stride(i) != v.stride(i)) refuse("k_cache and v_cache must have the same shape and strides");
   }
-  if (k.size(1) != plan.page_size || k.size(0) != plan.num_pages)
-    refuse("the plan is of ", plan.num_pages, " pages of ", plan.page_size, " tokens, the cache of ", k.size(0), " of ", k.size(1));
+  if (plan && (k.size(1) != plan->page_size || k.size(0) != plan->num_pages))
+    refuse("the plan is of ", plan->num_pages, " pages of ", plan->page_size, " tokens, the cache of ", k.size(0), " of ", k.size(1));
   if (k.stride(3) != 1 || v.stride(3) != 1) refuse("cache heads must be contiguous runs");
-  if (k.size(2) > 65535 || k.size(3) > 65535) refuse("too many or too wide heads: ", shape_of(k));
+  if (k.size(0) > INT32_MAX || k.size(1) > INT32_MAX || k.size(2) > 65535 || k.size(3) > 65535)
+    refuse("too many pages, or too many or too wide heads: ", shape_of(k));
   return smx_paged_cache{k.mutable_data_ptr(), v.mutable_data_ptr(), strides[0], strides[1], strides[2],
                          (int32_t)k.size(0), (int32_t)k.size(1), (int32_t)k.size(2), (int32_t)k.size(3)};
+}
+
+smx_paged_cache cache_of(PyObject* k, PyObject* v, const Plan& plan) {
+  return cache_layout(on_device(k, "k_cache", plan.device), on_device(v, "v_cache", plan.device), &plan);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -385,23 +401,41 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t) {
   });
 }
 
-// (q, k_cache, v_cache, plan, scale, window, out) -> out
+double scale_given(PyObject* o, int64_t head_dim) {
+  const double scale = given(o) ? real(o) : 1.0 / std::sqrt((double)head_dim);
+  if (!(std::isfinite(scale) && scale > 0)) refuse("scale must be positive and finite, got ", scale);
+  return scale;
+}
+
+int32_t window_given(PyObject* o) {
+  if (!given(o)) return 0;
+  if (!PyLong_Check(o)) refuse("window must be a positive number of tokens");
+  return (int32_t)integer(o, "window", 1, INT32_MAX);
+}
+
+// A float32 tensor that lies dense, of this shape.
+float* dense_floats(const Tensor& t, const char* name, at::IntArrayRef shape) {
+  if (t.scalar_type() != at::kFloat || t.sizes() != shape || !t.is_contiguous()) {
+    std::ostringstream want;
+    for (size_t i = 0; i < shape.size(); ++i) want << (i ? ", " : "") << shape[i];
+    refuse(name, " must be a contiguous float32 tensor of shape [", want.str(), "], got ", shape_of(t));
+  }
+  return t.mutable_data_ptr<float>();
+}
+
+// (q, k_cache, v_cache, plan, scale, window, out, lse) -> out
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t) {
   return guarded([&]() -> PyObject* {
-    no_gradients({a[0], a[1], a[2], a[6]});
+    no_gradients({a[0], a[1], a[2], a[6], a[7]});
     const Plan& plan = plan_of(a[3]);
     const smx_paged_cache cache = cache_of(a[1], a[2], plan);
     const int64_t head_dim = cache.head_dim;
     const c10::DeviceGuard guard(plan.device);
     Tensor hold, out;
     const smx_heads q = heads_of(a[0], "q", plan, -1, head_dim, &hold);
-    const double scale = given(a[4]) ? real(a[4]) : 1.0 / std::sqrt((double)head_dim);
-    if (!(std::isfinite(scale) && scale > 0)) refuse("scale must be positive and finite, got ", scale);
-    int64_t window = 0;
-    if (given(a[5])) {
-      if (!PyLong_Check(a[5])) refuse("window must be a positive number of tokens");
-      window = integer(a[5], "window", 1, INT32_MAX);
-    }
+    const double scale = scale_given(a[4], head_dim);
+    const int32_t window = window_given(a[5]);
+    float* const lse = given(a[7]) ? dense_floats(on_device(a[7], "lse", plan.device), "lse", {plan.step.tokens, q.heads}) : nullptr;
     smx_heads rows;
     const bool own = !given(a[6]);
     if (own) {
@@ -413,12 +447,204 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t) {
     int64_t need = 0;
     check(lib.attention_bytes((int32_t)head_dim, &need));
     const Tensor workspace = at::empty({need}, plan.memory.options().dtype(at::kByte));
-    check(lib.attention(&cache, &plan.step, &q, &rows, (float)scale, (int32_t)window, own, workspace.mutable_data_ptr(), need,
+    check(lib.attention(&cache, &plan.step, &q, &rows, (float)scale, window, own, lse, workspace.mutable_data_ptr(), need,
                         stream_of(plan.device)));
+    if (lse) written(tensor(a[7], "lse"));
     if (own) return THPVariable_Wrap(std::move(out));
     written(tensor(a[6], "out"));
     Py_INCREF(a[6]);
     return a[6];
+  });
+}
+
+// (q, k_cache, key_weights, plan, lse, scale, window) -> None
+PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t) {
+  return guarded([&]() -> PyObject* {
+    no_gradients({a[0], a[1], a[2], a[4]});
+    const Plan& plan = plan_of(a[3]);
+    const smx_paged_cache cache = cache_of(a[1], a[1], plan);  // (values are not read)
+    const c10::DeviceGuard guard(plan.device);
+    Tensor hold;
+    const smx_heads q = heads_of(a[0], "q", plan, -1, cache.head_dim, &hold);
+    const Tensor& weights = on_device(a[2], "key_weights", plan.device);
+    float* const to = dense_floats(weights, "key_weights", {cache.num_pages, cache.kv_heads, cache.page_size});
+    const float* const lse = dense_floats(on_device(a[4], "lse", plan.device), "lse", {plan.step.tokens, q.heads});
+    const double scale = scale_given(a[5], cache.head_dim);
+    const int32_t window = window_given(a[6]);
+    int64_t need = 0;
+    check(lib.weights_bytes(&need));
+    const Tensor workspace = at::empty({need}, plan.memory.options().dtype(at::kByte));
+    check(lib.weights(&cache, &plan.step, &q, lse, (float)scale, window, to, workspace.mutable_data_ptr(), need,
+                      stream_of(plan.device)));
+    written(weights);
+    Py_RETURN_NONE;
+  });
+}
+
+// (k_cache, v_cache, key_weights, context_lens, block_tables, keep, recent, max_context) -> lens
+PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t) {
+  return guarded([&]() -> PyObject* {
+    no_gradients({a[0], a[1], a[2]});
+    const Tensor& k = on_device(a[0], "k_cache");
+    const at::Device device = k.device();
+    const Tensor &v = on_device(a[1], "v_cache", device), &weights = on_device(a[2], "key_weights", device);
+    const smx_paged_cache cache = cache_layout(k, v, nullptr);
+    float* const received = dense_floats(weights, "key_weights", {cache.num_pages, cache.kv_heads, cache.page_size});
+    const Tensor& context_lens = on_device(a[3], "context_lens", device);
+    if (context_lens.dim() != 1 || !context_lens.size(0)) refuse("context_lens must hold one length per request");
+    const int64_t requests = context_lens.size(0);
+    const int32_t* const context = int32_list(context_lens, "context_lens", requests);
+    const Tensor& tables = on_device(a[4], "block_tables", device);
+    const int32_t* const entries = table_rows(tables, requests);
+    const int64_t width = std::min<int64_t>(tables.size(1), INT32_MAX), stride = requests > 1 ? tables.stride(0) : width;
+    const int32_t* keep_lens = nullptr;
+    int64_t keep = -1;
+    if (THPVariable_Check(a[5]))
+      keep_lens = int32_list(on_device(a[5], "keep", device), "keep", requests);
+    else
+      keep = integer(a[5], "keep", 0, INT32_MAX);
+    const int64_t recent = integer(a[6], "recent", 0, INT32_MAX);
+    const int64_t holds = std::min<int64_t>(width * cache.page_size, SMX_PAGED_MAX_CONTEXT);
+    const int64_t max_context = given(a[7]) ? integer(a[7], "max_context", 0, INT32_MAX) : holds;
+    const c10::DeviceGuard guard(device);
+    int64_t need = 0;
+    check(lib.evict_bytes((int32_t)std::min<int64_t>(requests, INT32_MAX), cache.kv_heads, (int32_t)keep, (int32_t)max_context, &need));
+    Tensor lens = at::empty({requests}, context_lens.options());
+    const Tensor workspace = at::empty({need}, context_lens.options().dtype(at::kByte));
+    check(lib.evict(&cache, received, (int32_t)requests, (int32_t)width, context, entries, stride, keep_lens, (int32_t)keep,
+                    (int32_t)recent, (int32_t)max_context, lens.mutable_data_ptr<int32_t>(), workspace.mutable_data_ptr(), need,
+                    stream_of(device)));
+    for (const Tensor* x : {&k, &v, &weights}) written(*x);
+    return THPVariable_Wrap(std::move(lens));
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Rotary positions
+// ---------------------------------------------------------------------------
+
+// (x, positions, frequencies, interleaved, amplitude, norm, eps, out) -> out
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t) {
+  return guarded([&]() -> PyObject* {
+    no_gradients({a[0], a[1], a[2], a[5], a[7]});
+    const Tensor* x = &on_device(a[0], "x");
+    const at::Device device = x->device();
+    if ((x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kFloat) || x->dim() != 3)
+      refuse("x must be bf16 or float32 heads [tokens, heads, head_dim], got ", shape_of(*x));
+    const int64_t tokens = x->size(0), heads = x->size(1), head_dim = x->size(2);
+    if (heads > INT32_MAX || head_dim > INT32_MAX) refuse("too many or too wide heads: ", shape_of(*x));
+    int32_t flags = 0;
+    if (x->scalar_type() == at::kFloat) flags |= SMX_ROTARY_F32;
+    const c10::DeviceGuard guard(device);
+    Tensor hold[4], out;
+    const Tensor* positions = &on_device(a[1], "positions", device);
+    if (positions->dim() != 1 || positions->size(0) != tokens ||
+        (positions->scalar_type() != at::kInt && positions->scalar_type() != at::kLong))
+      refuse("positions must be int32 or int64 of shape (", tokens, ",), got ", shape_of(*positions));
+    if (!positions->is_contiguous()) positions = &(hold[0] = positions->contiguous());
+    if (positions->scalar_type() == at::kLong) flags |= SMX_ROTARY_POSITIONS_I64;
+    const Tensor* frequencies = &on_device(a[2], "frequencies", device);
+    if (frequencies->dim() != 1 || (frequencies->scalar_type() != at::kFloat && frequencies->scalar_type() != at::kDouble))
+      refuse("frequencies must be a list of float64 or float32 values, got ", shape_of(*frequencies));
+    if (frequencies->size(0) < 1 || 2 * frequencies->size(0) > head_dim)
+      refuse("frequencies must be 1 to head_dim / 2 = ", head_dim / 2, " values, one for each pair, got ", frequencies->size(0));
+    if (!frequencies->is_contiguous()) frequencies = &(hold[1] = frequencies->contiguous());
+    if (frequencies->scalar_type() == at::kFloat) flags |= SMX_ROTARY_FREQUENCIES_F32;
+    const int interleaved = PyObject_IsTrue(a[3]);
+    if (interleaved < 0) throw Raised();
+    if (interleaved) flags |= SMX_ROTARY_INTERLEAVED;
+    const void* norm = nullptr;
+    if (given(a[5])) {
+      const Tensor& w = on_device(a[5], "norm", device);
+      if (w.dim() != 1 || w.size(0) != head_dim) refuse("norm must have shape (", head_dim, ",), got ", shape_of(w));
+      const Tensor& y = laid_out(w, &hold[2]);
+      if (y.scalar_type() == at::kFloat) flags |= SMX_ROTARY_NORM_F32;
+      norm = y.data_ptr();
+    }
+    auto stride = [](const Tensor& t, int i) { return t.size(i) > 1 ? t.stride(i) : 0; };
+    const bool own = !given(a[7]);
+    if (own) {
+      out = at::empty({tokens, heads, head_dim}, x->options());
+    } else {
+      out = on_device(a[7], "out", device);
+      if (out.scalar_type() != x->scalar_type() || out.sizes() != x->sizes() || out.stride(2) != 1)
+        refuse("out must be like x, ", shape_of(*x), ", with contiguous heads, got ", shape_of(out));
+    }
+    const double amplitude = real(a[4]), eps = real(a[6]);
+    if (tokens) {
+      if (x->stride(2) != 1) x = &(hold[3] = x->clone(at::MemoryFormat::Contiguous));
+      const smx_heads from{x->data_ptr(), stride(*x, 0), stride(*x, 1), (int32_t)heads};
+      const smx_heads to{out.mutable_data_ptr(), stride(out, 0), stride(out, 1), (int32_t)heads};
+      check(lib.rotary((int32_t)std::min<int64_t>(tokens, INT32_MAX), (int32_t)head_dim, (int32_t)(2 * frequencies->size(0)), &from, &to,
+                       positions->data_ptr(), frequencies->data_ptr(), norm, flags, (float)amplitude, (float)eps, own,
+                       stream_of(device)));
+    }
+    if (own) return THPVariable_Wrap(std::move(out));
+    written(out);
+    Py_INCREF(a[7]);
+    return a[7];
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Verification of drafts
+// ---------------------------------------------------------------------------
+
+// (target, tokens, plan, accept, sample, draft) -> (tokens, counts)
+PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t) {
+  return guarded([&]() -> PyObject* {
+    no_gradients({a[0], a[3], a[4], a[5]});
+    const Plan& plan = plan_of(a[2]);
+    const int64_t rows = plan.step.tokens, requests = plan.step.requests;
+    const c10::DeviceGuard guard(plan.device);
+    Tensor hold[5];
+    const Tensor& target = on_device(a[0], "target", plan.device);
+    if (target.dim() != 2 || target.size(0) != rows || !target.size(1) || target.size(1) > SMX_VERIFY_MAX_VOCAB ||
+        (target.scalar_type() != at::kFloat && target.scalar_type() != at::kBFloat16))
+      refuse("target must be float32 or bf16 probabilities [", rows, ", vocab], got ", shape_of(target));
+    const int64_t vocab = target.size(1);
+    // rows of probabilities behind each other (laid out anew where they are not)
+    auto rows_of = [&](const Tensor& t, Tensor* copy) -> const Tensor& {
+      if ((vocab == 1 || t.stride(1) == 1) && (rows == 1 || t.stride(0) >= vocab)) return t;
+      return *copy = t.clone(at::MemoryFormat::Contiguous);
+    };
+    const Tensor& p = rows_of(target, &hold[0]);
+    const Tensor* q = nullptr;
+    if (given(a[5])) {
+      const Tensor& draft = on_device(a[5], "draft", plan.device);
+      if (draft.sizes() != target.sizes() || draft.scalar_type() != target.scalar_type())
+        refuse("draft must be like target, ", shape_of(target), ", got ", shape_of(draft));
+      q = &rows_of(draft, &hold[1]);
+    }
+    const Tensor* tokens = &on_device(a[1], "tokens", plan.device);
+    if (tokens->dim() != 1 || tokens->size(0) != rows || (tokens->scalar_type() != at::kInt && tokens->scalar_type() != at::kLong))
+      refuse("tokens must be int32 or int64 of shape (", rows, ",), got ", shape_of(*tokens));
+    if (!tokens->is_contiguous()) tokens = &(hold[2] = tokens->contiguous());
+    const float* numbers[2];
+    for (int i = 0; i < 2; ++i) {
+      const char* const name = i ? "sample" : "accept";
+      const int64_t length = i ? requests : rows;
+      const Tensor* u = &on_device(a[3 + i], name, plan.device);
+      if (u->dim() != 1 || u->size(0) != length || u->scalar_type() != at::kFloat)
+        refuse(name, " must be float32 of shape (", length, ",), got ", shape_of(*u));
+      if (!u->is_contiguous()) u = &(hold[3 + i] = u->contiguous());
+      numbers[i] = u->const_data_ptr<float>();
+    }
+    int32_t flags = 0;
+    if (target.scalar_type() == at::kBFloat16) flags |= SMX_VERIFY_BF16;
+    if (tokens->scalar_type() == at::kLong) flags |= SMX_VERIFY_TOKENS_I64;
+    Tensor out = at::empty({rows}, tokens->options()), counts = at::empty({requests}, plan.memory.options());
+    int64_t need = 0;
+    check(lib.verify_bytes((int32_t)requests, (int32_t)vocab, &need));
+    const Tensor workspace = at::empty({need}, plan.memory.options().dtype(at::kByte));
+    check(lib.verify(&plan.step, (int32_t)vocab, p.data_ptr(), rows > 1 ? p.stride(0) : vocab, q ? q->data_ptr() : nullptr,
+                     q && rows > 1 ? q->stride(0) : vocab, tokens->data_ptr(), numbers[0], numbers[1], flags, out.mutable_data_ptr(),
+                     counts.mutable_data_ptr<int32_t>(), workspace.mutable_data_ptr(), need, stream_of(plan.device)));
+    PyObject* const result = PyTuple_New(2);
+    if (!result) throw Raised();
+    PyTuple_SET_ITEM(result, 0, THPVariable_Wrap(std::move(out)));
+    PyTuple_SET_ITEM(result, 1, THPVariable_Wrap(std::move(counts)));
+    return result;
   });
 }
 
@@ -495,22 +721,21 @@ PyObject* int4(PyObject*, PyObject* const* a, Py_ssize_t) {
 
 // (addresses of the C ABI's entry points in Library's order, raw_stream)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* at[7];
-  if (n != 8) {
-    PyErr_SetString(PyExc_TypeError, "seven addresses and the stream lookup");
+  constexpr int kEntries = 14;
+  void* at[kEntries];
+  if (n != kEntries + 1) {
+    PyErr_SetString(PyExc_TypeError, "the addresses of the library's entry points and the stream lookup");
     return nullptr;
   }
-  for (int i = 0; i < 7; ++i) at[i] = PyLong_AsVoidPtr(a[i]);
+  for (int i = 0; i < kEntries; ++i) at[i] = PyLong_AsVoidPtr(a[i]);
   if (PyErr_Occurred()) return nullptr;
-  lib.plan = reinterpret_cast<decltype(lib.plan)>(at[0]);
-  lib.write = reinterpret_cast<decltype(lib.write)>(at[1]);
-  lib.attention = reinterpret_cast<decltype(lib.attention)>(at[2]);
-  lib.attention_bytes = reinterpret_cast<decltype(lib.attention_bytes)>(at[3]);
-  lib.int4 = reinterpret_cast<decltype(lib.int4)>(at[4]);
-  lib.int4_bytes = reinterpret_cast<decltype(lib.int4_bytes)>(at[5]);
-  lib.error = reinterpret_cast<decltype(lib.error)>(at[6]);
-  Py_INCREF(a[7]);
-  lib.raw_stream = a[7];
+  int i = 0;
+  auto next = [&](auto& entry) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(at[i++]); };
+  next(lib.plan), next(lib.write), next(lib.attention), next(lib.attention_bytes), next(lib.weights), next(lib.weights_bytes);
+  next(lib.evict), next(lib.evict_bytes), next(lib.rotary), next(lib.verify), next(lib.verify_bytes), next(lib.int4);
+  next(lib.int4_bytes), next(lib.error);
+  Py_INCREF(a[kEntries]);
+  lib.raw_stream = a[kEntries];
   Py_RETURN_NONE;
 }
 
@@ -522,6 +747,10 @@ PyCFunction method(F f) {
 PyMethodDef methods[] = {{"plan", method(plan), METH_FASTCALL, nullptr},
                          {"write", method(write), METH_FASTCALL, nullptr},
                          {"attention", method(attention), METH_FASTCALL, nullptr},
+                         {"key_weights", method(key_weights), METH_FASTCALL, nullptr},
+                         {"evict", method(evict), METH_FASTCALL, nullptr},
+                         {"rotary", method(rotary), METH_FASTCALL, nullptr},
+                         {"verify", method(verify), METH_FASTCALL, nullptr},
                          {"int4", method(int4), METH_FASTCALL, nullptr},
                          {"bind", method(bind), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

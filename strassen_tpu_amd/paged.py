@@ -1,6 +1,7 @@
 """A paged key/value cache for serving: the plan of a step, the write of its
-heads and the attention over the cache, on the kernels of ``csrc/paged_cache.hip``
-and ``csrc/paged_attention.hip``. The reference keeps no cache; these stand
+heads, the attention over the cache, the weight that keys receive in it and the eviction by that weight, on the
+kernels of ``csrc/paged_cache.hip``, ``csrc/paged_attention.hip``, ``csrc/paged_weights.hip`` and
+``csrc/paged_evict.hip``. The reference keeps no cache; these stand
 beside ``qwen3_block.attention``, which attends within one batch of whole
 sequences.
 
@@ -24,7 +25,7 @@ from __future__ import annotations
 
 from . import _lib
 
-__all__ = ["PagedPlan", "paged_plan", "paged_write", "paged_attention", "PAGED_OK", "PAGED_BAD_LENGTH",
+__all__ = ["PagedPlan", "paged_plan", "paged_write", "paged_attention", "paged_key_weights", "paged_evict", "PAGED_OK", "PAGED_BAD_LENGTH",
            "PAGED_OUT_OF_ROWS", "PAGED_OUT_OF_PAGES", "PAGED_BAD_PAGE"]
 
 # What a plan's status says of a request.
@@ -101,7 +102,7 @@ def paged_write(k, v, k_cache, v_cache, plan, *, q=None, rope_cos=None, rope_sin
     return _lib.host().write(k, v, k_cache, v_cache, plan._native, q, rope_cos, rope_sin, q_scale, k_scale, eps)
 
 
-def paged_attention(q, k_cache, v_cache, plan, *, scale=None, window=None, out=None):
+def paged_attention(q, k_cache, v_cache, plan, *, scale=None, window=None, out=None, lse=None):
     """Causal grouped-query attention of a step's new tokens ``q`` ``[tokens, heads, head_dim]``
     over the cache, the step's own keys and values (``paged_write``) among it: the row at
     position p of its request sees that request's positions 0 .. p, with ``window``
@@ -112,5 +113,47 @@ def paged_attention(q, k_cache, v_cache, plan, *, scale=None, window=None, out=N
     that sees none is zero (one all of whose scores are -inf is NaN). Infinities and NaN in the cache
     reach the rows that see them and no others. Rows of no admitted request are zero in a new result, and left as they
     were in ``out`` (bf16 ``[tokens, heads, head_dim]``, rows 16-byte aligned). ``out`` may be ``q``; else its rows
-    share memory neither with each other nor with ``q`` or the cache."""
-    return _lib.host().attention(q, k_cache, v_cache, plan._native, scale, window, out)
+    share memory neither with each other nor with ``q`` or the cache.
+
+    ``lse`` float32 ``[tokens, heads]``, contiguous and of memory of its own, receives the logarithm of each row's
+    sum of exponentials, for ``paged_key_weights``: -inf for a row that sees no key or whose scores are all
+    -inf. Rows of no admitted request are left as they were."""
+    return _lib.host().attention(q, k_cache, v_cache, plan._native, scale, window, out, lse)
+
+
+def paged_key_weights(q, k_cache, key_weights, plan, lse, *, scale=None, window=None):
+    """Add the attention weight that each cached key receives in a step to ``key_weights``
+    float32 ``[pages, kv_heads, page_size]`` (contiguous), in place::
+
+        out = paged_attention(q, k_cache, v_cache, plan, lse=lse)
+        paged_key_weights(q, k_cache, key_weights, plan, lse)
+
+    A key receives ``exp(scale q . k - lse)``, its softmax weight, from every row that sees it and
+    every query head of its key/value head. The step's own keys start from zero, so that slots of
+    reused pages need no clearing, as long as every step that writes keys is followed by this call. ``q``, ``scale``
+    and ``window`` are those of the attention that gave ``lse``. Scores and sums in FP32, in an order that depends on the
+    lengths alone. Slots that hold no key of an admitted request stay as they were, as do those of table entries that
+    are no page of the cache. Requests must not share pages. ``key_weights`` shares no memory with the other tensors."""
+    _lib.host().key_weights(q, k_cache, key_weights, plan._native, lse, scale, window)
+
+
+def paged_evict(k_cache, v_cache, key_weights, context_lens, block_tables, keep, *, recent=0, max_context=None):
+    """Cut requests of more than ``keep`` cached tokens (``context_lens`` int32 ``[requests]``) down to
+    ``keep``, a number or an int32 tensor of one for each request, in place, and return the
+    lengths that the cache then holds (int32 ``[requests]``).
+
+    Each key/value head keeps the last ``min(recent, keep)`` tokens and, of those before, the ones
+    with the largest ``key_weights`` (``paged_key_weights``; equal ones: the lowest index, NaN counts as
+    the largest). Keys, values and weights then lie at the request's indices 0 .. keep - 1, those
+    kept for their weight first, the recent ones behind them in their order: a survivor whose index is below ``keep -
+    min(recent, keep)`` stays, the j-th place that became free below it takes the j-th survivor from behind. So heads hold
+    different tokens at an index, and the index no longer says a token's position: rotate new heads by
+    positions of your own (``rotary``), and attend without a window. Every layer's cache is cut by a call of its
+    own, with the same ``block_tables`` and lengths.
+
+    A request is left as it was, and its length returned, if it holds ``keep`` tokens or fewer, if a
+    length is negative or above ``max_context`` (default: what the tables hold; it sizes the call's workspace,
+    4 to 8 bytes a token and head), or if a table entry of its tokens is no page of the cache. ``block_tables`` is not
+    changed: pages behind the last kept token stay the request's, for its next tokens or for the program to
+    take back. Requests must not share pages."""
+    return _lib.host().evict(k_cache, v_cache, key_weights, context_lens, block_tables, keep, recent, max_context)
