@@ -40,7 +40,8 @@ from .int4 import int4_matmul, int4_quantize, int4_weight_layout
 from .layouts import (rope_layout_tables, rope_layout_to_heads, rope_scale_layout, rope_weight_layout,
                       swiglu_weight_layout)
 from .packing import cubic_weight_layout, pack_activation, strassen_weight_layout
-from .paged import paged_attention, paged_write
+from .paged import paged_attention, paged_key_weights, paged_write
+from .rotary import rotary, rotary_frequencies
 from .strassen import cubic_matmul, strassen_matmul
 
 __all__ = ["Qwen3Dims", "QWEN3_32B", "BlockWeights", "PreparedBlock", "rms_norm", "apply_rope", "rope_values",
@@ -285,14 +286,24 @@ class ServingBlock:
 
     The query, key and value projections are one product. ``arm`` "strassen" and "cubic" pack
     the weights for tiles of ``(bn, bk)`` columns and K; "int4" quantises them in groups of
-    ``group`` (``int4_quantize``). ``max_context`` positions have RoPE tables."""
+    ``group`` (``int4_quantize``). ``max_context`` positions have RoPE tables. ``frequencies`` and
+    ``amplitude`` (``rotary_frequencies``; default: those of ``dims.theta``) rotate the heads of steps that say their
+    positions; where they are given, those of all steps, and no tables are made."""
 
-    def __init__(self, weights, dims, arm, *, max_context, tile=(1024, 512), group=128):
+    def __init__(self, weights, dims, arm, *, max_context, tile=(1024, 512), group=128, frequencies=None, amplitude=1.0):
         if arm not in SERVING_ARMS:
             raise ValueError(f"unknown arm {arm!r}; expected one of {SERVING_ARMS}")
         self.weights, self.dims, self.arm, self.tile = weights, dims, arm, tuple(tile)
         self.max_context = int(max_context)
-        self.cos, self.sin = rope_values(self.max_context, dims.head_dim, dims.theta, weights.query.device)
+        device = weights.query.device
+        if frequencies is None:
+            if amplitude != 1.0:
+                raise ValueError("amplitude= goes with frequencies=")
+            self.cos, self.sin = rope_values(self.max_context, dims.head_dim, dims.theta, device)
+            self.frequencies, self.amplitude = rotary_frequencies(dims.head_dim, dims.theta, device=device)
+        else:
+            self.cos = self.sin = None
+            self.frequencies, self.amplitude = frequencies.to(device), amplitude
         qkv = torch.cat((weights.query, weights.key, weights.value), dim=1)
         if arm == "int4":
             def pack(w, epilogue=None):
@@ -320,23 +331,39 @@ class ServingBlock:
         return matmul(x, w, bm=bm, bn=self.tile[0], bk=self.tile[1], **kw)
 
 
-def block_step(x, block, k_cache, v_cache, plan, *, window=None):
+def block_step(x, block, k_cache, v_cache, plan, *, window=None, positions=None, key_weights=None):
     """One serving step through a decoder block: ``x [plan.tokens, hidden]`` bf16 -> same
     shape, the new tokens' keys and values stored in the layer's cache and attended to
     together with those before them (``paged_plan``, ``paged_write``, ``paged_attention``).
     The "strassen" and "cubic" arms take tokens in whole sixteens (the plan may have padding
     rows). Rows of no admitted request touch no cache and no other row. "strassen", whose products combine rows
     (an infinity or NaN in one admitted row reaches others of its tile), takes them as zero; in the other arms
-    they pass through as rows of their own."""
+    they pass through as rows of their own.
+
+    ``positions`` (int32 or int64 ``[plan.tokens]``) are the rows' positions where they are not their indices in the
+    cache: after an eviction, whose keys were rotated where they stood (``rotary``). ``key_weights``
+    float32 ``[pages, kv_heads, page_size]`` receives the attention weight of the layer's keys
+    (``paged_key_weights``), by which ``paged_evict`` cuts the cache."""
     d, w = block.dims, block.weights
     if block.arm == "strassen":
         x = x.masked_fill((plan.positions < 0)[:, None], 0)
     normalized = _row_rms_norm(x, w.attention_norm, d.eps)
     heads = block.product(normalized, block.qkv).view(plan.tokens, d.heads + 2 * d.kv_heads, d.head_dim)
     query, key, value = heads.split((d.heads, d.kv_heads, d.kv_heads), dim=1)
-    query = paged_write(key, value, k_cache, v_cache, plan, q=query, rope_cos=block.cos, rope_sin=block.sin,
-                        q_scale=w.query_norm, k_scale=w.key_norm, eps=d.eps)
-    attended = paged_attention(query, k_cache, v_cache, plan, window=window).flatten(1)
+    if positions is None and block.cos is not None:
+        query = paged_write(key, value, k_cache, v_cache, plan, q=query, rope_cos=block.cos, rope_sin=block.sin,
+                            q_scale=w.query_norm, k_scale=w.key_norm, eps=d.eps)
+    else:
+        at = plan.positions if positions is None else positions
+        query, key = (rotary(part, at, block.frequencies, amplitude=block.amplitude, norm=norm, eps=d.eps)
+                      for part, norm in ((query, w.query_norm), (key, w.key_norm)))
+        paged_write(key, value, k_cache, v_cache, plan)
+    lse = None
+    if key_weights is not None:
+        lse = torch.empty(plan.tokens, d.heads, dtype=torch.float32, device=query.device)
+    attended = paged_attention(query, k_cache, v_cache, plan, window=window, lse=lse).flatten(1)
+    if key_weights is not None:
+        paged_key_weights(query, k_cache, key_weights, plan, lse, window=window)
     residual = block.product(attended, block.attention_output, epilogue="residual_add", residual=x)
     normalized = _row_rms_norm(residual, w.mlp_norm, d.eps)
     activated = block.product(normalized, block.gate_up, epilogue="swiglu")
