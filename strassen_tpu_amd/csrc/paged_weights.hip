@@ -29,6 +29,7 @@ struct WeightArgs {
   const float* lse;
   float* weights;  // [pages, kv_heads, page_size]
   int32_t requests, group, kv_heads, page_shift, num_pages, window, min_span;
+  uint32_t per_group;    // 2^16 / group, upwards
   float scale;           // times log2 e
   double per_workgroup;  // 1 / workgroups
   float* partial;
@@ -45,9 +46,9 @@ constexpr float kLog2E = 1.44269504088896341f;
 // n / d downwards, d > 0.
 __device__ __forceinline__ int64_t floor_div(int64_t n, int64_t d) { return n >= 0 ? n / d : -((-n + d - 1) / d); }
 
-// The key tiles of one request, of kTile keys, and the steps of 32 rows that see each. An item (one of them) counts kItem
+// The key tiles of one request, of kTile keys, and the steps of kStepRows rows that see each. An item (one of them) counts kItem
 // units before its steps, for its start and end.
-constexpr int kTile = 256, kStepRows = 32, kItem = 3;
+constexpr int kBlocks = 3, kWave = 32 * kBlocks, kTile = 4 * kWave, kStepRows = 32, kItem = 3;
 struct KeyTiles {
   int32_t context, fresh, group, window, first, tiles;
 
@@ -120,18 +121,31 @@ __device__ __forceinline__ float* weight_of(const WeightArgs& p, int page, int k
 // Register e of half h holds row 8 (e / 4) + 4 h + e % 4 of a step.
 __device__ __forceinline__ int row_of_register(int e, int half) { return 8 * (e >> 2) + 4 * half + (e & 3); }
 
-// Many rows: a workgroup of four waves holds 256 keys, 64 a wave, and its rows pass through LDS, 32 at a time.
-template <int D>
+// Sixteen or four bytes a lane from memory into LDS, lane l's at `to` + its size times l.
+__device__ __forceinline__ void dma16(const void* from, void* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+__device__ __forceinline__ void dma4(const void* from, void* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)from,
+                                   (__attribute__((address_space(3))) void*)to, 4, 0, 0);
+}
+
+// Many rows: a workgroup of four waves holds 384 keys, 96 a wave, and its rows pass through LDS, 32 a step, fetched
+// three steps ahead.
+template <int D, bool kWhole>
 __global__ __launch_bounds__(256, 2) void key_weights_many(WeightArgs p) {
-  constexpr int kRow = 2 * D, kChunks = D / 8, kLoads = kStepRows * kChunks / 256;
-  __shared__ __attribute__((aligned(1024))) uint8_t q_tiles[2][kStepRows * kRow];
-  __shared__ __attribute__((aligned(16))) float sums[2][kStepRows];
-  __shared__ __attribute__((aligned(16))) int32_t places[2][kStepRows];
+  constexpr int kRow = 2 * D, kChunks = D / 8, kLoads = kStepRows * kChunks / 256, kRing = 4;
+  // (LDS of a size that the launch says: behind arrays that the compiler knows it waits for every DMA before a read)
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  constexpr int kStep = kStepRows * kRow;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   WeightRecord* const record = p.records + blockIdx.x;
   if (threadIdx.x == 0) record->others = 0;
   Span s;
   if (!find_span<KeyTiles, 4>(p, &s)) return;
+  const int64_t heads = (int64_t)p.group * p.kv_heads;
+  const int step_tokens = kStepRows / p.group, step_heads = kStepRows - step_tokens * p.group;
 
   while (s.left > 0) {
     const KeyTiles r = KeyTiles::uniform(p, s.context, s.fresh);
@@ -140,121 +154,216 @@ __global__ __launch_bounds__(256, 2) void key_weights_many(WeightArgs p) {
     const int before = max(0, s.skip - kItem), upto = max(0, s.skip + units - kItem);
     const int from = r.begin(s.tile) + before, count = upto - before;
     if (count > 0) {
-      const int length = s.context + s.fresh, key0 = (r.first + s.tile) * kTile + 64 * wave;
+      const int length = s.context + s.fresh, key0 = (r.first + s.tile) * kTile + kWave * wave;
       const int32_t* const table = p.tables + s.request * p.table_stride;
       const int64_t start = scalar_at(p.starts, s.request);
       const int rows = s.fresh * p.group;
-      Keys<D> k[2];
-      int page[2];
-      bool held[2];
+      // The rows that see a key are consecutive: of the tokens at it and behind it, less than a window from it.
+      auto first_row = [&](int key) __attribute__((always_inline)) { return max(0, key - s.context) * p.group; };
+      auto last_row = [&](int key) __attribute__((always_inline)) {
+        return p.window ? max(0, min(s.fresh, key - s.context + p.window)) * p.group : rows;
+      };
+      Keys<D> k[kBlocks];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int key = min(key0 + 32 * x + (lane & 31), length - 1);
-        held[x] = find_key(p, table, key0 + 32 * x + (lane & 31), length, &page[x]);
-        load_keys<D>(p, k[x], page[x], key, s.head);
+      for (int x = 0; x < kBlocks; ++x) {
+        const int key = key0 + 32 * x + (lane & 31);
+        int page;
+        find_key(p, table, key, length, &page);
+        load_keys<D>(p, k[x], page, min(key, length - 1), s.head);
       }
-      // The thread's part of a step's rows: chunks of 16 bytes, and (the first 32) a row's sum and place.
-      u32x4 chunk[kLoads];
-      float sum = 0.f;
-      int32_t place = 0;
-      auto load_rows = [&](int step) __attribute__((always_inline)) {
+      const int all_from = first_row(key0 + kWave - 1), all_upto = last_row(key0);  // rows that see all of the wave's keys
+      // The rows of the next step to be fetched: chunks of 16 bytes, and a row's lse, from the first row's token on (the host
+      // made sure that a step's queries lie within 2^32 bytes). Rows behind the last are fetched as that one, and count for
+      // nothing. In steps of whole tokens (kWhole) a lane keeps its place in them and in the last one.
+      const int last_step = (rows - 1) / kStepRows;
+      int fetched = min(from, last_step);
+      const int token0 = (uint32_t)(fetched * kStepRows) / (uint32_t)p.group;
+      int head0 = fetched * kStepRows - token0 * p.group;  // of the step's first row
+      const uint8_t* q_from = reinterpret_cast<const uint8_t*>(p.q + (start + token0) * p.q_token + (int64_t)s.head * p.group * p.q_head);
+      const uint8_t* lse_from = reinterpret_cast<const uint8_t*>(p.lse + (start + token0) * heads + s.head * p.group);
+      // bytes to the lane's row of DMA i (kLoads: the lse), none behind row `most` of the step
+      auto place = [&](int i, int most) __attribute__((always_inline)) -> uint32_t {
+        const uint32_t in = i < kLoads ? ((kLoads * wave + i) * 64 + lane) / kChunks : lane & 31;
+        const uint32_t row = head0 + min(in, (uint32_t)most);               // below 32 + 128: exact
+        const uint32_t token = row * p.per_group >> 16, head = row - token * p.group;
+        if (i == kLoads) return 4 * (token * (uint32_t)heads + head);
+        return 2 * (token * (uint32_t)p.q_token + head * (uint32_t)p.q_head) + 16 * (lane % kChunks ^ (in & (kChunks - 1)));
+      };
+      uint32_t at[kLoads + 1], at_last[kLoads + 1];
+      if constexpr (kWhole)
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int at = threadIdx.x + 256 * i, row = min(step * kStepRows + at / kChunks, rows - 1);
-          const int token = (uint32_t)row / (uint32_t)p.group, head = row - token * p.group;
-          chunk[i] = *reinterpret_cast<const u32x4*>(p.q + (start + token) * p.q_token +
-                                                     (int64_t)(s.head * p.group + head) * p.q_head + at % kChunks * 8);
+        for (int i = 0; i <= kLoads; ++i) at[i] = place(i, kStepRows - 1), at_last[i] = place(i, rows - 1 - last_step * kStepRows);
+      auto fetch = [&](int i) __attribute__((always_inline)) {
+        const int buffer = i & (kRing - 1);
+        uint8_t* const to = lds + buffer * kStep + kLoads * 1024 * wave;
+        const bool last = fetched >= last_step;  // uniform
+#pragma unroll
+        for (int x = 0; x < kLoads; ++x)
+          dma16(q_from + (!kWhole ? place(x, rows - 1 - fetched * kStepRows) : last ? at_last[x] : at[x]), to + 1024 * x);
+        dma4(lse_from + (!kWhole ? place(kLoads, rows - 1 - fetched * kStepRows) : last ? at_last[kLoads] : at[kLoads]),
+             lds + kRing * kStep + 256 * (kRing * wave + buffer));  // a wave's own: each row's lse, twice
+        const int heads_on = head0 + step_heads, wraps = heads_on >= p.group;  // on to the next step, if there is one
+        fetched += last ? 0 : 1;
+        if constexpr (!kWhole) head0 = last ? head0 : heads_on - (wraps ? p.group : 0);
+        const int64_t tokens = last ? 0 : step_tokens + (kWhole ? 0 : wraps);
+        q_from += 2 * tokens * p.q_token, lse_from += 4 * tokens * heads;
+      };
+      float total[kBlocks];
+#pragma unroll
+      for (int x = 0; x < kBlocks; ++x) total[x] = 0.f;
+      // Weights of a block's scores, added up.
+      auto weigh = [&](f32x16& score, const f32x4 (&lse)[4], int x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          score[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[e], p.scale, lse[e >> 2][e & 3]));
+        float part[2] = {score[0], score[1]};
+#pragma unroll
+        for (int e = 2; e < 16; ++e) part[e & 1] += score[e];
+        total[x] += part[0] + part[1];
+      };
+      // The same of rows some of which do not see some of the keys.
+      auto weigh_some = [&](f32x16& score, const f32x4 (&lse)[4], int x, int row0) __attribute__((always_inline)) {
+        float sum = 0.f;
+        const int key = key0 + 32 * x + (lane & 31), first = first_row(key) - row0 - 4 * half, last = last_row(key) - row0 - 4 * half;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int row = row_of_register(e, 0);  // (less row0 + 4 half, as the bounds)
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score[e], p.scale, lse[e >> 2][e & 3]));
+          sum += row >= first && row < last ? w : 0.f;
         }
-        if (threadIdx.x < kStepRows) {
-          const int at = step * kStepRows + (int)threadIdx.x, row = min(at, rows - 1);
-          const int token = (uint32_t)row / (uint32_t)p.group, head = row - token * p.group;
-          const float lse = p.lse[(start + token) * ((int64_t)p.group * p.kv_heads) + s.head * p.group + head];
-          sum = at < rows ? lse * kLog2E : INFINITY;
-          place = s.context + token;
+        total[x] += sum;
+      };
+      bf16x8 q[D / 16];
+      f32x16 score[2];
+      auto slot_of = [&](int i) { return i & (kRing - 1); };
+      auto lse_slot = [&](int i) { return reinterpret_cast<float*>(lds + kRing * kStep + 256 * (kRing * wave + slot_of(i))); };
+      auto read_row = [&](int i, int t) __attribute__((always_inline)) {
+        q[t] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(lds + slot_of(i) * kStep + (lane & 31) * kRow +
+                                                                         16 * ((2 * t + half) ^ (lane & (kChunks - 1)))));
+      };
+      auto read_lse = [&](int i, f32x4 (&lse)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lse[e] = *reinterpret_cast<const f32x4*>(lse_slot(i) + 8 * e + 4 * half);
+      };
+      auto multiply = [&](f32x16& score, int x, int next) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) score[e] = 0.f;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+          score = __builtin_amdgcn_mfma_f32_32x32x16_bf16(q[t], k[x].k[t], score, 0, 0, 0);
+          if (next) read_row(next, t);
         }
       };
-      auto store_rows = [&](int buffer) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int at = threadIdx.x + 256 * i, row = at / kChunks, c = at % kChunks;
-          *reinterpret_cast<u32x4*>(q_tiles[buffer] + row * kRow + 16 * (c ^ (row & (kChunks - 1)))) = chunk[i];
-        }
-        if (threadIdx.x < kStepRows) sums[buffer][threadIdx.x] = sum, places[buffer][threadIdx.x] = place;
+      // all but the fetches of `steps` steps, of every wave
+      auto arrived = [&](auto steps) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(decltype(steps)::value * (kLoads + 1)) : "memory");
       };
-      float total[2] = {0.f, 0.f};
-      __syncthreads();  // the item before has read its rows
-      load_rows(from);
-      store_rows(0);
-      for (int i = 0; i < count; ++i) {
-        const int buffer = i & 1;
-        __syncthreads();
-        if (i + 1 < count) load_rows(from + i + 1);
-        bf16x8 q[D / 16];
-#pragma unroll
-        for (int t = 0; t < D / 16; ++t)
-          q[t] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q_tiles[buffer] + (lane & 31) * kRow +
-                                                                           16 * ((2 * t + half) ^ (lane & (kChunks - 1)))));
+      // the next step's rows are there, and every wave has read this one's
+      auto next_step = [&](int i) __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
+        arrived(std::integral_constant<int, kRing - 2>());
+        fetch(i + kRing);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      // A step some of whose rows do not see some of the keys.
+      auto some = [&](int i) __attribute__((always_inline)) {
         f32x4 lse[4];
+        read_lse(i, lse);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) lse[e] = *reinterpret_cast<const f32x4*>(&sums[buffer][8 * e + 4 * half]);
-        f32x16 score[2];
+        for (int e = 0; e < 4; ++e) lse[e] *= -kLog2E;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < kBlocks; ++x) {
+          multiply(score[0], x, 0);
+          weigh_some(score[0], lse, x, (from + i) * kStepRows);
+        }
+        next_step(i);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) score[x][e] = 0.f;
+        for (int t = 0; t < D / 16; ++t) read_row(i + 1, t);
+      };
+      // A step whose rows see all keys. A block's products run beside the weights of the block before: a matrix instruction,
+      // then as much vector work as the matrix core takes for it. The next step's rows are read beside the last
+      // block's. `before`: lse (times -log2 e) of the step before, `now` of this one, by way of LDS: a lane's row
+      // is scaled by one instruction, and then read as the registers need it. kFirst: where the first block's scores go.
+      float mine = 0.f;
+      auto all = [&](auto kFirst, int i, const f32x4 (&before)[4], f32x4 (&now)[4]) __attribute__((always_inline)) {
+        lse_slot(i)[lane] = mine * -kLog2E;
+        read_lse(i, now);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t)
+        for (int x = 0; x < kBlocks; ++x) {
+          const int to = (decltype(kFirst)::value + x) & 1;
+          const bool ends = x == kBlocks - 1;
+          if (ends) next_step(i);
+          multiply(score[to], x, ends ? i + 1 : 0);
+          if (ends) mine = lse_slot(i + 1)[lane];
+          weigh(score[to ^ 1], x ? now : before, x ? x - 1 : kBlocks - 1);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) score[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(q[t], k[x].k[t], score[x], 0, 0, 0);
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            score[x][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[x][e], p.scale, -lse[e >> 2][e & 3]));
-        const int low = places[buffer][0], high = places[buffer][kStepRows - 1];
-        if (key0 + 63 > low || (p.window && key0 <= high - p.window)) {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int key = key0 + 32 * x + (lane & 31);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int at = places[buffer][row_of_register(e, half)];
-              score[x][e] = key <= at && (!p.window || key > at - p.window) ? score[x][e] : 0.f;
-            }
+          for (int t = 0; t < D / 16; ++t) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // a matrix instruction
+            __builtin_amdgcn_sched_group_barrier(0x002, 4 * 128 / D, 0);  // vector ones
+            __builtin_amdgcn_sched_group_barrier(0x400, 2 * 128 / D, 0);  // exponentials
+            if (ends) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // a read of LDS
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
+      };
+      // the item before: its rows are read, its fetches have arrived
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < kRing; ++i) fetch(i);
+      arrived(std::integral_constant<int, kRing - 1>());
 #pragma unroll
-          for (int e = 0; e < 16; ++e) part[e & 3] += score[x][e];
-          total[x] += (part[0] + part[1]) + (part[2] + part[3]);
+      for (int t = 0; t < D / 16; ++t) read_row(0, t);
+      // (uniform) the steps whose rows see all of the wave's keys lie between others
+      const int all_begin = min(count, max(0, (all_from + kStepRows - 1) / kStepRows - from));
+      const int all_end = min(count, max(all_begin, all_upto / kStepRows - from));
+      int i = 0;
+#pragma unroll 1
+      for (; i < all_begin; ++i) some(i);
+      if (i < all_end) {
+        constexpr std::integral_constant<int, 0> kEven{};
+        constexpr std::integral_constant<int, kBlocks & 1> kOdd{};
+        f32x4 lse[2][4];
+        // nothing is left of a step before: scores of -inf, whose weights are zero
+#pragma unroll
+        for (int e = 0; e < 16; ++e) score[1][e] = -INFINITY, lse[0][e >> 2][e & 3] = 0.f;
+        mine = lse_slot(i)[lane];
+#pragma unroll 1
+        for (; i + 1 < all_end; i += 2) all(kEven, i, lse[0], lse[1]), all(kOdd, i + 1, lse[1], lse[0]);
+        if (i < all_end) {
+          all(kEven, i, lse[0], lse[1]), ++i;
+          weigh(score[(kBlocks - 1) & 1], lse[1], kBlocks - 1);
+        } else {
+          weigh(score[1], lse[0], kBlocks - 1);
         }
-        if (i + 1 < count) store_rows(buffer ^ 1);
       }
+#pragma unroll 1
+      for (; i < count; ++i) some(i);
+      const int begins = before == 0;
+      float* const part = p.partial + (2 * (int64_t)s.worker + begins) * kTile + kWave * wave;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) total[x] += other_half(total[x]);
-      const float mine = half ? total[1] : total[0];
-      const bool here = half ? held[1] : held[0];
-      if (count == tile_count) {
-        const int key = key0 + lane;
-        if (here) {
-          float* const to = weight_of(p, half ? page[1] : page[0], key, s.head);
-          *to = (key < s.context ? *to : 0.f) + mine;
+      for (int x = 0; x < kBlocks; ++x) {
+        total[x] += other_half(total[x]);
+        if (half) continue;  // (both halves hold the sum)
+        const int key = key0 + 32 * x + lane;
+        int page;
+        if (count < tile_count) {
+          part[32 * x + lane] = total[x];
+        } else if (find_key(p, table, key, length, &page)) {
+          float* const to = weight_of(p, page, key, s.head);
+          *to = (key < s.context ? *to : 0.f) + total[x];
         }
-      } else {
-        const int begins = before == 0;
-        p.partial[(2 * (int64_t)s.worker + begins) * kTile + 64 * wave + lane] = mine;
-        if (begins && threadIdx.x == 0) {
-          record->worker = s.worker, record->head = s.head, record->request = s.request, record->tile = s.tile;
-          record->others = (int)quotient(rest + s.each - 1, s.each);
-        }
+      }
+      if (count < tile_count && begins && threadIdx.x == 0) {
+        record->worker = s.worker, record->head = s.head, record->request = s.request, record->tile = s.tile;
+        record->others = (int)quotient(rest + s.each - 1, s.each);
       }
     }
     s.left -= units;
     if (s.left <= 0) break;
     next_item(p, &s, r.tiles);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outlives the workgroup
 }
 
 // Adds up the sums of an item that several workgroups share: a thread per key.
@@ -293,13 +402,25 @@ struct FewTiles {
   __device__ int64_t all() const { return fresh > 0 ? steps + 1 : 0; }  // one for its start
 };
 
-// Few rows (at most 32 of a request, decoding): a wave holds them and its keys go by, 32 at a time, straight from memory into
-// registers. Bound by memory.
+// Few rows (at most 32 of a request, decoding): a wave holds them and its keys go by, 32 at a time, through a ring of
+// four tiles in LDS, so that three are on their way. Bound by memory.
 template <int D>
 __global__ __launch_bounds__(64) void key_weights_few(WeightArgs p) {
+  constexpr int kRow = 2 * D, kChunks = D / 8, kDmaRows = 64 / kChunks, kDmas = 32 / kDmaRows, kRing = 4;
+  constexpr int kSlot = 32 * kRow + 256;  // a tile's keys, and its weights before the step (twice)
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x, half = lane >> 5;
   Span s;
   if (!find_span<FewTiles, 1>(p, &s)) return;
+  // The lane's part of eight rows of a page, of a tile's even and odd groups of them: DMA i of a group brings kDmaRows rows.
+  uint32_t at[2][8 / kDmaRows];
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int i = 0; i < 8 / kDmaRows; ++i) {
+      const int row = i * kDmaRows + lane / kChunks;
+      at[g][i] = (uint32_t)row * (uint32_t)p.slot_stride * 2 + 16 * (lane % kChunks ^ ((8 * g + row) & (kChunks - 1)));
+    }
   while (s.left > 0) {
     const FewTiles r = FewTiles::uniform(p, s.context, s.fresh);
     const int units = (int)min((int64_t)(r.steps + 1 - s.skip), s.left);
@@ -310,38 +431,55 @@ __global__ __launch_bounds__(64) void key_weights_few(WeightArgs p) {
       const int64_t start = scalar_at(p.starts, s.request);
       const int row = min(lane & 31, rows - 1), token = row / p.group, head = s.head * p.group + row - token * p.group;
       const uint16_t* const from = p.q + (start + token) * p.q_token + (int64_t)head * p.q_head + 8 * half;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the item before: its last fetches and stores
       bf16x8 q[D / 16];
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) q[t] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(from + 16 * t));
       const float mine = lane < rows ? p.lse[(start + token) * ((int64_t)p.group * p.kv_heads) + head] * kLog2E : INFINITY;
       float lse[16];
-      int32_t places[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        lse[e] = __shfl(mine, row_of_register(e, half));
-        places[e] = s.context + __shfl(token, row_of_register(e, half));
-      }
+      for (int e = 0; e < 16; ++e) lse[e] = __shfl(mine, row_of_register(e, half));
       const int low = s.context, high = s.context + s.fresh - 1;
-      const int key_first = (r.first + before) * FewTiles::kKeys;
-      struct Ahead {
-        Keys<D> k;
-        int page;
-        bool held;
-        float weight;
+      const int key_first = (r.first + before) * FewTiles::kKeys, last_page = (length - 1) >> p.page_shift;
+      // Lane l holds entry l of 64 table entries, and of the 64 behind them; no tile's pages lie in both.
+      int first_page = key_first >> p.page_shift;
+      auto entries_of = [&](int page) __attribute__((always_inline)) { return table[min(page + lane, last_page)]; };
+      int entries = entries_of(first_page), more = entries_of(first_page + 64);
+      // Starts a tile's fetches; the lane's key's page. Tiles past the item's last are fetched as that one again, so that the
+      // number of fetches in flight stays the same.
+      auto fetch = [&](int i) __attribute__((always_inline)) {
+        const int key0 = key_first + min(i, count - 1) * FewTiles::kKeys;
+        uint8_t* const to = lds + (i & (kRing - 1)) * kSlot;
+        if ((key0 >> p.page_shift) - first_page >= 64) {  // uniform
+          first_page += 64;
+          entries = more, more = entries_of(first_page + 64);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int key = key0 + 8 * g, entry = __builtin_amdgcn_readlane(entries, (key >> p.page_shift) - first_page);
+          const int64_t page = (uint32_t)entry < (uint32_t)p.num_pages ? entry : 0;
+          const uint8_t* const base = reinterpret_cast<const uint8_t*>(
+              p.k + page * p.page_stride + (int64_t)(key & ((1 << p.page_shift) - 1)) * p.slot_stride + (int64_t)s.head * p.head_stride);
+#pragma unroll
+          for (int x = 0; x < 8 / kDmaRows; ++x) dma16(base + at[g & 1][x], to + (g * 8 + x * kDmaRows) * kRow);
+        }
+        const int key = key0 + (lane & 31), entry = __shfl(entries, (key >> p.page_shift) - first_page);
+        dma4(weight_of(p, (uint32_t)entry < (uint32_t)p.num_pages ? entry : 0, key, s.head), to + 32 * kRow);
+        return entry;
       };
-      auto fetch = [&](int i, Ahead& a) __attribute__((always_inline)) {
-        const int key = key_first + i * FewTiles::kKeys + (lane & 31), at = min(key, length - 1);
-        a.held = find_key(p, table, key, length, &a.page);
-        load_keys<D>(p, a.k, a.page, at, s.head);
-        a.weight = *weight_of(p, a.page, at, s.head);
-      };
-      auto add = [&](int i, const Ahead& a) __attribute__((always_inline)) {
+      auto add = [&](int i, int entry) __attribute__((always_inline)) {
         const int key0 = key_first + i * FewTiles::kKeys, key = key0 + (lane & 31);
+        const uint8_t* const tile = lds + (i & (kRing - 1)) * kSlot;
+        bf16x8 k[D / 16];
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+          k[t] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(tile + (lane & 31) * kRow + 16 * ((2 * t + half) ^ (lane & (kChunks - 1)))));
+        const float old = *reinterpret_cast<const float*>(tile + 32 * kRow + 4 * lane);
         f32x16 score;
 #pragma unroll
         for (int e = 0; e < 16; ++e) score[e] = 0.f;
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t) score = __builtin_amdgcn_mfma_f32_32x32x16_bf16(q[t], a.k.k[t], score, 0, 0, 0);
+        for (int t = 0; t < D / 16; ++t) score = __builtin_amdgcn_mfma_f32_32x32x16_bf16(q[t], k[t], score, 0, 0, 0);
         const bool masked = key0 + FewTiles::kKeys - 1 > low || (p.window && key0 <= high - p.window);
         float sum = 0.f;
 #pragma unroll
@@ -350,36 +488,53 @@ __global__ __launch_bounds__(64) void key_weights_few(WeightArgs p) {
 #pragma unroll
             for (int j = e; j < e + 4; ++j) {
               float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score[j], p.scale, -lse[j]));
-              if (masked) w = key <= places[j] && (!p.window || key > places[j] - p.window) ? w : 0.f;
+              if (masked) {
+                const int place = s.context + __shfl(token, row_of_register(j, half));
+                w = key <= place && (!p.window || key > place - p.window) ? w : 0.f;
+              }
               sum += w;
             }
           }
         sum += other_half(sum);
-        if (!half && a.held) *weight_of(p, a.page, key, s.head) = (key < s.context ? a.weight : 0.f) + sum;
+        if (!half && key < length && (uint32_t)entry < (uint32_t)p.num_pages)
+          *weight_of(p, entry, key, s.head) = (key < s.context ? old : 0.f) + sum;
       };
-      Ahead a, b;
-      fetch(0, a);
-      for (int i = 0; i < count; i += 2) {
-        if (i + 1 < count) fetch(i + 1, b);
-        add(i, a);
-        if (i + 2 < count) fetch(i + 2, a);
-        if (i + 1 < count) add(i + 1, b);
+      int entry[kRing];  // of this tile and those on their way
+#pragma unroll
+      for (int i = 0; i < kRing - 1; ++i) entry[i] = fetch(i);
+      for (int i = 0; i < count; ++i) {
+        // all but the fetches of the two tiles behind this one
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"((kRing - 2) * (kDmas + 1)) : "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        entry[kRing - 1] = fetch(i + kRing - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        add(i, entry[0]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x + 1 < kRing; ++x) entry[x] = entry[x + 1];
       }
     }
     s.left -= units;
     if (s.left <= 0) break;
     next_item(p, &s, r.tiles);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outlives the wave
 }
 
-// Workgroups of a launch, a multiple of the 8 XCDs: as many as a CU holds.
-int workgroups(int cus, bool few) { return ((few ? 8 : 2) * cus + 7) / 8 * 8; }
+// Workgroups of a launch, a multiple of the 8 XCDs. Of few rows as many as a CU holds, by their LDS (33 KB at head_dim
+// 128, of which five would fit but not even out: 222 us for four contexts of 131,000 tokens, with eight 235). Of many rows
+// twice as many: a CU serves the workgroup that came first before the other, so that the last ones run alone
+// (2048 rows of 64 heads on 16384 keys: 672 us with as many as fit, 604 with twice as many, 605 with four times).
+int few_workgroups(int cus, int head_dim) { return ((head_dim == 128 ? 4 : 8) * cus + 7) / 8 * 8; }
+int many_workgroups(int cus) { return (4 * cus + 7) / 8 * 8; }
 
-int64_t workspace_of(int cus) { return workgroups(cus, false) * (int64_t)(sizeof(WeightRecord) + 2 * 4 * kTile); }
+int64_t workspace_of(int cus) { return many_workgroups(cus) * (int64_t)(sizeof(WeightRecord) + 2 * 4 * kTile); }
 
 template <int D>
 int launch_weights(const WeightArgs& p, bool few, unsigned blocks, hipStream_t stream) {
-  hipLaunchKernelGGL(few ? key_weights_few<D> : key_weights_many<D>, dim3(blocks), dim3(few ? 64 : 256), 0, stream, p);
+  auto many = kStepRows % p.group == 0 ? key_weights_many<D, true> : key_weights_many<D, false>;
+  hipLaunchKernelGGL(few ? key_weights_few<D> : many, dim3(blocks), dim3(few ? 64 : 256),
+                     few ? 4 * (32 * 2 * D + 256) : 4 * (kStepRows * 2 * D + 4 * 256), stream, p);
   if (int rc = check_launch()) return rc;
   if (few) return SMX_OK;
   hipLaunchKernelGGL(key_weights_join, dim3(blocks), dim3(kTile), 0, stream, p);
@@ -417,6 +572,11 @@ int smx_paged_key_weights(const smx_paged_cache* cache, const smx_paged_step* st
     return fail(SMX_ERR_INVALID, "%d query heads are not 1 to 128 for each of %d key/value heads", q->heads, cache->kv_heads);
   if ((uintptr_t)q->data % 16 || q->token_stride % 8 || q->head_stride % 8 || q->token_stride < 0 || q->head_stride < 0)
     return fail(SMX_ERR_INVALID, "head rows must be 16-byte aligned");
+  // (offsets within a step's rows are of 32 bits)
+  const int64_t group = q->heads / cache->kv_heads, tokens = kStepRows / group + 2;
+  if (q->token_stride > INT32_MAX / tokens || q->head_stride > INT32_MAX / group ||
+      tokens * q->token_stride + group * q->head_stride + cache->head_dim > INT32_MAX)
+    return fail(SMX_ERR_UNSUPPORTED, "the query heads of %d rows must lie within 2^32 bytes", kStepRows);
   if ((uintptr_t)lse % 4 || (uintptr_t)key_weights % 16) return fail(SMX_ERR_INVALID, "misaligned lse or key_weights");
   const Runs to{key_weights, 2 * (int64_t)cache->num_pages * cache->kv_heads * cache->page_size, {{1, 0}, {1, 0}, {1, 0}}};
   const Runs sums{lse, 2 * (int64_t)step->tokens * q->heads, {{1, 0}, {1, 0}, {1, 0}}};
@@ -440,9 +600,10 @@ int smx_paged_key_weights(const smx_paged_cache* cache, const smx_paged_step* st
   p.page_shift = __builtin_ctz(cache->page_size), p.num_pages = cache->num_pages;
   p.window = window < SMX_PAGED_MAX_CONTEXT ? window : 0;  // wider than any request: none
   const bool few = (int64_t)max(1, step->max_new) * p.group <= kStepRows;
-  const int blocks = workgroups(cus, few);
+  const int blocks = few ? few_workgroups(cus, cache->head_dim) : many_workgroups(cus);
   p.min_span = few ? 2 : kItem + 4;
   p.scale = scale * kLog2E;
+  p.per_group = (65535 + p.group) / p.group;
   p.per_workgroup = 1. / blocks;
   p.records = (WeightRecord*)workspace;
   p.partial = (float*)((char*)workspace + blocks * sizeof(WeightRecord));

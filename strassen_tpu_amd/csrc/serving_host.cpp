@@ -465,7 +465,13 @@ PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t) {
     const smx_paged_cache cache = cache_of(a[1], a[1], plan);  // (values are not read)
     const c10::DeviceGuard guard(plan.device);
     Tensor hold;
-    const smx_heads q = heads_of(a[0], "q", plan, -1, cache.head_dim, &hold);
+    smx_heads q = heads_of(a[0], "q", plan, -1, cache.head_dim, &hold);
+    // rows that are too far from each other for the kernel's offsets (heads of some 10 million tokens outside the tokens) are
+    // laid out too
+    if (q.token_stride > 1 << 25 || q.head_stride > (1 << 29) / std::max(1, q.heads / std::max(1, cache.kv_heads))) {
+      hold = tensor(a[0], "q").clone(at::MemoryFormat::Contiguous);
+      q = smx_heads{hold.mutable_data_ptr(), q.heads * (int64_t)cache.head_dim, cache.head_dim, q.heads};
+    }
     const Tensor& weights = on_device(a[2], "key_weights", plan.device);
     float* const to = dense_floats(weights, "key_weights", {cache.num_pages, cache.kv_heads, cache.page_size});
     const float* const lse = dense_floats(on_device(a[4], "lse", plan.device), "lse", {plan.step.tokens, q.heads});

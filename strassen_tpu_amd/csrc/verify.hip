@@ -27,7 +27,7 @@ struct VerifyArgs {
   int32_t requests, count, vocab, slice, slices, flags;
 };
 
-constexpr int kVerifyThreads = 256, kSlice = 4096, kMostSlices = 1024;
+constexpr int kVerifyThreads = 256;
 
 // Probabilities that are no positive finite numbers count as zero.
 __device__ __forceinline__ float probability(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
@@ -61,38 +61,78 @@ __device__ int accepted_of(const VerifyArgs& p, int64_t start, int drafts) {
   return drafts;
 }
 
-// What a request draws from: value(i) of token i, and p(i).
+// Four values of a row, of any alignment.
+typedef f32x4 f32x4_loose __attribute__((aligned(4)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+typedef u16x4 u16x4_loose __attribute__((aligned(2)));
+
+// What a request draws from: max(p - q, 0) of the row whose draft was refused, or p.
 template <bool kBf16>
 struct Row {
   const void *target, *draft;
   int64_t at, draft_at;
   int64_t left_out;  // a token whose value is zero: a refused one that had no distribution
-  bool whole;
 
   __device__ Row(const VerifyArgs& p, int64_t start, int drafts, int accepted)
       : target(p.target), draft(accepted < drafts ? p.draft : nullptr), at((start + accepted) * p.target_row),
         draft_at((start + accepted) * p.draft_row), left_out(-1) {
     if (accepted < drafts && !p.draft) left_out = token_at(p, start + accepted + 1);
   }
-  __device__ double both(int i, double* p) const {
-    const float mine = value_at<kBf16>(target, at + i);
-    *p = mine;
-    if (draft) return max((double)mine - (double)value_at<kBf16>(draft, draft_at + i), 0.);
-    return i == left_out ? 0. : (double)mine;
+  // Values i .. i + 3 of the row at `from`, zeros from `end` on.
+  __device__ __forceinline__ static f32x4 four(const void* p, int64_t from, int i, int end) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (i + 4 <= end) {
+      if constexpr (kBf16) {
+        const u16x4 v = *reinterpret_cast<const u16x4_loose*>((const uint16_t*)p + from + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = bf16_to_f32(v[j]);
+      } else {
+        x = *reinterpret_cast<const f32x4_loose*>((const float*)p + from + i);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j < end) x[j] = kBf16 ? bf16_to_f32(((const uint16_t*)p)[from + i + j]) : ((const float*)p)[from + i + j];
+    }
+    return x;
   }
-  // Of a row whose max(p - q, 0) is all zero, p itself.
-  __device__ double value(int i, bool plain) const {
-    double p;
-    const double rest = both(i, &p);
-    return plain ? p : rest;
+  struct Four {
+    f32x4 p, q;
+  };
+  __device__ __forceinline__ Four load(int i, int end) const {
+    Four f;
+    f.p = four(target, at, i, end);
+    f.q = draft ? four(draft, draft_at, i, end) : f32x4{0.f, 0.f, 0.f, 0.f};
+    return f;
+  }
+  // Value j of those from i on; `plain`: p itself, for a row whose max(p - q, 0) is all zero.
+  __device__ __forceinline__ double value(const Four& f, int i, int j, bool plain) const {
+    const double p = probability(f.p[j]);
+    if (plain) return p;
+    if (draft) return max(p - (double)probability(f.q[j]), 0.);
+    return i + j == left_out ? 0. : p;
   }
 };
 
+// Sum over a wave's lanes, in every lane.
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
   return x;
 }
+
+// Inclusive sum over a wave's lanes.
+__device__ __forceinline__ double lane_scan(double x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+constexpr int kWaves = kVerifyThreads / 64, kRun = 4 * kVerifyThreads;  // tokens that the workgroup loads at once
 
 template <bool kBf16>
 __global__ __launch_bounds__(kVerifyThreads) void verify_sums(VerifyArgs p) {
@@ -104,140 +144,118 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sums(VerifyArgs p) {
   const Row<kBf16> row(p, start, fresh - 1, accepted);
   const int from = blockIdx.x * p.slice, to = min(p.vocab, from + p.slice);
   double rest = 0., whole = 0.;
-#pragma unroll 8
-  for (int i = from + (int)threadIdx.x; i < to; i += kVerifyThreads) {
-    double mine;
-    rest += row.both(i, &mine);
-    whole += mine;
+#pragma unroll 4
+  for (int i = from + 4 * (int)threadIdx.x; i < to; i += kRun) {
+    const auto f = row.load(i, to);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) rest += row.value(f, i, j, false), whole += row.value(f, i, j, true);
   }
-  __shared__ double parts[2][kVerifyThreads / 64];
+  __shared__ double parts[2][kWaves];
   rest = wave_sum(rest), whole = wave_sum(whole);
   if ((threadIdx.x & 63) == 0) parts[0][threadIdx.x >> 6] = rest, parts[1][threadIdx.x >> 6] = whole;
   __syncthreads();
   if (threadIdx.x < 2) {
     double sum = 0.;
-    for (int w = 0; w < kVerifyThreads / 64; ++w) sum += parts[threadIdx.x][w];
+    for (int w = 0; w < kWaves; ++w) sum += parts[threadIdx.x][w];
     p.sums[((int64_t)request * p.slices + blockIdx.x) * 2 + threadIdx.x] = sum;
   }
 }
 
-// Inclusive sum over the workgroup's threads.
-__device__ double block_scan(double x, double* waves) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  __syncthreads();
-  if (lane == 63) waves[wave] = x;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) x += waves[w];
-  return x;
+__device__ __forceinline__ void emit(const VerifyArgs& p, int64_t row, int64_t token) {
+  if (p.flags & SMX_VERIFY_TOKENS_I64) ((int64_t*)p.out)[row] = token; else ((int32_t*)p.out)[row] = (int32_t)token;
 }
 
 template <bool kBf16>
 __global__ __launch_bounds__(kVerifyThreads) void verify_draw(VerifyArgs p) {
-  const int request = blockIdx.x, fresh = p.rows[request];
+  const int request = blockIdx.x, fresh = p.rows[request], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // rows of no request
   for (int64_t r = (int64_t)request * kVerifyThreads + threadIdx.x; r < p.count; r += (int64_t)gridDim.x * kVerifyThreads)
-    if (p.positions[r] < 0) {
-      if (p.flags & SMX_VERIFY_TOKENS_I64) ((int64_t*)p.out)[r] = -1; else ((int32_t*)p.out)[r] = -1;
-    }
+    if (p.positions[r] < 0) emit(p, r, -1);
   if (fresh <= 0) {
     if (threadIdx.x == 0) p.counts[request] = 0;
     return;
   }
-  __shared__ double waves[kVerifyThreads / 64], base;
-  __shared__ int chosen, token, last;
-  if (threadIdx.x == 0) chosen = token = INT32_MAX, last = -1;
   const int64_t start = p.starts[request];
   const int accepted = p.accepted[request];
+  const Row<kBf16> row(p, start, fresh - 1, accepted);
+  // Every wave finds the slice: a lane each (at most 64).
   const double* const sums = p.sums + (int64_t)request * p.slices * 2;
-  // a thread's slices, one behind the other
-  constexpr int kEach = kMostSlices / kVerifyThreads;
-  double mine[2][kEach], total[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    double sum = 0.;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int s = (int)threadIdx.x * kEach + i;
-      mine[k][i] = s < p.slices ? sums[2 * s + k] : 0.;
-      sum += mine[k][i];
-    }
-    total[k] = sum;
+  const double mine_rest = lane < p.slices ? sums[2 * lane] : 0., mine_whole = lane < p.slices ? sums[2 * lane + 1] : 0.;
+  const bool plain = !__any(mine_rest > 0.);
+  const double mine = plain ? mine_whole : mine_rest, upto = lane_scan(mine);
+  const double goal = (double)p.sample[request] * __shfl(upto, 63);
+  // the first whose running sum passes the goal, or (by rounding, or a number that is not below 1) the last one that
+  // holds anything
+  const uint64_t any = __ballot(mine > 0.), over = __ballot(mine > 0. && upto > goal);
+  if (!any) {
+    for (int i = threadIdx.x; i < fresh; i += kVerifyThreads) emit(p, start + i, i < accepted ? token_at(p, start + i + 1) : -1);
+    if (threadIdx.x == 0) p.counts[request] = accepted + 1;
+    return;
   }
-  const double upto_rest = block_scan(total[0], waves), upto_whole = block_scan(total[1], waves);
-  __shared__ double all[2];
-  if (threadIdx.x == kVerifyThreads - 1) all[0] = upto_rest, all[1] = upto_whole;
-  __syncthreads();
-  const bool plain = !(all[0] > 0.);
-  const double goal = (double)p.sample[request] * (plain ? all[1] : all[0]);
-  double before = (plain ? upto_whole : upto_rest) - (plain ? total[1] : total[0]);
-  // the first slice whose running sum passes the goal, or (by rounding, or a number that is not below 1)
-  // the last one that holds anything
+  const int slice = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
+  double base = __shfl(upto - mine, slice);
+  const int from = slice * p.slice, to = min(p.vocab, from + p.slice);
+
+  __shared__ double waves[2][kWaves];
+  __shared__ int first_of[kWaves], last_of[kWaves];
+  int hit = -1, most = -1, buffer = 0;  // the thread's first token past the goal, and its last of any probability
+  // A run of the slice after another, four tokens a thread; the next one's are on their way.
+  auto f = row.load(from + 4 * (int)threadIdx.x, to);
+  for (int run = from; run < to; run += kRun, buffer ^= 1) {
+    const int i = run + 4 * (int)threadIdx.x;
+    const auto now = f;
+    f = row.load(i + kRun, to);
+    double value[4], sum = 0.;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int s = (int)threadIdx.x * kEach + i;
-    const double part = plain ? mine[1][i] : mine[0][i];
-    if (part > 0.) {
-      if (before + part > goal) atomicMin(&chosen, s);
-      atomicMax(&last, s);
+    for (int j = 0; j < 4; ++j) {
+      value[j] = row.value(now, i, j, plain), sum += value[j];
+      if (value[j] > 0.) most = i + j;
     }
-    before += part;
-  }
-  __syncthreads();
-  const bool beyond = chosen == INT32_MAX;
-  const int slice = beyond ? last : chosen;
-  if (slice >= 0) {
-    if (slice / kEach == (int)threadIdx.x) {
-      double b = (plain ? upto_whole : upto_rest) - (plain ? total[1] : total[0]);
-#pragma unroll
-      for (int i = 0; i < kEach; ++i)
-        if (i < slice % kEach) b += plain ? mine[1][i] : mine[0][i];
-      base = b;
-    }
+    const double scanned = lane_scan(sum);
+    if (lane == 63) waves[buffer][wave] = scanned;
     __syncthreads();
-    if (threadIdx.x == 0) last = -1;
-    const Row<kBf16> row(p, start, fresh - 1, accepted);
-    const int from = slice * p.slice, to = min(p.vocab, from + p.slice), each = p.slice / kVerifyThreads;
-    const int first = from + (int)threadIdx.x * each, end = min(to, first + each);
-    double sum = 0.;
-#pragma unroll 4
-    for (int i = first; i < end; ++i) sum += row.value(i, plain);
-    const double upto = base + block_scan(sum, waves);
-    double running = upto - sum;
-    // a thread's tokens: the first whose running sum passes the goal, and the last with any
-    if (sum > 0.) {
-      int hit = INT32_MAX, most = -1;
-      for (int i = first; i < end; ++i) {
-        const double v = row.value(i, plain);
-        running += v;
-        if (v > 0.) {
-          most = i;
-          if (running > goal && hit == INT32_MAX) hit = i;
-        }
+    double running = base + scanned - sum;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) running += waves[buffer][w];
+      base += waves[buffer][w];
+    }
+    if (over && base > goal) {  // uniform: here
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        running += value[j];
+        if (value[j] > 0. && running > goal && hit < 0) hit = i + j;
       }
-      if (!beyond && hit != INT32_MAX) atomicMin(&token, hit);
-      atomicMax(&last, most);
+      break;
     }
-    __syncthreads();
   }
-  const int drawn = slice < 0 ? -1 : token != INT32_MAX ? token : last;
-  for (int i = threadIdx.x; i < fresh; i += kVerifyThreads) {
-    const int64_t value = i < accepted ? token_at(p, start + i + 1) : i == accepted ? drawn : -1;
-    if (p.flags & SMX_VERIFY_TOKENS_I64) ((int64_t*)p.out)[start + i] = value; else ((int32_t*)p.out)[start + i] = (int32_t)value;
+  // The first token past the goal; where sums in another order leave none, the last of any probability.
+  const uint64_t hits = __ballot(hit >= 0);  // (of one run, whose tokens are in the threads' order)
+  const int wave_hit = hits ? __shfl(hit, __builtin_ctzll(hits)) : -1;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d));
+  if (lane == 0) first_of[wave] = wave_hit, last_of[wave] = most;
+  __syncthreads();
+  int drawn = -1, last = -1;
+  for (int w = 0; w < kWaves; ++w) {
+    if (drawn < 0) drawn = first_of[w];
+    last = max(last, last_of[w]);
   }
+  if (drawn < 0) drawn = last;
+  for (int i = threadIdx.x; i < fresh; i += kVerifyThreads)
+    emit(p, start + i, i < accepted ? token_at(p, start + i + 1) : i == accepted ? drawn : -1);
   if (threadIdx.x == 0) p.counts[request] = accepted + 1;
 }
 
-// Tokens of a slice, a multiple of the workgroup's threads.
-int slice_of(int vocab) {
-  const int64_t least = ((int64_t)vocab + kMostSlices - 1) / kMostSlices;
-  return (int)max((int64_t)kSlice, (least + kVerifyThreads - 1) / kVerifyThreads * kVerifyThreads);
+// Tokens of a slice, a multiple of the workgroup's loads: at most 64 slices, of 2048 tokens at least, and no more
+// than fill the chip with workgroups.
+int slice_of(int vocab, int requests) {
+  const int64_t slices = max(1, min(64, 2048 / requests)), least = ((int64_t)vocab + slices - 1) / slices;
+  return (int)max((int64_t)2048, (least + kRun - 1) / kRun * kRun);
 }
-int slices_of(int vocab) { return (int)(((int64_t)vocab + slice_of(vocab) - 1) / slice_of(vocab)); }
+int slices_of(int vocab, int requests) {
+  const int slice = slice_of(vocab, requests);
+  return (int)(((int64_t)vocab + slice - 1) / slice);
+}
 
 }  // namespace
 }  // namespace smx
@@ -252,7 +270,7 @@ int smx_verify_workspace_bytes(int32_t requests, int32_t vocab, int64_t* bytes) 
   if (requests <= 0 || requests > SMX_PAGED_MAX_REQUESTS || vocab <= 0 || vocab > SMX_VERIFY_MAX_VOCAB)
     return fail(SMX_ERR_INVALID, "1 to %d requests and 1 to %d tokens in the vocabulary (requests=%d, vocab=%d)",
                 SMX_PAGED_MAX_REQUESTS, SMX_VERIFY_MAX_VOCAB, requests, vocab);
-  *bytes = (int64_t)requests * (slices_of(vocab) * 16 + 8);
+  *bytes = (int64_t)requests * (slices_of(vocab, requests) * 16 + 8);
   return SMX_OK;
 }
 
@@ -279,7 +297,7 @@ int smx_verify_drafts(const smx_paged_step* step, int32_t vocab, const void* tar
   p.target = target, p.draft = draft, p.target_row = target_row, p.draft_row = draft_row, p.tokens = tokens;
   p.starts = step->starts, p.rows = step->rows, p.positions = step->positions, p.accept = accept, p.sample = sample;
   p.out = out, p.counts = counts, p.requests = step->requests, p.count = step->tokens, p.vocab = vocab, p.flags = flags;
-  p.slice = slice_of(vocab), p.slices = slices_of(vocab);
+  p.slice = slice_of(vocab, p.requests), p.slices = slices_of(vocab, p.requests);
   p.sums = (double*)workspace;
   p.accepted = (int32_t*)(p.sums + 2 * (int64_t)p.requests * p.slices);
   const bool bf16 = flags & SMX_VERIFY_BF16;
