@@ -8,7 +8,7 @@
 // head moves 24,800.
 //
 // evict_select (a workgroup per head and request) finds the need-th largest weight: weights as integers in their order,
-// a histogram over 2048 equal parts of their range, the part that holds it, and so on until its keys fit in LDS,
+// a histogram of their leading 11 bits, the part that holds it, and so on until its keys fit in LDS,
 // where they are compared with each other. evict_move then moves the rows.
 #include "launch.hpp"
 
@@ -33,7 +33,7 @@ struct Found {
   int32_t count, early, recent, from, to, unused[3];
 };
 
-constexpr int kSelectThreads = 1024, kSelectWaves = 16, kBins = 2048, kNear = 512, kQuads = 8;
+constexpr int kBins = 2048, kNear = 256, kQuads = 8;
 
 // Weights in the order of their values; NaN above everything, -0 as 0.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -42,186 +42,221 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  return x;
+// x of the lanes that kControl names, in the rows of 16 lanes that kRows names; zero where there are none.
+template <int kControl, int kRows>
+__device__ __forceinline__ int moved(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, kControl, kRows, 15, false);
 }
 
-// Inclusive sum over a wave's lanes.
+// Inclusive sum over a wave's lanes: within rows of 16 lanes, then a row's last value to the next row, and the
+// lower half's to the upper.
 __device__ __forceinline__ int lane_scan(int x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+  x += moved<0x111, 15>(x);
+  x += moved<0x112, 15>(x);
+  x += moved<0x114, 15>(x);
+  x += moved<0x118, 15>(x);
+  x += moved<0x142, 10>(x);
+  x += moved<0x143, 12>(x);
   return x;
 }
 
-__global__ __launch_bounds__(kSelectThreads) void evict_select(EvictArgs p) {
+// kThreads * 4 * kQuads weights are held in registers, more are read once for each look at them.
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void evict_select(EvictArgs p) {
+  constexpr int kWaves = kThreads / 64;
   const int head = blockIdx.x, request = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Found* const found = p.found + (int64_t)request * p.kv_heads + head;
-  __shared__ int bins[kBins], waves[kSelectWaves][8], bad, near_count;
-  __shared__ uint32_t near[kNear], low_key, high_key, edge_key;
-  __shared__ int edge_ties, early, picked[2];
+  __shared__ int bins[kBins], scans[kWaves], counts[kWaves][4], bad, near_count, early, picked[3];
+  __shared__ __attribute__((aligned(16))) uint32_t near[kNear];
+  __shared__ uint32_t edge_key, lows[kWaves], highs[kWaves];
+  __shared__ int edge_ties, near_at[kNear];
   const int32_t n = p.context[request], given = p.keep_lens ? p.keep_lens[request] : p.keep;
   const int32_t* const table = p.tables + request * p.table_stride;
   const int32_t mask = (1 << p.page_shift) - 1;
-  if (threadIdx.x == 0) bad = near_count = early = 0, low_key = ~0u, high_key = 0;
+  if (n <= given || n > p.max_context || given < 0) {  // uniform
+    if (threadIdx.x == 0) {
+      *found = Found{};
+      if (head == 0) p.lens[request] = n;
+    }
+    return;
+  }
+  if (threadIdx.x == 0) bad = near_count = early = 0;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) bins[i] = 0;
+  if (threadIdx.x < kNear) near[threadIdx.x] = 0;  // below every key
+  const int recent = min(p.recent, given), need = given - recent, m = n - recent;
+
+  // A wave's indices lie one behind the other, four to a lane, in batches of kQuads times 256.
+  const int each = (m + kWaves * 256 - 1) / (kWaves * 256), begin = wave * each * 256;
+  const bool held = each <= kQuads;
+  uint32_t keys[kQuads][4];
+  bool missing = false;
+  auto load = [&](int first) __attribute__((always_inline)) {
+    f32x4 w[kQuads];
+    int entry[kQuads];
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const int at = begin + (first + i) * 256 + 4 * lane;
+      entry[i] = first + i < each && at < m ? table[at >> p.page_shift] : 0;
+      missing |= (uint32_t)entry[i] >= (uint32_t)p.num_pages;
+      if ((uint32_t)entry[i] >= (uint32_t)p.num_pages) entry[i] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const int at = begin + (first + i) * 256 + 4 * lane;
+      if (first + i < each && at < m)
+        w[i] = *reinterpret_cast<const f32x4*>(p.weights + (((int64_t)entry[i] * p.kv_heads + head) << p.page_shift) + (at & mask));
+    }
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) keys[i][j] = order_of(w[i][j]);
+  };
+  // f(four keys, index of the first) over the wave's indices, in their order; f is called by all lanes
+  auto over = [&](auto f) __attribute__((always_inline)) {
+    for (int first = 0; first < each; first += kQuads) {
+      if (!held) load(first);
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i)
+        if (first + i < each) f(keys[i], begin + (first + i) * 256 + 4 * lane);
+    }
+  };
+
+  // The range of the weights (of the first batch, where they are more): parts of equal size of the values that
+  // are there hold few weights each, and the histogram's additions meet rarely.
+  load(0);
+  uint32_t low = ~0u, high = 0;
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i < each && begin + i * 256 + 4 * lane + j < m) low = min(low, keys[i][j]), high = max(high, keys[i][j]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) low = min(low, (uint32_t)__shfl_xor((int)low, d)), high = max(high, (uint32_t)__shfl_xor((int)high, d));
+  if (lane == 0) lows[wave] = low, highs[wave] = high;
+  // every page of the request has to be there, the recent tokens' too
+  for (int i = (m >> p.page_shift) + (int)threadIdx.x; i <= (n - 1) >> p.page_shift; i += kThreads)
+    missing |= (uint32_t)table[i] >= (uint32_t)p.num_pages;
   __syncthreads();
-  bool whole = n <= given || n > p.max_context || given < 0;
-  if (!whole)  // every page of the request has to be there (uniform bounds)
-    for (int i = threadIdx.x; i <= (n - 1) >> p.page_shift; i += kSelectThreads)
-      if ((uint32_t)table[i] >= (uint32_t)p.num_pages) bad = 1;
+  for (int w = 0; w < kWaves; ++w) low = min(low, lows[w]), high = max(high, highs[w]);
+
+  // The need-th largest lies between `least` and `most`, the `ties`-th largest of the keys there. (Without need nothing
+  // survives: none of the largest keys.)
+  uint32_t least = ~0u, most = ~0u;
+  int ties = 0;
+  if (need > 0) {
+    // Keys below `low` count to the first part of the histogram, those above `high` to the last.
+    int wanted = need;
+    least = 0;
+    for (;;) {
+      const int shift = max(0, 32 - (high > low ? (int)__builtin_clz(high - low) : 32) - 11);
+      over([&](const uint32_t (&key)[4], int at) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (at + j < m && key[j] >= least && key[j] <= most)
+            atomicAdd(&bins[key[j] <= low ? 0 : min((key[j] - low) >> shift, (uint32_t)kBins - 1)], 1);
+      });
+      __syncthreads();
+      // The part that holds it: sums from the highest one down, kEach parts a thread.
+      constexpr int kEach = kBins / kThreads;
+      const int top = kBins - 1 - (int)threadIdx.x * kEach;
+      int own[kEach], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) own[i] = bins[top - i], sum += own[i];
+      const int all = sum;
+      sum = lane_scan(sum);
+      if (lane == 63) scans[wave] = sum;
+      __syncthreads();
+      for (int w = 0; w < wave; ++w) sum += scans[w];
+      int above = sum - all;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (above < wanted && wanted <= above + own[i]) picked[0] = top - i, picked[1] = wanted - above, picked[2] = own[i];
+        above += own[i];
+        bins[top - i] = 0;
+      }
+      __syncthreads();
+      const int part = picked[0], count = picked[2];
+      wanted = picked[1];
+      const uint64_t first = low + ((uint64_t)part << shift);
+      if (part) least = (uint32_t)first;
+      if (part < kBins - 1) most = (uint32_t)min((uint64_t)most, first + ((uint64_t)1 << shift) - 1);
+      low = least, high = most;
+      if (least == most || count <= kNear) break;  // else another look, at this part alone
+    }
+    ties = wanted;
+  }
+  if (missing) bad = 1;
+
+  // Places to fill and survivors behind them, in index order: a wave counts its own first. Keys of the part found are
+  // compared with each other, unless they are equal.
+  const bool apart = least < most;
+  int count[4] = {0, 0, 0, 0};  // below need: of keys below the part, in it; behind: above it, in it
+  over([&](const uint32_t (&key)[4], int at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool inside = at + j < m, front = at + j < need, in = inside && key[j] >= least && key[j] <= most;
+      count[0] += inside && front && key[j] < least, count[1] += in && front;
+      count[2] += inside && !front && key[j] > most, count[3] += in && !front;
+      if (in && apart) {
+        const int place = atomicAdd(&near_count, 1);
+        if (place < kNear) near[place] = key[j], near_at[place] = at + j;  // (always, while nobody changes the weights)
+      }
+    }
+  });
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int sum = lane_scan(count[c]);
+    if (lane == 63) counts[wave][c] = apart && (c & 1) ? 0 : sum;
+  }
   __syncthreads();
-  whole = whole || bad;
-  if (head == 0 && threadIdx.x == 0) p.lens[request] = whole ? n : given;
-  if (whole) {
+  if (head == 0 && threadIdx.x == 0) p.lens[request] = bad ? n : given;
+  if (bad) {  // uniform
     if (threadIdx.x == 0) *found = Found{};
     return;
   }
-  const int recent = min(p.recent, given), need = given - recent, m = n - recent;
-
-  // A wave's indices lie one behind the other, four to a lane.
-  const int each = (m + kSelectWaves * 256 - 1) / (kSelectWaves * 256), begin = wave * each * 256;
-  const bool held = each <= kQuads;  // all weights stay in registers
-  uint32_t keys[kQuads][4];
-  // the slot of index i (of four from a multiple of 4 on: the same page)
-  auto slot_of = [&](int i) __attribute__((always_inline)) { return (table[i >> p.page_shift] << p.page_shift) + (i & mask); };
-  auto load = [&](int i, uint32_t (&key)[4]) __attribute__((always_inline)) {
-    const int at = begin + i * 256 + 4 * lane;
-    f32x4 w = {0.f, 0.f, 0.f, 0.f};
-    if (at < m)
-      w = *reinterpret_cast<const f32x4*>(p.weights + (((int64_t)table[at >> p.page_shift] * p.kv_heads + head) << p.page_shift) +
-                                          (at & mask));
+  // Survivors: keys above the edge, and the first `ties` of those equal to it.
+  uint32_t edge = most;
+  if (apart) {
+    const int near_all = min(near_count, kNear);
+    const uint32_t mine = (int)threadIdx.x < near_all ? near[threadIdx.x] : 0;
+    if (mine) {
+      int larger = 0, equal = 0;
+      for (int x = 0; x < near_all; x += 4) {
+        const u32x4 other = *reinterpret_cast<const u32x4*>(near + x);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) key[j] = order_of(w[j]);
-  };
-  if (held) {
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i)
-      if (i < each) load(i, keys[i]);
-  }
-  // f(key, index) of every weight
-  auto over = [&](auto f) __attribute__((always_inline)) {
-    if (held) {
-#pragma unroll
-      for (int i = 0; i < kQuads; ++i)
-        if (i < each)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int at = begin + i * 256 + 4 * lane + j;
-            if (at < m) f(keys[i][j], at);
-          }
-    } else {
-      for (int i = 0; i < each; ++i) {
-        uint32_t key[4];
-        load(i, key);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int at = begin + i * 256 + 4 * lane + j;
-          if (at < m) f(key[j], at);
-        }
+        for (int j = 0; j < 4; ++j) larger += other[j] > mine, equal += other[j] == mine;
       }
+      if (larger < ties && ties <= larger + equal) edge_key = mine, edge_ties = ties - larger;
     }
-  };
-
-  uint32_t edge = ~0u;  // survivors: keys above it, and `ties` of those equal to it
-  int ties = 0;
-  if (need > 0) {
-    uint32_t low = ~0u, high = 0;
-    over([&](uint32_t key, int) { low = min(low, key), high = max(high, key); });
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) low = min(low, (uint32_t)__shfl_xor((int)low, d)), high = max(high, (uint32_t)__shfl_xor((int)high, d));
-    if (lane == 0) atomicMin(&low_key, low), atomicMax(&high_key, high);
     __syncthreads();
-    low = low_key, high = high_key;
-    int wanted = need;
-    for (;;) {  // the range shrinks by a factor of 2048 each time, or the loop ends
-      const uint32_t range = high - low;
-      if (!range) {
-        edge = low, ties = wanted;
-        break;
-      }
-      const int shift = max(0, 32 - (int)__builtin_clz(range) - 11);
-      for (int i = threadIdx.x; i < kBins; i += kSelectThreads) bins[i] = 0;
-      __syncthreads();
-      over([&](uint32_t key, int) {
-        if (key >= low && key <= high) atomicAdd(&bins[(key - low) >> shift], 1);
-      });
-      __syncthreads();
-      // sums from the highest part down: thread t holds parts 2 t' and 2 t' + 1, t' = 1023 - t
-      const int pair = kSelectThreads - 1 - (int)threadIdx.x, upper = bins[2 * pair + 1], lower = bins[2 * pair];
-      int sum = lane_scan(upper + lower);
-      if (lane == 63) waves[wave][0] = sum;
-      __syncthreads();
-      for (int w = 0; w < wave; ++w) sum += waves[w][0];
-      const int above = sum - upper - lower;
-      if (above < wanted && wanted <= sum) {
-        const bool first = wanted <= above + upper;
-        picked[0] = 2 * pair + first, picked[1] = wanted - above - (first ? 0 : upper);
-      }
-      __syncthreads();
-      const int part = picked[0], count = bins[part];
-      wanted = picked[1];
-      low += (uint32_t)part << shift;
-      high = low + min(high - low, (1u << shift) - 1);
-      __syncthreads();
-      if (!shift) {
-        edge = low, ties = wanted;
-        break;
-      }
-      if (count > kNear) continue;
-      over([&](uint32_t key, int) {
-        if (key >= low && key <= high) near[atomicAdd(&near_count, 1)] = key;
-      });
-      __syncthreads();
-      if ((int)threadIdx.x < count) {
-        const uint32_t mine = near[threadIdx.x];
-        int larger = 0, equal = 0;
-        for (int i = 0; i < count; ++i) larger += near[i] > mine, equal += near[i] == mine;
-        if (larger < wanted && wanted <= larger + equal) edge_key = mine, edge_ties = wanted - larger;
-      }
-      __syncthreads();
-      edge = edge_key, ties = edge_ties;
-      break;
+    edge = edge_key, ties = edge_ties;
+    if (mine) {
+      const int at = near_at[threadIdx.x], of = at / (each * 256);
+      if (mine == edge) atomicAdd(&counts[of][at < need ? 1 : 3], 1);
+      else if (mine < edge && at < need) atomicAdd(&counts[of][0], 1);
+      else if (mine > edge && at >= need) atomicAdd(&counts[of][2], 1);
     }
+    __syncthreads();
   }
-
-  // Places to fill and survivors behind them, in index order: a wave counts its own first. Of the equal keys
-  // the first `ties` survive.
-  int count[4] = {0, 0, 0, 0};  // evicted for certain below need, equal there, survivors behind, equal there
-  over([&](uint32_t key, int at) {
-    const bool front = at < need;
-    count[0] += front && key < edge, count[1] += front && key == edge;
-    count[2] += !front && key > edge, count[3] += !front && key == edge;
-  });
-#pragma unroll
-  for (int c = 0; c < 4; ++c) count[c] = wave_sum(count[c]);
-  __syncthreads();
-  if (lane == 0)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) waves[wave][c] = count[c];
-  __syncthreads();
   // equal keys, places and survivors before this wave; survivors in all
   int seen = 0, to = 0, from = 0, all = 0, equals = 0, places_before = 0;
-  for (int w = 0; w < kSelectWaves; ++w) {
+  for (int w = 0; w < kWaves; ++w) {
     if (w == wave) seen = equals, to = places_before, from = all;
-    const int front = waves[w][1], back = waves[w][3];  // (its front part comes before its back part)
+    const int front = counts[w][1], back = counts[w][3];  // (its front part comes before its back part)
     const int kept_front = min(front, max(0, ties - equals)), kept_back = min(back, max(0, ties - equals - front));
-    places_before += waves[w][0] + front - kept_front, all += waves[w][2] + kept_back, equals += front + back;
+    places_before += counts[w][0] + front - kept_front, all += counts[w][2] + kept_back, equals += front + back;
   }
 
   int32_t* const fill = p.lists + ((int64_t)request * p.kv_heads + head) * 2 * p.moves;
   int32_t* const take = fill + p.moves;
   int mine_early = 0;
-  auto emit = [&](const uint32_t (&key)[4], int at) __attribute__((always_inline)) {
+  over([&](const uint32_t (&key)[4], int at) __attribute__((always_inline)) {
     // equal keys of the lanes before
     int equal = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) equal += at + j < m && key[j] == edge;
-    const int equal_upto = lane_scan(equal);
+    int equal_upto = 0;
+    if (__any(equal)) equal_upto = lane_scan(equal);  // (few batches hold any)
     int rank = seen + equal_upto - equal, places = 0, sources = 0;
     bool place[4], source[4];
 #pragma unroll
@@ -232,33 +267,23 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select(EvictArgs p) {
       place[j] = inside && at + j < need && !stays, source[j] = stays && at + j >= need;
       places += place[j], sources += source[j];
     }
-    const int places_upto = lane_scan(places), sources_upto = lane_scan(sources);
+    // both sums in one: 256 at most
+    const int both = lane_scan(places | sources << 16), places_upto = both & 0xffff, sources_upto = both >> 16;
     int next_place = to + places_upto - places, next_source = from + sources_upto - sources;
     if (places || sources) {
       const int slot = (table[at >> p.page_shift] << p.page_shift) + (at & mask);  // four of one page
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (place[j]) fill[next_place++] = slot + j;
-        if (source[j]) take[next_source++] = slot + j, mine_early += at + j < given;
+        if (place[j] && next_place < p.moves) fill[next_place++] = slot + j;
+        if (source[j] && next_source < p.moves) take[next_source++] = slot + j, mine_early += at + j < given;
       }
     }
     seen += __shfl(equal_upto, 63), to += __shfl(places_upto, 63), from += __shfl(sources_upto, 63);
-  };
-  if (held) {
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i)
-      if (i < each) emit(keys[i], begin + i * 256 + 4 * lane);
-  } else {
-    for (int i = 0; i < each; ++i) {
-      uint32_t key[4];
-      load(i, key);
-      emit(key, begin + i * 256 + 4 * lane);
-    }
-  }
-  mine_early = wave_sum(mine_early);
-  if (lane == 0) atomicAdd(&early, mine_early);
+  });
+  mine_early = lane_scan(mine_early);
+  if (lane == 63) atomicAdd(&early, mine_early);
   __syncthreads();
-  if (threadIdx.x == 0) *found = Found{all, early, recent, m, need, {0, 0, 0}};
+  if (threadIdx.x == 0) *found = Found{min(all, p.moves), early, recent, m, need, {0, 0, 0}};
 }
 
 constexpr int kMoveThreads = 256, kAhead = 4;
@@ -392,8 +417,10 @@ int smx_paged_evict(const smx_paged_cache* cache, float* key_weights, int32_t re
   const int pairs = requests * cache->kv_heads;
   p.found = (Found*)workspace;
   p.lists = (int32_t*)(p.found + pairs);
-  hipLaunchKernelGGL(evict_select, dim3((unsigned)cache->kv_heads, (unsigned)requests), dim3(kSelectThreads), 0,
-                     (hipStream_t)stream, p);
+  // Four waves where they hold the longest context, else sixteen.
+  const bool few = max_context <= 256 * 4 * kQuads;
+  hipLaunchKernelGGL(few ? evict_select<256> : evict_select<1024>, dim3((unsigned)cache->kv_heads, (unsigned)requests),
+                     dim3(few ? 256 : 1024), 0, (hipStream_t)stream, p);
   if (int rc = check_launch()) return rc;
   // Workgroups of a head and request: enough to fill the chip, of 64 rows at least.
   p.tails = cache->head_dim / 32;
