@@ -8,8 +8,9 @@
 // head moves 24,800.
 //
 // evict_select (a workgroup per head and request) finds the need-th largest weight: weights as integers in their order,
-// a histogram of their leading 11 bits, the part that holds it, and so on until its keys fit in LDS,
-// where they are compared with each other. evict_move then moves the rows.
+// a histogram of equal parts of their range, the part that holds it, and so on until its keys fit in LDS,
+// where they are compared with each other. Where contexts are long and heads few, the same is done in parts by several workgroups a
+// head (evict_histogram, evict_collect, evict_list). evict_move then moves the rows.
 #include "launch.hpp"
 
 namespace smx {
@@ -25,6 +26,12 @@ struct EvictArgs {
   int32_t requests, kv_heads, head_dim, page_shift, num_pages, keep, recent, max_context, moves, movers, tails;
   struct Found* found;  // [requests * kv_heads]
   int32_t* lists;       // [requests * kv_heads][2][moves]: slots to fill, slots to take from
+  // of long contexts, in `parts` parts of a head and request
+  int32_t parts;
+  struct Looked* looked;          // [requests * kv_heads]
+  struct Candidate* candidates;   // [requests * kv_heads][kCrowd]
+  int32_t *bad, *counts;          // [requests * kv_heads][parts], [..][parts][waves][4]
+  uint16_t* histograms;           // [requests * kv_heads][parts][kBins]
 };
 
 // What evict_select leaves for evict_move: rows of the lists, those of them whose source lies among the places of the recent
@@ -60,130 +67,246 @@ __device__ __forceinline__ int lane_scan(int x) {
   return x;
 }
 
-// kThreads * 4 * kQuads weights are held in registers, more are read once for each look at them.
-template <int kThreads>
-__global__ __launch_bounds__(kThreads) void evict_select(EvictArgs p) {
-  constexpr int kWaves = kThreads / 64;
-  const int head = blockIdx.x, request = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  Found* const found = p.found + (int64_t)request * p.kv_heads + head;
-  __shared__ int bins[kBins], scans[kWaves], counts[kWaves][4], bad, near_count, early, picked[3];
-  __shared__ __attribute__((aligned(16))) uint32_t near[kNear];
-  __shared__ uint32_t edge_key, lows[kWaves], highs[kWaves];
-  __shared__ int edge_ties, near_at[kNear];
-  const int32_t n = p.context[request], given = p.keep_lens ? p.keep_lens[request] : p.keep;
-  const int32_t* const table = p.tables + request * p.table_stride;
-  const int32_t mask = (1 << p.page_shift) - 1;
-  if (n <= given || n > p.max_context || given < 0) {  // uniform
-    if (threadIdx.x == 0) {
-      *found = Found{};
-      if (head == 0) p.lens[request] = n;
-    }
-    return;
+// What a request is cut to.
+struct Cut {
+  int32_t n, given, recent, need, m;  // its tokens, those kept, the recent among them, the others; the older tokens
+
+  // Whether anything is to be cut.
+  __device__ __forceinline__ bool of(const EvictArgs& p, int request) {
+    n = p.context[request], given = p.keep_lens ? p.keep_lens[request] : p.keep;
+    recent = min(p.recent, given), need = given - recent, m = n - recent;
+    return n > given && n <= p.max_context && given >= 0;
   }
-  if (threadIdx.x == 0) bad = near_count = early = 0;
-  for (int i = threadIdx.x; i < kBins; i += kThreads) bins[i] = 0;
-  if (threadIdx.x < kNear) near[threadIdx.x] = 0;  // below every key
-  const int recent = min(p.recent, given), need = given - recent, m = n - recent;
+};
+
+typedef uint32_t Keys[kQuads][4];
+
+// The keys of indices begin + 256 i + 4 lane .. + 3, i < count, below m. Entries that are no page of the cache are told in
+// `missing` and read as page 0.
+__device__ __forceinline__ void load_keys(const EvictArgs& p, const int32_t* table, int head, int begin, int count, int m, Keys& keys,
+                                          bool& missing) {
+  const int lane = threadIdx.x & 63, mask = (1 << p.page_shift) - 1;
+  f32x4 w[kQuads];
+  int entry[kQuads];
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i) {
+    const int at = begin + i * 256 + 4 * lane;
+    entry[i] = i < count && at < m ? table[at >> p.page_shift] : 0;
+    missing |= (uint32_t)entry[i] >= (uint32_t)p.num_pages;
+    if ((uint32_t)entry[i] >= (uint32_t)p.num_pages) entry[i] = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i) {
+    const int at = begin + i * 256 + 4 * lane;
+    if (i < count && at < m)
+      w[i] = *reinterpret_cast<const f32x4*>(p.weights + (((int64_t)entry[i] * p.kv_heads + head) << p.page_shift) + (at & mask));
+  }
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) keys[i][j] = order_of(w[i][j]);
+}
+
+// The range of the workgroup's keys (two barriers apart from each other's use of `ends`: one within).
+template <int kWaves>
+__device__ __forceinline__ void range_of(uint32_t& low, uint32_t& high, uint32_t (&ends)[2][kWaves]) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) low = min(low, (uint32_t)__shfl_xor((int)low, d)), high = max(high, (uint32_t)__shfl_xor((int)high, d));
+  if ((threadIdx.x & 63) == 0) ends[0][threadIdx.x >> 6] = low, ends[1][threadIdx.x >> 6] = high;
+  __syncthreads();
+  for (int w = 0; w < kWaves; ++w) low = min(low, ends[0][w]), high = max(high, ends[1][w]);
+}
+
+// A histogram over the keys from low to high: those below low, low itself (weights of which many are zero end here),
+// and equal parts of the others, the last with those above high. Parts of the values that are there hold few keys each, so that
+// additions meet rarely (leading bits alone, of which most weights share some: 66 us instead of 23 for 8100 keys of
+// 512 heads).
+struct Look {
+  int bins[kBins], scans[16], picked[3];
+
+  __device__ __forceinline__ void clear() {
+    for (int i = threadIdx.x; i < kBins; i += blockDim.x) bins[i] = 0;
+    if (threadIdx.x < 3) picked[threadIdx.x] = 0;
+  }
+};
+
+__device__ __forceinline__ int shift_of(uint32_t low, uint32_t high) {
+  const uint32_t range = high > low ? high - low : 0;
+  const int shift = max(0, 32 - (range ? (int)__builtin_clz(range) : 32) - 11);
+  return shift + (range >> shift > kBins - 2);
+}
+
+__device__ __forceinline__ int part_of(uint32_t key, uint32_t low, int shift) {
+  return key <= low ? key == low : (int)min(((key - low - 1) >> shift) + 2, (uint32_t)kBins - 1);
+}
+
+// The wanted-th largest key of those from least to most, of a filled histogram: its part's ends (also as the next
+// histogram's), the rank within the part, and how many keys are there. The histogram is cleared.
+template <int kThreads>
+__device__ __forceinline__ int pick(Look& look, uint32_t& low, uint32_t& high, uint32_t& least, uint32_t& most, int& wanted) {
+  constexpr int kEach = kBins / kThreads;
+  const int shift = shift_of(low, high), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // sums from the highest part down, kEach parts a thread
+  const int top = kBins - 1 - (int)threadIdx.x * kEach;
+  __syncthreads();
+  int own[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) own[i] = look.bins[top - i], sum += own[i];
+  const int all = sum;
+  sum = lane_scan(sum);
+  if (lane == 63) look.scans[wave] = sum;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) sum += look.scans[w];
+  int above = sum - all;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (above < wanted && wanted <= above + own[i]) look.picked[0] = top - i, look.picked[1] = wanted - above, look.picked[2] = own[i];
+    above += own[i];
+    look.bins[top - i] = 0;
+  }
+  __syncthreads();
+  const int part = look.picked[0], count = look.picked[2];
+  wanted = look.picked[1];
+  if (part == 0) most = low ? low - 1 : 0;
+  else if (part == 1) least = most = low;
+  else {
+    const uint64_t first = (uint64_t)low + 1 + ((uint64_t)(part - 2) << shift);
+    least = (uint32_t)first;
+    if (part < kBins - 1) most = (uint32_t)min((uint64_t)most, first + ((uint64_t)1 << shift) - 1);
+  }
+  low = least, high = most;
+  return count;
+}
+
+// Few keys, compared with each other.
+struct Near {
+  __attribute__((aligned(16))) uint32_t key[kNear];
+  uint32_t edge;
+  int at[kNear], count, ties;
+
+  __device__ __forceinline__ void clear() {
+    if (threadIdx.x < kNear) key[threadIdx.x] = 0;  // below every key
+    if (threadIdx.x == 0) count = 0;
+  }
+  __device__ __forceinline__ void add(uint32_t k, int index) {
+    const int place = atomicAdd(&count, 1);
+    if (place < kNear) key[place] = k, at[place] = index;  // (always, while nobody changes the weights)
+  }
+  // The wanted-th largest, and its rank among those equal to it.
+  __device__ __forceinline__ uint32_t resolve(int* wanted) {
+    const int all = min(count, kNear);
+    const uint32_t mine = (int)threadIdx.x < all ? key[threadIdx.x] : 0;
+    if (mine) {
+      int larger = 0, equal = 0;
+      for (int x = 0; x < all; x += 4) {
+        const u32x4 other = *reinterpret_cast<const u32x4*>(key + x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) larger += other[j] > mine, equal += other[j] == mine;
+      }
+      if (larger < *wanted && *wanted <= larger + equal) edge = mine, ties = *wanted - larger;
+    }
+    __syncthreads();
+    *wanted = ties;
+    return edge;
+  }
+};
+
+// Puts the places to fill and the survivors behind them on the lists, four indices a lane. seen, to and from: equal keys,
+// places and survivors before these (uniform). Returns how many of the lane's survivors lie before `given`.
+__device__ __forceinline__ int list_four(const EvictArgs& p, const int32_t* table, const Cut& c, uint32_t edge, int ties, int32_t* fill,
+                                         int32_t* take, const uint32_t (&key)[4], int at, int& seen, int& to, int& from) {
+  // equal keys of the lanes before
+  int equal = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) equal += at + j < c.m && key[j] == edge;
+  int equal_upto = 0;
+  if (__any(equal)) equal_upto = lane_scan(equal);  // (few hold any)
+  int rank = seen + equal_upto - equal, places = 0, sources = 0, early = 0;
+  bool place[4], source[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool inside = at + j < c.m, tie = inside && key[j] == edge;
+    const bool stays = inside && (key[j] > edge || (tie && rank < ties));
+    rank += tie;
+    place[j] = inside && at + j < c.need && !stays, source[j] = stays && at + j >= c.need;
+    places += place[j], sources += source[j];
+  }
+  // both sums in one: 256 at most
+  const int both = lane_scan(places | sources << 16);
+  int next_place = to + (both & 0xffff) - places, next_source = from + (both >> 16) - sources;
+  if (places || sources) {
+    const int slot = (table[at >> p.page_shift] << p.page_shift) + (at & ((1 << p.page_shift) - 1));  // four of one page
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (place[j] && next_place < p.moves) fill[next_place++] = slot + j;
+      if (source[j] && next_source < p.moves) take[next_source++] = slot + j, early += at + j < c.given;
+    }
+  }
+  seen += __builtin_amdgcn_readlane(equal_upto, 63);
+  const int sums = __builtin_amdgcn_readlane(both, 63);
+  to += sums & 0xffff, from += sums >> 16;
+  return early;
+}
+
+__device__ __forceinline__ int32_t* lists_of(const EvictArgs& p, int64_t pair) { return p.lists + pair * 2 * p.moves; }
+
+// The whole of one head and request by one workgroup. kThreads * 4 * kQuads weights are held in registers, more are read
+// once for each look at them.
+template <int kThreads>
+__device__ void select_whole(const EvictArgs& p, const Cut& c, int head, int request, Look& look, Near& near) {
+  constexpr int kWaves = kThreads / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t pair = (int64_t)request * p.kv_heads + head;
+  __shared__ int counts[kWaves][4], bad, early;
+  __shared__ uint32_t ends[2][kWaves];
+  const int32_t* const table = p.tables + request * p.table_stride;
+  if (threadIdx.x == 0) bad = early = 0;
+  near.clear();
+  look.clear();
 
   // A wave's indices lie one behind the other, four to a lane, in batches of kQuads times 256.
-  const int each = (m + kWaves * 256 - 1) / (kWaves * 256), begin = wave * each * 256;
+  const int each = (c.m + kWaves * 256 - 1) / (kWaves * 256), begin = wave * each * 256;
   const bool held = each <= kQuads;
-  uint32_t keys[kQuads][4];
+  Keys keys;
   bool missing = false;
-  auto load = [&](int first) __attribute__((always_inline)) {
-    f32x4 w[kQuads];
-    int entry[kQuads];
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i) {
-      const int at = begin + (first + i) * 256 + 4 * lane;
-      entry[i] = first + i < each && at < m ? table[at >> p.page_shift] : 0;
-      missing |= (uint32_t)entry[i] >= (uint32_t)p.num_pages;
-      if ((uint32_t)entry[i] >= (uint32_t)p.num_pages) entry[i] = 0;
-    }
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i) {
-      const int at = begin + (first + i) * 256 + 4 * lane;
-      if (first + i < each && at < m)
-        w[i] = *reinterpret_cast<const f32x4*>(p.weights + (((int64_t)entry[i] * p.kv_heads + head) << p.page_shift) + (at & mask));
-    }
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) keys[i][j] = order_of(w[i][j]);
-  };
   // f(four keys, index of the first) over the wave's indices, in their order; f is called by all lanes
   auto over = [&](auto f) __attribute__((always_inline)) {
     for (int first = 0; first < each; first += kQuads) {
-      if (!held) load(first);
+      if (!held) load_keys(p, table, head, begin + first * 256, each - first, c.m, keys, missing);
 #pragma unroll
       for (int i = 0; i < kQuads; ++i)
         if (first + i < each) f(keys[i], begin + (first + i) * 256 + 4 * lane);
     }
   };
-
-  // The range of the weights (of the first batch, where they are more): parts of equal size of the values that
-  // are there hold few weights each, and the histogram's additions meet rarely.
-  load(0);
+  // the range of the weights (of the first batch, where they are more)
+  load_keys(p, table, head, begin, each, c.m, keys, missing);
   uint32_t low = ~0u, high = 0;
 #pragma unroll
   for (int i = 0; i < kQuads; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (i < each && begin + i * 256 + 4 * lane + j < m) low = min(low, keys[i][j]), high = max(high, keys[i][j]);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) low = min(low, (uint32_t)__shfl_xor((int)low, d)), high = max(high, (uint32_t)__shfl_xor((int)high, d));
-  if (lane == 0) lows[wave] = low, highs[wave] = high;
+      if (i < each && begin + i * 256 + 4 * lane + j < c.m) low = min(low, keys[i][j]), high = max(high, keys[i][j]);
   // every page of the request has to be there, the recent tokens' too
-  for (int i = (m >> p.page_shift) + (int)threadIdx.x; i <= (n - 1) >> p.page_shift; i += kThreads)
+  for (int i = (c.m >> p.page_shift) + (int)threadIdx.x; i <= (c.n - 1) >> p.page_shift; i += kThreads)
     missing |= (uint32_t)table[i] >= (uint32_t)p.num_pages;
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) low = min(low, lows[w]), high = max(high, highs[w]);
+  range_of<kWaves>(low, high, ends);
 
   // The need-th largest lies between `least` and `most`, the `ties`-th largest of the keys there. (Without need nothing
   // survives: none of the largest keys.)
   uint32_t least = ~0u, most = ~0u;
   int ties = 0;
-  if (need > 0) {
-    // Keys below `low` count to the first part of the histogram, those above `high` to the last.
-    int wanted = need;
-    least = 0;
-    for (;;) {
-      const int shift = max(0, 32 - (high > low ? (int)__builtin_clz(high - low) : 32) - 11);
+  if (c.need > 0) {
+    ties = c.need, least = 0;
+    int count;
+    do {
+      const int shift = shift_of(low, high);
       over([&](const uint32_t (&key)[4], int at) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (at + j < m && key[j] >= least && key[j] <= most)
-            atomicAdd(&bins[key[j] <= low ? 0 : min((key[j] - low) >> shift, (uint32_t)kBins - 1)], 1);
+          if (at + j < c.m && key[j] >= least && key[j] <= most) atomicAdd(&look.bins[part_of(key[j], low, shift)], 1);
       });
-      __syncthreads();
-      // The part that holds it: sums from the highest one down, kEach parts a thread.
-      constexpr int kEach = kBins / kThreads;
-      const int top = kBins - 1 - (int)threadIdx.x * kEach;
-      int own[kEach], sum = 0;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) own[i] = bins[top - i], sum += own[i];
-      const int all = sum;
-      sum = lane_scan(sum);
-      if (lane == 63) scans[wave] = sum;
-      __syncthreads();
-      for (int w = 0; w < wave; ++w) sum += scans[w];
-      int above = sum - all;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        if (above < wanted && wanted <= above + own[i]) picked[0] = top - i, picked[1] = wanted - above, picked[2] = own[i];
-        above += own[i];
-        bins[top - i] = 0;
-      }
-      __syncthreads();
-      const int part = picked[0], count = picked[2];
-      wanted = picked[1];
-      const uint64_t first = low + ((uint64_t)part << shift);
-      if (part) least = (uint32_t)first;
-      if (part < kBins - 1) most = (uint32_t)min((uint64_t)most, first + ((uint64_t)1 << shift) - 1);
-      low = least, high = most;
-      if (least == most || count <= kNear) break;  // else another look, at this part alone
-    }
-    ties = wanted;
+      count = pick<kThreads>(look, low, high, least, most, ties);
+    } while (least < most && count > kNear);  // another look, at the part alone
   }
   if (missing) bad = 1;
 
@@ -194,47 +317,33 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs p) {
   over([&](const uint32_t (&key)[4], int at) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const bool inside = at + j < m, front = at + j < need, in = inside && key[j] >= least && key[j] <= most;
+      const bool inside = at + j < c.m, front = at + j < c.need, in = inside && key[j] >= least && key[j] <= most;
       count[0] += inside && front && key[j] < least, count[1] += in && front;
       count[2] += inside && !front && key[j] > most, count[3] += in && !front;
-      if (in && apart) {
-        const int place = atomicAdd(&near_count, 1);
-        if (place < kNear) near[place] = key[j], near_at[place] = at + j;  // (always, while nobody changes the weights)
-      }
+      if (in && apart) near.add(key[j], at + j);
     }
   });
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int sum = lane_scan(count[c]);
-    if (lane == 63) counts[wave][c] = apart && (c & 1) ? 0 : sum;
+  for (int x = 0; x < 4; ++x) {
+    const int sum = lane_scan(count[x]);
+    if (lane == 63) counts[wave][x] = apart && (x & 1) ? 0 : sum;
   }
   __syncthreads();
-  if (head == 0 && threadIdx.x == 0) p.lens[request] = bad ? n : given;
+  if (head == 0 && threadIdx.x == 0) p.lens[request] = bad ? c.n : c.given;
   if (bad) {  // uniform
-    if (threadIdx.x == 0) *found = Found{};
+    if (threadIdx.x == 0) p.found[pair] = Found{};
     return;
   }
   // Survivors: keys above the edge, and the first `ties` of those equal to it.
   uint32_t edge = most;
   if (apart) {
-    const int near_all = min(near_count, kNear);
-    const uint32_t mine = (int)threadIdx.x < near_all ? near[threadIdx.x] : 0;
-    if (mine) {
-      int larger = 0, equal = 0;
-      for (int x = 0; x < near_all; x += 4) {
-        const u32x4 other = *reinterpret_cast<const u32x4*>(near + x);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) larger += other[j] > mine, equal += other[j] == mine;
-      }
-      if (larger < ties && ties <= larger + equal) edge_key = mine, edge_ties = ties - larger;
-    }
-    __syncthreads();
-    edge = edge_key, ties = edge_ties;
-    if (mine) {
-      const int at = near_at[threadIdx.x], of = at / (each * 256);
-      if (mine == edge) atomicAdd(&counts[of][at < need ? 1 : 3], 1);
-      else if (mine < edge && at < need) atomicAdd(&counts[of][0], 1);
-      else if (mine > edge && at >= need) atomicAdd(&counts[of][2], 1);
+    edge = near.resolve(&ties);
+    if ((int)threadIdx.x < min(near.count, kNear)) {
+      const uint32_t mine = near.key[threadIdx.x];
+      const int at = near.at[threadIdx.x], of = at / (each * 256);
+      if (mine == edge) atomicAdd(&counts[of][at < c.need ? 1 : 3], 1);
+      else if (mine < edge && at < c.need) atomicAdd(&counts[of][0], 1);
+      else if (mine > edge && at >= c.need) atomicAdd(&counts[of][2], 1);
     }
     __syncthreads();
   }
@@ -246,44 +355,284 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs p) {
     const int kept_front = min(front, max(0, ties - equals)), kept_back = min(back, max(0, ties - equals - front));
     places_before += counts[w][0] + front - kept_front, all += counts[w][2] + kept_back, equals += front + back;
   }
-
-  int32_t* const fill = p.lists + ((int64_t)request * p.kv_heads + head) * 2 * p.moves;
-  int32_t* const take = fill + p.moves;
+  int32_t* const fill = lists_of(p, pair);
   int mine_early = 0;
   over([&](const uint32_t (&key)[4], int at) __attribute__((always_inline)) {
-    // equal keys of the lanes before
-    int equal = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) equal += at + j < m && key[j] == edge;
-    int equal_upto = 0;
-    if (__any(equal)) equal_upto = lane_scan(equal);  // (few batches hold any)
-    int rank = seen + equal_upto - equal, places = 0, sources = 0;
-    bool place[4], source[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool inside = at + j < m, tie = inside && key[j] == edge;
-      const bool stays = inside && (key[j] > edge || (tie && rank < ties));
-      rank += tie;
-      place[j] = inside && at + j < need && !stays, source[j] = stays && at + j >= need;
-      places += place[j], sources += source[j];
-    }
-    // both sums in one: 256 at most
-    const int both = lane_scan(places | sources << 16), places_upto = both & 0xffff, sources_upto = both >> 16;
-    int next_place = to + places_upto - places, next_source = from + sources_upto - sources;
-    if (places || sources) {
-      const int slot = (table[at >> p.page_shift] << p.page_shift) + (at & mask);  // four of one page
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (place[j] && next_place < p.moves) fill[next_place++] = slot + j;
-        if (source[j] && next_source < p.moves) take[next_source++] = slot + j, mine_early += at + j < given;
-      }
-    }
-    seen += __shfl(equal_upto, 63), to += __shfl(places_upto, 63), from += __shfl(sources_upto, 63);
+    mine_early += list_four(p, table, c, edge, ties, fill, fill + p.moves, key, at, seen, to, from);
   });
   mine_early = lane_scan(mine_early);
   if (lane == 63) atomicAdd(&early, mine_early);
   __syncthreads();
-  if (threadIdx.x == 0) *found = Found{min(all, p.moves), early, recent, m, need, {0, 0, 0}};
+  if (threadIdx.x == 0) p.found[pair] = Found{min(all, p.moves), early, c.recent, c.m, c.need, {0, 0, 0}};
+}
+
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void evict_select(EvictArgs p) {
+  __shared__ Look look;
+  __shared__ Near near;
+  const int head = blockIdx.x, request = blockIdx.y;
+  Cut c;
+  if (c.of(p, request)) return select_whole<kThreads>(p, c, head, request, look, near);  // uniform
+  if (threadIdx.x == 0) {
+    p.found[(int64_t)request * p.kv_heads + head] = Found{};
+    if (head == 0) p.lens[request] = c.n;
+  }
+}
+
+// Long contexts: the older tokens in parts of 8192, a workgroup each, in three launches, for which one workgroup took
+// 127 us at 131,000 tokens. evict_histogram counts each part's weights over the range that the first thousand have,
+// evict_collect finds the part of the range that holds the edge and collects its keys, evict_list finds
+// the edge among them and puts each part's places and survivors on the lists.
+constexpr int kPart = 8192, kPartThreads = 256, kPartWaves = 4, kCrowd = 4096, kMostParts = 64;
+
+// What the three launches leave for each other, of a head and request.
+struct Looked {
+  uint32_t low, high, least, most;
+  int32_t ties, crowd, mode, unused;  // mode 0: nothing is cut, 1: parts, 2: too many keys at the edge, one workgroup does it all
+};
+struct Candidate {
+  uint32_t key;
+  int32_t at;
+};
+
+__device__ __forceinline__ int parts_of(const Cut& c) { return (c.m + kPart - 1) / kPart; }
+
+__global__ __launch_bounds__(kPartThreads) void evict_histogram(EvictArgs p) {
+  const int head = blockIdx.x, request = blockIdx.y, part = blockIdx.z, wave = threadIdx.x >> 6;
+  const int64_t pair = (int64_t)request * p.kv_heads + head;
+  Looked* const looked = p.looked + pair;
+  Cut c;
+  if (!c.of(p, request)) {  // uniform
+    if (threadIdx.x == 0 && part == 0) {
+      looked->mode = 0;
+      p.found[pair] = Found{};
+      if (head == 0) p.lens[request] = c.n;
+    }
+    return;
+  }
+  if (part >= max(1, parts_of(c))) return;
+  __shared__ int bins[kBins], bad;
+  __shared__ uint32_t ends[2][kPartWaves];
+  for (int i = threadIdx.x; i < kBins; i += kPartThreads) bins[i] = 0;
+  if (threadIdx.x == 0) bad = 0;
+  const int32_t* const table = p.tables + request * p.table_stride;
+  bool missing = false;
+  Keys keys;
+  uint32_t low = ~0u, high = 0;
+  load_keys(p, table, head, wave * 256, 1, c.m, keys, missing);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (4 * (int)threadIdx.x + j < c.m) low = min(low, keys[0][j]), high = max(high, keys[0][j]);
+  const int begin = part * kPart + wave * (kPart / kPartWaves);
+  load_keys(p, table, head, begin, kQuads, c.m, keys, missing);
+  if (part == 0)
+    for (int i = (c.m >> p.page_shift) + (int)threadIdx.x; i <= (c.n - 1) >> p.page_shift; i += kPartThreads)
+      missing |= (uint32_t)table[i] >= (uint32_t)p.num_pages;
+  range_of<kPartWaves>(low, high, ends);
+  if (missing) bad = 1;
+  const int shift = shift_of(low, high);
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (begin + i * 256 + 4 * (int)(threadIdx.x & 63) + j < c.m) atomicAdd(&bins[part_of(keys[i][j], low, shift)], 1);
+  __syncthreads();
+  u32x4 eight;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) eight[j] = (uint32_t)bins[8 * threadIdx.x + 2 * j] | (uint32_t)bins[8 * threadIdx.x + 2 * j + 1] << 16;
+  reinterpret_cast<u32x4*>(p.histograms)[(pair * p.parts + part) * kPartThreads + threadIdx.x] = eight;
+  if (threadIdx.x == 0) {
+    p.bad[pair * p.parts + part] = bad;
+    if (part == 0) looked->low = low, looked->high = high, looked->crowd = 0, p.found[pair].early = 0;
+  }
+}
+
+__global__ __launch_bounds__(kPartThreads) void evict_collect(EvictArgs p) {
+  const int head = blockIdx.x, request = blockIdx.y, part = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t pair = (int64_t)request * p.kv_heads + head;
+  Looked* const looked = p.looked + pair;
+  Cut c;
+  if (!c.of(p, request)) return;
+  const int parts = max(1, parts_of(c));
+  if (part >= parts) return;
+  __shared__ Look look;
+  __shared__ Candidate candidates[kCrowd];
+  __shared__ int count, base;
+  if (threadIdx.x == 0) count = 0;
+  if (threadIdx.x < 3) look.picked[threadIdx.x] = 0;
+  const int32_t* const table = p.tables + request * p.table_stride;
+  const int begin = part * kPart + wave * (kPart / kPartWaves);
+  Keys keys;
+  bool missing = false;
+  load_keys(p, table, head, begin, kQuads, c.m, keys, missing);
+  uint32_t low = looked->low, high = looked->high, least = ~0u, most = ~0u;
+  int ties = 0, crowd = 0;
+  const bool bad = __syncthreads_or((int)threadIdx.x < parts && p.bad[pair * p.parts + threadIdx.x]);
+  if (c.need > 0 && !bad) {  // uniform
+    int sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const u32x4* const from = reinterpret_cast<const u32x4*>(p.histograms) + pair * p.parts * kPartThreads + threadIdx.x;
+#pragma unroll 4
+    for (int x = 0; x < parts; ++x) {
+      const u32x4 eight = from[x * kPartThreads];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sums[2 * j] += eight[j] & 0xffff, sums[2 * j + 1] += eight[j] >> 16;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) look.bins[8 * threadIdx.x + j] = sums[j];
+    ties = c.need, least = 0;
+    crowd = pick<kPartThreads>(look, low, high, least, most, ties);
+  }
+  const int mode = bad ? 0 : least < most && crowd > kCrowd ? 2 : 1;
+  if (threadIdx.x == 0 && part == 0) {
+    looked->least = least, looked->most = most, looked->ties = ties, looked->mode = mode;
+    if (bad) p.found[pair] = Found{};
+    if (head == 0) p.lens[request] = bad ? c.n : c.given;
+  }
+  if (mode != 1) return;
+  // The wave's keys that are evicted or survive for certain, and those of the part found.
+  int certain[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = begin + i * 256 + 4 * lane + j;
+      const uint32_t key = keys[i][j];
+      if (at >= c.m) continue;
+      certain[0] += at < c.need && key < least, certain[1] += at >= c.need && key > most;
+      if (c.need > 0 && key >= least && key <= most && least < most) {
+        const int place = atomicAdd(&count, 1);
+        if (place < kCrowd) candidates[place] = Candidate{key, at};
+      }
+    }
+  if (least == most) {
+    // all of the part found are equal: counted in place of candidates
+    int equal[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = begin + i * 256 + 4 * lane + j;
+        if (at < c.m && keys[i][j] == least) ++equal[at >= c.need];
+      }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int sum = lane_scan(equal[x]);
+      if (lane == 63) p.counts[((pair * p.parts + part) * kPartWaves + wave) * 4 + 2 + x] = sum;
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int sum = lane_scan(certain[x]);
+    if (lane == 63) p.counts[((pair * p.parts + part) * kPartWaves + wave) * 4 + x] = sum;
+  }
+  __syncthreads();
+  const int mine = min(count, kCrowd);
+  if (threadIdx.x == 0 && mine) base = atomicAdd(&looked->crowd, mine);  // (their order does not matter)
+  __syncthreads();
+  for (int i = threadIdx.x; i < mine; i += kPartThreads)
+    if (base + i < kCrowd) p.candidates[pair * kCrowd + base + i] = candidates[i];
+}
+
+__global__ __launch_bounds__(kPartThreads) void evict_list(EvictArgs p) {
+  const int head = blockIdx.x, request = blockIdx.y, part = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t pair = (int64_t)request * p.kv_heads + head;
+  __shared__ Look look;
+  __shared__ Near near;
+  __shared__ int sums[kPartWaves + 1][4], early;
+  Cut c;
+  if (!c.of(p, request)) return;
+  const int parts = max(1, parts_of(c));
+  const Looked looked = p.looked[pair];
+  if (part >= parts || looked.mode == 0) return;
+  if (looked.mode == 2) {
+    if (part == 0) select_whole<kPartThreads>(p, c, head, request, look, near);
+    return;
+  }
+  const int32_t* const table = p.tables + request * p.table_stride;
+  const int begin = part * kPart + wave * (kPart / kPartWaves);
+  Keys keys;
+  bool missing = false;
+  load_keys(p, table, head, begin, kQuads, c.m, keys, missing);
+  near.clear();
+  look.clear();
+  if (threadIdx.x < 4 * (kPartWaves + 1)) (&sums[0][0])[threadIdx.x] = 0;
+  if (threadIdx.x == 0) early = 0;
+  __syncthreads();
+  // The edge, among the candidates (every workgroup finds it for itself).
+  constexpr int kEach = kCrowd / kPartThreads;
+  uint32_t least = looked.least, most = looked.most, edge = most;
+  int ties = looked.ties;
+  const bool apart = least < most;
+  const int crowd = apart ? min(looked.crowd, kCrowd) : 0;
+  Candidate mine[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {  // (mostly few of these are there)
+    const int at = i * kPartThreads + (int)threadIdx.x;
+    mine[i] = at < crowd ? p.candidates[pair * kCrowd + at] : Candidate{0, 0};
+  }
+  if (apart) {
+    uint32_t low = least, high = most;
+    int count = crowd;
+    while (least < most && count > kNear) {
+      const int shift = shift_of(low, high);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (mine[i].key >= least && mine[i].key <= most && mine[i].key) atomicAdd(&look.bins[part_of(mine[i].key, low, shift)], 1);
+      count = pick<kPartThreads>(look, low, high, least, most, ties);
+    }
+    edge = most;
+    if (least < most) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (mine[i].key && mine[i].key >= least && mine[i].key <= most) near.add(mine[i].key, mine[i].at);
+      __syncthreads();
+      edge = near.resolve(&ties);
+    }
+  }
+  // Before each wave's indices, and (the last) in all: places for certain, survivors for certain, and of the keys equal to the
+  // edge those below need, and all.
+  const int* const counts = p.counts + pair * p.parts * kPartWaves * 4;
+#pragma unroll
+  for (int b = 0; b <= kPartWaves; ++b) {
+    const int upto = b == kPartWaves ? parts * kPart : part * kPart + b * (kPart / kPartWaves);
+    int before[4] = {0, 0, 0, 0};
+    const int w = threadIdx.x;  // (at most 256 waves)
+    if (w < upto / (kPart / kPartWaves)) {
+      before[0] = counts[4 * w], before[1] = counts[4 * w + 1];
+      if (!apart) before[2] = counts[4 * w + 2], before[3] = counts[4 * w + 2] + counts[4 * w + 3];
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (i * kPartThreads < crowd) {  // uniform
+        const uint32_t key = mine[i].key;
+        const int at = mine[i].at;
+        const bool in = key && at < upto, front = at < c.need;
+        before[0] += in && key < edge && front, before[1] += in && key > edge && !front;
+        before[2] += in && key == edge && front, before[3] += in && key == edge;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int sum = lane_scan(before[x]);
+      if (lane == 63) atomicAdd(&sums[b][x], sum);
+    }
+  }
+  __syncthreads();
+  auto places = [&](int b) { return sums[b][0] + sums[b][2] - min(ties, sums[b][2]); };
+  auto sources = [&](int b) { return sums[b][1] + min(ties, sums[b][3]) - min(ties, sums[b][2]); };
+  int seen = sums[wave][3], to = places(wave), from = sources(wave), mine_early = 0;
+  int32_t* const fill = lists_of(p, pair);
+#pragma unroll
+  for (int i = 0; i < kQuads; ++i)
+    mine_early += list_four(p, table, c, edge, ties, fill, fill + p.moves, keys[i], begin + i * 256 + 4 * lane, seen, to, from);
+  mine_early = lane_scan(mine_early);
+  if (lane == 63) atomicAdd(&early, mine_early);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    Found* const found = p.found + pair;
+    if (early) atomicAdd(&found->early, early);
+    if (part == 0) found->count = min(sources(kPartWaves), p.moves), found->recent = c.recent, found->from = c.m, found->to = c.need;
+  }
 }
 
 constexpr int kMoveThreads = 256, kAhead = 4;
@@ -365,6 +714,30 @@ int moves_of(int keep, bool given, int max_context) {
   return max(1, given ? max_context / 2 : min(keep, max(0, max_context - keep)));
 }
 
+// Parts of the longest context where it is long and the heads are few; 0: one workgroup a head and request. Selection
+// took, of one workgroup and of parts: 31 and 36 us for 8 heads of 32,000 tokens, which sixteen waves hold in registers, 100 and 43
+// for 32 heads of 131,000, and 119 and 124 for 128 of them, which fill half the chip as they are.
+int parts_of(int64_t pairs, int max_context) {
+  const int64_t parts = ((int64_t)max_context + kPart - 1) / kPart;
+  return max_context > 1024 * 4 * kQuads && parts <= kMostParts && pairs < 128 ? (int)parts : 0;
+}
+
+// Where the workspace's pieces lie, behind each other; the last is its size.
+struct Pieces {
+  int64_t found, looked, candidates, bad, counts, histograms, lists, end;
+  Pieces(int64_t pairs, int parts, int moves) {
+    auto next = [](int64_t from, int64_t bytes) { return from + (bytes + 15) / 16 * 16; };
+    found = 0;
+    looked = next(found, pairs * sizeof(Found));
+    candidates = next(looked, parts ? pairs * sizeof(Looked) : 0);
+    bad = next(candidates, parts ? pairs * kCrowd * sizeof(Candidate) : 0);
+    counts = next(bad, pairs * parts * 4);
+    histograms = next(counts, pairs * parts * kPartWaves * 16);
+    lists = next(histograms, pairs * parts * kBins * 2);
+    end = next(lists, pairs * moves * 8);
+  }
+};
+
 }  // namespace
 }  // namespace smx
 
@@ -381,7 +754,7 @@ int smx_paged_evict_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t 
   if (max_context < 0 || max_context > SMX_PAGED_MAX_CONTEXT)
     return fail(SMX_ERR_INVALID, "max_context must be 0 to %d, got %d", SMX_PAGED_MAX_CONTEXT, max_context);
   // keep < 0: a length for each request
-  *bytes = (int64_t)requests * kv_heads * (sizeof(Found) + 8 * (int64_t)moves_of(keep, keep < 0, max_context));
+  *bytes = Pieces((int64_t)requests * kv_heads, parts_of((int64_t)requests * kv_heads, max_context), moves_of(keep, keep < 0, max_context)).end;
   return SMX_OK;
 }
 
@@ -415,16 +788,28 @@ int smx_paged_evict(const smx_paged_cache* cache, float* key_weights, int32_t re
   p.head_dim = cache->head_dim, p.page_shift = __builtin_ctz(cache->page_size), p.num_pages = cache->num_pages;
   p.keep = keep, p.recent = recent, p.max_context = max_context, p.moves = moves_of(keep, keep < 0, max_context);
   const int pairs = requests * cache->kv_heads;
-  p.found = (Found*)workspace;
-  p.lists = (int32_t*)(p.found + pairs);
-  // Four waves where they hold the longest context, else sixteen.
-  const bool few = max_context <= 256 * 4 * kQuads;
-  hipLaunchKernelGGL(few ? evict_select<256> : evict_select<1024>, dim3((unsigned)cache->kv_heads, (unsigned)requests),
-                     dim3(few ? 256 : 1024), 0, (hipStream_t)stream, p);
-  if (int rc = check_launch()) return rc;
-  // Workgroups of a head and request: enough to fill the chip, of 64 rows at least.
+  p.parts = parts_of(pairs, max_context);
+  const Pieces at(pairs, p.parts, p.moves);
+  char* const base = (char*)workspace;
+  p.found = (Found*)(base + at.found), p.looked = (Looked*)(base + at.looked), p.candidates = (Candidate*)(base + at.candidates);
+  p.bad = (int32_t*)(base + at.bad), p.counts = (int32_t*)(base + at.counts), p.histograms = (uint16_t*)(base + at.histograms);
+  p.lists = (int32_t*)(base + at.lists);
+  const dim3 heads((unsigned)cache->kv_heads, (unsigned)requests, (unsigned)max(1, p.parts));
+  if (p.parts) {
+    for (auto kern : {evict_histogram, evict_collect, evict_list}) {
+      hipLaunchKernelGGL(kern, heads, dim3(kPartThreads), 0, (hipStream_t)stream, p);
+      if (int rc = check_launch()) return rc;
+    }
+  } else {
+    // four waves where they hold the longest context, else sixteen
+    const bool few = max_context <= kPart;
+    hipLaunchKernelGGL(few ? evict_select<256> : evict_select<1024>, heads, dim3(few ? 256 : 1024), 0, (hipStream_t)stream, p);
+    if (int rc = check_launch()) return rc;
+  }
+  // Workgroups of a head and request: of 64 rows at least, and so many that they even out (139 us for 64 requests; 142 of half
+  // as many, 149 of a quarter).
   p.tails = cache->head_dim / 32;
-  p.movers = min((p.moves + 63) / 64, max(1, 8192 / pairs));
+  p.movers = min((p.moves + 63) / 64, max(1, 16384 / pairs));
   hipLaunchKernelGGL(cache->head_dim == 128 ? evict_move<128> : evict_move<64>, dim3((unsigned)pairs, (unsigned)(p.tails + p.movers)),
                      dim3(kMoveThreads), 0, (hipStream_t)stream, p);
   return check_launch();

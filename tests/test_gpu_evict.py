@@ -146,6 +146,53 @@ def test_long_contexts(context, keep, recent, page):
     check(make_cache(context, kv_heads=1, page=page, seed=4), context, keep, recent)
 
 
+@pytest.mark.parametrize("kind", ["any", "equal", "few", "zeros", "odd", "close", "halves", "rising", "falling"])
+def test_long_contexts_in_parts(kind):
+    """Several workgroups a head: weights that crowd at the edge, that are equal across parts, that rise or fall along a request (so
+    that the first thousand say little about the others), next to short requests and those that stay."""
+    context = [50000, 8192, 8193, 40, 0, 33000, 16384, 20000]
+    cache = make_cache(context, page=32, seed=20)
+    k, v, w, lens, tables = cache
+    g = torch.Generator(device=DEV).manual_seed(21)
+    random = torch.rand(w.shape, device=DEV, generator=g)
+    if kind == "equal":
+        w.fill_(0.25)
+    elif kind == "few":
+        w.copy_(torch.randint(0, 4, w.shape, device=DEV, generator=g))
+    elif kind == "zeros":
+        w.mul_(random < 0.1)
+    elif kind == "odd":
+        w[random < 0.3], w[random < 0.2], w[random < 0.1] = math.inf, math.nan, -math.inf
+        w[random > 0.95] = -math.nan
+    elif kind == "close":
+        w.copy_((torch.full(w.shape, 1.0, device=DEV).view(torch.int32) + (random * 5).int()).view(torch.float32))
+    elif kind == "halves":  # all within a part of the range, more than are collected
+        w.copy_(1 + random * 2**-12)
+        w.view(-1)[::997] = 1e30
+    elif kind in ("rising", "falling"):
+        for row, n in zip(tables.tolist(), context):
+            for i in range(-(-n // 32)):
+                at = torch.arange(32, device=DEV) + 32 * i + 1.0
+                w[row[i]] = at if kind == "rising" else 1 / at
+    if kind == "any":
+        tables[6, 300], tables[7, 624] = -1, k.shape[0]
+    check(cache, context, [20000, 4000, 8191, 20, 0, 1, 16000, 300], 250)
+
+
+@pytest.mark.parametrize("context,keep,recent", [([50000], 49999, 0), ([50000], 0, 0), ([50000], 1, 0), ([50000], 700, 700),
+                                                 ([50000], 40000, 39990), ([32769], 32768, 1), ([40960, 40961], 8192, 0)])
+def test_long_contexts_in_parts_at_their_ends(context, keep, recent):
+    check(make_cache(context, page=64, kv_heads=1, seed=22), context, keep, recent)
+
+
+def test_a_bound_beyond_the_parts():
+    """The longest contexts that are allowed for, whatever the requests hold."""
+    k, v, weights, lens, tables = make_cache([9000, 100], page=1024, kv_heads=2, seed=23, width=600)
+    check((k, v, weights, lens, tables), [9000, 100], 500, 20)
+    k, v, weights, lens, tables = make_cache([40000, 9000], page=1024, kv_heads=64, seed=24)  # many heads
+    check((k, v, weights, lens, tables), [40000, 9000], 5000, 20)
+
+
 def test_a_long_recent_part_moves_over_itself():
     for shift in (1, 3, 129, 1000):
         context = [4000 + shift]
