@@ -501,7 +501,8 @@ int smx_paged_attention_lse(const smx_paged_cache* cache, const smx_paged_step* 
  * keys start from zero. lse is that of smx_paged_attention_lse for the same queries, scale and window. Scores and sums in
  * FP32; the same call gives the same bits. Slots that no admitted request's keys lie in are left as they are, and so are
  * those of pages that are not in the cache. The cache's values are not read (v may be k). Requests share no pages.
- * key_weights shares no memory with the keys, the queries and lse. The workspace
+ * key_weights shares no memory with the keys, the queries and lse. The query heads of 32 rows lie within 2^32 bytes
+ * (SMX_ERR_UNSUPPORTED otherwise). The workspace
  * (smx_paged_key_weights_workspace_bytes, for the current device) is overwritten. Asynchronous on stream.
  */
 int smx_paged_key_weights(const smx_paged_cache* cache, const smx_paged_step* step, const smx_heads* q, const float* lse,
@@ -563,7 +564,8 @@ int smx_rotary(int32_t tokens, int32_t head_dim, int32_t rotary_dim, const smx_h
  * of any probability if there is none). Probabilities that are no positive finite numbers count as zero, a draft outside the
  * vocabulary is refused; products and sums in 64 bits. Out: counts [requests], the accepted drafts and one (0 for a request
  * without rows); out [step tokens], from each request's first row on its accepted drafts, the drawn token (-1 if its
- * row holds no probability at all) and -1. workspace: smx_verify_workspace_bytes. Asynchronous on stream.
+ * row holds no probability at all) and -1. out and counts share no memory with anything that is read. workspace:
+ * smx_verify_workspace_bytes. Asynchronous on stream.
  */
 int smx_verify_drafts(const smx_paged_step* step, int32_t vocab, const void* target, int64_t target_row,
                       const void* draft, int64_t draft_row, const void* tokens, const float* accept,

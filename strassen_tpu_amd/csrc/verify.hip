@@ -289,8 +289,8 @@ int smx_verify_drafts(const smx_paged_step* step, int32_t vocab, const void* tar
     return fail(SMX_ERR_INVALID, "rows must be at least vocab=%d apart", vocab);
   const int size = flags & SMX_VERIFY_BF16 ? 2 : 4;
   if ((uintptr_t)target % size || (uintptr_t)draft % size || (uintptr_t)tokens % (flags & SMX_VERIFY_TOKENS_I64 ? 8 : 4) ||
-      (uintptr_t)out % (flags & SMX_VERIFY_TOKENS_I64 ? 8 : 4))
-    return fail(SMX_ERR_INVALID, "misaligned probabilities or tokens");
+      (uintptr_t)out % (flags & SMX_VERIFY_TOKENS_I64 ? 8 : 4) || (uintptr_t)accept % 4 || (uintptr_t)sample % 4 || (uintptr_t)counts % 4)
+    return fail(SMX_ERR_INVALID, "misaligned probabilities, tokens, random numbers or counts");
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)
     return fail(SMX_ERR_INVALID, "the call needs a 16-byte aligned workspace of %lld bytes", (long long)need);
   VerifyArgs p{};

@@ -53,6 +53,8 @@ def rotary_frequencies(rotary_dim, theta=1e6, *, scaling=None, factor=1.0, origi
         return (base ** (-2 * half / rotary_dim)).to(device), 1.0
     if original_context is None or original_context <= 0:
         raise ValueError(f"scaling={scaling!r} needs original_context=, the tokens that the model was trained on")
+    if scaling == "yarn" and theta <= 1:
+        raise ValueError(f"scaling='yarn' needs theta above 1, got {theta}")
     fast = fast if fast is not None else 32.0 if scaling == "yarn" else 4.0
     slow = 1.0 if slow is None else slow
     if not fast > slow > 0:
