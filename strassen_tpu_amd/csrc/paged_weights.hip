@@ -601,7 +601,7 @@ int smx_paged_key_weights(const smx_paged_cache* cache, const smx_paged_step* st
   p.window = window < SMX_PAGED_MAX_CONTEXT ? window : 0;  // wider than any request: none
   const bool few = (int64_t)max(1, step->max_new) * p.group <= kStepRows;
   const int blocks = few ? few_workgroups(cus, cache->head_dim) : many_workgroups(cus);
-  p.min_span = few ? 2 : kItem + 4;
+  p.min_span = few ? 1 : kItem + 1;
   p.scale = scale * kLog2E;
   p.per_group = (65535 + p.group) / p.group;
   p.per_workgroup = 1. / blocks;
