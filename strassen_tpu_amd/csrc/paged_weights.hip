@@ -132,7 +132,9 @@ __device__ __forceinline__ void dma4(const void* from, void* to) {
 }
 
 // Many rows: a workgroup of four waves holds 384 keys, 96 a wave, and its rows pass through LDS, 32 a step, fetched
-// three steps ahead.
+// three steps ahead. Bound by the matrix instructions and what has to run beside them: 2048 rows of 64 heads on 16384
+// keys, 0.58 TFLOP, take 600 us (970 TFLOP/s; with each wave's own reads of the rows from memory 888). Without the reads of LDS
+// it would be 459, without those, the DMA and the barriers 357, at a clock that falls to 2.1 GHz.
 template <int D, bool kWhole>
 __global__ __launch_bounds__(256, 2) void key_weights_many(WeightArgs p) {
   constexpr int kRow = 2 * D, kChunks = D / 8, kLoads = kStepRows * kChunks / 256, kRing = 4;
@@ -403,7 +405,8 @@ struct FewTiles {
 };
 
 // Few rows (at most 32 of a request, decoding): a wave holds them and its keys go by, 32 at a time, through a ring of
-// four tiles in LDS, so that three are on their way. Bound by memory.
+// four tiles in LDS, so that three are on their way. Bound by memory: 64 requests of 64 heads on 4200 keys on average,
+// 550 MB, take 120 us (4.6 TB/s), four on 131,000, 1.1 GB, 221 us (5.0 TB/s).
 template <int D>
 __global__ __launch_bounds__(64) void key_weights_few(WeightArgs p) {
   constexpr int kRow = 2 * D, kChunks = D / 8, kDmaRows = 64 / kChunks, kDmas = 32 / kDmaRows, kRing = 4;
@@ -601,6 +604,8 @@ int smx_paged_key_weights(const smx_paged_cache* cache, const smx_paged_step* st
   p.window = window < SMX_PAGED_MAX_CONTEXT ? window : 0;  // wider than any request: none
   const bool few = (int64_t)max(1, step->max_new) * p.group <= kStepRows;
   const int blocks = few ? few_workgroups(cus, cache->head_dim) : many_workgroups(cus);
+  // Small steps are spread over more workgroups than have whole items: 14 requests of up to 22 tokens take 12.5 us, with spans
+  // of kItem + 4 units 15.6; 3 of up to 465 21.5, with kItem - 1 27.5.
   p.min_span = few ? 1 : kItem + 1;
   p.scale = scale * kLog2E;
   p.per_group = (65535 + p.group) / p.group;

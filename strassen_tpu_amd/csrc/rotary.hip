@@ -17,7 +17,7 @@ struct RotaryArgs {
   const void *x, *positions, *frequencies, *norm;
   void* out;
   int64_t x_token, x_head, out_token, out_head;
-  int32_t tokens, heads, dim, half, flags, zero_rows, per_block;
+  int32_t tokens, heads, dim, half, flags, zero_rows, per_block, heads_each;
   float amplitude, eps;
 };
 
@@ -87,8 +87,8 @@ struct Run {
 
 // Heads whose values fall into aligned runs of 16 bytes: a lane takes two of them, half of the turned (or of the other)
 // values apart, so that a wave's loads are consecutive, and goes from head to head with the next one's on their way (the
-// first one's while the angles are worked out). Bound by memory: 302 MB of bf16 in 53 us, 5.7 TB/s (with the runs of a lane
-// next to each other and no loads ahead 64), 123 MB of float32 in 22 us, 5.6 TB/s (32).
+// first one's while the angles are worked out). Bound by memory: 302 MB of bf16 in 64 us, as long as a copy of them, 123 MB of
+// float32 in 24 us, 5.2 TB/s (with the runs of a lane next to each other and no loads ahead 32).
 template <bool kF32, bool kInterleaved, bool kNorm>
 __global__ __launch_bounds__(256) void rotary_runs(RotaryArgs p) {
   constexpr int kValues = Run<kF32>::kValues;
@@ -105,16 +105,17 @@ __global__ __launch_bounds__(256) void rotary_runs(RotaryArgs p) {
   const int first = turned ? kValues * lane : 2 * p.half + kValues * (lane - turning);
   const int second = first + (turned ? p.half : kValues * ((others + 1) / 2));
   const bool two = second < p.dim;
+  const int head0 = blockIdx.y * p.heads_each, heads = min(p.heads_each, p.heads - head0);
   int row = 0, head = slot;
   auto settle = [&] {
-    while (head >= p.heads) head -= p.heads, ++row;
+    while (head >= heads) head -= heads, ++row;
   };
   settle();
   if (slot >= slots) row = rows;  // (with a norm 256 is a multiple of lanes)
   Run<kF32> wa, wb, a, b;
   auto load = [&] {
     if (row >= rows) return;
-    const int64_t from = (row0 + row) * p.x_token + head * p.x_head;
+    const int64_t from = (row0 + row) * p.x_token + (head0 + head) * p.x_head;
     a.template load<kF32>(p.x, from + first);
     if (two) b.template load<kF32>(p.x, from + second);
   };
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(256) void rotary_runs(RotaryArgs p) {
 
   while (row < rows) {
     const int64_t token = row0 + row;
-    const int64_t to = token * p.out_token + head * p.out_head;
+    const int64_t to = token * p.out_token + (head0 + head) * p.out_head;
     const int angles = row * p.half;
     Run<kF32> x = a, y = b;
     head += slots;
@@ -288,14 +289,18 @@ int smx_rotary(int32_t tokens, int32_t head_dim, int32_t rotary_dim, const smx_h
     return check_launch();
   }
   // Rows of a workgroup: several where enough workgroups remain to fill the chip (72 heads of 128; one, two and four
-  // rows: 6, 8 and 12 us for 16 tokens, 18, 16 and 19 for 2045, 56, 54 and 53 for 8192).
+  // rows: 22, 20 and 23 us for 2045 tokens, 55, 53 and 53 for 8192).
   p.per_block = tokens >= 4096 ? 4 : tokens >= 1536 ? 2 : 1;
   const unsigned blocks = (unsigned)((tokens + p.per_block - 1) / p.per_block);
+  // Of few tokens a row's heads are shared out, as many to a workgroup as it takes at once (72 heads of 128; shared and not:
+  // 4.3 and 6.1 us for 16 tokens, 6.5 and 7.6 for 400, 12.7 and 10.8 for 1000).
+  const int turning = p.half / run, lanes = turning + (head_dim / run - 2 * turning + 1) / 2;
+  p.heads_each = blocks <= 512 ? min(p.heads, max(1, 256 / lanes)) : p.heads;
   const int lds = 2 * p.per_block * p.half * 4;
   const bool wide = flags & SMX_ROTARY_INTERLEAVED;
   auto kern = flags & SMX_ROTARY_F32 ? (wide ? runs_kernel<true, true>(norm) : runs_kernel<true, false>(norm))
                                      : (wide ? runs_kernel<false, true>(norm) : runs_kernel<false, false>(norm));
-  hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), lds, (hipStream_t)stream, p);
+  hipLaunchKernelGGL(kern, dim3(blocks, (unsigned)((p.heads + p.heads_each - 1) / p.heads_each)), dim3(256), lds, (hipStream_t)stream, p);
   return check_launch();
 }
 

@@ -8,7 +8,10 @@
 // on the order of the additions.
 //
 // Work. One row of p and one of q a request, whatever the number of drafts: verify_sums cuts the row in slices, a workgroup
-// each, verify_draw finds the slice that the draw falls in and looks through that slice alone.
+// each, verify_draw finds the slice that the draw falls in and looks through that slice alone. Where requests fill the chip or
+// the vocabulary is small verify_whole does both in one launch. Bound by memory where requests
+// are many: 64 requests with drafts on 151,936 tokens, 78 MB of FP32, take 22 us, 17 of them the sums (4.7 TB/s); one
+// request takes 9.5 us, 8 of them in two launches that wait for a chain of lengths, tokens, their probabilities and the row.
 #include "launch.hpp"
 
 namespace smx {
@@ -112,6 +115,16 @@ struct Row {
     if (draft) return max(p - (double)probability(f.q[j]), 0.);
     return i + j == left_out ? 0. : p;
   }
+  // The sums of a share of the tokens from .. to - 1: thread `mine` of kThreads.
+  template <int kThreads>
+  __device__ __forceinline__ void add(int from, int to, int mine, double& rest, double& whole) const {
+#pragma unroll 4
+    for (int i = from + 4 * mine; i < to; i += 4 * kThreads) {
+      const auto f = load(i, to);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) rest += value(f, i, j, false), whole += value(f, i, j, true);
+    }
+  }
 };
 
 // Sum over a wave's lanes, in every lane.
@@ -132,24 +145,18 @@ __device__ __forceinline__ double lane_scan(double x) {
   return x;
 }
 
-constexpr int kWaves = kVerifyThreads / 64, kRun = 4 * kVerifyThreads;  // tokens that the workgroup loads at once
-
 template <bool kBf16>
 __global__ __launch_bounds__(kVerifyThreads) void verify_sums(VerifyArgs p) {
   const int request = blockIdx.y, fresh = p.rows[request];
-  if (fresh <= 0) return;
   const int64_t start = p.starts[request];
+  if (fresh <= 0) return;
   const int accepted = accepted_of<kBf16>(p, start, fresh - 1);
   if (blockIdx.x == 0 && threadIdx.x == 0) p.accepted[request] = accepted;
   const Row<kBf16> row(p, start, fresh - 1, accepted);
-  const int from = blockIdx.x * p.slice, to = min(p.vocab, from + p.slice);
+  const int from = blockIdx.x * p.slice;
   double rest = 0., whole = 0.;
-#pragma unroll 4
-  for (int i = from + 4 * (int)threadIdx.x; i < to; i += kRun) {
-    const auto f = row.load(i, to);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) rest += row.value(f, i, j, false), whole += row.value(f, i, j, true);
-  }
+  row.template add<kVerifyThreads>(from, min(p.vocab, from + p.slice), threadIdx.x, rest, whole);
+  constexpr int kWaves = kVerifyThreads / 64;
   __shared__ double parts[2][kWaves];
   rest = wave_sum(rest), whole = wave_sum(whole);
   if ((threadIdx.x & 63) == 0) parts[0][threadIdx.x >> 6] = rest, parts[1][threadIdx.x >> 6] = whole;
@@ -165,30 +172,29 @@ __device__ __forceinline__ void emit(const VerifyArgs& p, int64_t row, int64_t t
   if (p.flags & SMX_VERIFY_TOKENS_I64) ((int64_t*)p.out)[row] = token; else ((int32_t*)p.out)[row] = (int32_t)token;
 }
 
-template <bool kBf16>
-__global__ __launch_bounds__(kVerifyThreads) void verify_draw(VerifyArgs p) {
-  const int request = blockIdx.x, fresh = p.rows[request], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // rows of no request
-  for (int64_t r = (int64_t)request * kVerifyThreads + threadIdx.x; r < p.count; r += (int64_t)gridDim.x * kVerifyThreads)
+// Rows of no request, shared out over all workgroups.
+template <int kThreads>
+__device__ __forceinline__ void emit_others(const VerifyArgs& p, int request) {
+  for (int64_t r = (int64_t)request * kThreads + threadIdx.x; r < p.count; r += (int64_t)p.requests * kThreads)
     if (p.positions[r] < 0) emit(p, r, -1);
-  if (fresh <= 0) {
-    if (threadIdx.x == 0) p.counts[request] = 0;
-    return;
-  }
-  const int64_t start = p.starts[request];
-  const int accepted = p.accepted[request];
-  const Row<kBf16> row(p, start, fresh - 1, accepted);
-  // Every wave finds the slice: a lane each (at most 64).
-  const double* const sums = p.sums + (int64_t)request * p.slices * 2;
-  const double mine_rest = lane < p.slices ? sums[2 * lane] : 0., mine_whole = lane < p.slices ? sums[2 * lane + 1] : 0.;
+}
+
+// A request's token, drawn by its slices' sums (at most 64, one a lane: of what is drawn from, and of p alone), and all that it
+// emits.
+template <bool kBf16, int kThreads>
+__device__ __forceinline__ void draw(const VerifyArgs& p, int request, int64_t start, int fresh, int accepted,
+                                     const Row<kBf16>& row, double sample, double mine_rest, double mine_whole) {
+  constexpr int kWaves = kThreads / 64, kRun = 4 * kThreads;  // tokens that the workgroup loads at once
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // Every wave finds the slice.
   const bool plain = !__any(mine_rest > 0.);
   const double mine = plain ? mine_whole : mine_rest, upto = lane_scan(mine);
-  const double goal = (double)p.sample[request] * __shfl(upto, 63);
+  const double goal = sample * __shfl(upto, 63);
   // the first whose running sum passes the goal, or (by rounding, or a number that is not below 1) the last one that
   // holds anything
   const uint64_t any = __ballot(mine > 0.), over = __ballot(mine > 0. && upto > goal);
   if (!any) {
-    for (int i = threadIdx.x; i < fresh; i += kVerifyThreads) emit(p, start + i, i < accepted ? token_at(p, start + i + 1) : -1);
+    for (int i = threadIdx.x; i < fresh; i += kThreads) emit(p, start + i, i < accepted ? token_at(p, start + i + 1) : -1);
     if (threadIdx.x == 0) p.counts[request] = accepted + 1;
     return;
   }
@@ -241,15 +247,73 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw(VerifyArgs p) {
     last = max(last, last_of[w]);
   }
   if (drawn < 0) drawn = last;
-  for (int i = threadIdx.x; i < fresh; i += kVerifyThreads)
+  for (int i = threadIdx.x; i < fresh; i += kThreads)
     emit(p, start + i, i < accepted ? token_at(p, start + i + 1) : i == accepted ? drawn : -1);
   if (threadIdx.x == 0) p.counts[request] = accepted + 1;
 }
 
+template <bool kBf16>
+__global__ __launch_bounds__(kVerifyThreads) void verify_draw(VerifyArgs p) {
+  // (all that does not wait for anything else is read at once; accepted and sums are none of a request without rows)
+  const int request = blockIdx.x, lane = threadIdx.x & 63;
+  const double* const sums = p.sums + (int64_t)request * p.slices * 2;
+  const int fresh = p.rows[request], accepted = p.accepted[request];
+  const int64_t start = p.starts[request];
+  const double sample = p.sample[request];
+  const double rest = lane < p.slices ? sums[2 * lane] : 0., whole = lane < p.slices ? sums[2 * lane + 1] : 0.;
+  if (fresh > 0)
+    draw<kBf16, kVerifyThreads>(p, request, start, fresh, accepted, Row<kBf16>(p, start, fresh - 1, accepted), sample, rest, whole);
+  else if (threadIdx.x == 0)
+    p.counts[request] = 0;
+  emit_others<kVerifyThreads>(p, request);
+}
+
+// The whole of a request by one workgroup, a slice a wave.
+template <bool kBf16, int kThreads>
+__global__ __launch_bounds__(kThreads) void verify_whole(VerifyArgs p) {
+  constexpr int kWaves = kThreads / 64;
+  const int request = blockIdx.x, fresh = p.rows[request], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t start = p.starts[request];
+  const double sample = p.sample[request];
+  if (fresh > 0) {
+    const int accepted = accepted_of<kBf16>(p, start, fresh - 1);
+    const Row<kBf16> row(p, start, fresh - 1, accepted);
+    __shared__ double sums[2][kWaves];
+    double rest = 0., whole = 0.;
+    const int from = wave * p.slice;
+    row.template add<64>(from, min(p.vocab, from + p.slice), lane, rest, whole);
+    rest = wave_sum(rest), whole = wave_sum(whole);
+    if (lane == 0) sums[0][wave] = rest, sums[1][wave] = whole;
+    __syncthreads();
+    draw<kBf16, kThreads>(p, request, start, fresh, accepted, row, sample, lane < kWaves ? sums[0][lane] : 0.,
+                          lane < kWaves ? sums[1][lane] : 0.);
+  } else if (threadIdx.x == 0) {
+    p.counts[request] = 0;
+  }
+  emit_others<kThreads>(p, request);
+}
+
+// Threads of a workgroup that takes the whole of a request, which saves a launch and the second chain of loads; 0: the request is
+// shared out. In us, shared out, of 1024 threads and of 512 (bf16, two drafts looked up):
+//             8 requests         128                200                256                400
+//   2453    9.9  8.7  7.4    10.1  9.1  7.7     10.2  9.3  7.7    10.3  9.1  7.8     11.0 14.9  9.0
+//   8000    9.6  9.1 10.6    10.3  9.4 10.1     10.8  9.5 10.2    10.9  9.5 10.0     14.2 16.1 12.2
+//  32001    9.6 13.4 15.3    14.8 15.6 17.7     18.6 15.8 20.1    21.3 16.0 20.0     27.5 28.6 21.7
+// 151936     11   28   43      30   35   60       38   35   61      47   40   69       77   80   79
+int whole_threads(int vocab, int requests) {
+  constexpr int kCus = 256;
+  if (requests > 2 * kCus) return 0;  // (a second round: 600 requests of 32,001 tokens 37, shared out 32)
+  if (vocab <= 4096) return 512;
+  if (requests > kCus) return vocab <= 65536 ? 512 : 0;
+  return vocab <= 8192 || requests >= 192 ? 1024 : 0;
+}
+
 // Tokens of a slice, a multiple of the workgroup's loads: at most 64 slices, of 2048 tokens at least, and no more
-// than fill the chip with workgroups.
+// than fill the chip with workgroups twice (64 requests 25.4 us, once 26.7; 200 of 32,001 tokens 18.7 and 20.1).
 int slice_of(int vocab, int requests) {
-  const int64_t slices = max(1, min(64, 2048 / requests)), least = ((int64_t)vocab + slices - 1) / slices;
+  if (const int waves = whole_threads(vocab, requests) / 64) return (vocab + 4 * waves - 1) / (4 * waves) * 4;
+  constexpr int kRun = 4 * kVerifyThreads;
+  const int64_t slices = max(1, min(64, 4096 / requests)), least = ((int64_t)vocab + slices - 1) / slices;
   return (int)max((int64_t)2048, (least + kRun - 1) / kRun * kRun);
 }
 int slices_of(int vocab, int requests) {
@@ -301,6 +365,12 @@ int smx_verify_drafts(const smx_paged_step* step, int32_t vocab, const void* tar
   p.sums = (double*)workspace;
   p.accepted = (int32_t*)(p.sums + 2 * (int64_t)p.requests * p.slices);
   const bool bf16 = flags & SMX_VERIFY_BF16;
+  if (const int threads = whole_threads(vocab, p.requests)) {
+    auto kern = threads == 512 ? (bf16 ? verify_whole<true, 512> : verify_whole<false, 512>)
+                               : (bf16 ? verify_whole<true, 1024> : verify_whole<false, 1024>);
+    hipLaunchKernelGGL(kern, dim3((unsigned)p.requests), dim3((unsigned)threads), 0, (hipStream_t)stream, p);
+    return check_launch();
+  }
   hipLaunchKernelGGL(bf16 ? verify_sums<true> : verify_sums<false>, dim3((unsigned)p.slices, (unsigned)p.requests),
                      dim3(kVerifyThreads), 0, (hipStream_t)stream, p);
   if (int rc = check_launch()) return rc;

@@ -101,6 +101,16 @@ def test_verify(new, vocab, dtype, model):
         assert {1, 4} < set(counts)  # some refused at once, some taken whole
 
 
+@pytest.mark.parametrize("requests,vocab,dtype,model", [
+    # a workgroup a request, of 512 threads and of 1024, and requests shared out, on both sides of each border
+    (3, 4096, torch.float32, True), (3, 4097, torch.float32, True), (3, 8192, torch.bfloat16, False), (3, 8193, torch.bfloat16, True),
+    (191, 9001, torch.bfloat16, False), (192, 9001, torch.bfloat16, False), (256, 8001, torch.float32, True),
+    (257, 8001, torch.float32, True), (512, 65536, torch.bfloat16, False), (260, 65537, torch.bfloat16, False),
+    (513, 300, torch.float32, True), (200, 32001, torch.float32, True), (700, 2049, torch.bfloat16, False)])
+def test_requests_whole_and_shared_out(requests, vocab, dtype, model):
+    check([(7 * b + 1) % 4 for b in range(requests)], vocab, dtype, model=model, pad=5)
+
+
 def test_vocabulary_of_more_slices_than_threads():
     check([3, 1], 4_500_001, tokens_dtype=torch.int32)
 
