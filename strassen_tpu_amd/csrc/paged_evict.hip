@@ -780,6 +780,11 @@ int smx_paged_evict(const smx_paged_cache* cache, float* key_weights, int32_t re
   if (meet(keys, values)) return fail(SMX_ERR_INVALID, "keys and values must share no memory of the cache");
   const Runs all{key_weights, 2 * (int64_t)cache->num_pages * cache->kv_heads * cache->page_size, {{1, 0}, {1, 0}, {1, 0}}};
   if (meet(all, keys) || meet(all, values)) return fail(SMX_ERR_INVALID, "key_weights must share no memory with the cache");
+  // lens are written while other workgroups read the lengths
+  const auto list = [](const void* at, int64_t entries) { return Runs{at, 2 * entries, {{1, 0}, {1, 0}, {1, 0}}}; };
+  if (meet(list(lens, requests), list(context_lens, requests)) || (keep_lens && meet(list(lens, requests), list(keep_lens, requests))) ||
+      meet(list(lens, requests), list(block_tables, (requests - 1) * table_stride + width)))
+    return fail(SMX_ERR_INVALID, "lens must share no memory with context_lens, keep_lens and block_tables");
   EvictArgs p{};
   p.k = (uint16_t*)cache->k, p.v = (uint16_t*)cache->v;
   p.page_stride = cache->page_stride, p.slot_stride = cache->slot_stride, p.head_stride = cache->head_stride;

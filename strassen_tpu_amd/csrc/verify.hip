@@ -357,6 +357,9 @@ int smx_verify_drafts(const smx_paged_step* step, int32_t vocab, const void* tar
     return fail(SMX_ERR_INVALID, "misaligned probabilities, tokens, random numbers or counts");
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)
     return fail(SMX_ERR_INVALID, "the call needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+  const int64_t units = (int64_t)step->tokens * (flags & SMX_VERIFY_TOKENS_I64 ? 4 : 2);
+  const auto list = [&](const void* at) { return Runs{at, units, {{1, 0}, {1, 0}, {1, 0}}}; };
+  if (meet(list(out), list(tokens))) return fail(SMX_ERR_INVALID, "out and tokens must share no memory");
   VerifyArgs p{};
   p.target = target, p.draft = draft, p.target_row = target_row, p.draft_row = draft_row, p.tokens = tokens;
   p.starts = step->starts, p.rows = step->rows, p.positions = step->positions, p.accept = accept, p.sample = sample;

@@ -257,8 +257,8 @@ def test_past_32_bit_offsets():
     assert same(both[used][:, 0], want[0]) and same(both[used][:, 1], want[1]) and same(weights[used], want[2])
 
 
-def test_in_a_graph_and_on_two_streams():
-    context = [500, 77, 900]
+@pytest.mark.parametrize("context", [[500, 77, 900], [40000, 33]])
+def test_in_a_graph_and_on_two_streams(context):
     first = make_cache(context, seed=14)
     second = make_cache(context, seed=15)
     masters = [[x.clone() for x in c[:3]] for c in (first, second)]

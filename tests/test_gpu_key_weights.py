@@ -262,6 +262,25 @@ def test_queries_of_odd_strides(max_new):
     assert all(torch.equal(r, results[0]) for r in results)
 
 
+@pytest.mark.parametrize("max_new", [None, 1])
+@pytest.mark.parametrize("far", ["tokens", "heads"])
+def test_queries_far_from_each_other(max_new, far):
+    """Strides beyond the kernel's offsets within a step's rows."""
+    context, new = [300, 40], [1, 1]
+    plan, k, v, *_, g = make_step(context, new, page=16, kv_heads=2, dim=64)
+    plan = smx.paged_plan(i32(context), i32(new), plan.block_tables, page_size=16, num_pages=plan.num_pages, tokens=2, max_new=max_new)
+    q = torch.randn(2, 8, 64, device=DEV, generator=g).to(torch.bfloat16)
+    strides = ((1 << 29) + 8, 64, 1) if far == "tokens" else (64, (1 << 27) + 8, 1)
+    view = torch.empty(strides[0] + 7 * strides[1] + 64, dtype=torch.bfloat16, device=DEV).as_strided((2, 8, 64), strides)
+    view.copy_(q)
+    lse = torch.empty(2, 8, device=DEV)
+    smx.paged_attention(q, k, v, plan, lse=lse)
+    results = [torch.zeros(k.shape[0], 2, 16, device=DEV) for _ in range(2)]
+    for x, weights in zip((q, view), results):
+        smx.paged_key_weights(x, k, weights, plan, lse)
+    assert torch.equal(*results) and results[0].any()
+
+
 @pytest.mark.parametrize("max_new", [1, 40])
 def test_in_a_graph(max_new):
     """Replays after lengths, tables, queries and keys changed in place, eager work between; two graphs at once keep

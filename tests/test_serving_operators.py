@@ -73,6 +73,7 @@ def _verify(step=None, vocab=100, target=P, target_row=100, draft=None, draft_ro
     (dict(draft=P + 2, draft_row=100), "misaligned"), (dict(tokens=P + 4, flags=2), "misaligned"), (dict(out=P + 4, flags=2), "misaligned"),
     (dict(accept=P + 2), "misaligned"), (dict(sample=P + 1), "misaligned"), (dict(counts=P + 2), "misaligned"),
     (dict(workspace=None), "workspace"), (dict(workspace=P + 8), "workspace"), (dict(size=16), "workspace"),
+    (dict(out=P + 28), "share no memory"), (dict(tokens=P + 56, flags=2), "share no memory"),
 ])
 def test_verify_refusals(change, message):
     refused(_verify(**change), message)
@@ -94,6 +95,8 @@ def _evict(cache=None, weights=FAR, requests=2, width=4, context=P, tables=P, st
     (dict(cache=_cache(k=OUT, v=OUT + (1 << 24), page_stride=16 * 256 - 128)), "each other"),
     (dict(cache=_cache(k=OUT, v=OUT)), "keys and values"), (dict(cache=_cache(k=OUT, v=OUT + 256)), "keys and values"),
     (dict(weights=OUT + 1024), "key_weights must share"), (dict(weights=OUT + (1 << 24) - 16), "key_weights must share"),
+    (dict(context=1 << 20, tables=1 << 21, lens=(1 << 20) + 4), "lens must share"), (dict(context=1 << 20, tables=1 << 21, lens=(1 << 21) + 28), "lens must share"),
+    (dict(context=1 << 20, tables=1 << 21, keep_lens=P), "lens must share"),
 ])
 def test_evict_refusals(change, message):
     refused(_evict(**change), message)
