@@ -132,9 +132,10 @@ __device__ __forceinline__ void dma4(const void* from, void* to) {
 }
 
 // Many rows: a workgroup of four waves holds 384 keys, 96 a wave, and its rows pass through LDS, 32 a step, fetched
-// three steps ahead. Bound by the matrix instructions and what has to run beside them: 2048 rows of 64 heads on 16384
-// keys, 0.58 TFLOP, take 600 us (970 TFLOP/s; with each wave's own reads of the rows from memory 888). Without the reads of LDS
-// it would be 459, without those, the DMA and the barriers 357, at a clock that falls to 2.1 GHz.
+// three steps ahead. Bound by the matrix instructions, the vector work beside them and the power that both draw: 2048 rows of
+// 64 heads on 16384 keys, 0.58 TFLOP, take 600 us (970 TFLOP/s; with each wave's own reads of the rows from memory 888) at a
+// clock that falls to 2.0 GHz; 485 where all values are zero. More blocks of keys or a deeper pipeline in a wave did not
+// shorten it.
 template <int D, bool kWhole>
 __global__ __launch_bounds__(256, 2) void key_weights_many(WeightArgs p) {
   constexpr int kRow = 2 * D, kChunks = D / 8, kLoads = kStepRows * kChunks / 256, kRing = 4;
