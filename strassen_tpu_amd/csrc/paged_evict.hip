@@ -198,6 +198,7 @@ struct Near {
     const uint32_t mine = (int)threadIdx.x < all ? key[threadIdx.x] : 0;
     if (mine) {
       int larger = 0, equal = 0;
+#pragma unroll 4
       for (int x = 0; x < all; x += 4) {
         const u32x4 other = *reinterpret_cast<const u32x4*>(key + x);
 #pragma unroll
@@ -538,7 +539,7 @@ __global__ __launch_bounds__(kPartThreads) void evict_list(EvictArgs p) {
   const int64_t pair = (int64_t)request * p.kv_heads + head;
   __shared__ Look look;
   __shared__ Near near;
-  __shared__ int sums[kPartWaves + 1][4], early;
+  __shared__ int early;
   Cut c;
   if (!c.of(p, request)) return;
   const int parts = max(1, parts_of(c));
@@ -555,7 +556,6 @@ __global__ __launch_bounds__(kPartThreads) void evict_list(EvictArgs p) {
   load_keys(p, table, head, begin, kQuads, c.m, keys, missing);
   near.clear();
   look.clear();
-  if (threadIdx.x < 4 * (kPartWaves + 1)) (&sums[0][0])[threadIdx.x] = 0;
   if (threadIdx.x == 0) early = 0;
   __syncthreads();
   // The edge, among the candidates (every workgroup finds it for itself).
@@ -589,38 +589,29 @@ __global__ __launch_bounds__(kPartThreads) void evict_list(EvictArgs p) {
       edge = near.resolve(&ties);
     }
   }
-  // Before each wave's indices, and (the last) in all: places for certain, survivors for certain, and of the keys equal to the
-  // edge those below need, and all.
-  const int* const counts = p.counts + pair * p.parts * kPartWaves * 4;
-#pragma unroll
-  for (int b = 0; b <= kPartWaves; ++b) {
-    const int upto = b == kPartWaves ? parts * kPart : part * kPart + b * (kPart / kPartWaves);
-    int before[4] = {0, 0, 0, 0};
-    const int w = threadIdx.x;  // (at most 256 waves)
-    if (w < upto / (kPart / kPartWaves)) {
-      before[0] = counts[4 * w], before[1] = counts[4 * w + 1];
-      if (!apart) before[2] = counts[4 * w + 2], before[3] = counts[4 * w + 2] + counts[4 * w + 3];
-    }
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      if (i * kPartThreads < crowd) {  // uniform
-        const uint32_t key = mine[i].key;
-        const int at = mine[i].at;
-        const bool in = key && at < upto, front = at < c.need;
-        before[0] += in && key < edge && front, before[1] += in && key > edge && !front;
-        before[2] += in && key == edge && front, before[3] += in && key == edge;
-      }
-    }
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int sum = lane_scan(before[x]);
-      if (lane == 63) atomicAdd(&sums[b][x], sum);
-    }
+  // Before the wave's indices: places for certain, survivors for certain, and of the keys equal to the edge those below
+  // need, and all.
+  typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+  const i32x4* const counts = reinterpret_cast<const i32x4*>(p.counts) + pair * p.parts * kPartWaves;
+  const Candidate* const candidates = p.candidates + pair * kCrowd;
+  int before[4] = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int w = lane; w < part * kPartWaves + wave; w += 64) {
+    const i32x4 of = counts[w];
+    before[0] += of[0], before[1] += of[1];
+    if (!apart) before[2] += of[2], before[3] += of[2] + of[3];
   }
-  __syncthreads();
-  auto places = [&](int b) { return sums[b][0] + sums[b][2] - min(ties, sums[b][2]); };
-  auto sources = [&](int b) { return sums[b][1] + min(ties, sums[b][3]) - min(ties, sums[b][2]); };
-  int seen = sums[wave][3], to = places(wave), from = sources(wave), mine_early = 0;
+#pragma unroll 4
+  for (int i = lane; i < crowd; i += 64) {
+    const Candidate x = candidates[i];
+    const bool in = x.at < begin, front = x.at < c.need;
+    before[0] += in && x.key < edge && front, before[1] += in && x.key > edge && !front;
+    before[2] += in && x.key == edge && front, before[3] += in && x.key == edge;
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x) before[x] = __builtin_amdgcn_readlane(lane_scan(before[x]), 63);
+  int seen = before[3], to = before[0] + before[2] - min(ties, before[2]), mine_early = 0;
+  int from = before[1] + min(ties, before[3]) - min(ties, before[2]);
   int32_t* const fill = lists_of(p, pair);
 #pragma unroll
   for (int i = 0; i < kQuads; ++i)
@@ -631,8 +622,9 @@ __global__ __launch_bounds__(kPartThreads) void evict_list(EvictArgs p) {
   if (threadIdx.x == 0) {
     Found* const found = p.found + pair;
     if (early) atomicAdd(&found->early, early);
-    if (part == 0) found->count = min(sources(kPartWaves), p.moves), found->recent = c.recent, found->from = c.m, found->to = c.need;
+    if (part == 0) found->recent = c.recent, found->from = c.m, found->to = c.need;
   }
+  if (part == parts - 1 && threadIdx.x == kPartThreads - 1) p.found[pair].count = min(from, p.moves);  // behind the last wave: all
 }
 
 constexpr int kMoveThreads = 256, kAhead = 4;
@@ -715,11 +707,11 @@ int moves_of(int keep, bool given, int max_context) {
 }
 
 // Parts of the longest context where it is long and the heads are few; 0: one workgroup a head and request. Selection
-// took, of one workgroup and of parts: 31 and 36 us for 8 heads of 32,000 tokens, which sixteen waves hold in registers, 100 and 43
-// for 32 heads of 131,000, and 119 and 124 for 128 of them, which fill half the chip as they are.
+// took, of one workgroup and of parts: 30 and 32 us for 8 heads of 32,000 tokens, which sixteen waves hold in registers, 100 and 40
+// for 32 heads of 131,000, 119 and 110 for 128 of them, and 331 and 43 for 8 of 500,000.
 int parts_of(int64_t pairs, int max_context) {
   const int64_t parts = ((int64_t)max_context + kPart - 1) / kPart;
-  return max_context > 1024 * 4 * kQuads && parts <= kMostParts && pairs < 128 ? (int)parts : 0;
+  return max_context > 1024 * 4 * kQuads && parts <= kMostParts && pairs <= 128 ? (int)parts : 0;
 }
 
 // Where the workspace's pieces lie, behind each other; the last is its size.

@@ -189,7 +189,7 @@ def test_a_bound_beyond_the_parts():
     """The longest contexts that are allowed for, whatever the requests hold."""
     k, v, weights, lens, tables = make_cache([9000, 100], page=1024, kv_heads=2, seed=23, width=600)
     check((k, v, weights, lens, tables), [9000, 100], 500, 20)
-    k, v, weights, lens, tables = make_cache([40000, 9000], page=1024, kv_heads=64, seed=24)  # many heads
+    k, v, weights, lens, tables = make_cache([40000, 9000], page=1024, kv_heads=65, seed=24)  # many heads
     check((k, v, weights, lens, tables), [40000, 9000], 5000, 20)
 
 
