@@ -405,12 +405,12 @@ struct FewTiles {
   __device__ int64_t all() const { return fresh > 0 ? steps + 1 : 0; }  // one for its start
 };
 
-// Few rows (at most 32 of a request, decoding): a wave holds them and its keys go by, 32 at a time, through a ring of
-// four tiles in LDS, so that three are on their way. Bound by memory: 64 requests of 64 heads on 4200 keys on average,
-// 550 MB, take 120 us (4.6 TB/s), four on 131,000, 1.1 GB, 221 us (5.0 TB/s).
+// Few rows (at most 32 of a request, decoding): a wave holds them and its keys go by, 32 at a time, through two tiles in
+// LDS, one on its way while the other is weighed. Bound by memory: 64 requests of 64 heads on 4200 keys on average, 550 MB,
+// take 118 us (4.7 TB/s), four on 131,000, 1.1 GB, 222 us (5.0 TB/s); without the stores of the weights 104 and 192.
 template <int D>
 __global__ __launch_bounds__(64) void key_weights_few(WeightArgs p) {
-  constexpr int kRow = 2 * D, kChunks = D / 8, kDmaRows = 64 / kChunks, kDmas = 32 / kDmaRows, kRing = 4;
+  constexpr int kRow = 2 * D, kChunks = D / 8, kDmaRows = 64 / kChunks, kDmas = 32 / kDmaRows, kRing = 2;
   constexpr int kSlot = 32 * kRow + 256;  // a tile's keys, and its weights before the step (twice)
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x, half = lane >> 5;
@@ -507,7 +507,7 @@ __global__ __launch_bounds__(64) void key_weights_few(WeightArgs p) {
 #pragma unroll
       for (int i = 0; i < kRing - 1; ++i) entry[i] = fetch(i);
       for (int i = 0; i < count; ++i) {
-        // all but the fetches of the two tiles behind this one
+        // all but the fetches of the tiles behind this one
         asm volatile("s_waitcnt vmcnt(%0)" ::"i"((kRing - 2) * (kDmas + 1)) : "memory");
         __builtin_amdgcn_sched_barrier(0);
         entry[kRing - 1] = fetch(i + kRing - 1);
@@ -525,11 +525,12 @@ __global__ __launch_bounds__(64) void key_weights_few(WeightArgs p) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA outlives the wave
 }
 
-// Workgroups of a launch, a multiple of the 8 XCDs. Of few rows as many as a CU holds, by their LDS (33 KB at head_dim
-// 128, of which five would fit but not even out: 222 us for four contexts of 131,000 tokens, with eight 235). Of many rows
+// Workgroups of a launch, a multiple of the 8 XCDs. Of few rows as many as a CU holds, by their LDS (17 KB at head_dim 128,
+// of which nine would fit but not even out: four contexts of 131,000 tokens 222 us, with nine 225). With rings of four tiles
+// and half as many waves 64 requests took 120 us in place of 118, 18 requests of head_dim 64 37 in place of 35. Of many rows
 // twice as many: a CU serves the workgroup that came first before the other, so that the last ones run alone
 // (2048 rows of 64 heads on 16384 keys: 672 us with as many as fit, 604 with twice as many, 605 with four times).
-int few_workgroups(int cus, int head_dim) { return ((head_dim == 128 ? 4 : 8) * cus + 7) / 8 * 8; }
+int few_workgroups(int cus, int head_dim) { return ((head_dim == 128 ? 8 : 16) * cus + 7) / 8 * 8; }
 int many_workgroups(int cus) { return (4 * cus + 7) / 8 * 8; }
 
 int64_t workspace_of(int cus) { return many_workgroups(cus) * (int64_t)(sizeof(WeightRecord) + 2 * 4 * kTile); }
@@ -538,7 +539,7 @@ template <int D>
 int launch_weights(const WeightArgs& p, bool few, unsigned blocks, hipStream_t stream) {
   auto many = kStepRows % p.group == 0 ? key_weights_many<D, true> : key_weights_many<D, false>;
   hipLaunchKernelGGL(few ? key_weights_few<D> : many, dim3(blocks), dim3(few ? 64 : 256),
-                     few ? 4 * (32 * 2 * D + 256) : 4 * (kStepRows * 2 * D + 4 * 256), stream, p);
+                     few ? 2 * (32 * 2 * D + 256) : 4 * (kStepRows * 2 * D + 4 * 256), stream, p);
   if (int rc = check_launch()) return rc;
   if (few) return SMX_OK;
   hipLaunchKernelGGL(key_weights_join, dim3(blocks), dim3(kTile), 0, stream, p);
