@@ -519,8 +519,9 @@ int smx_paged_key_weights_workspace_bytes(int64_t* bytes);
  * was. keep is keep_lens[b] where keep_lens is not NULL. lens [requests] becomes keep, or n where nothing is cut: n <= keep,
  * n over max_context, a negative length, or a page of the request that is not in the cache. block_tables is not
  * changed: the pages behind the last kept token are the caller's to reuse. Requests share no pages. The cache's rows lie apart
- * from each other and from key_weights, and lens from context_lens, keep_lens and block_tables. workspace: smx_paged_evict_workspace_bytes, with the same keep (-1 with
- * keep_lens) and max_context, which bounds the contexts and is at most width * page_size. Asynchronous on stream.
+ * from each other and from key_weights, and lens from context_lens, keep_lens and block_tables. workspace:
+ * smx_paged_evict_workspace_bytes, with the same keep (-1 with keep_lens) and max_context, which bounds the contexts and is
+ * at most width * page_size. Asynchronous on stream.
  */
 int smx_paged_evict(const smx_paged_cache* cache, float* key_weights, int32_t requests, int32_t width,
                     const int32_t* context_lens, const int32_t* block_tables, int64_t table_stride,

@@ -153,7 +153,7 @@ def paged_evict(k_cache, v_cache, key_weights, context_lens, block_tables, keep,
 
     A request is left as it was, and its length returned, if it holds ``keep`` tokens or fewer, if a
     length is negative or above ``max_context`` (default: what the tables hold; it sizes the call's workspace,
-    4 to 8 bytes a token and head), or if a table entry of its tokens is no page of the cache. ``block_tables`` is not
+    about 5 bytes a token and head), or if a table entry of its tokens is no page of the cache. ``block_tables`` is not
     changed: pages behind the last kept token stay the request's, for its next tokens or for the program to
     take back. Requests must not share pages."""
     return _lib.host().evict(k_cache, v_cache, key_weights, context_lens, block_tables, keep, recent, max_context)
