@@ -121,10 +121,12 @@ __device__ __forceinline__ float* weight_of(const WeightArgs& p, int page, int k
 // Register e of half h holds row 8 (e / 4) + 4 h + e % 4 of a step.
 __device__ __forceinline__ int row_of_register(int e, int half) { return 8 * (e >> 2) + 4 * half + (e & 3); }
 
-// Sixteen or four bytes a lane from memory into LDS, lane l's at `to` + its size times l.
+// Sixteen or four bytes a lane from memory into LDS, lane l's at `to` + its size times l. kOnce: nothing reads them again soon,
+// and they need not push out of the caches what is written there.
+template <bool kOnce = false>
 __device__ __forceinline__ void dma16(const void* from, void* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)from,
-                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, kOnce ? 2 : 0);
 }
 __device__ __forceinline__ void dma4(const void* from, void* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(uintptr_t)from,
@@ -406,8 +408,9 @@ struct FewTiles {
 };
 
 // Few rows (at most 32 of a request, decoding): a wave holds them and its keys go by, 32 at a time, through two tiles in
-// LDS, one on its way while the other is weighed. Bound by memory: 64 requests of 64 heads on 4200 keys on average, 550 MB,
-// take 118 us (4.7 TB/s), four on 131,000, 1.1 GB, 222 us (5.0 TB/s); without the stores of the weights 104 and 192.
+// LDS, one on its way while the other is weighed. Keys are loaded as such that are read once, so that the weights written wait
+// in the caches for more of their kind. Bound by memory: 64 requests of 64 heads on 4200 keys on average, 550 MB, take 108 us
+// (5.1 TB/s; keys loaded like any others 118), four on 131,000, 1.1 GB, 202 us (5.5 TB/s; 222).
 template <int D>
 __global__ __launch_bounds__(64) void key_weights_few(WeightArgs p) {
   constexpr int kRow = 2 * D, kChunks = D / 8, kDmaRows = 64 / kChunks, kDmas = 32 / kDmaRows, kRing = 2;
@@ -465,7 +468,7 @@ __global__ __launch_bounds__(64) void key_weights_few(WeightArgs p) {
           const uint8_t* const base = reinterpret_cast<const uint8_t*>(
               p.k + page * p.page_stride + (int64_t)(key & ((1 << p.page_shift) - 1)) * p.slot_stride + (int64_t)s.head * p.head_stride);
 #pragma unroll
-          for (int x = 0; x < 8 / kDmaRows; ++x) dma16(base + at[g & 1][x], to + (g * 8 + x * kDmaRows) * kRow);
+          for (int x = 0; x < 8 / kDmaRows; ++x) dma16<true>(base + at[g & 1][x], to + (g * 8 + x * kDmaRows) * kRow);
         }
         const int key = key0 + (lane & 31), entry = __shfl(entries, (key >> p.page_shift) - first_page);
         dma4(weight_of(p, (uint32_t)entry < (uint32_t)p.num_pages ? entry : 0, key, s.head), to + 32 * kRow);
@@ -526,8 +529,8 @@ __global__ __launch_bounds__(64) void key_weights_few(WeightArgs p) {
 }
 
 // Workgroups of a launch, a multiple of the 8 XCDs. Of few rows as many as a CU holds, by their LDS (17 KB at head_dim 128,
-// of which nine would fit but not even out: four contexts of 131,000 tokens 222 us, with nine 225). With rings of four tiles
-// and half as many waves 64 requests took 120 us in place of 118, 18 requests of head_dim 64 37 in place of 35. Of many rows
+// of which nine would fit but not even out). With rings of four tiles and half as many waves 64 requests took 120 us in place of
+// 118, 18 requests of head_dim 64 37 in place of 35 (both before keys were loaded as read once). Of many rows
 // twice as many: a CU serves the workgroup that came first before the other, so that the last ones run alone
 // (2048 rows of 64 heads on 16384 keys: 672 us with as many as fit, 604 with twice as many, 605 with four times).
 int few_workgroups(int cus, int head_dim) { return ((head_dim == 128 ? 8 : 16) * cus + 7) / 8 * 8; }
