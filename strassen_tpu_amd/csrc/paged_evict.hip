@@ -638,11 +638,23 @@ __device__ __forceinline__ float* weight_at(const EvictArgs& p, int slot, int he
   return p.weights + ((((int64_t)(slot >> p.page_shift) * p.kv_heads + head) << p.page_shift) + (slot & ((1 << p.page_shift) - 1)));
 }
 
+// kOnce: as values that are not wanted again soon.
+template <bool kOnce>
+__device__ __forceinline__ u32x4 load_row(const uint16_t* from) {
+  const u32x4* const at = reinterpret_cast<const u32x4*>(from);
+  return kOnce ? __builtin_nontemporal_load(at) : *at;
+}
+template <bool kOnce>
+__device__ __forceinline__ void store_row(uint16_t* to, u32x4 x) {
+  u32x4* const at = reinterpret_cast<u32x4*>(to);
+  if constexpr (kOnce) __builtin_nontemporal_store(x, at); else *at = x;
+}
+
 // The rows on a head's lists, and its recent ones. The first p.tails workgroups of a head and request take the recent rows, each
 // a share of a row's columns: first the survivors out of the places where those go, then the recent ones from the
 // front on, all of a block read before any of it is written, since their old and new places may overlap. The other
 // workgroups share the rest of the lists. No other two rows meet: bound by memory.
-template <int D>
+template <int D, bool kOnce>
 __global__ __launch_bounds__(kMoveThreads) void evict_move(EvictArgs p) {
   constexpr int kChunks = D / 8;  // of 16 bytes in a row of keys, and as many of values
   const int pair = blockIdx.x, head = pair % p.kv_heads, request = pair / p.kv_heads;
@@ -659,10 +671,10 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move(EvictArgs p) {
       u32x4 value[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        if (j + u * rows < last) value[u] = *reinterpret_cast<const u32x4*>(row_at(p, cache, take[j + u * rows], head));
+        if (j + u * rows < last) value[u] = load_row<kOnce>(row_at(p, cache, take[j + u * rows], head));
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        if (j + u * rows < last) *reinterpret_cast<u32x4*>(row_at(p, cache, fill[j + u * rows], head)) = value[u];
+        if (j + u * rows < last) store_row<kOnce>(row_at(p, cache, fill[j + u * rows], head), value[u]);
     }
   };
   if (!tail) {
@@ -684,7 +696,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move(EvictArgs p) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int at = i + u * rows + row;
-      if (at < f.recent) value[u] = *reinterpret_cast<const u32x4*>(row_at(p, cache, slot_of(f.from + at), head));
+      if (at < f.recent) value[u] = load_row<kOnce>(row_at(p, cache, slot_of(f.from + at), head));
     }
     const int at_weight = i + (int)threadIdx.x;
     const bool weighs = blockIdx.y == 0 && (int)threadIdx.x < rows * kAhead && at_weight < f.recent;
@@ -695,7 +707,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move(EvictArgs p) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int at = i + u * rows + row;
-      if (at < f.recent) *reinterpret_cast<u32x4*>(row_at(p, cache, slot_of(f.to + at), head)) = value[u];
+      if (at < f.recent) store_row<kOnce>(row_at(p, cache, slot_of(f.to + at), head), value[u]);
     }
     if (weighs) *weight_at(p, slot_of(f.to + at_weight), head) = weight;
   }
@@ -807,8 +819,12 @@ int smx_paged_evict(const smx_paged_cache* cache, float* key_weights, int32_t re
   // as many, 149 of a quarter).
   p.tails = cache->head_dim / 32;
   p.movers = min((p.moves + 63) / 64, max(1, 16384 / pairs));
-  hipLaunchKernelGGL(cache->head_dim == 128 ? evict_move<128> : evict_move<64>, dim3((unsigned)pairs, (unsigned)(p.tails + p.movers)),
-                     dim3(kMoveThreads), 0, (hipStream_t)stream, p);
+  // Rows that do not fit into the caches anyway pass them by: four prompts of 131,000 216 us (else 227), 64 requests 133 (138), 47 of
+  // which 100 MB may move 59.6 (63.0); but 45 requests with 20 MB 26.0 (23.0), 31 with 14 MB 23.0 (21.0).
+  const bool once = (int64_t)pairs * (p.moves + min(recent, max_context)) * 4 * p.head_dim > (64 << 20);
+  auto move = cache->head_dim == 128 ? (once ? evict_move<128, true> : evict_move<128, false>)
+                                     : (once ? evict_move<64, true> : evict_move<64, false>);
+  hipLaunchKernelGGL(move, dim3((unsigned)pairs, (unsigned)(p.tails + p.movers)), dim3(kMoveThreads), 0, (hipStream_t)stream, p);
   return check_launch();
 }
 
