@@ -57,18 +57,20 @@ struct Run {
   static constexpr int kValues = kF32 ? 4 : 8;
   float v[kValues];
 
-  template <bool kFrom32>
+  template <bool kFrom32, bool kOnce = false>
   __device__ __forceinline__ void load(const void* p, int64_t at) {
     if constexpr (kFrom32) {
 #pragma unroll
       for (int j = 0; j < kValues / 4; ++j) {
-        const f32x4 x = reinterpret_cast<const f32x4*>((const float*)p + at)[j];
+        const f32x4* const from = reinterpret_cast<const f32x4*>((const float*)p + at) + j;
+        const f32x4 x = kOnce ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[4 * j + i] = x[i];
       }
     } else {
       typedef uint32_t Words __attribute__((ext_vector_type(kValues / 2)));
-      const Words x = *reinterpret_cast<const Words*>((const uint16_t*)p + at);
+      const Words* const from = reinterpret_cast<const Words*>((const uint16_t*)p + at);
+      const Words x = kOnce ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
       for (int i = 0; i < kValues / 2; ++i) v[2 * i] = lo_f32(x[i]), v[2 * i + 1] = hi_f32(x[i]);
     }
@@ -87,9 +89,9 @@ struct Run {
 
 // Heads whose values fall into aligned runs of 16 bytes: a lane takes two of them, half of the turned (or of the other)
 // values apart, so that a wave's loads are consecutive, and goes from head to head with the next one's on their way (the
-// first one's while the angles are worked out). Bound by memory: 302 MB of bf16 in 64 us, as long as a copy of them, 123 MB of
-// float32 in 24 us, 5.2 TB/s (with the runs of a lane next to each other and no loads ahead 32).
-template <bool kF32, bool kInterleaved, bool kNorm>
+// first one's while the angles are worked out). Bound by memory: 302 MB of bf16 in 54 us, 5.5 TB/s, 123 MB of float32 in 24 us,
+// 5.2 TB/s (with the runs of a lane next to each other and no loads ahead 32).
+template <bool kF32, bool kInterleaved, bool kNorm, bool kOnce>
 __global__ __launch_bounds__(256) void rotary_runs(RotaryArgs p) {
   constexpr int kValues = Run<kF32>::kValues;
   extern __shared__ __attribute__((aligned(16))) float rotary_lds[];
@@ -116,8 +118,8 @@ __global__ __launch_bounds__(256) void rotary_runs(RotaryArgs p) {
   auto load = [&] {
     if (row >= rows) return;
     const int64_t from = (row0 + row) * p.x_token + (head0 + head) * p.x_head;
-    a.template load<kF32>(p.x, from + first);
-    if (two) b.template load<kF32>(p.x, from + second);
+    a.template load<kF32, kOnce>(p.x, from + first);
+    if (two) b.template load<kF32, kOnce>(p.x, from + second);
   };
 #pragma unroll
   for (int i = 0; i < kValues; ++i) a.v[i] = b.v[i] = 0.f;
@@ -224,8 +226,9 @@ __global__ __launch_bounds__(256) void rotary_values(RotaryArgs p) {
 }
 
 template <bool kF32, bool kInterleaved>
-auto runs_kernel(bool norm) {
-  return norm ? rotary_runs<kF32, kInterleaved, true> : rotary_runs<kF32, kInterleaved, false>;
+auto runs_kernel(bool norm, bool once) {
+  return norm ? (once ? rotary_runs<kF32, kInterleaved, true, true> : rotary_runs<kF32, kInterleaved, true, false>)
+              : (once ? rotary_runs<kF32, kInterleaved, false, true> : rotary_runs<kF32, kInterleaved, false, false>);
 }
 
 // Overlap checks count in two-byte units.
@@ -297,9 +300,12 @@ int smx_rotary(int32_t tokens, int32_t head_dim, int32_t rotary_dim, const smx_h
   const int turning = p.half / run, lanes = turning + (head_dim / run - 2 * turning + 1) / 2;
   p.heads_each = blocks <= 512 ? min(p.heads, max(1, 256 / lanes)) : p.heads;
   const int lds = 2 * p.per_block * p.half * 4;
+  // Heads that do not fit into the caches (256 MB) together with the result leave them to the result, which is read next: 302 MB in
+  // calls one behind another 54 us (else 65), 270 MB 47 (58); but 80 MB, which fit, 24 (21).
+  const bool once = x->data != out->data && 2 * (int64_t)size * tokens * p.heads * head_dim > (int64_t)200 << 20;
   const bool wide = flags & SMX_ROTARY_INTERLEAVED;
-  auto kern = flags & SMX_ROTARY_F32 ? (wide ? runs_kernel<true, true>(norm) : runs_kernel<true, false>(norm))
-                                     : (wide ? runs_kernel<false, true>(norm) : runs_kernel<false, false>(norm));
+  auto kern = flags & SMX_ROTARY_F32 ? (wide ? runs_kernel<true, true>(norm, once) : runs_kernel<true, false>(norm, once))
+                                     : (wide ? runs_kernel<false, true>(norm, once) : runs_kernel<false, false>(norm, once));
   hipLaunchKernelGGL(kern, dim3(blocks, (unsigned)((p.heads + p.heads_each - 1) / p.heads_each)), dim3(256), lds, (hipStream_t)stream, p);
   return check_launch();
 }
