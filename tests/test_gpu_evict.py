@@ -193,6 +193,13 @@ def test_a_bound_beyond_the_parts():
     check((k, v, weights, lens, tables), [40000, 9000], 5000, 20)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_more_rows_than_the_caches_hold(dim):
+    """By the bound on what may move; the requests are of every kind."""
+    context = [9000, 8001, 8000, 300, 0]
+    check(make_cache(context, page=1024, kv_heads=8, dim=dim, seed=25, width=20), context, 8000, 700)
+
+
 def test_a_long_recent_part_moves_over_itself():
     for shift in (1, 3, 129, 1000):
         context = [4000 + shift]

@@ -91,6 +91,23 @@ def test_rotary_behind_a_norm(dim, rotated, dtype, norm_dtype, interleaved):
     check(smx.rotary(x, positions, frequencies, **args), want, size)
 
 
+@pytest.mark.parametrize("dtype,norm,interleaved", [(torch.bfloat16, False, False), (torch.bfloat16, True, True), (torch.float32, True, False),
+                                                    (torch.float32, False, True)])
+def test_rotary_of_more_than_the_caches_hold(dtype, norm, interleaved):
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(4111 if dtype == torch.bfloat16 else 2051, 103, 128, device=DEV, generator=g).to(dtype)
+    assert 2 * x.numel() * x.element_size() > 200 << 20
+    positions = torch.randint(-1, 100000, (x.shape[0],), device=DEV, generator=g)
+    positions[7] = -3
+    frequencies, _ = smx.rotary_frequencies(64, device=DEV)
+    args = dict(interleaved=interleaved, norm=1 + 0.1 * torch.randn(128, device=DEV, generator=g) if norm else None)
+    got = smx.rotary(x, positions, frequencies, **args)
+    inside = positions >= 0
+    check(got[inside], *rotate64(x[inside], positions[inside], frequencies, **args))
+    assert got[~inside].eq(0).all()
+    assert torch.equal(smx.rotary(x, positions, frequencies, out=x.clone(), **args)[inside], got[inside])
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_rotary_of_far_positions(dtype):
     """Positions past 2^31, and frequencies of whole turns, where a position's own digits are all that is left."""
