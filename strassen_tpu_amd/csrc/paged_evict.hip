@@ -309,7 +309,6 @@ __device__ void select_whole(const EvictArgs& p, const Cut& c, int head, int req
       count = pick<kThreads>(look, low, high, least, most, ties);
     } while (least < most && count > kNear);  // another look, at the part alone
   }
-  if (missing) bad = 1;
 
   // Places to fill and survivors behind them, in index order: a wave counts its own first. Keys of the part found are
   // compared with each other, unless they are equal.
@@ -324,6 +323,9 @@ __device__ void select_whole(const EvictArgs& p, const Cut& c, int head, int req
       if (in && apart) near.add(key[j], at + j);
     }
   });
+  // (now at the latest every page has been looked at: without need there was no look, and keys that are not held were read in
+  // this pass for the first time)
+  if (missing) bad = 1;
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     const int sum = lane_scan(count[x]);
