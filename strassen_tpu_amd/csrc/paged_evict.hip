@@ -383,7 +383,7 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs p) {
 }
 
 // Long contexts: the older tokens in parts of 8192, a workgroup each, in three launches, for which one workgroup took
-// 127 us at 131,000 tokens. evict_histogram counts each part's weights over the range that the first thousand have,
+// 127 us at 131,000 tokens. evict_histogram counts each part's weights over the range that a thousand of them have,
 // evict_collect finds the part of the range that holds the edge and collects its keys, evict_list finds
 // the edge among them and puts each part's places and survivors on the lists.
 constexpr int kPart = 8192, kPartThreads = 256, kPartWaves = 4, kCrowd = 4096, kMostParts = 64;
@@ -391,7 +391,9 @@ constexpr int kPart = 8192, kPartThreads = 256, kPartWaves = 4, kCrowd = 4096, k
 // What the three launches leave for each other, of a head and request.
 struct Looked {
   uint32_t low, high, least, most;
-  int32_t ties, crowd, mode, unused;  // mode 0: nothing is cut, 1: parts, 2: too many keys at the edge, one workgroup does it all
+  // mode 0: nothing is cut, 1: parts, 2: too many keys at the edge, one workgroup does it all (weights all within 2^-12 of each
+  // other but for a thousandth far above: four contexts of 131,000 cut to 32,768 634 us, by one workgroup of sixteen waves 437)
+  int32_t ties, crowd, mode, unused;
 };
 struct Candidate {
   uint32_t key;
@@ -422,10 +424,14 @@ __global__ __launch_bounds__(kPartThreads) void evict_histogram(EvictArgs p) {
   bool missing = false;
   Keys keys;
   uint32_t low = ~0u, high = 0;
-  load_keys(p, table, head, wave * 256, 1, c.m, keys, missing);
+  // Four weights a thread, evenly apart over all older tokens: what keys receive falls with their index, so that the first of them
+  // alone have a range above the others (weights of log(n / j), four contexts of 131,000 cut to 4096: 62 us; from the range of
+  // the first thousand 293, since more keys lie below it than are collected).
+  const int four = 4 * (int)((int64_t)threadIdx.x * ((c.m + 3) / 4) / kPartThreads);  // below m
+  load_keys(p, table, head, four - 4 * (int)(threadIdx.x & 63), 1, c.m, keys, missing);
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    if (4 * (int)threadIdx.x + j < c.m) low = min(low, keys[0][j]), high = max(high, keys[0][j]);
+    if (four + j < c.m) low = min(low, keys[0][j]), high = max(high, keys[0][j]);
   const int begin = part * kPart + wave * (kPart / kPartWaves);
   load_keys(p, table, head, begin, kQuads, c.m, keys, missing);
   if (part == 0)
