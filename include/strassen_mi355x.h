@@ -542,8 +542,8 @@ int smx_paged_evict_workspace_bytes(int32_t requests, int32_t kv_heads, int32_t 
  * of the heads' type) are rotated, pair i by the angle positions[token] * frequencies[i], and multiplied by
  * amplitude; the values behind them are copied. With norm [head_dim] the whole head is RMS-normalised and scaled first.
  * Angles are reduced in 64 bits, the rest is FP32 with one rounding. Rows of negative position are left as they are in
- * out, or become zero with zero_rows. out is x (same address and strides) or shares no memory with it; its rows lie apart from
- * each other. head_dim 2 to 1024. Asynchronous on stream.
+ * out, or become zero with zero_rows. out is x (same address and strides) or shares no memory with it, and none with
+ * positions, frequencies and norm; its rows lie apart from each other. head_dim 2 to 1024. Asynchronous on stream.
  */
 int smx_rotary(int32_t tokens, int32_t head_dim, int32_t rotary_dim, const smx_heads* x, const smx_heads* out,
                const void* positions, const void* frequencies, const void* norm, int32_t flags, float amplitude,

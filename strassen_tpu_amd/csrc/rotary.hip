@@ -275,6 +275,12 @@ int smx_rotary(int32_t tokens, int32_t head_dim, int32_t rotary_dim, const smx_h
   if (!lie_apart(to)) return fail(SMX_ERR_INVALID, "out holds rows that lie on each other");
   if (!same_runs(from, to) && meet(from, to))
     return fail(SMX_ERR_INVALID, "out must be x itself or share no memory with it");
+  // ... and read beside positions, frequencies and norm, by every workgroup for itself.
+  const auto list = [](const void* at, int64_t count, int bytes) { return Runs{at, count * (bytes / 2), {{1, 0}, {1, 0}, {1, 0}}}; };
+  if (meet(to, list(positions, tokens, flags & SMX_ROTARY_POSITIONS_I64 ? 8 : 4)) ||
+      meet(to, list(frequencies, rotary_dim / 2, flags & SMX_ROTARY_FREQUENCIES_F32 ? 4 : 8)) ||
+      (norm && meet(to, list(norm, head_dim, flags & SMX_ROTARY_NORM_F32 ? 4 : 2))))
+    return fail(SMX_ERR_INVALID, "out must share no memory with positions, frequencies and norm");
   RotaryArgs p{};
   p.x = x->data, p.out = out->data, p.positions = positions, p.frequencies = frequencies, p.norm = norm;
   p.x_token = x->token_stride, p.x_head = x->head_stride, p.out_token = out->token_stride, p.out_head = out->head_stride;

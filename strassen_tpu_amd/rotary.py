@@ -82,6 +82,6 @@ def rotary(x, positions, frequencies, *, interleaved=False, amplitude=1.0, norm=
     Query and key heads that are columns of one projection are one ``x``. Angles are reduced in 64 bits from
     ``frequencies`` float64 (or float32, taken as they are), so that far positions lose nothing; the rest is FP32
     with one rounding. Rows of negative position (a plan's rows of no admitted request) are zero in a new result and left
-    as they were in ``out``, which is ``x`` itself or shares no memory with it. ``head_dim`` up to 1024, up to 2^20 tokens.
-    No gradients."""
+    as they were in ``out``, which is ``x`` itself or shares no memory with it, and none with the other tensors. ``head_dim`` up
+    to 1024, up to 2^20 tokens. No gradients."""
     return _lib.host().rotary(x, positions, frequencies, interleaved, amplitude, norm, eps, out)

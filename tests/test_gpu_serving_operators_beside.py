@@ -1,0 +1,48 @@
+"""Operands of the serving operators that lie back to back in one allocation, as a program's own arena holds them."""
+
+import pytest
+import torch
+
+import strassen_tpu_amd as smx
+from test_gpu_parity import DEV, say
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _announce(request):
+    say(f"\n[gpu] {request.node.nodeid}")
+    yield
+    torch.cuda.synchronize()
+
+
+def arena(*parts):
+    """Copies of the tensors behind each other, each where the one before ends (sizes are multiples of 16 bytes)."""
+    memory = torch.empty(sum(x.numel() * x.element_size() for x in parts), dtype=torch.uint8, device=DEV)
+    views, at = [], 0
+    for x in parts:
+        size = x.numel() * x.element_size()
+        assert size % 16 == 0
+        views.append(memory[at:at + size].view(x.dtype).view(x.shape).copy_(x))
+        at += size
+    return views
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2, 3), (1, 0, 2, 3), (2, 1, 0, 3), (3, 2, 1, 0)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rotary_beside_what_it_reads(dtype, order):
+    g = torch.Generator(device=DEV).manual_seed(50)
+    x = torch.randn(16, 8, 128, device=DEV, generator=g).to(dtype)
+    positions = torch.randint(0, 5000, (16,), device=DEV, generator=g, dtype=torch.int32)
+    f = smx.rotary_frequencies(128, device=DEV)[0]
+    norm = torch.randn(128, device=DEV, generator=g).to(dtype)
+    want = smx.rotary(x, positions, f, norm=norm)
+    parts = [torch.zeros_like(x), positions, f, norm]
+    laid = arena(*(parts[i] for i in order))
+    out, positions, f, norm = (laid[order.index(i)] for i in range(4))
+    assert smx.rotary(x, positions, f, norm=norm, out=out) is out
+    assert torch.equal(out, want)
+    out.copy_(x)  # in place
+    assert torch.equal(smx.rotary(out, positions, f, norm=norm, out=out), want)
+    with pytest.raises(ValueError, match="positions, frequencies and norm"):
+        smx.rotary(x, out.view(torch.int32).flatten()[:16], f, out=out)
