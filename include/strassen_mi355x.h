@@ -501,7 +501,7 @@ int smx_paged_attention_lse(const smx_paged_cache* cache, const smx_paged_step* 
  * keys start from zero. lse is that of smx_paged_attention_lse for the same queries, scale and window. Scores and sums in
  * FP32; the same call gives the same bits. Slots that no admitted request's keys lie in are left as they are, and so are
  * those of pages that are not in the cache. The cache's values are not read (v may be k). Requests share no pages.
- * key_weights shares no memory with the keys, the queries and lse. The query heads of 32 rows lie within 2^32 bytes
+ * key_weights shares no memory with the keys, the queries, lse and the step's lists. The query heads of 32 rows lie within 2^32 bytes
  * (SMX_ERR_UNSUPPORTED otherwise). The workspace
  * (smx_paged_key_weights_workspace_bytes, for the current device) is overwritten. Asynchronous on stream.
  */

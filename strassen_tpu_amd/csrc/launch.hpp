@@ -27,6 +27,16 @@ inline Runs head_runs(const smx_heads& x, int64_t tokens, int64_t head_dim) {
   return Runs{x.data, head_dim, {{tokens, x.token_stride}, {x.heads, x.head_stride}, {1, 0}}};
 }
 
+// Whether `bytes` from `at` on share memory with the lists that a step is read from (of a table, whose width the step does not
+// say, each row's first entry).
+inline bool meets_step(const void* at, int64_t bytes, const smx_paged_step& s) {
+  const Runs x{at, bytes / 2, {{1, 0}, {1, 0}, {1, 0}}};
+  for (const int32_t* list : {s.starts, s.rows, s.context})
+    if (meet(x, Runs{list, 2 * (int64_t)s.requests, {{1, 0}, {1, 0}, {1, 0}}})) return true;
+  return (s.positions && meet(x, Runs{s.positions, 2 * (int64_t)s.tokens, {{1, 0}, {1, 0}, {1, 0}}})) ||
+         list_meets_table(at, bytes / 4, s.block_tables, s.requests, 1, s.table_stride, 4);
+}
+
 inline int check_launch() {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(SMX_ERR_LAUNCH, "kernel launch: %s", hipGetErrorString(e));

@@ -590,6 +590,8 @@ int smx_paged_key_weights(const smx_paged_cache* cache, const smx_paged_step* st
   const Runs sums{lse, 2 * (int64_t)step->tokens * q->heads, {{1, 0}, {1, 0}, {1, 0}}};
   if (meet(to, cache_runs(*cache, cache->k)) || meet(to, head_runs(*q, step->tokens, cache->head_dim)) || meet(to, sums))
     return fail(SMX_ERR_INVALID, "key_weights must share no memory with the keys, the queries and lse");
+  // (a workgroup's lengths and tables are read while others store)
+  if (meets_step(key_weights, 2 * to.width, *step)) return fail(SMX_ERR_INVALID, "key_weights must share no memory with the step's lists");
   if (!(scale > 0.f) || !(scale * kLog2E < INFINITY))
     return fail(SMX_ERR_INVALID, "scale must be positive and finite, also times log2 e");
   if (window < 0) return fail(SMX_ERR_INVALID, "window must not be negative (0: none)");

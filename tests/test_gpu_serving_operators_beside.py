@@ -46,3 +46,25 @@ def test_rotary_beside_what_it_reads(dtype, order):
     assert torch.equal(smx.rotary(out, positions, f, norm=norm, out=out), want)
     with pytest.raises(ValueError, match="positions, frequencies and norm"):
         smx.rotary(x, out.view(torch.int32).flatten()[:16], f, out=out)
+
+
+@pytest.mark.parametrize("max_new", [1, 40])
+def test_key_weights_beside_the_steps_lists(max_new):
+    """Weights between the tables and the lengths, the plan made from both."""
+    g = torch.Generator(device=DEV).manual_seed(51)
+    k = torch.randn(12, 16, 2, 128, device=DEV, generator=g).to(torch.bfloat16)
+    q = torch.randn(4 * max_new, 4, 128, device=DEV, generator=g).to(torch.bfloat16)
+    tables = torch.randperm(12, device=DEV, generator=g)[:12].view(4, 3).to(torch.int32)
+    lens, new = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, 5, 7, 8], [max_new] * 4))
+    first = torch.rand(12, 2, 16, device=DEV, generator=g)
+
+    def run(tables, weights, lens, lse):
+        plan = smx.paged_plan(lens, new, tables, page_size=16, num_pages=12, tokens=4 * max_new, max_new=max_new)
+        smx.paged_attention(q, k, k, plan, lse=lse)
+        smx.paged_key_weights(q, k, weights, plan, lse)
+        return weights, lse
+
+    lse = torch.zeros(4 * max_new, 4, device=DEV)
+    want = run(tables, first.clone(), lens, lse)
+    got = run(*arena(tables, first, lens, lse))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))

@@ -3,8 +3,8 @@ launch."""
 
 import pytest
 
-from test_serving_operators import OUT, _rotary, refused
-from test_serving_surface import _heads
+from test_serving_operators import FAR, OUT, _key_weights, _rotary, refused
+from test_serving_surface import _heads, _step
 
 
 # eight rows of eight heads of 128: 16384 bytes of bf16, 32768 of float32
@@ -17,3 +17,13 @@ from test_serving_surface import _heads
 ])
 def test_rotary_refuses_results_over_what_it_reads(change):
     refused(_rotary(**change), "positions, frequencies and norm")
+
+
+# eight pages of two heads of 16 slots: 1024 bytes; two requests, eight tokens, tables of four entries
+@pytest.mark.parametrize("change", [
+    dict(starts=FAR), dict(starts=FAR + 1020), dict(starts=FAR - 4), dict(rows=FAR + 512), dict(rows=FAR - 4), dict(context=FAR),
+    dict(context=FAR + 1020), dict(positions=FAR - 28), dict(positions=FAR + 1020), dict(tables=FAR), dict(tables=FAR + 1020),
+    dict(tables=FAR - 16),
+])
+def test_key_weights_refuse_weights_over_the_steps_lists(change):
+    refused(_key_weights(step=_step(**change)), "step's lists")
