@@ -519,7 +519,7 @@ int smx_paged_key_weights_workspace_bytes(int64_t* bytes);
  * was. keep is keep_lens[b] where keep_lens is not NULL. lens [requests] becomes keep, or n where nothing is cut: n <= keep,
  * n over max_context, a negative length, or a page of the request that is not in the cache. block_tables is not
  * changed: the pages behind the last kept token are the caller's to reuse. Requests share no pages. The cache's rows lie apart
- * from each other and from key_weights, and lens from context_lens, keep_lens and block_tables. workspace:
+ * from each other and from key_weights, and both and lens from context_lens, keep_lens and block_tables. workspace:
  * smx_paged_evict_workspace_bytes, with the same keep (-1 with keep_lens) and max_context, which bounds the contexts and is
  * at most width * page_size. Asynchronous on stream.
  */

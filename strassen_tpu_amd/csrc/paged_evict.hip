@@ -797,6 +797,11 @@ int smx_paged_evict(const smx_paged_cache* cache, float* key_weights, int32_t re
   if (meet(list(lens, requests), list(context_lens, requests)) || (keep_lens && meet(list(lens, requests), list(keep_lens, requests))) ||
       meet(list(lens, requests), list(block_tables, (requests - 1) * table_stride + width)))
     return fail(SMX_ERR_INVALID, "lens must share no memory with context_lens, keep_lens and block_tables");
+  // rows and weights are moved while others look up where theirs lie
+  for (const Runs& moved : {keys, values, all})
+    if (meet(moved, list(lens, requests)) || meet(moved, list(context_lens, requests)) || (keep_lens && meet(moved, list(keep_lens, requests))) ||
+        meet(moved, list(block_tables, (requests - 1) * table_stride + width)))
+      return fail(SMX_ERR_INVALID, "the cache and key_weights must share no memory with the lengths and block_tables");
   EvictArgs p{};
   p.k = (uint16_t*)cache->k, p.v = (uint16_t*)cache->v;
   p.page_stride = cache->page_stride, p.slot_stride = cache->slot_stride, p.head_stride = cache->head_stride;

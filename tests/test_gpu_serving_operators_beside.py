@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import strassen_tpu_amd as smx
+from test_gpu_evict import expected, make_cache, same
 from test_gpu_parity import DEV, say
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +69,16 @@ def test_key_weights_beside_the_steps_lists(max_new):
     want = run(tables, first.clone(), lens, lse)
     got = run(*arena(tables, first, lens, lse))
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_eviction_beside_the_lists():
+    """Keys, lengths, values, tables and weights one behind the other."""
+    context, keep = [100, 30, 65, 77], [40, 40, 8, 70]
+    k, v, w, lens, tables = make_cache(context, page=8, seed=52, width=16)
+    want = expected(k, v, w, context, tables, keep, 6)
+    goals = torch.tensor(keep, dtype=torch.int32, device=DEV)
+    k, lens, v, tables, w, goals = arena(k, lens, v, tables, w, goals)
+    assert smx.paged_evict(k, v, w, lens, tables, goals, recent=6).tolist() == want[3] and lens.tolist() == context
+    assert same(k, want[0]) and same(v, want[1]) and same(w, want[2])
+    with pytest.raises(ValueError, match="lengths and block_tables"):
+        smx.paged_evict(k, v, w, w.view(torch.int32).flatten()[:4], tables, goals, recent=6)

@@ -3,7 +3,7 @@ launch."""
 
 import pytest
 
-from test_serving_operators import FAR, OUT, _key_weights, _rotary, refused
+from test_serving_operators import FAR, OUT, _evict, _key_weights, _rotary, refused
 from test_serving_surface import _heads, _step
 
 
@@ -27,3 +27,15 @@ def test_rotary_refuses_results_over_what_it_reads(change):
 ])
 def test_key_weights_refuse_weights_over_the_steps_lists(change):
     refused(_key_weights(step=_step(**change)), "step's lists")
+
+
+# eight pages of sixteen rows of two heads of 128: 65536 bytes of keys, as many of values 2^24 behind them, 1024 of weights
+@pytest.mark.parametrize("base,size", [(OUT, 65536), (OUT + (1 << 24), 65536), (FAR, 1024)])
+@pytest.mark.parametrize("change", [
+    dict(context=0), dict(context=-4), dict(lens=-4), dict(keep_lens=-4), dict(tables=-28), dict(tables=-4), dict(context="end"),
+    dict(lens="end"), dict(keep_lens="end"), dict(tables="end"),
+])
+def test_evict_refuses_rows_and_weights_over_the_lists(base, size, change):
+    apart = dict(context=1 << 20, tables=1 << 21, lens=1 << 22)
+    refused(_evict(**{**apart, **{name: base + (size - 4 if at == "end" else at) for name, at in change.items()}}),
+            "lengths and block_tables")
