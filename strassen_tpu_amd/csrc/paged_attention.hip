@@ -998,6 +998,7 @@ int smx_paged_attention_lse(const smx_paged_cache* cache, const smx_paged_step* 
     if ((uintptr_t)lse % 4 || meet(sums, from) || meet(sums, to) || meet(sums, cache_runs(*cache, cache->k)) ||
         meet(sums, cache_runs(*cache, cache->v)))
       return fail(SMX_ERR_INVALID, "lse must be aligned and share no memory with the queries, out or the cache");
+    if (meets_step(lse, 2 * sums.width, *step)) return fail(SMX_ERR_INVALID, "lse must share no memory with the step's lists");
   }
   constexpr float kLog2E = 1.44269504088896341f;  // (the kernels' exponentials are powers of two)
   if (!(scale > 0.f) || !(scale * kLog2E < INFINITY))

@@ -3,8 +3,9 @@ launch."""
 
 import pytest
 
+from strassen_tpu_amd import _lib
 from test_serving_operators import FAR, OUT, _evict, _key_weights, _rotary, refused
-from test_serving_surface import _heads, _step
+from test_serving_surface import P, _cache, _heads, _step
 
 
 # eight rows of eight heads of 128: 16384 bytes of bf16, 32768 of float32
@@ -39,3 +40,13 @@ def test_evict_refuses_rows_and_weights_over_the_lists(base, size, change):
     apart = dict(context=1 << 20, tables=1 << 21, lens=1 << 22)
     refused(_evict(**{**apart, **{name: base + (size - 4 if at == "end" else at) for name, at in change.items()}}),
             "lengths and block_tables")
+
+
+# eight rows of eight heads: 256 bytes
+@pytest.mark.parametrize("change", [
+    dict(starts=FAR), dict(starts=FAR + 252), dict(rows=FAR - 4), dict(context=FAR + 128), dict(positions=FAR - 28),
+    dict(positions=FAR + 252), dict(tables=FAR + 252), dict(tables=FAR - 16),
+])
+def test_attention_refuses_row_sums_over_the_steps_lists(change):
+    refused(_lib.load().smx_paged_attention_lse(_cache(k=OUT, v=OUT + (1 << 24)), _step(**change), _heads(data=1 << 30),
+                                                _heads(data=1 << 30), 0.1, 0, 0, FAR, P, 0, None), "step's lists")
