@@ -4,7 +4,7 @@ launch."""
 import pytest
 
 from strassen_tpu_amd import _lib
-from test_serving_operators import FAR, OUT, _evict, _key_weights, _rotary, refused
+from test_serving_operators import FAR, OUT, _evict, _key_weights, _rotary, _verify, refused
 from test_serving_surface import P, _cache, _heads, _step
 
 
@@ -50,3 +50,15 @@ def test_evict_refuses_rows_and_weights_over_the_lists(base, size, change):
 def test_attention_refuses_row_sums_over_the_steps_lists(change):
     refused(_lib.load().smx_paged_attention_lse(_cache(k=OUT, v=OUT + (1 << 24)), _step(**change), _heads(data=1 << 30),
                                                 _heads(data=1 << 30), 0.1, 0, 0, FAR, P, 0, None), "step's lists")
+
+
+# eight rows of 100 probabilities, two requests: `out` of 32 bytes at OUT (64 of int64), `counts` of 8 at FAR
+@pytest.mark.parametrize("change", [
+    dict(counts=OUT), dict(counts=OUT + 28), dict(counts=OUT + 60, flags=2), dict(counts=OUT - 4), dict(accept=OUT - 28), dict(accept=FAR + 4),
+    dict(sample=OUT + 28), dict(sample=FAR - 4), dict(tokens=FAR - 28), dict(tokens=FAR - 56, flags=2), dict(target=OUT + 28),
+    dict(target=OUT - 4 * (700 + 100) + 4), dict(target=FAR - 4 * (7 * 128 + 100) + 4, target_row=128), dict(draft=OUT + 28, draft_row=100),
+    dict(draft=FAR - 2 * 800 + 4, draft_row=100, flags=1), dict(step=_step(starts=FAR)), dict(step=_step(rows=FAR)),
+    dict(step=_step(rows=OUT + 28)), dict(step=_step(positions=FAR - 28)), dict(step=_step(positions=OUT)), dict(step=_step(context=OUT)),
+])
+def test_verify_refuses_results_over_what_it_reads(change):
+    refused(_verify(**{**dict(out=OUT, counts=FAR), **change}), "share no memory")
