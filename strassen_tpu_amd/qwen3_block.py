@@ -288,7 +288,12 @@ class ServingBlock:
     the weights for tiles of ``(bn, bk)`` columns and K; "int4" quantises them in groups of
     ``group`` (``int4_quantize``). ``max_context`` positions have RoPE tables. ``frequencies`` and
     ``amplitude`` (``rotary_frequencies``; default: those of ``dims.theta``) rotate the heads of steps that say their
-    positions; where they are given, those of all steps, and no tables are made."""
+    positions; where they are given, those of all steps, and no tables are made.
+
+    The tables hold bf16 values of FP32 angles, ``rotary`` works with the angles themselves: the two differ by a bf16 rounding of
+    cos and sin and by at most ``position * frequency * 2 ** -21`` radians (a hundredth at a position of 100,000). A cache
+    whose steps will say their positions some day (one that is evicted from) is best filled by one of them throughout: give
+    ``frequencies``, or positions from the first step on."""
 
     def __init__(self, weights, dims, arm, *, max_context, tile=(1024, 512), group=128, frequencies=None, amplitude=1.0):
         if arm not in SERVING_ARMS:
