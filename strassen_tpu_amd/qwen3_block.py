@@ -346,7 +346,9 @@ def block_step(x, block, k_cache, v_cache, plan, *, window=None, positions=None,
     they pass through as rows of their own.
 
     ``positions`` (int32 or int64 ``[plan.tokens]``) are the rows' positions where they are not their indices in the
-    cache: after an eviction, whose keys were rotated where they stood (``rotary``). ``key_weights``
+    cache: after an eviction, whose keys were rotated where they stood (``rotary``). ``window`` counts indices in the cache
+    whatever the positions: of a cache that was evicted from, whose indices say nothing of the order, none is the
+    right one. ``key_weights``
     float32 ``[pages, kv_heads, page_size]`` receives the attention weight of the layer's keys
     (``paged_key_weights``), by which ``paged_evict`` cuts the cache."""
     d, w = block.dims, block.weights
