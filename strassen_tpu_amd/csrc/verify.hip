@@ -5,7 +5,7 @@
 // replaced by a token drawn from max(p_i - q_i, 0); behind an accepted last one a token is drawn from the last
 // row's p. A draw takes the first token whose running sum exceeds v times the whole sum. Products and
 // sums are in 64 bits: a sum of 150,000 values in FP32 is off by more than many of them, and the token would depend
-// on the order of the additions.
+// on the order of the additions (which is another one where a request is shared out, below).
 //
 // Work. One row of p and one of q a request, whatever the number of drafts: verify_sums cuts the row in slices, a workgroup
 // each, verify_draw finds the slice that the draw falls in and looks through that slice alone. Where requests fill the chip or

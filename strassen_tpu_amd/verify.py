@@ -27,8 +27,10 @@ def verify_drafts(target, tokens, plan, accept, sample, *, draft=None):
     ``x`` behind row ``i`` is accepted if ``accept[i] * draft[i, x] < target[i, x]`` and those before it were. The next token
     is drawn from ``max(target - draft, 0)`` of the row whose draft was refused (from ``target`` where that is zero everywhere),
     or from ``target`` of the last row: the first token whose running sum exceeds ``sample`` times the whole. Products and sums
-    are in 64 bits, so that the same numbers give the same tokens whatever the order of the sums; probabilities need not
-    add up to 1, and such as are no positive finite numbers count as zero (a draft outside the vocabulary too).
+    are in 64 bits: the same call gives the same tokens, and a request in calls of other sizes (whose sums go in another
+    order) the same but for numbers within the rounding of such sums, 2^-50 or so of the whole, of a border between two
+    tokens. Probabilities need not add up to 1, and such as are no positive finite numbers count as zero (a draft outside the
+    vocabulary too).
 
     Returns ``emitted [plan.tokens]`` (as ``tokens``) with each request's accepted drafts and its next token from its first
     row on, -1 behind them and in rows of no admitted request, and ``counts`` int32 ``[requests]``: how
