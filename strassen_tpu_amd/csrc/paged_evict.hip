@@ -3,9 +3,9 @@
 // Of the n tokens of a request, each key/value head keeps `keep`: the last `recent`, and of the m older ones the
 // need = keep - recent with the largest weights (ties: the lowest index). Survivors with an index below need stay
 // where they are. The places of the evicted ones there are as many as the survivors behind, and the j-th of
-// the one takes the j-th of the other; the recent ones move to need .. keep - 1 in order. That is the least that can be
-// moved with the cache left without gaps, and no row is moved twice: of 131,000 tokens cut to 32,768 a
-// head moves 24,800.
+// the one takes the j-th of the other: of those kept for their weight no fewer can move if there are to be no gaps. The recent ones
+// all move, to need .. keep - 1, since they stay in their order. No row is moved twice: of 131,000 tokens cut to 32,768, 512
+// of them the last, a head moves 24,800.
 //
 // evict_select (a workgroup per head and request) finds the need-th largest weight: weights as integers in their order,
 // a histogram of equal parts of their range, the part that holds it, and so on until its keys fit in LDS,
