@@ -119,8 +119,8 @@ __device__ __forceinline__ void range_of(uint32_t& low, uint32_t& high, uint32_t
 
 // A histogram over the keys from low to high: those below low, low itself (weights of which many are zero end here),
 // and equal parts of the others, the last with those above high. Parts of the values that are there hold few keys each, so that
-// additions meet rarely (leading bits alone, of which most weights share some: 66 us instead of 23 for 8100 keys of
-// 512 heads).
+// additions meet rarely (leading bits alone, of which most weights share some: 66 us for 8100 keys
+// of 512 heads, and 23 of equal parts in the same state of the rest; 21 now).
 struct Look {
   int bins[kBins], scans[16], picked[3];
 
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs p) {
 }
 
 // Long contexts: the older tokens in parts of 8192, a workgroup each, in three launches, for which one workgroup took
-// 127 us at 131,000 tokens. evict_histogram counts each part's weights over the range that a thousand of them have,
+// 128 us for 32 heads of 131,000 tokens (in parts 40). evict_histogram counts each part's weights over the range that a thousand of them have,
 // evict_collect finds the part of the range that holds the edge and collects its keys, evict_list finds
 // the edge among them and puts each part's places and survivors on the lists.
 constexpr int kPart = 8192, kPartThreads = 256, kPartWaves = 4, kCrowd = 4096, kMostParts = 64;
@@ -727,8 +727,8 @@ int moves_of(int keep, bool given, int max_context) {
 }
 
 // Parts of the longest context where it is long and the heads are few; 0: one workgroup a head and request. Selection
-// took, of one workgroup and of parts: 30 and 32 us for 8 heads of 32,000 tokens, which sixteen waves hold in registers, 100 and 40
-// for 32 heads of 131,000, 119 and 110 for 128 of them, and 331 and 43 for 8 of 500,000.
+// takes in its kernels, of one workgroup and of parts: 30 and 31 us for 8 heads of 32,000 tokens, which sixteen waves hold in
+// registers, 128 and 40 for 32 heads of 131,000, 145 and 114 for 128 of them, and 452 and 44 for 8 of 500,000.
 int parts_of(int64_t pairs, int max_context) {
   const int64_t parts = ((int64_t)max_context + kPart - 1) / kPart;
   return max_context > 1024 * 4 * kQuads && parts <= kMostParts && pairs <= 128 ? (int)parts : 0;
@@ -828,8 +828,8 @@ int smx_paged_evict(const smx_paged_cache* cache, float* key_weights, int32_t re
     hipLaunchKernelGGL(few ? evict_select<256> : evict_select<1024>, heads, dim3(few ? 256 : 1024), 0, (hipStream_t)stream, p);
     if (int rc = check_launch()) return rc;
   }
-  // Workgroups of a head and request: of 64 rows at least, and so many that they even out (139 us for 64 requests; 142 of half
-  // as many, 149 of a quarter).
+  // Workgroups of a head and request: of 64 rows at least, and so many that they even out (64 requests, weights copied back
+  // before each: 133 us; 135 of half as many, 142 of a quarter).
   p.tails = cache->head_dim / 32;
   p.movers = min((p.moves + 63) / 64, max(1, 16384 / pairs));
   // Rows that do not fit into the caches anyway pass them by: four prompts of 131,000 216 us (else 227), 64 requests 133 (138), 47 of

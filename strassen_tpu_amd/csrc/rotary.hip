@@ -297,12 +297,12 @@ int smx_rotary(int32_t tokens, int32_t head_dim, int32_t rotary_dim, const smx_h
                        2 * p.half * 4, (hipStream_t)stream, p);
     return check_launch();
   }
-  // Rows of a workgroup: several where enough workgroups remain to fill the chip (72 heads of 128; one, two and four
-  // rows: 22, 20 and 23 us for 2045 tokens, 55, 53 and 53 for 8192).
+  // Rows of a workgroup: several where enough workgroups remain to fill the chip (72 heads of 128, three sets of them in turn; one,
+  // two and four rows: 14.2, 14.3 and 14.0 us for 2045 tokens, 53, 52 and 51 for 8192).
   p.per_block = tokens >= 4096 ? 4 : tokens >= 1536 ? 2 : 1;
   const unsigned blocks = (unsigned)((tokens + p.per_block - 1) / p.per_block);
-  // Of few tokens a row's heads are shared out, as many to a workgroup as it takes at once (72 heads of 128; shared and not:
-  // 4.3 and 6.1 us for 16 tokens, 6.5 and 7.6 for 400, 12.7 and 10.8 for 1000).
+  // Of few tokens a row's heads are shared out, as many to a workgroup as it takes at once (72 heads of 128 without a norm; shared
+  // and not, in the kernel: 4.0 and 5.3 us for 16 tokens, 5.7 and 6.4 for 400, 9.7 and 9.0 for 1000).
   const int turning = p.half / run, lanes = turning + (head_dim / run - 2 * turning + 1) / 2;
   p.heads_each = blocks <= 512 ? min(p.heads, max(1, 256 / lanes)) : p.heads;
   const int lds = 2 * p.per_block * p.half * 4;

@@ -309,7 +309,7 @@ int whole_threads(int vocab, int requests) {
 }
 
 // Tokens of a slice, a multiple of the workgroup's loads: at most 64 slices, of 2048 tokens at least, and no more
-// than fill the chip with workgroups twice (64 requests 25.4 us, once 26.7; 200 of 32,001 tokens 18.7 and 20.1).
+// than fill the chip with workgroups twice (64 requests 23.3 us, once 24.7; 100 of 32,001 tokens 14.8 either way).
 int slice_of(int vocab, int requests) {
   if (const int waves = whole_threads(vocab, requests) / 64) return (vocab + 4 * waves - 1) / (4 * waves) * 4;
   constexpr int kRun = 4 * kVerifyThreads;
