@@ -152,8 +152,10 @@ def paged_evict(k_cache, v_cache, key_weights, context_lens, block_tables, keep,
     own, with the same ``block_tables`` and lengths.
 
     A request is left as it was, and its length returned, if it holds ``keep`` tokens or fewer, if a
-    length is negative or above ``max_context`` (default: what the tables hold; it sizes the call's workspace,
-    about 5 bytes a token and head), or if a table entry of its tokens is no page of the cache. ``block_tables`` is not
+    length is negative or above ``max_context`` (default: what the tables hold), or if a table entry of its tokens is no page of
+    the cache. ``max_context`` sizes the call's workspace, about 5 bytes a token and head, and picks its kernels: where tables
+    hold far more than the requests do, a bound near their lengths is faster (eight requests cut from 1040 tokens to 1024: 11 us
+    by a bound of 1040, 23 by that of tables for 131,072). ``block_tables`` is not
     changed: pages behind the last kept token stay the request's, for its next tokens or for the program to
     take back. Requests must not share pages."""
     return _lib.host().evict(k_cache, v_cache, key_weights, context_lens, block_tables, keep, recent, max_context)

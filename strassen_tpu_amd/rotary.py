@@ -83,5 +83,8 @@ def rotary(x, positions, frequencies, *, interleaved=False, amplitude=1.0, norm=
     ``frequencies`` float64 (or float32, taken as they are), so that far positions lose nothing; the rest is FP32
     with one rounding. Rows of negative position (a plan's rows of no admitted request) are zero in a new result and left
     as they were in ``out``, which is ``x`` itself or shares no memory with it, and none with the other tensors. ``head_dim`` up
-    to 1024, up to 2^20 tokens. No gradients."""
+    to 1024, up to 2^20 tokens. No gradients.
+
+    Heads whose rotated halves and width are whole runs of 16 bytes (8 bf16 values) at aligned places, behind a norm also a power
+    of two wide, run at what memory gives; others take some three times as long."""
     return _lib.host().rotary(x, positions, frequencies, interleaved, amplitude, norm, eps, out)
