@@ -34,7 +34,7 @@ inline bool meets_step(const void* at, int64_t bytes, const smx_paged_step& s) {
   for (const int32_t* list : {s.starts, s.rows, s.context})
     if (meet(x, Runs{list, 2 * (int64_t)s.requests, {{1, 0}, {1, 0}, {1, 0}}})) return true;
   return (s.positions && meet(x, Runs{s.positions, 2 * (int64_t)s.tokens, {{1, 0}, {1, 0}, {1, 0}}})) ||
-         (s.block_tables && list_meets_table(at, bytes / 4, s.block_tables, s.requests, 1, s.table_stride, 4));
+         list_meets_table(at, bytes / 4, s.block_tables, s.requests, 1, s.table_stride, 4);
 }
 
 inline int check_launch() {

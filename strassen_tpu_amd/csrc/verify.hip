@@ -359,16 +359,22 @@ int smx_verify_drafts(const smx_paged_step* step, int32_t vocab, const void* tar
     return fail(SMX_ERR_INVALID, "the call needs a 16-byte aligned workspace of %lld bytes", (long long)need);
   // a request's tokens and count are stored while others read theirs
   const auto list = [](const void* at, int64_t count, int bytes) { return Runs{at, count * (bytes / 2), {{1, 0}, {1, 0}, {1, 0}}}; };
-  const auto rows_of = [&](const void* at, int64_t row) { return Runs{at, (int64_t)vocab * (size / 2), {{step->tokens, row * (size / 2)}, {1, 0}, {1, 0}}}; };
+  const auto rows_of = [&](const void* at, int64_t row) {
+    return Runs{at, (int64_t)vocab * (size / 2), {{step->tokens, row * (size / 2)}, {1, 0}, {1, 0}}};
+  };
   const int64_t rows = step->tokens, requests = step->requests;
   const int token = flags & SMX_VERIFY_TOKENS_I64 ? 8 : 4;
   const Runs stored[] = {list(out, rows, token), list(counts, requests, 4)};
   if (meet(stored[0], list(tokens, rows, token))) return fail(SMX_ERR_INVALID, "out and tokens must share no memory");
   if (meet(stored[0], stored[1])) return fail(SMX_ERR_INVALID, "out and counts must share no memory");
-  for (const Runs& to : stored)
-    if (meet(to, list(tokens, rows, token)) || meet(to, list(accept, rows, 4)) || meet(to, list(sample, requests, 4)) ||
-        meet(to, rows_of(target, target_row)) || (draft && meet(to, rows_of(draft, draft_row))) || meets_step(to.at, 2 * to.width, *step))
-      return fail(SMX_ERR_INVALID, "out and counts must share no memory with what the call reads");
+  // (of the step, starts, rows and positions; the rest of it need not be there)
+  const Runs read[] = {list(tokens, rows, token), list(accept, rows, 4), list(sample, requests, 4), list(step->starts, requests, 4),
+                       list(step->rows, requests, 4), list(step->positions, rows, 4), rows_of(target, target_row)};
+  for (const Runs& to : stored) {
+    bool meets = draft && meet(to, rows_of(draft, draft_row));
+    for (const Runs& from : read) meets = meets || meet(to, from);
+    if (meets) return fail(SMX_ERR_INVALID, "out and counts must share no memory with what the call reads");
+  }
   VerifyArgs p{};
   p.target = target, p.draft = draft, p.target_row = target_row, p.draft_row = draft_row, p.tokens = tokens;
   p.starts = step->starts, p.rows = step->rows, p.positions = step->positions, p.accept = accept, p.sample = sample;

@@ -1,9 +1,12 @@
 """What verify_drafts reads stays as it was, and a request's tokens are the same in calls of other sizes."""
 
+import ctypes
+
 import pytest
 import torch
 
 import strassen_tpu_amd as smx
+from strassen_tpu_amd import _lib
 from test_gpu_parity import DEV, say
 from test_gpu_verify import distributions, drawn, make_plan
 
@@ -52,3 +55,27 @@ def test_a_request_in_calls_of_other_sizes():
     got, counts = smx.verify_drafts(many(target, 100), many(tokens, 100), make_plan(new * 100), many(accept, 100), many(sample, 100),
                                     draft=many(draft, 100))
     assert got.tolist() == alone[0] * 100 and counts.tolist() == alone[1] * 100
+
+
+@pytest.mark.parametrize("vocab", [1000, 32001])
+def test_the_c_entry_reads_three_lists_of_a_step(vocab):
+    """No tables, no stride and no contexts are asked for; results behind the lists that are read."""
+    g = torch.Generator(device=DEV).manual_seed(72)
+    new = [3, 0, 5, 1]
+    target, draft = distributions(g, 9, vocab, torch.float32)
+    tokens = drawn(g, draft).to(torch.int32)
+    accept, sample = torch.rand(9, device=DEV, generator=g), torch.rand(4, device=DEV, generator=g)
+    plan = make_plan(new)
+    want = smx.verify_drafts(target, tokens, plan, accept, sample, draft=draft)
+    lists = torch.cat((plan.starts[:4], plan.rows, plan.positions, torch.zeros(9 + 4, dtype=torch.int32, device=DEV)))
+    starts, rows, positions, out, counts = lists.split((4, 4, 9, 9, 4))
+    at = lambda x: x.data_ptr()
+    step = _lib.SmxPagedStep(4, 9, 0, None, 0, at(starts), at(rows), None, at(positions))
+    need = ctypes.c_int64()
+    assert _lib.load().smx_verify_workspace_bytes(4, vocab, ctypes.byref(need)) == _lib.SMX_OK
+    workspace = torch.empty(need.value, dtype=torch.uint8, device=DEV)
+    rc = _lib.load().smx_verify_drafts(ctypes.byref(step), vocab, at(target), vocab, at(draft), vocab, at(tokens), at(accept), at(sample), 0,
+                                       at(out), at(counts), at(workspace), need.value, torch.cuda.current_stream().cuda_stream)
+    assert rc == _lib.SMX_OK, _lib.last_error()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want[0]) and torch.equal(counts, want[1])

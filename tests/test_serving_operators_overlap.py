@@ -58,7 +58,7 @@ def test_attention_refuses_row_sums_over_the_steps_lists(change):
     dict(sample=OUT + 28), dict(sample=FAR - 4), dict(tokens=FAR - 28), dict(tokens=FAR - 56, flags=2), dict(target=OUT + 28),
     dict(target=OUT - 4 * (700 + 100) + 4), dict(target=FAR - 4 * (7 * 128 + 100) + 4, target_row=128), dict(draft=OUT + 28, draft_row=100),
     dict(draft=FAR - 2 * 800 + 4, draft_row=100, flags=1), dict(step=_step(starts=FAR)), dict(step=_step(rows=FAR)),
-    dict(step=_step(rows=OUT + 28)), dict(step=_step(positions=FAR - 28)), dict(step=_step(positions=OUT)), dict(step=_step(context=OUT)),
+    dict(step=_step(rows=OUT + 28)), dict(step=_step(positions=FAR - 28)), dict(step=_step(positions=OUT)),
 ])
 def test_verify_refuses_results_over_what_it_reads(change):
     refused(_verify(**{**dict(out=OUT, counts=FAR), **change}), "share no memory")
