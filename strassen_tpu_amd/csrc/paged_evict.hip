@@ -382,9 +382,9 @@ __global__ __launch_bounds__(kThreads) void evict_select(EvictArgs p) {
   }
 }
 
-// Long contexts: the older tokens in parts of 8192, a workgroup each, in three launches, for which one workgroup took
-// 128 us for 32 heads of 131,000 tokens (in parts 40). evict_histogram counts each part's weights over the range that a thousand of them have,
-// evict_collect finds the part of the range that holds the edge and collects its keys, evict_list finds
+// Long contexts: the older tokens in parts of 8192, a workgroup each, in three launches, for which one workgroup took 128 us for
+// 32 heads of 131,000 tokens (in parts 40). evict_histogram counts each part's weights over the range that a thousand of them
+// have, evict_collect finds the part of the range that holds the edge and collects its keys, evict_list finds
 // the edge among them and puts each part's places and survivors on the lists.
 constexpr int kPart = 8192, kPartThreads = 256, kPartWaves = 4, kCrowd = 4096, kMostParts = 64;
 
@@ -799,8 +799,8 @@ int smx_paged_evict(const smx_paged_cache* cache, float* key_weights, int32_t re
     return fail(SMX_ERR_INVALID, "lens must share no memory with context_lens, keep_lens and block_tables");
   // rows and weights are moved while others look up where theirs lie
   for (const Runs& moved : {keys, values, all})
-    if (meet(moved, list(lens, requests)) || meet(moved, list(context_lens, requests)) || (keep_lens && meet(moved, list(keep_lens, requests))) ||
-        meet(moved, list(block_tables, (requests - 1) * table_stride + width)))
+    if (meet(moved, list(lens, requests)) || meet(moved, list(context_lens, requests)) ||
+        (keep_lens && meet(moved, list(keep_lens, requests))) || meet(moved, list(block_tables, (requests - 1) * table_stride + width)))
       return fail(SMX_ERR_INVALID, "the cache and key_weights must share no memory with the lengths and block_tables");
   EvictArgs p{};
   p.k = (uint16_t*)cache->k, p.v = (uint16_t*)cache->v;
